@@ -35,9 +35,10 @@ extern "C" {
 
 /* cfg.flags */
 #define G4A_KV_F32    0x1u /* caches hold f32 (the reference's own cache type); default f16 */
-#define G4A_IN_F16    0x2u /* g4a_kv_write: k/v inputs are f16 (kvnorm_b); default f32 (kvnorm) */
-#define G4A_NO_V_NORM 0x4u /* g4a_kv_write, g4a_decode_kv: store v as given instead of RMSNorm(v) */
-#define G4A_OUT_F32   0x8u /* g4a_prefill: f32 output (attn_prefill's "out"); default f16 (attnh) */
+#define G4A_IN_F16    0x2u /* g4a_kv_write, g4a_paged_write: k/v inputs are f16 (kvnorm_b); default f32 (kvnorm) */
+#define G4A_NO_V_NORM 0x4u /* g4a_kv_write, g4a_decode_kv, g4a_paged_*: store v as given instead of RMSNorm(v) */
+#define G4A_OUT_F32   0x8u /* g4a_prefill, g4a_paged_decode, g4a_paged_prefill: f32 output (attn_prefill's
+                              "out"); default f16 (attnh) */
 #define G4A_Q_HILO    0x10u /* g4a_prefill: keep q at f32 accuracy (f16 hi + lo MFMA operands),
                                as attn_prefill's f32 q (kernels_dsl.py:2007-2014); default rounds
                                q to f16 as qprep_b does (kernels_dsl.py:1872-1873) */
@@ -193,6 +194,87 @@ int g4a_qprep(const g4a_cfg* cfg, int S, const float* q, const float* q_gain,
 int g4a_kv_write(const g4a_cfg* cfg, int S, int start_pos, const void* k, const void* v,
                  float k_in_q, float v_in_q, const float* k_gain, const float* rope_cos,
                  const float* rope_sin, void* k_cache, void* v_cache, void* stream);
+
+/*
+ * ---- A paged K/V cache --------------------------------------------------------------------
+ * Many sequences in one pool of pages, for a server that cannot set max_seq rows aside for each.
+ * No counterpart in the reference, whose runners hold one sequence. The operations are those of
+ * g4a_kv_write, g4a_decode / g4a_decode_kv and g4a_prefill, over ragged batches.
+ *
+ *   k_pages/v_pages [n_pages][page_size][n_kv_heads][head_dim], f16, or f32 with G4A_KV_F32.
+ *               page_size a power of two, 16 .. 65536.
+ *   page_table  int32, device: position p of sequence b is row p % page_size of page
+ *               page_table[b * table_stride + p / page_size], table_cols entries a sequence.
+ *               An entry outside [0, n_pages) is a page that is not there: its positions are
+ *               neither written nor attended (-1 for the pages behind a sliding window that were
+ *               given back). Entries at or past ceil(key_len / page_size) are not used.
+ *   key_len     int32 [n_seq], device: keys of each sequence, the tokens of this call included;
+ *               0 = an idle sequence.
+ *   max_key_len host upper bound of key_len[] (a longer one is taken as max_key_len), at most
+ *               table_cols * page_size; sizes the workspaces and the grids.
+ * Packed tokens: sequence b's rows of the packed inputs are cu_q[b] .. cu_q[b + 1] - 1 (cu_q
+ * int32 [n_seq + 1], device, ascending from 0), at positions key_len[b] - (cu_q[b + 1] - cu_q[b])
+ * .. key_len[b] - 1. Rows from cu_q[n_seq] on belong to nobody: they are not read, and their
+ * outputs are left as they were. A token at a position below zero attends nothing (zeros).
+ * RoPE tables: f32 [max_key_len][head_dim / 2] at least, indexed by absolute position.
+ * Two rows of one call that map to the same cache row (a page listed twice) must not be written.
+ * Zero-initialise the struct: later versions may take over its reserved words.
+ */
+typedef struct g4a_paged {
+    void* k_pages;
+    void* v_pages;
+    const int32_t* page_table;
+    const int32_t* key_len;
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t n_seq;
+    int32_t table_cols;
+    int32_t table_stride;
+    int32_t max_key_len;
+    int32_t reserved[2]; /* 0 */
+} g4a_paged;
+
+/*
+ * Appends the k/v rows of n_tokens packed tokens: each row prepared as g4a_kv_write prepares it
+ * (the same values to the bit) and stored at its position's row.
+ *   k, v        [n_tokens][n_kv_heads][head_dim], f32, or f16 with G4A_IN_F16.
+ */
+int g4a_paged_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q, const void* k,
+                    const void* v, float k_in_q, float v_in_q, const float* k_gain, const float* rope_cos,
+                    const float* rope_sin, void* stream);
+
+/*
+ * Decode attention of one new token per sequence: query b sits at position key_len[b] - 1 and
+ * attends keys [max(0, key_len[b] - W), key_len[b]) whose pages are there; zeros if there is none.
+ *   q           f32 [n_seq][n_q_heads][head_dim] raw, q_gain and RoPE applied as g4a_decode does.
+ *   k_new/v_new f32 [n_seq][n_kv_heads][head_dim] or both NULL: the step's raw rows, prepared and
+ *               stored at position key_len[b] - 1 first, as g4a_decode_kv does (k_in_q, v_in_q and
+ *               k_gain are theirs).
+ *   out         [n_seq][n_q_heads][head_dim], f16, or f32 with G4A_OUT_F32; srq'd with out_q.
+ *   ws          at least g4a_paged_decode_ws_bytes() bytes, 256-byte aligned, uninitialised;
+ *               concurrent calls need distinct ones.
+ */
+size_t g4a_paged_decode_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg);
+int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, const float* q_gain,
+                     const float* rope_cos, const float* rope_sin, const float* k_new, const float* v_new,
+                     float k_in_q, float v_in_q, const float* k_gain, void* out, void* ws, size_t ws_bytes,
+                     void* stream);
+
+/*
+ * Causal attention of n_tokens packed tokens, prompts or pieces of them, over the cache that
+ * already holds their own rows (g4a_paged_write): the token at position p attends keys
+ * [max(0, p + 1 - W), p] whose pages are there.
+ *   q           f32 [n_tokens][n_q_heads][head_dim] raw; q_gain and RoPE are applied and the
+ *               result rounded to f16, as g4a_prefill does without G4A_Q_HILO (refused here).
+ *   out         [n_tokens][n_q_heads][head_dim], f16, or f32 with G4A_OUT_F32; srq'd with out_q.
+ *   ws          at least g4a_paged_prefill_ws_bytes() bytes, 256-byte aligned, uninitialised;
+ *               concurrent calls need distinct ones. f32 caches are converted to f16 in it
+ *               (n_seq * max_key_len rows of K and V).
+ */
+size_t g4a_paged_prefill_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens);
+int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q, const float* q,
+                      const float* q_gain, const float* rope_cos, const float* rope_sin, void* out, void* ws,
+                      size_t ws_bytes, void* stream);
 
 /*
  * ---- The q/k/v producer: projections with QAT weights --------------------------------

@@ -28,6 +28,7 @@ EXPORTS = (
     "g4a_decode_ws_bytes", "g4a_decode", "g4a_decode_kv", "g4a_decode_noalloc",
     "g4a_prefill_ws_bytes", "g4a_prefill", "g4a_qprep",
     "g4a_kv_write",
+    "g4a_paged_write", "g4a_paged_decode_ws_bytes", "g4a_paged_decode", "g4a_paged_prefill_ws_bytes", "g4a_paged_prefill",
     "g4a_dequant", "g4a_qkv_gemv", "g4a_qkv_gemv_norm", "g4a_srqh", "g4a_gemm16",
     "g4a_gemm16_ws_bytes", "g4a_gemm16_ws", "g4a_gemm16_geglu",
     "g4a_qgemv", "g4a_qgemv_geglu", "g4a_qgemv_gelu_mul", "g4a_gemv_f16", "g4a_rms_norm", "g4a_geglu",
@@ -65,6 +66,23 @@ class G4AGemmMat(ctypes.Structure):
         ("out_f32", ctypes.c_int),
         ("out_q", ctypes.c_float),
         ("alpha", ctypes.c_float),
+    ]
+
+
+class G4APaged(ctypes.Structure):
+    """struct g4a_paged: a paged K/V cache and the sequences in it."""
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("key_len", ctypes.c_void_p),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_seq", ctypes.c_int32),
+        ("table_cols", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+        ("max_key_len", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 2),
     ]
 
 
@@ -134,6 +152,17 @@ def load() -> ctypes.CDLL:
     lib.g4a_kv_write.argtypes = [cfgp, ctypes.c_int, ctypes.c_int, P, P, ctypes.c_float,
                                  ctypes.c_float, P, P, P, P, P, P]
     i, f = ctypes.c_int, ctypes.c_float
+    pgp, zp = ctypes.POINTER(G4APaged), ctypes.c_size_t
+    lib.g4a_paged_write.restype = ctypes.c_int
+    lib.g4a_paged_write.argtypes = [cfgp, pgp, i, P, P, P, f, f, P, P, P, P]
+    lib.g4a_paged_decode_ws_bytes.restype = zp
+    lib.g4a_paged_decode_ws_bytes.argtypes = [cfgp, pgp]
+    lib.g4a_paged_decode.restype = ctypes.c_int
+    lib.g4a_paged_decode.argtypes = [cfgp, pgp, P, P, P, P, P, P, f, f, P, P, P, zp, P]
+    lib.g4a_paged_prefill_ws_bytes.restype = zp
+    lib.g4a_paged_prefill_ws_bytes.argtypes = [cfgp, pgp, i]
+    lib.g4a_paged_prefill.restype = ctypes.c_int
+    lib.g4a_paged_prefill.argtypes = [cfgp, pgp, i, P, P, P, P, P, P, P, zp, P]
     lib.g4a_dequant.restype = ctypes.c_int
     lib.g4a_dequant.argtypes = [i, i, i, P, P, P, P]
     lib.g4a_qkv_gemv.restype = ctypes.c_int

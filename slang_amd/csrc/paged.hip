@@ -1,0 +1,425 @@
+// The paged K/V cache: appending rows, and the attention over it in its plainest form -- one
+// workgroup per (token, kv head), each wave every fourth key, an online softmax per wave.
+#include "paged.hpp"
+
+namespace g4a {
+
+static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
+// the outputs of n_tokens rows must not lie over the rows of q
+static bool out_over_q(const g4a_cfg* cfg, int n_tokens, const float* q, const void* out) {
+    const size_t n = (size_t)n_tokens * cfg->n_q_heads * cfg->head_dim, osz = (cfg->flags & G4A_OUT_F32) ? 4 : 2;
+    const uintptr_t a = (uintptr_t)q, b = (uintptr_t)out;
+    if (a < b + n * osz && b < a + n * 4) {
+        set_error("out must not overlap q");
+        return true;
+    }
+    return false;
+}
+
+int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8) {
+    if (!check_cfg(cfg, need_group_le8)) return G4A_EINVAL;
+    if (!pg) {
+        set_error("pg is NULL");
+        return G4A_EINVAL;
+    }
+    if (!pg->k_pages || !pg->v_pages || !pg->page_table || !pg->key_len) {
+        set_error("k_pages, v_pages, page_table and key_len must be non-NULL");
+        return G4A_EINVAL;
+    }
+    if (!aligned16(pg->k_pages) || !aligned16(pg->v_pages) || (uintptr_t)pg->page_table % 4 || (uintptr_t)pg->key_len % 4) {
+        set_error("k_pages and v_pages must be 16-byte aligned, page_table and key_len 4-byte aligned");
+        return G4A_EINVAL;
+    }
+    const int ps = pg->page_size;
+    if (ps < 16 || ps > 65536 || (ps & (ps - 1))) {
+        set_error("page_size must be a power of two of 16 .. 65536 (got %d)", ps);
+        return G4A_EUNSUPPORTED;
+    }
+    if (pg->n_pages <= 0 || pg->n_seq <= 0 || pg->table_cols <= 0 || pg->table_stride < pg->table_cols) {
+        set_error("n_pages (%d), n_seq (%d) and table_cols (%d) must be positive, table_stride (%d) at least table_cols",
+                  pg->n_pages, pg->n_seq, pg->table_cols, pg->table_stride);
+        return G4A_EINVAL;
+    }
+    if (pg->max_key_len <= 0 || (int64_t)pg->max_key_len > (int64_t)pg->table_cols * ps || pg->max_key_len > 1 << 30) {
+        set_error("max_key_len (%d) must be in [1, table_cols * page_size] and at most 2^30", pg->max_key_len);
+        return G4A_EINVAL;
+    }
+    if (pg->reserved[0] || pg->reserved[1]) {
+        set_error("g4a_paged's reserved words must be 0");
+        return G4A_EINVAL;
+    }
+    if (cfg->head_dim != 256 && cfg->head_dim != 512) {
+        set_error("head_dim %u not supported (256 or 512)", cfg->head_dim);
+        return G4A_EUNSUPPORTED;
+    }
+    if (cfg->n_kv_heads > 4096 || cfg->n_q_heads > 32768 || (int64_t)pg->n_seq * cfg->n_kv_heads > 65535) {
+        set_error("n_kv_heads (%u), n_q_heads (%u) or n_seq * n_kv_heads (n_seq %d) too large", cfg->n_kv_heads,
+                  cfg->n_q_heads, pg->n_seq);
+        return G4A_EINVAL;
+    }
+    if (cfg->window > 1u << 30) {
+        set_error("window (%u) must be at most 2^30", cfg->window);
+        return G4A_EINVAL;
+    }
+    return G4A_OK;
+}
+
+PageTab page_tab(const g4a_paged* pg) {
+    return PageTab{pg->page_table, pg->key_len, pg->n_seq, pg->table_stride, pg->table_cols, pg->n_pages,
+                   __builtin_ctz((unsigned)pg->page_size), pg->max_key_len};
+}
+
+struct PagedWriteArgs {
+    PageTab t;
+    const int32_t* cu;
+    const void* k;
+    const void* v;
+    const float* k_gain;
+    const float* rcos;
+    const float* rsin;
+    void* kc;
+    void* vc;
+    int n_tokens, n_kv_heads, v_norm;
+    float k_in_q, v_in_q, eps;
+};
+
+template <int HD, typename IT, typename CT>
+__global__ __launch_bounds__(HD / 2) void paged_write_kernel(PagedWriteArgs a) {
+    constexpr int HALF = HD / 2, NW = HALF / 64;
+    __shared__ float red[2 * NW];
+    const int t = threadIdx.x, tok = blockIdx.x, kh = blockIdx.y;
+    int b = tok, p;  // without cu, row b is sequence b's last key
+    if (a.cu) {
+        b = seq_of_row(a.cu, a.t.n_seq, tok);
+        if (b >= a.t.n_seq) return;
+        const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
+        if (tok < r.lo || tok >= r.hi) return;
+        p = r.keys - r.hi + tok;
+    } else {
+        p = paged_len(a.t, b) - 1;
+    }
+    if (p < 0) return;
+    const int page = page_at(a.t, b, p);
+    if (!page_ok(a.t, page)) return;
+    const size_t row = ((size_t)tok * a.n_kv_heads + kh) * HD;
+    const IT* kin = reinterpret_cast<const IT*>(a.k) + row;
+    const IT* vin = reinterpret_cast<const IT*>(a.v) + row;
+    float k0 = (float)kin[t], k1 = (float)kin[t + HALF], v0 = (float)vin[t], v1 = (float)vin[t + HALF];
+    kv_pair_prep<HD>(k0, k1, v0, v1, a.k_gain, a.rcos ? a.rcos + (size_t)p * HALF : nullptr,
+                     a.rsin ? a.rsin + (size_t)p * HALF : nullptr, a.v_norm != 0, a.eps, a.k_in_q, a.v_in_q, red, t);
+    const size_t crow = paged_row(a.t, page, p, a.n_kv_heads * HD) + (size_t)kh * HD;
+    CT* kc = reinterpret_cast<CT*>(a.kc) + crow;
+    CT* vc = reinterpret_cast<CT*>(a.vc) + crow;
+    store_elem(kc + t, k0);
+    store_elem(kc + t + HALF, k1);
+    store_elem(vc + t, v0);
+    store_elem(vc + t + HALF, v1);
+}
+
+typedef void (*paged_write_fn)(PagedWriteArgs);
+template <int HD>
+static paged_write_fn pick_write(bool in16, bool c32) {
+    if (in16) return c32 ? paged_write_kernel<HD, half_t, float> : paged_write_kernel<HD, half_t, half_t>;
+    return c32 ? paged_write_kernel<HD, float, float> : paged_write_kernel<HD, float, half_t>;
+}
+
+static int launch_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu, bool in16, const void* k,
+                        const void* v, float k_in_q, float v_in_q, const float* k_gain, const float* rcos,
+                        const float* rsin, hipStream_t stream) {
+    PagedWriteArgs a;
+    a.t = page_tab(pg);
+    a.cu = cu;
+    a.k = k;
+    a.v = v;
+    a.k_gain = k_gain;
+    a.rcos = rcos;
+    a.rsin = rsin;
+    a.kc = pg->k_pages;
+    a.vc = pg->v_pages;
+    a.n_tokens = n_tokens;
+    a.n_kv_heads = (int)cfg->n_kv_heads;
+    a.v_norm = (cfg->flags & G4A_NO_V_NORM) ? 0 : 1;
+    a.k_in_q = k_in_q;
+    a.v_in_q = v_in_q;
+    a.eps = cfg->eps;
+    const bool c32 = (cfg->flags & G4A_KV_F32) != 0;
+    hipLaunchKernelGGL(cfg->head_dim == 256 ? pick_write<256>(in16, c32) : pick_write<512>(in16, c32),
+                       dim3((unsigned)n_tokens, cfg->n_kv_heads), dim3(cfg->head_dim / 2), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? G4A_OK : hip_error(e, "paged write launch");
+}
+
+struct PagedAttnArgs {
+    PageTab t;
+    const int32_t* cu;  // NULL: decode, token b of sequence b at position key_len - 1
+    const float* q;
+    const float* q_gain;
+    const float* rcos;
+    const float* rsin;
+    const void* kc;
+    const void* vc;
+    void* out;
+    int n_tokens, n_q_heads, n_kv_heads, window, out32;
+    float scale_log2, eps, out_q;
+};
+
+template <int HD, int G, typename KVT>
+__global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
+    constexpr int E = HD / 64;  // dims of a lane: d0 .. d0 + E/2 - 1 and the same + HD/2
+    __shared__ float sm[4][G], sl[4][G];
+    __shared__ float so[4][G][HD];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tok = blockIdx.x, kh = blockIdx.y;
+    int b, p;
+    if (a.cu) {
+        b = seq_of_row(a.cu, a.t.n_seq, tok);
+        if (b >= a.t.n_seq) return;
+        const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
+        if (tok < r.lo || tok >= r.hi) return;
+        p = r.keys - r.hi + tok;
+    } else {
+        b = tok;
+        p = paged_len(a.t, b) - 1;
+    }
+    float x[G][E], o[G][E], m[G], l[G];
+    const int d0 = E / 2 * lane;
+    for (int h = 0; h < G; ++h) {
+        const float* qr = a.q + ((size_t)tok * a.n_q_heads + kh * G + h) * HD;
+        float ss = 0.0f;
+        for (int e = 0; e < E / 2; ++e) {
+            x[h][e] = qr[d0 + e];
+            x[h][e + E / 2] = qr[d0 + e + HD / 2];
+            ss += x[h][e] * x[h][e] + x[h][e + E / 2] * x[h][e + E / 2];
+        }
+        const float rs = a.q_gain ? 1.0f / sqrtf(wave_sum(ss) / (float)HD + a.eps) : 1.0f;
+        for (int e = 0; e < E / 2; ++e) {
+            const float x0 = a.q_gain ? x[h][e] * rs * a.q_gain[d0 + e] : x[h][e];
+            const float x1 = a.q_gain ? x[h][e + E / 2] * rs * a.q_gain[d0 + e + HD / 2] : x[h][e + E / 2];
+            const float c = a.rcos && p >= 0 ? a.rcos[(size_t)p * (HD / 2) + d0 + e] : 1.0f;
+            const float s = a.rcos && p >= 0 ? a.rsin[(size_t)p * (HD / 2) + d0 + e] : 0.0f;
+            x[h][e] = (x0 * c - x1 * s) * a.scale_log2;
+            x[h][e + E / 2] = (x1 * c + x0 * s) * a.scale_log2;
+        }
+        for (int e = 0; e < E; ++e) o[h][e] = 0.0f;
+        m[h] = kNegInf;
+        l[h] = 0.0f;
+    }
+    const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
+    for (int t = lo + wave; t <= p; t += 4) {
+        const int page = page_at(a.t, b, t);
+        if (!page_ok(a.t, page)) continue;
+        const size_t row = paged_row(a.t, page, t, a.n_kv_heads * HD) + (size_t)kh * HD;
+        const KVT* kr = reinterpret_cast<const KVT*>(a.kc) + row;
+        const KVT* vr = reinterpret_cast<const KVT*>(a.vc) + row;
+        float kx[E], vx[E];
+        for (int e = 0; e < E / 2; ++e) {
+            kx[e] = (float)kr[d0 + e];
+            kx[e + E / 2] = (float)kr[d0 + e + HD / 2];
+            vx[e] = (float)vr[d0 + e];
+            vx[e + E / 2] = (float)vr[d0 + e + HD / 2];
+        }
+        for (int h = 0; h < G; ++h) {
+            float s = 0.0f;
+            for (int e = 0; e < E; ++e) s += x[h][e] * kx[e];
+            s = wave_sum(s);
+            const float mn = fmaxf(m[h], s), mu = mn == kNegInf ? 0.0f : mn;
+            const float c = fexp2(m[h] - mu), w = fexp2(s - mu);
+            for (int e = 0; e < E; ++e) o[h][e] = o[h][e] * c + w * vx[e];
+            l[h] = l[h] * c + w;
+            m[h] = mn;
+        }
+    }
+    for (int h = 0; h < G; ++h) {
+        for (int e = 0; e < E / 2; ++e) {
+            so[wave][h][d0 + e] = o[h][e];
+            so[wave][h][d0 + e + HD / 2] = o[h][e + E / 2];
+        }
+        if (lane == 0) {
+            sm[wave][h] = m[h];
+            sl[wave][h] = l[h];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < G * HD; i += 256) {
+        const int h = i / HD, d = i % HD;
+        float M = kNegInf, L = 0.0f, O = 0.0f;
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w][h]);
+        for (int w = 0; w < 4; ++w) {
+            const float wt = sm[w][h] == kNegInf ? 0.0f : fexp2(sm[w][h] - M);
+            L += wt * sl[w][h];
+            O += wt * so[w][h][d];
+        }
+        const float y = L > 0.0f ? srq(O / L, a.out_q) : 0.0f;
+        const size_t at = ((size_t)tok * a.n_q_heads + kh * G + h) * HD + d;
+        if (a.out32) reinterpret_cast<float*>(a.out)[at] = y;
+        else reinterpret_cast<half_t*>(a.out)[at] = (half_t)y;
+    }
+}
+
+typedef void (*paged_attn_fn)(PagedAttnArgs);
+template <int HD, typename KVT>
+static paged_attn_fn pick_attn(int G) {
+    switch (G) {
+        case 1: return paged_attn_kernel<HD, 1, KVT>;
+        case 2: return paged_attn_kernel<HD, 2, KVT>;
+        case 4: return paged_attn_kernel<HD, 4, KVT>;
+        case 8: return paged_attn_kernel<HD, 8, KVT>;
+    }
+    return nullptr;
+}
+
+static int launch_attn(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu, const float* q,
+                       const float* q_gain, const float* rcos, const float* rsin, void* out, hipStream_t stream) {
+    PagedAttnArgs a;
+    a.t = page_tab(pg);
+    a.cu = cu;
+    a.q = q;
+    a.q_gain = q_gain;
+    a.rcos = rcos;
+    a.rsin = rsin;
+    a.kc = pg->k_pages;
+    a.vc = pg->v_pages;
+    a.out = out;
+    a.n_tokens = n_tokens;
+    a.n_q_heads = (int)cfg->n_q_heads;
+    a.n_kv_heads = (int)cfg->n_kv_heads;
+    a.window = (int)cfg->window;
+    a.out32 = (cfg->flags & G4A_OUT_F32) != 0;
+    a.scale_log2 = cfg->scale * kLog2e;
+    a.eps = cfg->eps;
+    a.out_q = cfg->out_q;
+    const int G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
+    const bool c32 = (cfg->flags & G4A_KV_F32) != 0;
+    const paged_attn_fn fn = cfg->head_dim == 256 ? (c32 ? pick_attn<256, float>(G) : pick_attn<256, half_t>(G))
+                                                  : (c32 ? pick_attn<512, float>(G) : pick_attn<512, half_t>(G));
+    hipLaunchKernelGGL(fn, dim3((unsigned)n_tokens, cfg->n_kv_heads), dim3(256), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? G4A_OK : hip_error(e, "paged attention launch");
+}
+
+static int check_rope(const float* rcos, const float* rsin) {
+    if ((rcos == nullptr) != (rsin == nullptr)) {
+        set_error("rope_cos and rope_sin must both be given or both be NULL");
+        return G4A_EINVAL;
+    }
+    return G4A_OK;
+}
+static int check_steps(float k_in_q, float v_in_q) {
+    if (!(k_in_q >= 0.0f) || !(v_in_q >= 0.0f)) {
+        set_error("k_in_q/v_in_q must be >= 0");
+        return G4A_EINVAL;
+    }
+    return G4A_OK;
+}
+static int check_tokens(const g4a_cfg* cfg, int n_tokens, const int32_t* cu) {
+    if (n_tokens <= 0 || !cu || (uintptr_t)cu % 4) {
+        set_error("n_tokens (%d) must be positive and cu_q non-NULL and 4-byte aligned", n_tokens);
+        return G4A_EINVAL;
+    }
+    if ((int64_t)n_tokens * cfg->n_q_heads > 0x7fffffff - 64) {
+        set_error("n_tokens * n_q_heads too large");
+        return G4A_EINVAL;
+    }
+    return G4A_OK;
+}
+
+}  // namespace g4a
+
+using namespace g4a;
+
+extern "C" int g4a_paged_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q,
+                               const void* k, const void* v, float k_in_q, float v_in_q, const float* k_gain,
+                               const float* rope_cos, const float* rope_sin, void* stream) {
+    if (const int rc = check_paged(cfg, pg, false)) return rc;
+    if (const int rc = check_tokens(cfg, n_tokens, cu_q)) return rc;
+    if (const int rc = check_rope(rope_cos, rope_sin)) return rc;
+    if (const int rc = check_steps(k_in_q, v_in_q)) return rc;
+    if (!k || !v) {
+        set_error("k and v must be non-NULL");
+        return G4A_EINVAL;
+    }
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_gain) || !aligned16(rope_cos) || !aligned16(rope_sin)) {
+        set_error("k, v, k_gain and the rope tables must be 16-byte aligned");
+        return G4A_EINVAL;
+    }
+    return launch_write(cfg, pg, n_tokens, cu_q, (cfg->flags & G4A_IN_F16) != 0, k, v, k_in_q, v_in_q, k_gain, rope_cos,
+                        rope_sin, (hipStream_t)stream);
+}
+
+extern "C" size_t g4a_paged_decode_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg) {
+    return check_paged(cfg, pg, true) ? 0 : 512;
+}
+
+extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, const float* q_gain,
+                                const float* rope_cos, const float* rope_sin, const float* k_new, const float* v_new,
+                                float k_in_q, float v_in_q, const float* k_gain, void* out, void* ws,
+                                size_t ws_bytes, void* stream) {
+    if (const int rc = check_paged(cfg, pg, true)) return rc;
+    if (const int rc = check_rope(rope_cos, rope_sin)) return rc;
+    if (const int rc = check_steps(k_in_q, v_in_q)) return rc;
+    if (!q || !out) {
+        set_error("q and out must be non-NULL");
+        return G4A_EINVAL;
+    }
+    if ((k_new == nullptr) != (v_new == nullptr)) {
+        set_error("k_new and v_new must both be given or both be NULL");
+        return G4A_EINVAL;
+    }
+    if (cfg->flags & G4A_IN_F16) {
+        set_error("g4a_paged_decode takes f32 k/v rows (G4A_IN_F16 not supported)");
+        return G4A_EUNSUPPORTED;
+    }
+    if (!aligned16(q) || !aligned16(out) || !aligned16(q_gain) || !aligned16(rope_cos) || !aligned16(rope_sin) ||
+        !aligned16(k_new) || !aligned16(v_new) || !aligned16(k_gain)) {
+        set_error("q, out, the gains, the rope tables, k_new and v_new must be 16-byte aligned");
+        return G4A_EINVAL;
+    }
+    if (out_over_q(cfg, pg->n_seq, q, out)) return G4A_EINVAL;
+    const size_t need = g4a_paged_decode_ws_bytes(cfg, pg);
+    if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
+        set_error("paged decode workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
+        return G4A_EWORKSPACE;
+    }
+    if (k_new) {
+        if (const int rc = launch_write(cfg, pg, pg->n_seq, nullptr, false, k_new, v_new, k_in_q, v_in_q, k_gain, rope_cos,
+                                        rope_sin, (hipStream_t)stream))
+            return rc;
+    }
+    return launch_attn(cfg, pg, pg->n_seq, nullptr, q, q_gain, rope_cos, rope_sin, out, (hipStream_t)stream);
+}
+
+extern "C" size_t g4a_paged_prefill_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens) {
+    if (check_paged(cfg, pg, true)) return 0;
+    if (n_tokens <= 0) {
+        set_error("n_tokens (%d) must be positive", n_tokens);
+        return 0;
+    }
+    return 512;
+}
+
+extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q,
+                                 const float* q, const float* q_gain, const float* rope_cos, const float* rope_sin,
+                                 void* out, void* ws, size_t ws_bytes, void* stream) {
+    if (const int rc = check_paged(cfg, pg, true)) return rc;
+    if (const int rc = check_tokens(cfg, n_tokens, cu_q)) return rc;
+    if (const int rc = check_rope(rope_cos, rope_sin)) return rc;
+    if (!q || !out) {
+        set_error("q and out must be non-NULL");
+        return G4A_EINVAL;
+    }
+    if (cfg->flags & G4A_Q_HILO) {
+        set_error("g4a_paged_prefill rounds q to f16 (G4A_Q_HILO not supported)");
+        return G4A_EUNSUPPORTED;
+    }
+    if (!aligned16(q) || !aligned16(out) || !aligned16(q_gain) || !aligned16(rope_cos) || !aligned16(rope_sin)) {
+        set_error("q, out, q_gain and the rope tables must be 16-byte aligned");
+        return G4A_EINVAL;
+    }
+    if (out_over_q(cfg, n_tokens, q, out)) return G4A_EINVAL;
+    const size_t need = g4a_paged_prefill_ws_bytes(cfg, pg, n_tokens);
+    if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
+        set_error("paged prefill workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
+        return G4A_EWORKSPACE;
+    }
+    return launch_attn(cfg, pg, n_tokens, cu_q, q, q_gain, rope_cos, rope_sin, out, (hipStream_t)stream);
+}
