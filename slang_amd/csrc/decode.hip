@@ -33,9 +33,13 @@
 //    agent-scope release has to write back the XCD's L2 and the merger then walks every
 //    partial serially.)
 // Scores are in the log2 domain (q carries scale*log2 e), so the softmax uses exp2.
+// A paged cache (g4a_paged_decode) runs the same kernels with PagedDecodeArgs: a 16-key block lies
+// in one page, so splits start at multiples of 16 and each block's rows come through buffer
+// resources of their own; everything else, the plan and the merge included, is shared.
 #include <mutex>
+#include <type_traits>
 
-#include "common.hpp"
+#include "paged.hpp"
 
 namespace g4a {
 
@@ -68,6 +72,13 @@ struct DecodeArgs {
     void* vc_out;
     float k_in_q, v_in_q;
     int v_norm;
+};
+
+// the same over a paged cache: key_len, kc, vc and fixed_len are not used, seq_stride neither; the RoPE
+// tables hold a row per absolute position
+struct PagedDecodeArgs : DecodeArgs {
+    PageTab t;
+    int out16;  // f16 output
 };
 
 template <int HD, int G>
@@ -154,6 +165,13 @@ __device__ __forceinline__ float dpp_row_shl(float x) {
 // keys of sequence s: from the device array, or the host-given length when there is none
 // (a batch-1 decode knows its position on the host, as the reference's params do)
 __device__ __forceinline__ int seq_len(const DecodeArgs& a, int s) { return a.key_len ? a.key_len[s] : a.fixed_len; }
+__device__ __forceinline__ int seq_len(const PagedDecodeArgs& a, int s) { return paged_len(a.t, s); }
+
+// first key of the splits of a sequence of T keys: the first attended one, on a paged cache the start of
+// its 16-key block (the keys before it are masked)
+__device__ __forceinline__ int first_key(const DecodeArgs& a, int T) { return (a.window > 0 && T > a.window) ? T - a.window : 0; }
+__device__ __forceinline__ int split_lo(const DecodeArgs& a, int T) { return first_key(a, T); }
+__device__ __forceinline__ int split_lo(const PagedDecodeArgs& a, int T) { return first_key(a, T) & ~15; }
 
 // Keys attended by sequence b and how they are split: active keys [lo, hi), split c covers
 // [lo + c*chunk, min(lo + (c+1)*chunk, hi)); split c is live when c*chunk < hi - lo. No
@@ -162,10 +180,11 @@ __device__ __forceinline__ int seq_len(const DecodeArgs& a, int s) { return a.ke
 struct SplitPlan {
     int lo, hi, active, chunk;
 };
-__device__ __forceinline__ SplitPlan split_plan(const DecodeArgs& a, int b) {
+template <typename A>
+__device__ __forceinline__ SplitPlan split_plan(const A& a, int b) {
     SplitPlan p;
     p.hi = seq_len(a, b);
-    p.lo = (a.window > 0 && p.hi > a.window) ? p.hi - a.window : 0;
+    p.lo = split_lo(a, p.hi);
     p.active = p.hi - p.lo;
     p.chunk = a.chunk;
     if (p.active > a.max_splits * a.chunk)
@@ -185,11 +204,13 @@ __device__ __forceinline__ SplitPlan split_plan(const DecodeArgs& a, int b) {
 __device__ __forceinline__ int active_keys(const DecodeArgs& a, int T) {
     return T <= 0 ? 0 : (a.window > 0 && T > a.window) ? a.window : T;
 }
+__device__ __forceinline__ int active_keys(const PagedDecodeArgs& a, int T) { return T - split_lo(a, T); }
 __device__ __forceinline__ int ceil_div(int x, int d) { return x / d + (x % d != 0); }
 
 // chunk of the plan; act0 returns this lane's sequence of the first 64 (its active keys),
 // so a batch of up to 64 sequences reads key_len once
-__device__ __forceinline__ int list_chunk(const DecodeArgs& a, int& act0) {
+template <typename A>
+__device__ __forceinline__ int list_chunk(const A& a, int& act0) {
     const int lane = threadIdx.x & 63;
     unsigned long long tot = 0;
     act0 = 0;
@@ -208,7 +229,8 @@ __device__ __forceinline__ int list_chunk(const DecodeArgs& a, int& act0) {
     return __builtin_amdgcn_readfirstlane((int)c);
 }
 
-__device__ __forceinline__ int list_active(const DecodeArgs& a, int s0, int act0, int n) {
+template <typename A>
+__device__ __forceinline__ int list_active(const A& a, int s0, int act0, int n) {
     const int s = s0 + (threadIdx.x & 63);
     return s0 == 0 ? (s < n ? act0 : 0) : (s < n ? active_keys(a, seq_len(a, s)) : 0);
 }
@@ -217,7 +239,8 @@ struct ListUnit {
     int b, kh, ci, splits;
 };
 // the unit of workgroup L (b = -1: past the last unit)
-__device__ __forceinline__ ListUnit list_unit(const DecodeArgs& a, int chunk, int act0, int L) {
+template <typename A>
+__device__ __forceinline__ ListUnit list_unit(const A& a, int chunk, int act0, int L) {
     int base = 0;  // units of the sequences before this group of 64
     for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
         const int sp = ceil_div(list_active(a, s0, act0, a.n_seq), chunk);
@@ -252,9 +275,10 @@ __device__ __forceinline__ void bload_q(rsrc_t r, int off, float (&x)[QP]) {
 // LIST: the unit comes from the work-list plan (several sequences); KVW: the fused KV write
 // of g4a_decode_kv. Both are template switches so the plain single-sequence kernel carries
 // neither (their code measured 0.2 us on the latency-bound T 4096 call).
-template <int HD, int G, typename KVT, bool LIST, bool KVW>
+template <int HD, int G, typename KVT, bool LIST, bool KVW, typename A = DecodeArgs>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 256 && sizeof(KVT) == 2 ? 2 : 1)))
-void decode_kernel(DecodeArgs a) {
+void decode_kernel(A a) {
+    constexpr bool PAGED = std::is_same_v<A, PagedDecodeArgs>;
     using Sh = DecodeShape<HD, G>;
     constexpr int KSTEPS = Sh::KSTEPS, NDT = Sh::NDT, VLANES = Sh::VLANES, VROWS = Sh::VROWS;
     constexpr int VLOADS = Sh::VLOADS, VSTR = Sh::VSTR, QSTR = Sh::QSTR;
@@ -299,7 +323,7 @@ void decode_kernel(DecodeArgs a) {
         // merge needs no plan of its own (a pair without keys has no unit and no entry)
         if (ci == 0 && tid == 0) a.list_tab[b * a.n_kv_heads + kh] = make_int2((int)blockIdx.x, u.splits);
         sp.hi = seq_len(a, b);
-        sp.lo = (a.window > 0 && sp.hi > a.window) ? sp.hi - a.window : 0;
+        sp.lo = split_lo(a, sp.hi);
         sp.active = sp.hi - sp.lo;
         sp.chunk = chunk;
         slot = blockIdx.x;
@@ -308,7 +332,10 @@ void decode_kernel(DecodeArgs a) {
         sp = split_plan(a, b);  // scalar load of key_len, issued first
         slot = (size_t)(b * a.n_kv_heads + kh) * a.max_splits + ci;
     }
-    float* outp = a.out + ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD;
+    const size_t outo = ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD;
+    float* outp = a.out + outo;
+    bool out16 = false;  // paged: outp's rows are f16
+    if constexpr (PAGED) out16 = a.out16;
 
     // ---- q operand loads: they depend on nothing but the sequence and kv head.
     // Wave w prepares heads w, w+4 (a head >= G reads past the q range: zeros, no traffic).
@@ -317,8 +344,9 @@ void decode_kernel(DecodeArgs a) {
     const int d0 = QP * lane;             // this lane: dims d0.. and d0+HD/2..
     const rsrc_t rq = make_rsrc(a.q + ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD, G * HD * 4);
     const rsrc_t rg = make_rsrc(a.q_gain, a.q_gain ? HD * 4 : 0);
-    const rsrc_t rc = make_rsrc(a.rcos ? a.rcos + (size_t)b * (HD / 2) : nullptr, a.rcos ? HD * 2 : 0);
-    const rsrc_t rs = make_rsrc(a.rsin ? a.rsin + (size_t)b * (HD / 2) : nullptr, a.rsin ? HD * 2 : 0);
+    const int rrow = PAGED ? max(sp.hi - 1, 0) : b;  // the query's row of the RoPE tables
+    const rsrc_t rc = make_rsrc(a.rcos ? a.rcos + (size_t)rrow * (HD / 2) : nullptr, a.rcos ? HD * 2 : 0);
+    const rsrc_t rs = make_rsrc(a.rsin ? a.rsin + (size_t)rrow * (HD / 2) : nullptr, a.rsin ? HD * 2 : 0);
     float qx[NQH][2][QP], qgv[2][QP], qcv[QP], qsv[QP];
 #pragma unroll
     for (int j = 0; j < NQH; ++j) {
@@ -336,7 +364,10 @@ void decode_kernel(DecodeArgs a) {
     const bool single = a.max_splits == 1;
     if (ci * sp.chunk >= sp.active) {
         if (single) {
-            for (int e = tid; e < G * HD; e += 256) outp[e] = 0.0f;  // no keys: zeros
+            for (int e = tid; e < G * HD; e += 256) {  // no keys: zeros
+                if (PAGED && out16) reinterpret_cast<half_t*>(a.out)[outo + e] = (half_t)0.0f;
+                else outp[e] = 0.0f;
+            }
         } else if (tid < G) {
             a.part_ml[slot * G + tid] = make_float2(kNegInf, 0.0f);
         }
@@ -353,8 +384,8 @@ void decode_kernel(DecodeArgs a) {
     float nk0 = 0.0f, nk1 = 0.0f, nv0 = 0.0f, nv1 = 0.0f;
     KvPairOps nops{1.0f, 1.0f, 1.0f, 0.0f};
     if (owns_new) {  // with the raw row, ahead of the block loads (which they would wait behind)
-        nops = kv_pair_ops<HD>(a.k_gain, a.rcos ? a.rcos + (size_t)b * HALF : nullptr,
-                               a.rsin ? a.rsin + (size_t)b * HALF : nullptr, tid);
+        nops = kv_pair_ops<HD>(a.k_gain, a.rcos ? a.rcos + (size_t)rrow * HALF : nullptr,
+                               a.rsin ? a.rsin + (size_t)rrow * HALF : nullptr, tid);
     }
     if (owns_new && tid < HALF) {
         const size_t ro = ((size_t)b * a.n_kv_heads + kh) * HD;
@@ -371,16 +402,49 @@ void decode_kernel(DecodeArgs a) {
     // A layout (lane n,g: key n, dims 32s+8g..), V rows of VLANES lanes.
     const size_t rstride = (size_t)a.n_kv_heads * HD;  // elements per cache row
     const int rsb = (int)(rstride * ESZ);               // bytes per cache row
-    const uint32_t range = (uint32_t)(k1 - k0) * (uint32_t)rsb;
-    const size_t row0 = (size_t)b * a.seq_stride + (size_t)k0 * rstride + (size_t)kh * HD;
+    const uint32_t range = PAGED ? 0 : (uint32_t)(k1 - k0) * (uint32_t)rsb;
+    const size_t row0 = PAGED ? 0 : (size_t)b * a.seq_stride + (size_t)k0 * rstride + (size_t)kh * HD;
     const rsrc_t rk = make_rsrc(reinterpret_cast<const KVT*>(a.kc) + row0, range);
     const rsrc_t rv = make_rsrc(reinterpret_cast<const KVT*>(a.vc) + row0, range);
+    // paged: lane j holds the table entry of this wave's block j (of 64 at a time); a block reads rows
+    // [max(blk, first attended key), k1) of its page, all others as zeros, whatever they hold
+    const int key_lo = PAGED ? first_key(a, sp.hi) : 0;
+    int entries = -1, blk_page = -1;  // blk_page: the page of the block in the registers
+    auto load_entries = [&](int blk) {
+        if constexpr (PAGED) {
+            const rsrc_t rt = make_rsrc(a.t.table + (size_t)b * a.t.stride, (uint32_t)a.t.cols * 4);
+            entries = __builtin_amdgcn_raw_buffer_load_b32(rt, ((blk + 64 * lane) >> a.t.shift) * 4, 0, 0);
+        }
+    };
     const int vrow = lane / VLANES;
     const int koff = n * rsb + 8 * g * ESZ, voff = vrow * rsb + 8 * (lane % VLANES) * ESZ;
     kraw_t kr[KROW ? 1 : KSTEPS];
     half8 krow[KROW ? VLOADS : 1];
     vraw_t vr[VLOADS];
     auto load_block = [&](int blk) {
+        if constexpr (PAGED) {
+            const int j = (blk - k0) >> 6;
+            if (j != 0 && (j & 63) == 0) load_entries(blk);
+            blk_page = __builtin_amdgcn_readlane(entries, j & 63);
+            const bool ok = page_ok(a.t, blk_page);
+            const uint32_t bytes = ok ? (uint32_t)(min(max(k1 - blk, 0), 16) * rsb) : 0u;
+            const size_t at = paged_row(a.t, ok ? blk_page : 0, blk, (int)rstride) + (size_t)kh * HD;
+            const rsrc_t pk = make_rsrc(reinterpret_cast<const KVT*>(a.kc) + at, bytes);
+            const rsrc_t pv = make_rsrc(reinterpret_cast<const KVT*>(a.vc) + at, bytes);
+            // rows in front of the first attended key: an offset past every range (and with room for
+            // the second half of an f32 load)
+            const auto off = [&](int row, int o) { return blk + row < key_lo ? 0x7fffff00 : o; };
+            if constexpr (KROW) {
+#pragma unroll
+                for (int i = 0; i < VLOADS; ++i) krow[i] = bload_h8_nt(pk, off(VROWS * i + vrow, VROWS * i * rsb + voff));
+            } else {
+#pragma unroll
+                for (int s = 0; s < KSTEPS; ++s) kr[s] = KO::load(pk, off(n, koff + 32 * s * ESZ));
+            }
+#pragma unroll
+            for (int i = 0; i < VLOADS; ++i) vr[i] = VO::load(pv, off(VROWS * i + vrow, VROWS * i * rsb + voff));
+            return;
+        }
         const int r = (blk - k0) * rsb;
         if constexpr (KROW) {
 #pragma unroll
@@ -393,6 +457,7 @@ void decode_kernel(DecodeArgs a) {
         for (int i = 0; i < VLOADS; ++i) vr[i] = VO::load(rv, r + VROWS * i * rsb + voff);
     };
     int blk = k0 + wave * 16;
+    load_entries(blk);
     // in flight during the q prologue. Unconditional: a block past k1 reads zeros without
     // memory traffic. Under a branch, the join left the compiler unsure how many loads
     // followed q's, so the prologue waited for the block's loads too (vmcnt(4), not 20).
@@ -445,13 +510,23 @@ void decode_kernel(DecodeArgs a) {
         kv_pair_prep<HD>(nk0, nk1, nv0, nv1, nops, a.k_gain != nullptr, a.rcos != nullptr, a.v_norm != 0, a.eps,
                          a.k_in_q, a.v_in_q, kv_red, tid);
         if (tid < HALF) {
-            const size_t crow = (size_t)b * a.seq_stride + (size_t)p_new * a.n_kv_heads * HD + (size_t)kh * HD;
+            size_t crow;
+            bool there = true;
+            if constexpr (PAGED) {
+                const int page = page_at(a.t, b, p_new);
+                there = page_ok(a.t, page);
+                crow = paged_row(a.t, there ? page : 0, p_new, a.n_kv_heads * HD) + (size_t)kh * HD;
+            } else {
+                crow = (size_t)b * a.seq_stride + (size_t)p_new * a.n_kv_heads * HD + (size_t)kh * HD;
+            }
             KVT* kcw = reinterpret_cast<KVT*>(a.kc_out) + crow;
             KVT* vcw = reinterpret_cast<KVT*>(a.vc_out) + crow;
-            store_elem(kcw + tid, nk0);
-            store_elem(kcw + tid + HALF, nk1);
-            store_elem(vcw + tid, nv0);
-            store_elem(vcw + tid + HALF, nv1);
+            if (!PAGED || there) {
+                store_elem(kcw + tid, nk0);
+                store_elem(kcw + tid + HALF, nk1);
+                store_elem(vcw + tid, nv0);
+                store_elem(vcw + tid + HALF, nv1);
+            }
             sKn[tid] = (KVT)nk0;
             sKn[tid + HALF] = (KVT)nk1;
             sVn[tid] = (KVT)nv0;
@@ -478,6 +553,9 @@ void decode_kernel(DecodeArgs a) {
         // the block holding the new key: its row comes from the prepared copy, whatever
         // the load (issued before the store) returned
         const bool patch = owns_new && p_new >= blk && p_new < blk + 16;  // wave-uniform
+        // paged: the block's keys [lo_i, hi_i) attend, none if its page is not there
+        int lo_i = 0;
+        if constexpr (PAGED) lo_i = page_ok(a.t, blk_page) ? key_lo : k1;
         float4v c4 = float4v{0, 0, 0, 0};
         if constexpr (KROW) {
             // K and V rows into this wave's LDS blocks (the new key's row over whatever its
@@ -524,12 +602,13 @@ void decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float v = c4[i] + dpp_row_shl<G>(c4[i]);  // high + low column
-            sc[i] = (n < G && blk + 4 * g + i < k1) ? v : kNegInf;
+            sc[i] = (n < G && blk + 4 * g + i < k1 && (!PAGED || blk + 4 * g + i >= lo_i)) ? v : kNegInf;
             mloc = fmaxf(mloc, sc[i]);
         }
         mloc = max32(max16(mloc));
-        const float m_new = fmaxf(m_run, mloc);            // finite for heads: key blk is valid
-        const float m_use = (m_new == kNegInf) ? 0.0f : m_new;  // padding columns stay at zero
+        // finite for heads, as key blk is valid (but for a paged block without an attended key)
+        const float m_new = fmaxf(m_run, mloc);
+        const float m_use = (m_new == kNegInf) ? 0.0f : m_new;  // such columns and the padding's stay at zero
         half4 pb;
         float ps = 0.0f;
 #pragma unroll
@@ -583,11 +662,12 @@ void decode_kernel(DecodeArgs a) {
             o += *reinterpret_cast<const float4v*>(&lds[w * G * HD + e]) * wt;
         }
         if (single) {
-            const float inv = 1.0f / L;
+            const float inv = PAGED && !(L > 0.0f) ? 0.0f : 1.0f / L;  // paged: perhaps no page is there
             float4v r;
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = srq(o[i] * inv, a.out_q);
-            *reinterpret_cast<float4v*>(outp + e) = r;
+            if (PAGED && out16) store4(reinterpret_cast<half_t*>(a.out) + outo + e, r);
+            else *reinterpret_cast<float4v*>(outp + e) = r;
         } else {
             *reinterpret_cast<float4v*>(a.part_o + slot * (G * HD) + e) = o;
             if (e % HD == 0) a.part_ml[slot * G + hh] = make_float2(M, L);
@@ -603,8 +683,18 @@ void decode_kernel(DecodeArgs a) {
 // (NB batches of 64; slots past max_splits read as zeros through the buffer range), thread
 // t reads (m, l) of split t. A slot of weight 0 is dropped by a select, never multiplied
 // in: a marker slot's o holds whatever an earlier call left there.
-template <int HD, int G, int NB>
-__global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
+template <typename A>
+__device__ __forceinline__ void store_merged(const A& a, size_t at, float v) {
+    if constexpr (std::is_same_v<A, PagedDecodeArgs>) {
+        if (a.out16) {
+            reinterpret_cast<half_t*>(a.out)[at] = (half_t)v;
+            return;
+        }
+    }
+    a.out[at] = v;
+}
+template <int HD, int G, int NB, typename A = DecodeArgs>
+__global__ __launch_bounds__(256) void decode_merge_kernel(A a) {
     constexpr int E = G * HD, NU = 16 * NB;
     __shared__ float wts[256];
     __shared__ float red[4][64];
@@ -641,7 +731,7 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
         const float L = (s_red2[0] + s_red2[1]) + (s_red2[2] + s_red2[3]);
         const float t = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
         // L = 0 only when the sequence attends no key: defined output of zeros
-        a.out[((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e] = L > 0.0f ? srq(t * (1.0f / L), a.out_q) : 0.0f;
+        store_merged(a, ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e, L > 0.0f ? srq(t * (1.0f / L), a.out_q) : 0.0f);
     }
 }
 
@@ -650,8 +740,8 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(DecodeArgs a) {
 // by this call. Thread (sg, dim e) folds splits sg, sg+4, .. into a running (m, l, o) eight
 // loads at a time; the four split groups are combined through LDS. (The partials were just
 // written from other XCDs: non-temporal loads of them measured slower.)
-template <int HD, int G>
-__global__ __launch_bounds__(256) void decode_merge_list_kernel(DecodeArgs a) {
+template <int HD, int G, typename A = DecodeArgs>
+__global__ __launch_bounds__(256) void decode_merge_list_kernel(A a) {
     constexpr int E = G * HD;
     __shared__ float sm[4][64], sl[4][64], so[4][64];
     const int tid = threadIdx.x, lane = tid & 63, sg = tid >> 6;
@@ -681,7 +771,8 @@ __global__ __launch_bounds__(256) void decode_merge_list_kernel(DecodeArgs a) {
         float bm = M;
 #pragma unroll
         for (int j = 0; j < 8; ++j) bm = fmaxf(bm, ml[j].x);
-        const float c = M == kNegInf ? 0.0f : fexp2(M - bm);  // bm is finite: split s0 is live
+        // bm is finite, as split s0 is live (but for paged splits without a page)
+        const float c = M == kNegInf ? 0.0f : fexp2(M - bm);
         Ls *= c;
         O *= c;
 #pragma unroll
@@ -706,7 +797,7 @@ __global__ __launch_bounds__(256) void decode_merge_list_kernel(DecodeArgs a) {
             t = w != 0.0f ? fmaf(w, so[k][lane], t) : t;
         }
         // L = 0 only when the sequence attends no key: defined output of zeros
-        a.out[((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e] = L > 0.0f ? srq(t * (1.0f / L), a.out_q) : 0.0f;
+        store_merged(a, ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e, L > 0.0f ? srq(t * (1.0f / L), a.out_q) : 0.0f);
     }
 }
 
@@ -726,10 +817,14 @@ constexpr long kDecodeCus = 256;        // compute units of the MI355X
 // would take a second workgroup each stream twice the keys of the rest (config 5's decode,
 // T 8448, kvH 2: 264 workgroups of 64 keys ran 12.3 us a call, 212 of 80 keys 10.8 us).
 // At most 256 splits per sequence, chunk a multiple of the 16-key block.
-static int decode_chunk(const g4a_cfg* cfg, int n_seq, int max_key_len) {
+// paged: splits start at a multiple of 16, up to 15 keys in front of the window.
+static long longest_active(const g4a_cfg* cfg, int max_key_len, bool paged) {
+    const long w = (long)cfg->window + (paged ? 15 : 0);
+    return cfg->window > 0 && w < max_key_len ? w : max_key_len;
+}
+static int decode_chunk(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
     const long pairs = (long)n_seq * cfg->n_kv_heads;
-    long max_active = max_key_len;
-    if (cfg->window > 0 && (long)cfg->window < max_active) max_active = cfg->window;
+    const long max_active = longest_active(cfg, max_key_len, paged);
     const long target = kDecodeTargetWgs;
     const long min_chunk = kDecodeMinChunk;
     const long kp = max_active * pairs;
@@ -746,10 +841,9 @@ static int decode_chunk(const g4a_cfg* cfg, int n_seq, int max_key_len) {
     return (int)((chunk + 15) & ~15L);
 }
 
-static int decode_splits(const g4a_cfg* cfg, int n_seq, int max_key_len) {
-    long max_active = max_key_len;
-    if (cfg->window > 0 && (long)cfg->window < max_active) max_active = cfg->window;
-    const int chunk = decode_chunk(cfg, n_seq, max_key_len);
+static int decode_splits(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
+    const long max_active = longest_active(cfg, max_key_len, paged);
+    const int chunk = decode_chunk(cfg, n_seq, max_key_len, paged);
     const long s = (max_active + chunk - 1) / chunk;
     return (int)(s < 1 ? 1 : s);
 }
@@ -761,9 +855,9 @@ static int decode_splits(const g4a_cfg* cfg, int n_seq, int max_key_len) {
 struct ListPlan {
     int target, grid;
 };
-static ListPlan list_plan(const g4a_cfg* cfg, int n_seq, int max_key_len) {
+static ListPlan list_plan(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
     ListPlan p{0, 0};
-    if (n_seq <= 1 || decode_splits(cfg, n_seq, max_key_len) <= 1) return p;
+    if (n_seq <= 1 || decode_splits(cfg, n_seq, max_key_len, paged) <= 1) return p;
     const bool f32 = (cfg->flags & G4A_KV_F32) != 0;
     const int resident = cfg->head_dim == 256 && !f32 ? 512 : 256;
     const long pairs = (long)n_seq * cfg->n_kv_heads;
@@ -777,10 +871,10 @@ struct WsLayout {
 };
 
 // partial slots: max_splits per pair, or one per work-list unit
-static WsLayout ws_layout(const g4a_cfg* cfg, int n_seq, int max_key_len) {
-    const ListPlan lp = list_plan(cfg, n_seq, max_key_len);
+static WsLayout ws_layout(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
+    const ListPlan lp = list_plan(cfg, n_seq, max_key_len, paged);
     const size_t slots = lp.grid > 0 ? (size_t)lp.grid
-                                     : (size_t)n_seq * cfg->n_kv_heads * decode_splits(cfg, n_seq, max_key_len);
+                                     : (size_t)n_seq * cfg->n_kv_heads * decode_splits(cfg, n_seq, max_key_len, paged);
     const size_t G = cfg->n_q_heads / cfg->n_kv_heads;
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     WsLayout L;
@@ -791,52 +885,120 @@ static WsLayout ws_layout(const g4a_cfg* cfg, int n_seq, int max_key_len) {
     return L;
 }
 
-typedef void (*decode_fn)(DecodeArgs);
+template <typename A>
+using decode_fn = void (*)(A);
 
-template <int HD, int G, typename KVT>
-static decode_fn pick_mode(bool list, bool kvw) {
-    if (list) return kvw ? decode_kernel<HD, G, KVT, true, true> : decode_kernel<HD, G, KVT, true, false>;
-    return kvw ? decode_kernel<HD, G, KVT, false, true> : decode_kernel<HD, G, KVT, false, false>;
+template <int HD, int G, typename KVT, typename A>
+static decode_fn<A> pick_mode(bool list, bool kvw) {
+    if (list) return kvw ? decode_kernel<HD, G, KVT, true, true, A> : decode_kernel<HD, G, KVT, true, false, A>;
+    return kvw ? decode_kernel<HD, G, KVT, false, true, A> : decode_kernel<HD, G, KVT, false, false, A>;
 }
-template <int HD, int G>
-static decode_fn pick_kv(bool f32, bool list, bool kvw) {
-    return f32 ? pick_mode<HD, G, float>(list, kvw) : pick_mode<HD, G, half_t>(list, kvw);
+template <int HD, int G, typename A>
+static decode_fn<A> pick_kv(bool f32, bool list, bool kvw) {
+    return f32 ? pick_mode<HD, G, float, A>(list, kvw) : pick_mode<HD, G, half_t, A>(list, kvw);
 }
-template <int HD>
-static decode_fn pick_g(int G, bool f32, bool list, bool kvw) {
+template <int HD, typename A>
+static decode_fn<A> pick_g(int G, bool f32, bool list, bool kvw) {
     switch (G) {
-        case 1: return pick_kv<HD, 1>(f32, list, kvw);
-        case 2: return pick_kv<HD, 2>(f32, list, kvw);
-        case 4: return pick_kv<HD, 4>(f32, list, kvw);
-        case 8: return pick_kv<HD, 8>(f32, list, kvw);
+        case 1: return pick_kv<HD, 1, A>(f32, list, kvw);
+        case 2: return pick_kv<HD, 2, A>(f32, list, kvw);
+        case 4: return pick_kv<HD, 4, A>(f32, list, kvw);
+        case 8: return pick_kv<HD, 8, A>(f32, list, kvw);
     }
     return nullptr;
 }
-template <int HD, int G>
-static decode_fn pick_merge_nb(int splits) {
-    if (splits <= 64) return decode_merge_kernel<HD, G, 1>;
-    if (splits <= 128) return decode_merge_kernel<HD, G, 2>;
-    return decode_merge_kernel<HD, G, 4>;
+template <int HD, int G, typename A>
+static decode_fn<A> pick_merge_nb(int splits) {
+    if (splits <= 64) return decode_merge_kernel<HD, G, 1, A>;
+    if (splits <= 128) return decode_merge_kernel<HD, G, 2, A>;
+    return decode_merge_kernel<HD, G, 4, A>;
 }
-template <int HD>
-static decode_fn pick_merge_list(int G) {
+template <int HD, typename A>
+static decode_fn<A> pick_merge_list(int G) {
     switch (G) {
-        case 1: return decode_merge_list_kernel<HD, 1>;
-        case 2: return decode_merge_list_kernel<HD, 2>;
-        case 4: return decode_merge_list_kernel<HD, 4>;
-        case 8: return decode_merge_list_kernel<HD, 8>;
+        case 1: return decode_merge_list_kernel<HD, 1, A>;
+        case 2: return decode_merge_list_kernel<HD, 2, A>;
+        case 4: return decode_merge_list_kernel<HD, 4, A>;
+        case 8: return decode_merge_list_kernel<HD, 8, A>;
     }
     return nullptr;
 }
-template <int HD>
-static decode_fn pick_merge(int G, int splits) {
+template <int HD, typename A>
+static decode_fn<A> pick_merge(int G, int splits) {
     switch (G) {
-        case 1: return pick_merge_nb<HD, 1>(splits);
-        case 2: return pick_merge_nb<HD, 2>(splits);
-        case 4: return pick_merge_nb<HD, 4>(splits);
-        case 8: return pick_merge_nb<HD, 8>(splits);
+        case 1: return pick_merge_nb<HD, 1, A>(splits);
+        case 2: return pick_merge_nb<HD, 2, A>(splits);
+        case 4: return pick_merge_nb<HD, 4, A>(splits);
+        case 8: return pick_merge_nb<HD, 8, A>(splits);
     }
     return nullptr;
+}
+
+// what decode_impl and g4a_paged_decode set alike: the plan, the workspace's parts and the config
+static int decode_setup(DecodeArgs& a, const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged, void* ws) {
+    const int HD = (int)cfg->head_dim;
+    const size_t esz = (cfg->flags & G4A_KV_F32) != 0 ? 4 : 2;
+    const ListPlan lp = list_plan(cfg, n_seq, max_key_len, paged);
+    const WsLayout L = ws_layout(cfg, n_seq, max_key_len, paged);
+    char* w = (char*)ws;
+    a.part_ml = (float2*)(w + L.ml);
+    a.part_o = (float*)(w + L.o);
+    a.list_tab = (int2*)(w + L.tab);
+    a.n_q_heads = (int)cfg->n_q_heads;
+    a.n_kv_heads = (int)cfg->n_kv_heads;
+    a.window = (int)cfg->window;
+    const int64_t row_bytes = (int64_t)cfg->n_kv_heads * HD * (int64_t)esz;
+    a.n_seq = n_seq;
+    a.list_target = lp.target;
+    a.list_units = lp.grid;
+    if (lp.grid > 0) {
+        // work list: units of at least 64 keys (every wave of a workgroup busy); a unit's
+        // byte offsets stay within 32 bits
+        a.max_splits = 0;
+        a.chunk = 64;
+        a.chunk_cap = (int)(((0x7fffffff / row_bytes) - 64) & ~15LL);
+        if (a.chunk_cap < a.chunk) {
+            set_error("cache rows too large for 32-bit buffer offsets");
+            return G4A_EINVAL;
+        }
+    } else {
+        a.max_splits = decode_splits(cfg, n_seq, max_key_len, paged);
+        a.chunk = decode_chunk(cfg, n_seq, max_key_len, paged);
+        a.chunk_cap = 0;
+        if ((int64_t)(a.chunk + 64) * row_bytes > 0x7fffffff) {
+            set_error("keys per split too large for 32-bit buffer offsets");
+            return G4A_EINVAL;
+        }
+    }
+    a.scale_log2 = cfg->scale * kLog2e;
+    a.eps = cfg->eps;
+    a.out_q = cfg->out_q;
+    a.v_norm = (cfg->flags & G4A_NO_V_NORM) ? 0 : 1;
+    return G4A_OK;
+}
+
+// the decode kernel of `a` and, unless one split holds every key, the merge
+template <typename A>
+static int decode_launch(const A& a, const g4a_cfg* cfg, hipStream_t stream) {
+    const int HD = (int)cfg->head_dim, G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
+    const bool f32 = (cfg->flags & G4A_KV_F32) != 0, list = a.list_units > 0, kvw = a.k_new != nullptr;
+    const decode_fn<A> fn = HD == 256 ? pick_g<256, A>(G, f32, list, kvw) : pick_g<512, A>(G, f32, list, kvw);
+    if (!fn) {
+        set_error("no decode kernel for group size %d", G);
+        return G4A_EUNSUPPORTED;
+    }
+    const dim3 grid = list ? dim3(a.list_units) : dim3(a.max_splits, cfg->n_kv_heads, a.n_seq);
+    hipLaunchKernelGGL(fn, grid, dim3(256), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return hip_error(e, "decode launch");
+    if (list || a.max_splits > 1) {
+        const decode_fn<A> mf = list ? (HD == 256 ? pick_merge_list<256, A>(G) : pick_merge_list<512, A>(G))
+                                     : (HD == 256 ? pick_merge<256, A>(G, a.max_splits) : pick_merge<512, A>(G, a.max_splits));
+        hipLaunchKernelGGL(mf, dim3(G * HD / 64, cfg->n_kv_heads, a.n_seq), dim3(256), 0, stream, a);
+        e = hipGetLastError();
+        if (e != hipSuccess) return hip_error(e, "decode merge launch");
+    }
+    return G4A_OK;
 }
 
 }  // namespace g4a
@@ -872,13 +1034,12 @@ static int decode_impl(const g4a_cfg* cfg, int n_seq, int max_key_len, const int
         set_error("rope_cos and rope_sin must both be given or both be NULL");
         return G4A_EINVAL;
     }
-    const int HD = (int)cfg->head_dim, G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
+    const int HD = (int)cfg->head_dim;
     if (HD != 256 && HD != 512) {
         set_error("head_dim %d not supported (256 or 512)", HD);
         return G4A_EUNSUPPORTED;
     }
-    const bool f32 = (cfg->flags & G4A_KV_F32) != 0;
-    const size_t esz = f32 ? 4 : 2;
+    const size_t esz = (cfg->flags & G4A_KV_F32) != 0 ? 4 : 2;
     if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q | (uintptr_t)out) % 16 ||
         (q_gain && (uintptr_t)q_gain % 16) || (rope_cos && ((uintptr_t)rope_cos | (uintptr_t)rope_sin) % 16) ||
         (seq_stride * esz) % 16) {
@@ -889,8 +1050,6 @@ static int decode_impl(const g4a_cfg* cfg, int n_seq, int max_key_len, const int
         set_error("seq_stride %lld smaller than one cache row", (long long)seq_stride);
         return G4A_EINVAL;
     }
-    const int splits = decode_splits(cfg, n_seq, max_key_len);
-    const ListPlan lp = list_plan(cfg, n_seq, max_key_len);
     const WsLayout L = ws_layout(cfg, n_seq, max_key_len);
     if (!ws || ws_bytes < L.total || ((uintptr_t)ws % 256)) {
         set_error("decode workspace needs %zu bytes (256-byte aligned), got %zu", L.total, ws_bytes);
@@ -911,39 +1070,7 @@ static int decode_impl(const g4a_cfg* cfg, int n_seq, int max_key_len, const int
     a.vc = v_cache;
     a.seq_stride = seq_stride;
     a.out = out;
-    char* w = (char*)ws;
-    a.part_ml = (float2*)(w + L.ml);
-    a.part_o = (float*)(w + L.o);
-    a.list_tab = (int2*)(w + L.tab);
-    a.n_q_heads = (int)cfg->n_q_heads;
-    a.n_kv_heads = (int)cfg->n_kv_heads;
-    a.window = (int)cfg->window;
-    const int64_t row_bytes = (int64_t)cfg->n_kv_heads * HD * (int64_t)esz;
-    a.n_seq = n_seq;
-    a.list_target = lp.target;
-    a.list_units = lp.grid;
-    if (lp.grid > 0) {
-        // work list: units of at least 64 keys (every wave of a workgroup busy); a unit's
-        // byte offsets stay within 32 bits
-        a.max_splits = 0;
-        a.chunk = 64;
-        a.chunk_cap = (int)(((0x7fffffff / row_bytes) - 64) & ~15LL);
-        if (a.chunk_cap < a.chunk) {
-            set_error("cache rows too large for 32-bit buffer offsets");
-            return G4A_EINVAL;
-        }
-    } else {
-        a.max_splits = splits;
-        a.chunk = decode_chunk(cfg, n_seq, max_key_len);
-        a.chunk_cap = 0;
-        if ((int64_t)(a.chunk + 64) * row_bytes > 0x7fffffff) {
-            set_error("keys per split too large for 32-bit buffer offsets");
-            return G4A_EINVAL;
-        }
-    }
-    a.scale_log2 = cfg->scale * kLog2e;
-    a.eps = cfg->eps;
-    a.out_q = cfg->out_q;
+    if (const int rc = decode_setup(a, cfg, n_seq, max_key_len, false, ws)) return rc;
     a.k_new = kvn ? kvn->k : nullptr;
     a.v_new = kvn ? kvn->v : nullptr;
     a.k_gain = kvn ? kvn->k_gain : nullptr;
@@ -951,25 +1078,7 @@ static int decode_impl(const g4a_cfg* cfg, int n_seq, int max_key_len, const int
     a.vc_out = const_cast<void*>(v_cache);
     a.k_in_q = kvn ? kvn->k_in_q : 0.0f;
     a.v_in_q = kvn ? kvn->v_in_q : 0.0f;
-    a.v_norm = (cfg->flags & G4A_NO_V_NORM) ? 0 : 1;
-    const bool list = lp.grid > 0, kvw = kvn != nullptr;
-    decode_fn fn = HD == 256 ? pick_g<256>(G, f32, list, kvw) : pick_g<512>(G, f32, list, kvw);
-    if (!fn) {
-        set_error("no decode kernel for group size %d", G);
-        return G4A_EUNSUPPORTED;
-    }
-    const dim3 grid = lp.grid > 0 ? dim3(lp.grid) : dim3(splits, cfg->n_kv_heads, n_seq);
-    hipLaunchKernelGGL(fn, grid, dim3(256), 0, (hipStream_t)stream, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return hip_error(e, "decode launch");
-    if (lp.grid > 0 || splits > 1) {
-        decode_fn mf = lp.grid > 0 ? (HD == 256 ? pick_merge_list<256>(G) : pick_merge_list<512>(G))
-                                   : (HD == 256 ? pick_merge<256>(G, splits) : pick_merge<512>(G, splits));
-        hipLaunchKernelGGL(mf, dim3(G * HD / 64, cfg->n_kv_heads, n_seq), dim3(256), 0, (hipStream_t)stream, a);
-        e = hipGetLastError();
-        if (e != hipSuccess) return hip_error(e, "decode merge launch");
-    }
-    return G4A_OK;
+    return decode_launch(a, cfg, (hipStream_t)stream);
 }
 
 extern "C" int g4a_decode(const g4a_cfg* cfg, int n_seq, int max_key_len, const int32_t* key_len,
@@ -1068,4 +1177,53 @@ extern "C" int g4a_decode_noalloc(const g4a_cfg* cfg, int n_seq, int max_key_len
     if (rc != G4A_OK) return rc;
     return decode_impl(cfg, n_seq, max_key_len, key_len, q, q_gain, rope_cos, rope_sin, k_cache, v_cache,
                        seq_stride, out, ws, kDecodeScratchBytes, stream, nullptr);
+}
+
+// ---------------------------------------------------------------- a paged cache
+extern "C" size_t g4a_paged_decode_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg) {
+    if (check_paged(cfg, pg, true)) return 0;
+    return ws_layout(cfg, pg->n_seq, pg->max_key_len, true).total;
+}
+
+extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, const float* q_gain,
+                                const float* rope_cos, const float* rope_sin, const float* k_new, const float* v_new,
+                                float k_in_q, float v_in_q, const float* k_gain, void* out, void* ws, size_t ws_bytes,
+                                void* stream) {
+    if (const int rc = check_paged(cfg, pg, true)) return rc;
+    if (const int rc = check_paged_call(cfg, pg->n_seq, q, q_gain, rope_cos, rope_sin, out)) return rc;
+    if (const int rc = check_steps(k_in_q, v_in_q)) return rc;
+    if ((k_new == nullptr) != (v_new == nullptr)) {
+        set_error("k_new and v_new must both be given or both be NULL");
+        return G4A_EINVAL;
+    }
+    if (cfg->flags & G4A_IN_F16) {
+        set_error("g4a_paged_decode takes f32 k/v rows (G4A_IN_F16 not supported)");
+        return G4A_EUNSUPPORTED;
+    }
+    if (((uintptr_t)k_new | (uintptr_t)v_new | (uintptr_t)k_gain) % 16) {
+        set_error("k_new, v_new and k_gain must be 16-byte aligned");
+        return G4A_EINVAL;
+    }
+    const size_t need = ws_layout(cfg, pg->n_seq, pg->max_key_len, true).total;
+    if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
+        set_error("paged decode workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
+        return G4A_EWORKSPACE;
+    }
+    PagedDecodeArgs a{};
+    a.t = page_tab(pg);
+    a.q = q;
+    a.q_gain = q_gain;
+    a.rcos = rope_cos;
+    a.rsin = rope_sin;
+    a.kc = a.kc_out = pg->k_pages;
+    a.vc = a.vc_out = pg->v_pages;
+    a.out = (float*)out;
+    a.out16 = (cfg->flags & G4A_OUT_F32) == 0;
+    if (const int rc = decode_setup(a, cfg, pg->n_seq, pg->max_key_len, true, ws)) return rc;
+    a.k_new = k_new;
+    a.v_new = v_new;
+    a.k_gain = k_gain;
+    a.k_in_q = k_in_q;
+    a.v_in_q = v_in_q;
+    return decode_launch(a, cfg, (hipStream_t)stream);
 }

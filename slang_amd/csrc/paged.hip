@@ -5,17 +5,6 @@
 namespace g4a {
 
 static bool aligned16(const void* p) { return (uintptr_t)p % 16 == 0; }
-// the outputs of n_tokens rows must not lie over the rows of q
-static bool out_over_q(const g4a_cfg* cfg, int n_tokens, const float* q, const void* out) {
-    const size_t n = (size_t)n_tokens * cfg->n_q_heads * cfg->head_dim, osz = (cfg->flags & G4A_OUT_F32) ? 4 : 2;
-    const uintptr_t a = (uintptr_t)q, b = (uintptr_t)out;
-    if (a < b + n * osz && b < a + n * 4) {
-        set_error("out must not overlap q");
-        return true;
-    }
-    return false;
-}
-
 int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8) {
     if (!check_cfg(cfg, need_group_le8)) return G4A_EINVAL;
     if (!pg) {
@@ -297,16 +286,35 @@ static int launch_attn(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, co
     return e == hipSuccess ? G4A_OK : hip_error(e, "paged attention launch");
 }
 
-static int check_rope(const float* rcos, const float* rsin) {
+int check_rope(const float* rcos, const float* rsin) {
     if ((rcos == nullptr) != (rsin == nullptr)) {
         set_error("rope_cos and rope_sin must both be given or both be NULL");
         return G4A_EINVAL;
     }
     return G4A_OK;
 }
-static int check_steps(float k_in_q, float v_in_q) {
+int check_steps(float k_in_q, float v_in_q) {
     if (!(k_in_q >= 0.0f) || !(v_in_q >= 0.0f)) {
         set_error("k_in_q/v_in_q must be >= 0");
+        return G4A_EINVAL;
+    }
+    return G4A_OK;
+}
+int check_paged_call(const g4a_cfg* cfg, int n_tokens, const float* q, const float* q_gain, const float* rcos,
+                     const float* rsin, const void* out) {
+    if (const int rc = check_rope(rcos, rsin)) return rc;
+    if (!q || !out) {
+        set_error("q and out must be non-NULL");
+        return G4A_EINVAL;
+    }
+    if (!aligned16(q) || !aligned16(out) || !aligned16(q_gain) || !aligned16(rcos) || !aligned16(rsin)) {
+        set_error("q, out, q_gain and the rope tables must be 16-byte aligned");
+        return G4A_EINVAL;
+    }
+    const size_t n = (size_t)n_tokens * cfg->n_q_heads * cfg->head_dim, osz = (cfg->flags & G4A_OUT_F32) ? 4 : 2;
+    const uintptr_t x = (uintptr_t)q, y = (uintptr_t)out;
+    if (x < y + n * osz && y < x + n * 4) {
+        set_error("out must not overlap q");
         return G4A_EINVAL;
     }
     return G4A_OK;
@@ -346,48 +354,6 @@ extern "C" int g4a_paged_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_to
                         rope_sin, (hipStream_t)stream);
 }
 
-extern "C" size_t g4a_paged_decode_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg) {
-    return check_paged(cfg, pg, true) ? 0 : 512;
-}
-
-extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, const float* q_gain,
-                                const float* rope_cos, const float* rope_sin, const float* k_new, const float* v_new,
-                                float k_in_q, float v_in_q, const float* k_gain, void* out, void* ws,
-                                size_t ws_bytes, void* stream) {
-    if (const int rc = check_paged(cfg, pg, true)) return rc;
-    if (const int rc = check_rope(rope_cos, rope_sin)) return rc;
-    if (const int rc = check_steps(k_in_q, v_in_q)) return rc;
-    if (!q || !out) {
-        set_error("q and out must be non-NULL");
-        return G4A_EINVAL;
-    }
-    if ((k_new == nullptr) != (v_new == nullptr)) {
-        set_error("k_new and v_new must both be given or both be NULL");
-        return G4A_EINVAL;
-    }
-    if (cfg->flags & G4A_IN_F16) {
-        set_error("g4a_paged_decode takes f32 k/v rows (G4A_IN_F16 not supported)");
-        return G4A_EUNSUPPORTED;
-    }
-    if (!aligned16(q) || !aligned16(out) || !aligned16(q_gain) || !aligned16(rope_cos) || !aligned16(rope_sin) ||
-        !aligned16(k_new) || !aligned16(v_new) || !aligned16(k_gain)) {
-        set_error("q, out, the gains, the rope tables, k_new and v_new must be 16-byte aligned");
-        return G4A_EINVAL;
-    }
-    if (out_over_q(cfg, pg->n_seq, q, out)) return G4A_EINVAL;
-    const size_t need = g4a_paged_decode_ws_bytes(cfg, pg);
-    if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
-        set_error("paged decode workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
-        return G4A_EWORKSPACE;
-    }
-    if (k_new) {
-        if (const int rc = launch_write(cfg, pg, pg->n_seq, nullptr, false, k_new, v_new, k_in_q, v_in_q, k_gain, rope_cos,
-                                        rope_sin, (hipStream_t)stream))
-            return rc;
-    }
-    return launch_attn(cfg, pg, pg->n_seq, nullptr, q, q_gain, rope_cos, rope_sin, out, (hipStream_t)stream);
-}
-
 extern "C" size_t g4a_paged_prefill_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens) {
     if (check_paged(cfg, pg, true)) return 0;
     if (n_tokens <= 0) {
@@ -402,20 +368,11 @@ extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_
                                  void* out, void* ws, size_t ws_bytes, void* stream) {
     if (const int rc = check_paged(cfg, pg, true)) return rc;
     if (const int rc = check_tokens(cfg, n_tokens, cu_q)) return rc;
-    if (const int rc = check_rope(rope_cos, rope_sin)) return rc;
-    if (!q || !out) {
-        set_error("q and out must be non-NULL");
-        return G4A_EINVAL;
-    }
+    if (const int rc = check_paged_call(cfg, n_tokens, q, q_gain, rope_cos, rope_sin, out)) return rc;
     if (cfg->flags & G4A_Q_HILO) {
         set_error("g4a_paged_prefill rounds q to f16 (G4A_Q_HILO not supported)");
         return G4A_EUNSUPPORTED;
     }
-    if (!aligned16(q) || !aligned16(out) || !aligned16(q_gain) || !aligned16(rope_cos) || !aligned16(rope_sin)) {
-        set_error("q, out, q_gain and the rope tables must be 16-byte aligned");
-        return G4A_EINVAL;
-    }
-    if (out_over_q(cfg, n_tokens, q, out)) return G4A_EINVAL;
     const size_t need = g4a_paged_prefill_ws_bytes(cfg, pg, n_tokens);
     if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
         set_error("paged prefill workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
