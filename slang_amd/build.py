@@ -38,7 +38,7 @@ def hipcc() -> str:
 # per-file additions: the prefill kernels keep their MFMA accumulators in VGPRs, so the
 # online-softmax rescale of the 128 accumulator registers does not make the compiler copy
 # them between register files on every tile
-FILE_FLAGS = {"prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("prefill.hip", "paged_prefill.hip")}
 
 
 def _compile(src: str, verbose: bool) -> str:

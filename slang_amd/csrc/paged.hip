@@ -1,5 +1,4 @@
-// The paged K/V cache: appending rows, and the attention over it in its plainest form -- one
-// workgroup per (token, kv head), each wave every fourth key, an online softmax per wave.
+// The paged K/V cache: the checks that its entry points share, and appending rows.
 #include "paged.hpp"
 
 namespace g4a {
@@ -138,154 +137,6 @@ static int launch_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, c
     return e == hipSuccess ? G4A_OK : hip_error(e, "paged write launch");
 }
 
-struct PagedAttnArgs {
-    PageTab t;
-    const int32_t* cu;  // NULL: decode, token b of sequence b at position key_len - 1
-    const float* q;
-    const float* q_gain;
-    const float* rcos;
-    const float* rsin;
-    const void* kc;
-    const void* vc;
-    void* out;
-    int n_tokens, n_q_heads, n_kv_heads, window, out32;
-    float scale_log2, eps, out_q;
-};
-
-template <int HD, int G, typename KVT>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedAttnArgs a) {
-    constexpr int E = HD / 64;  // dims of a lane: d0 .. d0 + E/2 - 1 and the same + HD/2
-    __shared__ float sm[4][G], sl[4][G];
-    __shared__ float so[4][G][HD];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int tok = blockIdx.x, kh = blockIdx.y;
-    int b, p;
-    if (a.cu) {
-        b = seq_of_row(a.cu, a.t.n_seq, tok);
-        if (b >= a.t.n_seq) return;
-        const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
-        if (tok < r.lo || tok >= r.hi) return;
-        p = r.keys - r.hi + tok;
-    } else {
-        b = tok;
-        p = paged_len(a.t, b) - 1;
-    }
-    float x[G][E], o[G][E], m[G], l[G];
-    const int d0 = E / 2 * lane;
-    for (int h = 0; h < G; ++h) {
-        const float* qr = a.q + ((size_t)tok * a.n_q_heads + kh * G + h) * HD;
-        float ss = 0.0f;
-        for (int e = 0; e < E / 2; ++e) {
-            x[h][e] = qr[d0 + e];
-            x[h][e + E / 2] = qr[d0 + e + HD / 2];
-            ss += x[h][e] * x[h][e] + x[h][e + E / 2] * x[h][e + E / 2];
-        }
-        const float rs = a.q_gain ? 1.0f / sqrtf(wave_sum(ss) / (float)HD + a.eps) : 1.0f;
-        for (int e = 0; e < E / 2; ++e) {
-            const float x0 = a.q_gain ? x[h][e] * rs * a.q_gain[d0 + e] : x[h][e];
-            const float x1 = a.q_gain ? x[h][e + E / 2] * rs * a.q_gain[d0 + e + HD / 2] : x[h][e + E / 2];
-            const float c = a.rcos && p >= 0 ? a.rcos[(size_t)p * (HD / 2) + d0 + e] : 1.0f;
-            const float s = a.rcos && p >= 0 ? a.rsin[(size_t)p * (HD / 2) + d0 + e] : 0.0f;
-            x[h][e] = (x0 * c - x1 * s) * a.scale_log2;
-            x[h][e + E / 2] = (x1 * c + x0 * s) * a.scale_log2;
-        }
-        for (int e = 0; e < E; ++e) o[h][e] = 0.0f;
-        m[h] = kNegInf;
-        l[h] = 0.0f;
-    }
-    const int lo = a.window > 0 ? max(0, p + 1 - a.window) : 0;
-    for (int t = lo + wave; t <= p; t += 4) {
-        const int page = page_at(a.t, b, t);
-        if (!page_ok(a.t, page)) continue;
-        const size_t row = paged_row(a.t, page, t, a.n_kv_heads * HD) + (size_t)kh * HD;
-        const KVT* kr = reinterpret_cast<const KVT*>(a.kc) + row;
-        const KVT* vr = reinterpret_cast<const KVT*>(a.vc) + row;
-        float kx[E], vx[E];
-        for (int e = 0; e < E / 2; ++e) {
-            kx[e] = (float)kr[d0 + e];
-            kx[e + E / 2] = (float)kr[d0 + e + HD / 2];
-            vx[e] = (float)vr[d0 + e];
-            vx[e + E / 2] = (float)vr[d0 + e + HD / 2];
-        }
-        for (int h = 0; h < G; ++h) {
-            float s = 0.0f;
-            for (int e = 0; e < E; ++e) s += x[h][e] * kx[e];
-            s = wave_sum(s);
-            const float mn = fmaxf(m[h], s), mu = mn == kNegInf ? 0.0f : mn;
-            const float c = fexp2(m[h] - mu), w = fexp2(s - mu);
-            for (int e = 0; e < E; ++e) o[h][e] = o[h][e] * c + w * vx[e];
-            l[h] = l[h] * c + w;
-            m[h] = mn;
-        }
-    }
-    for (int h = 0; h < G; ++h) {
-        for (int e = 0; e < E / 2; ++e) {
-            so[wave][h][d0 + e] = o[h][e];
-            so[wave][h][d0 + e + HD / 2] = o[h][e + E / 2];
-        }
-        if (lane == 0) {
-            sm[wave][h] = m[h];
-            sl[wave][h] = l[h];
-        }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < G * HD; i += 256) {
-        const int h = i / HD, d = i % HD;
-        float M = kNegInf, L = 0.0f, O = 0.0f;
-        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w][h]);
-        for (int w = 0; w < 4; ++w) {
-            const float wt = sm[w][h] == kNegInf ? 0.0f : fexp2(sm[w][h] - M);
-            L += wt * sl[w][h];
-            O += wt * so[w][h][d];
-        }
-        const float y = L > 0.0f ? srq(O / L, a.out_q) : 0.0f;
-        const size_t at = ((size_t)tok * a.n_q_heads + kh * G + h) * HD + d;
-        if (a.out32) reinterpret_cast<float*>(a.out)[at] = y;
-        else reinterpret_cast<half_t*>(a.out)[at] = (half_t)y;
-    }
-}
-
-typedef void (*paged_attn_fn)(PagedAttnArgs);
-template <int HD, typename KVT>
-static paged_attn_fn pick_attn(int G) {
-    switch (G) {
-        case 1: return paged_attn_kernel<HD, 1, KVT>;
-        case 2: return paged_attn_kernel<HD, 2, KVT>;
-        case 4: return paged_attn_kernel<HD, 4, KVT>;
-        case 8: return paged_attn_kernel<HD, 8, KVT>;
-    }
-    return nullptr;
-}
-
-static int launch_attn(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu, const float* q,
-                       const float* q_gain, const float* rcos, const float* rsin, void* out, hipStream_t stream) {
-    PagedAttnArgs a;
-    a.t = page_tab(pg);
-    a.cu = cu;
-    a.q = q;
-    a.q_gain = q_gain;
-    a.rcos = rcos;
-    a.rsin = rsin;
-    a.kc = pg->k_pages;
-    a.vc = pg->v_pages;
-    a.out = out;
-    a.n_tokens = n_tokens;
-    a.n_q_heads = (int)cfg->n_q_heads;
-    a.n_kv_heads = (int)cfg->n_kv_heads;
-    a.window = (int)cfg->window;
-    a.out32 = (cfg->flags & G4A_OUT_F32) != 0;
-    a.scale_log2 = cfg->scale * kLog2e;
-    a.eps = cfg->eps;
-    a.out_q = cfg->out_q;
-    const int G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
-    const bool c32 = (cfg->flags & G4A_KV_F32) != 0;
-    const paged_attn_fn fn = cfg->head_dim == 256 ? (c32 ? pick_attn<256, float>(G) : pick_attn<256, half_t>(G))
-                                                  : (c32 ? pick_attn<512, float>(G) : pick_attn<512, half_t>(G));
-    hipLaunchKernelGGL(fn, dim3((unsigned)n_tokens, cfg->n_kv_heads), dim3(256), 0, stream, a);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? G4A_OK : hip_error(e, "paged attention launch");
-}
-
 int check_rope(const float* rcos, const float* rsin) {
     if ((rcos == nullptr) != (rsin == nullptr)) {
         set_error("rope_cos and rope_sin must both be given or both be NULL");
@@ -319,7 +170,7 @@ int check_paged_call(const g4a_cfg* cfg, int n_tokens, const float* q, const flo
     }
     return G4A_OK;
 }
-static int check_tokens(const g4a_cfg* cfg, int n_tokens, const int32_t* cu) {
+int check_tokens(const g4a_cfg* cfg, int n_tokens, const int32_t* cu) {
     if (n_tokens <= 0 || !cu || (uintptr_t)cu % 4) {
         set_error("n_tokens (%d) must be positive and cu_q non-NULL and 4-byte aligned", n_tokens);
         return G4A_EINVAL;
@@ -352,31 +203,4 @@ extern "C" int g4a_paged_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_to
     }
     return launch_write(cfg, pg, n_tokens, cu_q, (cfg->flags & G4A_IN_F16) != 0, k, v, k_in_q, v_in_q, k_gain, rope_cos,
                         rope_sin, (hipStream_t)stream);
-}
-
-extern "C" size_t g4a_paged_prefill_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens) {
-    if (check_paged(cfg, pg, true)) return 0;
-    if (n_tokens <= 0) {
-        set_error("n_tokens (%d) must be positive", n_tokens);
-        return 0;
-    }
-    return 512;
-}
-
-extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q,
-                                 const float* q, const float* q_gain, const float* rope_cos, const float* rope_sin,
-                                 void* out, void* ws, size_t ws_bytes, void* stream) {
-    if (const int rc = check_paged(cfg, pg, true)) return rc;
-    if (const int rc = check_tokens(cfg, n_tokens, cu_q)) return rc;
-    if (const int rc = check_paged_call(cfg, n_tokens, q, q_gain, rope_cos, rope_sin, out)) return rc;
-    if (cfg->flags & G4A_Q_HILO) {
-        set_error("g4a_paged_prefill rounds q to f16 (G4A_Q_HILO not supported)");
-        return G4A_EUNSUPPORTED;
-    }
-    const size_t need = g4a_paged_prefill_ws_bytes(cfg, pg, n_tokens);
-    if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
-        set_error("paged prefill workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
-        return G4A_EWORKSPACE;
-    }
-    return launch_attn(cfg, pg, n_tokens, cu_q, q, q_gain, rope_cos, rope_sin, out, (hipStream_t)stream);
 }

@@ -62,6 +62,7 @@ int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8);
 // ... of the operands that paged decode and prefill share, n_tokens rows of q and out
 int check_paged_call(const g4a_cfg* cfg, int n_tokens, const float* q, const float* q_gain, const float* rcos,
                      const float* rsin, const void* out);
+int check_tokens(const g4a_cfg* cfg, int n_tokens, const int32_t* cu);
 int check_rope(const float* rcos, const float* rsin);
 int check_steps(float k_in_q, float v_in_q);
 PageTab page_tab(const g4a_paged* pg);
