@@ -427,7 +427,7 @@ void decode_kernel(A a) {
             if (j != 0 && (j & 63) == 0) load_entries(blk);
             blk_page = __builtin_amdgcn_readlane(entries, j & 63);
             const bool ok = page_ok(a.t, blk_page);
-            const uint32_t bytes = ok ? (uint32_t)(min(max(k1 - blk, 0), 16) * rsb) : 0u;
+            const uint32_t bytes = ok ? (uint32_t)(clamp16(k1 - blk) * rsb) : 0u;
             const size_t at = paged_row(a.t, ok ? blk_page : 0, blk, (int)rstride) + (size_t)kh * HD;
             const rsrc_t pk = make_rsrc(reinterpret_cast<const KVT*>(a.kc) + at, bytes);
             const rsrc_t pv = make_rsrc(reinterpret_cast<const KVT*>(a.vc) + at, bytes);

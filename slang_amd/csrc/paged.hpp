@@ -25,6 +25,11 @@ __device__ __forceinline__ int page_at(const PageTab& t, int b, int p) {
     return t.table[(size_t)b * t.stride + (p >> t.shift)];
 }
 
+// rows of a 16-key block that lie in front of its end, n = end - block start, wave-uniform. (The clamp
+// is a vector instruction; left in a vector register it would make the buffer resource it enters look
+// divergent, and every load through it a loop over lanes.)
+__device__ __forceinline__ int clamp16(int n) { return __builtin_amdgcn_readfirstlane(min(max(n, 0), 16)); }
+
 // element offset of a position's row in the pools, `row` = kvH * hd elements
 __device__ __forceinline__ size_t paged_row(const PageTab& t, int page, int p, int row) {
     return (((size_t)page << t.shift) + (size_t)(p & ((1 << t.shift) - 1))) * (size_t)row;

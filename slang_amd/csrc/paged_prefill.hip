@@ -53,14 +53,14 @@ struct PagedPrefillArgs {
 };
 
 // ---------------------------------------------------------------- the work list
-__device__ __forceinline__ int wave_sum_i(int x) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) x += __shfl_xor(x, d);
-    return x;
-}
-__device__ __forceinline__ int wave_max_i(int x) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) x = max(x, __shfl_xor(x, d));
+// Inclusive prefix sum over the 64 lanes on DPP row shifts and broadcasts.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
     return x;
 }
 
@@ -71,30 +71,57 @@ __device__ __forceinline__ int block_tiles(const PagedPrefillArgs& a, int start,
     return max(0, (hi - (first & ~15) + a.kt - 1) / a.kt);
 }
 
-constexpr int kPlanThreads = 256, kBins = 256;
 // Cost of the units, in key tiles: a unit's own beside its tiles (q, epilogue), a partial's store and
-// merge, and the merge launch.
+// merge (its 3 bytes a value go to memory and back at a CU's share of the bandwidth, 20 GB/s), and
+// the merge launch. A tile takes about 2.1 us at hd 256 and 2.6 us at hd 512.
 struct PlanCost {
     float unit, part, merge;
 };
-__host__ __device__ inline PlanCost plan_cost(int kt) { return kt == 64 ? PlanCost{2.4f, 1.3f, 2.0f} : PlanCost{4.0f, 1.3f, 2.0f}; }
+__host__ __device__ inline PlanCost plan_cost(int kt) { return kt == 64 ? PlanCost{2.4f, 4.6f, 2.0f} : PlanCost{4.0f, 7.5f, 2.0f}; }
 
-// Written by one workgroup of kPlanThreads threads. The pieces a block is cut into follow from the most
-// tiles a piece may have, st: of st = longest / 1 .. longest / kMaxPieces the one whose units, dealt
-// longest first to kCus workgroups, end first (the mean load and a share of the longest unit).
+constexpr int kPlanThreads = 256;
+constexpr int kBins = 64;  // size classes of the sorted list
+
+// How the units of one candidate split would end: sums over a lane's sequences, whose blocks' tiles run
+// linearly from u to v over m blocks.
+struct SplitSums {
+    float units = 0.0f, slots = 0.0f, over[4] = {};  // over: pieces of at least (4 - i)/4 of the longest
+};
+__device__ __forceinline__ float ramp_over(float v, float m, float slope, float x) {  // blocks of more than x tiles
+    return v <= x ? 0.0f : m * fminf((v - x) * slope, 1.0f);
+}
+__device__ __forceinline__ void ramp_sums(SplitSums& t, float u, float v, float m, float st) {
+    const float slope = __builtin_amdgcn_rcpf(fmaxf(v - u, 1.0f));
+    float units = m, c1 = 0.0f;
+#pragma unroll
+    for (int j = 1; j < kMaxPieces; ++j) {
+        const float c = ramp_over(v, m, slope, st * (float)j);
+        if (j == 1) c1 = c;
+        units += c;
+    }
+    const float slots = units - m + c1;
+    t.units += units;
+    t.slots += slots;
+    // pieces of cut blocks count as longest (they hold half of st at least)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.over[i] += slots + fmaxf(ramp_over(v, m, slope, st * (float)(4 - i) * 0.25f - 0.5f) - c1, 0.0f);
+}
+
+// Written by one workgroup of kPlanThreads threads.
+// How many pieces: st, the most tiles a piece may have, is longest / 1 .. longest / kMaxPieces. Units
+// dealt longest first to kCus CUs end, to a good approximation, at the larger of the mean load and, for
+// any c, ceil(c / kCus) units of the size of the c-th longest; the st with the lowest such cost is
+// taken, from each sequence's block sizes as two linear ramps (first block to middle to last).
+// The list: size classes from the longest. (Dealing the blocks that read the same K/V to one XCD was
+// tried: L2 hits stayed at 80-85 %, the kernels' times within 3 %.)
 __device__ void plan_units(const PagedPrefillArgs& a) {
     __shared__ int s_lo[kPlanThreads], s_S[kPlanThreads], s_start[kPlanThreads], s_blk[kPlanThreads + 1];
-    __shared__ int s_wave[kPlanThreads / 64];
-    __shared__ int s_max, s_n[kMaxPieces + 1], s_slots[kMaxPieces + 1], s_bin[kBins], s_units, s_merges, s_slot;
-    __shared__ unsigned long long s_tiles;
+    __shared__ int s_wave[kPlanThreads / 64], s_max, s_cut, s_bin[kBins], s_slot, s_merge;
+    __shared__ float s_sum[kMaxPieces + 1][7];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int chunks = (a.t.n_seq + kPlanThreads - 1) / kPlanThreads;
-    if (tid <= kMaxPieces) s_n[tid] = s_slots[tid] = 0;
-    if (tid == 0) {
-        s_max = s_units = s_merges = s_slot = 0;
-        s_tiles = 0;
-    }
-    for (int i = tid; i < kBins; i += kPlanThreads) s_bin[i] = 0;
+    if (tid < kBins) s_bin[tid] = 0;
+    if (tid == 0) s_max = s_cut = s_slot = s_merge = 0;
 
     // the sequences c * kPlanThreads .. into LDS, with the prefix sum of their query blocks
     auto load_chunk = [&](int c) {
@@ -106,7 +133,7 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
         s_lo[tid] = r.lo;
         s_S[tid] = S;
         s_start[tid] = r.keys - S;
-        const int incl = wave_prefix_sum(nb);
+        const int incl = wave_scan(nb);
         if (lane == 63) s_wave[wave] = incl;
         __syncthreads();
         int base = 0;
@@ -115,134 +142,136 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
         if (tid == 0) s_blk[0] = 0;
         __syncthreads();
     };
-    // f(sequence in the chunk, its query block) for every block
-    auto for_blocks = [&](int c, auto f) {
-        if (chunks > 1) load_chunk(c);
-        const int n = s_blk[kPlanThreads];
-        for (int j = tid; j < n; j += kPlanThreads) {
-            int lo = 0, hi = kPlanThreads;  // s_blk[lo] <= j < s_blk[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (s_blk[mid] <= j) lo = mid;
-                else hi = mid;
+    // f(sequence of the chunk, query block, its tiles) for every block
+    auto for_blocks = [&](auto f) {
+        for (int c = 0; c < chunks; ++c) {
+            if (chunks > 1) load_chunk(c);
+            for (int j = tid; j < s_blk[kPlanThreads]; j += kPlanThreads) {
+                int lo = 0, hi = min(kPlanThreads, a.t.n_seq);  // s_blk[lo] <= j < s_blk[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (s_blk[mid] <= j) lo = mid;
+                    else hi = mid;
+                }
+                f(c * kPlanThreads + lo, lo, j - s_blk[lo], block_tiles(a, s_start[lo], s_S[lo], j - s_blk[lo]));
             }
-            f(lo, j - s_blk[lo]);
         }
     };
     load_chunk(0);
 
-    // the longest block, all tiles, all blocks
-    int mx = 0, cnt = 0;
-    unsigned long long tiles = 0;
-    for (int c = 0; c < chunks; ++c)
-        for_blocks(c, [&](int s, int qb) {
-            const int nt = block_tiles(a, s_start[s], s_S[s], qb);
-            mx = max(mx, nt);
-            tiles += (unsigned)nt;
-            ++cnt;
-        });
-    mx = wave_max_i(mx);
-    cnt = wave_sum_i(cnt);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) tiles += __shfl_xor(tiles, d);
-    if (lane == 0) {
-        atomicMax(&s_max, mx);
-        atomicAdd(&s_n[1], cnt);
-        atomicAdd(&s_tiles, tiles);
+    // the longest block: tiles do not fall along a sequence, but for a short last block
+    for (int c = 0; c < chunks; ++c) {
+        if (chunks > 1) load_chunk(c);
+        const int nb = s_blk[tid + 1] - s_blk[tid];
+        int mx = 0;
+        if (nb > 0) mx = block_tiles(a, s_start[tid], s_S[tid], nb - 1);
+        if (nb > 1) mx = max(mx, block_tiles(a, s_start[tid], s_S[tid], nb - 2));
+        mx = (int)wave_max((float)mx);  // (at most 2^25 tiles)
+        if (lane == 0) atomicMax(&s_max, mx);
     }
     __syncthreads();
     const int longest = s_max;
-    // at least 4 tiles of 32 keys (2 of 64) a piece
-    const int st_min = a.kt == 64 ? 2 : 4;
-    int st = max(longest, 1);
+    const int st_min = a.kt == 64 ? 2 : 4;  // tiles a piece at least
+    const auto cut = [&](int k) { return max((longest + k - 1) / k, k == 1 ? 1 : st_min); };
+    int st = cut(1);
     if (a.max_slots > 0 && longest > st_min) {  // workgroup-uniform
-        int n[kMaxPieces + 1] = {}, sl[kMaxPieces + 1] = {};
-        for (int c = 0; c < chunks; ++c)
-            for_blocks(c, [&](int s, int qb) {
-                const int nt = block_tiles(a, s_start[s], s_S[s], qb);
+        // wave w takes candidates w + 1, w + 5, .., a sequence a lane
+        SplitSums t[2];
+        float tiles = 0.0f;
+        static_assert(kMaxPieces == 2 * (kPlanThreads / 64), "two candidates a wave");
+        for (int c = 0; c < chunks; ++c) {
+            if (chunks > 1) load_chunk(c);
+            for (int i = lane; i < min(kPlanThreads, a.t.n_seq - c * kPlanThreads); i += 64) {
+                const int nb = s_blk[i + 1] - s_blk[i];
+                if (nb == 0) continue;
+                const int S = s_S[i], start = s_start[i];
+                const float n0 = (float)block_tiles(a, start, S, 0), n1 = (float)block_tiles(a, start, S, nb / 2);
+                const float n2 = (float)block_tiles(a, start, S, nb > 1 ? nb - 2 : 0), m1 = (float)(nb / 2), m2 = (float)(nb - nb / 2);
+                tiles += 0.5f * ((n0 + n1) * m1 + (n1 + n2) * m2);
 #pragma unroll
-                for (int k = 2; k <= kMaxPieces; ++k) {
-                    const int stk = max((longest + k - 1) / k, st_min), np = max(1, (nt + stk - 1) / stk);
-                    n[k] += np;
-                    sl[k] += np > 1 ? np : 0;
+                for (int q = 0; q < 2; ++q) {
+                    ramp_sums(t[q], n0, n1, m1, (float)cut(wave + 1 + 4 * q));
+                    ramp_sums(t[q], n1, n2, m2, (float)cut(wave + 1 + 4 * q));
                 }
-            });
-#pragma unroll
-        for (int k = 2; k <= kMaxPieces; ++k) {
-            const int nk = wave_sum_i(n[k]), sk = wave_sum_i(sl[k]);
-            if (lane == 0) {
-                atomicAdd(&s_n[k], nk);
-                atomicAdd(&s_slots[k], sk);
             }
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float v[7] = {wave_sum(t[q].units), wave_sum(t[q].slots), wave_sum(t[q].over[0]), wave_sum(t[q].over[1]),
+                                wave_sum(t[q].over[2]), wave_sum(t[q].over[3]), wave_sum(tiles)};
+            if (lane == 0)
+#pragma unroll
+                for (int i = 0; i < 7; ++i) s_sum[wave + 1 + 4 * q][i] = v[i];
         }
         __syncthreads();
+        // lane k of every wave prices candidate k
         const PlanCost pc = plan_cost(a.kt);
-        float best = 0.0f;
-        for (int k = 1; k <= kMaxPieces; ++k) {
-            const int stk = max((longest + k - 1) / k, k == 1 ? 1 : st_min);
-            if ((long long)s_slots[k] * a.n_kv_heads > a.max_slots) continue;
-            const float load = ((float)s_tiles + (float)s_n[k] * pc.unit + (float)s_slots[k] * pc.part) * (float)a.n_kv_heads / kCus;
-            const float lng = (float)stk + pc.unit + (k > 1 ? pc.part : 0.0f);
-            const float cost = fmaxf(lng, load + 0.3f * lng) + (s_slots[k] > 0 ? pc.merge : 0.0f);
-            if (k == 1 || cost < best) {
-                best = cost;
-                st = stk;
+        float cost = __builtin_huge_valf();
+        if (lane >= 1 && lane <= kMaxPieces) {
+            float v[7];
+#pragma unroll
+            for (int i = 0; i < 7; ++i) {
+                v[i] = s_sum[lane][i] * (float)a.n_kv_heads;
             }
+            const float stk = (float)cut(lane), part = v[1] > 0.5f ? pc.part : 0.0f;
+            cost = (v[6] + v[0] * pc.unit + v[1] * pc.part) * (1.0f / kCus);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (v[2 + i] >= 0.5f) cost = fmaxf(cost, ceilf(v[2 + i] * (1.0f / kCus)) * (stk * (float)(4 - i) * 0.25f + pc.unit + part));
+            if (v[1] > 0.5f) cost += pc.merge;
+            if (v[1] > (float)a.max_slots) cost = __builtin_huge_valf();
         }
+        const float best = -wave_max(-cost);
+        const unsigned long long m = __ballot(cost == best && lane >= 1 && lane <= kMaxPieces);
+        if (m) st = cut(__builtin_ctzll(m));
     }
-    const auto pieces = [&](int nt) { return max(1, (nt + st - 1) / st); };
-    // bin 0: the longest pieces
+    const auto pieces = [&](int nt) { return min(max(1, (nt + st - 1) / st), kMaxPieces); };
+    // class 0: the longest pieces
     const auto bin_of = [&](int nt, int np) { return kBins - 1 - min((nt + np - 1) / np * (kBins - 1) / st, kBins - 1); };
-    for (int c = 0; c < chunks; ++c)
-        for_blocks(c, [&](int s, int qb) {
-            const int nt = block_tiles(a, s_start[s], s_S[s], qb), np = pieces(nt);
+    for (int round = 0; round < 2; ++round) {
+        for_blocks([&](int, int, int, int nt) {
+            const int np = pieces(nt);
             atomicAdd(&s_bin[bin_of(nt, np)], np * a.n_kv_heads);
+            if (np > 1) atomicAdd(&s_cut, np * a.n_kv_heads);
         });
-    __syncthreads();
-    if (wave == 0) {  // first unit of each bin
-        int v[kBins / 64], sum = 0;
-#pragma unroll
-        for (int i = 0; i < kBins / 64; ++i) {
-            v[i] = s_bin[lane * (kBins / 64) + i];
-            sum += v[i];
-        }
-        int at = wave_prefix_sum(sum) - sum;
-        if (lane == 63) s_units = at + sum;
-#pragma unroll
-        for (int i = 0; i < kBins / 64; ++i) {
-            s_bin[lane * (kBins / 64) + i] = at;
-            at += v[i];
-        }
+        __syncthreads();
+        if (s_cut <= a.max_slots) break;
+        // the ramps missed: more pieces than there is room for their partials, so none at all
+        __syncthreads();
+        st = max(longest, 1);
+        if (tid < kBins) s_bin[tid] = 0;
+        if (tid == 0) s_cut = 0;
+        __syncthreads();
+    }
+    if (wave == 0) {  // first unit of each class
+        const int n = s_bin[lane], incl = wave_scan(n);
+        s_bin[lane] = incl - n;
+        if (lane == 63) a.counts[0] = min(incl, a.max_units);
     }
     __syncthreads();
-    for (int c = 0; c < chunks; ++c)
-        for_blocks(c, [&](int s, int qb) {
-            const int nt = block_tiles(a, s_start[s], s_S[s], qb), np = pieces(nt);
-            int at = atomicAdd(&s_bin[bin_of(nt, np)], np * a.n_kv_heads);
-            int slot = 0, mg = 0;
-            if (np > 1) {
-                slot = atomicAdd(&s_slot, np * a.n_kv_heads);
-                mg = atomicAdd(&s_merges, a.n_kv_heads);
+    for_blocks([&](int b, int s, int qb, int nt) {
+        const int np = pieces(nt);
+        int at = atomicAdd(&s_bin[bin_of(nt, np)], np * a.n_kv_heads), slot = 0, mg = 0;
+        if (np > 1) {
+            slot = atomicAdd(&s_slot, np * a.n_kv_heads);
+            mg = atomicAdd(&s_merge, a.n_kv_heads);
+        }
+        PagedUnit u{b, qb, 0, np, 0, 0, 0, s_lo[s], s_S[s], s_start[s], 0, 0};
+        for (int kh = 0; kh < a.n_kv_heads; ++kh) {
+            u.kh = kh;
+            for (int p = 0; p < np; ++p, ++at) {
+                u.slot = slot + kh * np + p;
+                u.t0 = (p * nt + np - 1) / np;
+                u.t1 = ((p + 1) * nt + np - 1) / np;
+                // (offsets out of order could list more blocks than there are packed rows: cut to the room)
+                if (at < a.max_units) a.units[at] = u;
             }
-            PagedUnit u{c * kPlanThreads + s, qb, 0, np, 0, 0, 0, s_lo[s], s_S[s], s_start[s], 0, 0};
-            // (offsets out of order could list more blocks than there are packed rows: cut to the room)
-            for (int kh = 0; kh < a.n_kv_heads; ++kh) {
-                u.kh = kh;
-                for (int p = 0; p < np; ++p, ++at) {
-                    u.slot = slot + kh * np + p;
-                    u.t0 = (p * nt + np - 1) / np;
-                    u.t1 = ((p + 1) * nt + np - 1) / np;
-                    if (at < a.max_units) a.units[at] = u;
-                }
-                u.slot = slot + kh * np;
-                if (np > 1) a.merges[mg + kh] = u;  // (st was chosen so that the slots hold every piece)
-            }
-        });
+            u.slot = slot + kh * np;
+            if (np > 1) a.merges[mg + kh] = u;
+        }
+    });
     __syncthreads();
-    if (tid == 0) {
-        a.counts[0] = min(s_units, a.max_units);
-        a.counts[1] = min(s_merges, a.max_slots / 2);
-    }
+    if (tid == 0) a.counts[1] = s_merge;
 }
 
 // q of packed rows to f16: RMSNorm * gain, then RoPE at the row's position (qprep_row512_kernel's
@@ -359,7 +388,7 @@ struct TilePages {
 __device__ __forceinline__ rsrc_t page_rows(const PageTab& t, const void* pool, int entry, int k0, int kv_hi, int row,
                                             int kh_off) {
     const bool ok = page_ok(t, entry);
-    const uint32_t bytes = ok ? (uint32_t)(min(max(kv_hi - k0, 0), 16) * row * 2) : 0u;
+    const uint32_t bytes = ok ? (uint32_t)(clamp16(kv_hi - k0) * row * 2) : 0u;
     return make_rsrc(reinterpret_cast<const half_t*>(pool) + paged_row(t, ok ? entry : 0, k0, row) + kh_off, bytes);
 }
 constexpr int kNoRow = 0x7fffff00;  // an offset past every such range, with room for a row's own bytes
@@ -402,30 +431,27 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
     // K/V rows of this kv head; wave w moves rows 16w .. 16w + 15 of a tile, two rows (1 KiB) an instruction
     const int rowg = a.n_kv_heads * HD * 2;  // bytes per cache row
     TilePages<KT> pages;
-    auto issue = [&](int t, int buf) {
-        char* kdst = lds + buf * 2 * TILEB;
-        const int kg = wg_lo + t * KT + 16 * wave;  // this wave's 16 rows
-        const int entry = __builtin_amdgcn_readlane(pages.entry, (t - t0) & 63);
-        const rsrc_t pk = page_rows(a.t, a.kc, entry, kg, kv_hi, rowg / 2, kh * HD);
-        const rsrc_t pv = page_rows(a.t, a.vc, entry, kg, kv_hi, rowg / 2, kh * HD);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int r = 16 * wave + 2 * j + h;  // tile row of this lane
-            const bool seen = kg + 2 * j + h >= first;
-            const int ro = (2 * j + h) * rowg;
-            char* d = kdst + (16 * wave + 2 * j) * ROWB;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pk, (__attribute__((address_space(3))) void*)d, 16,
-                                                     seen ? ro + 16 * (n32 ^ (r & 31)) : kNoRow, 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pv, (__attribute__((address_space(3))) void*)(d + TILEB), 16,
-                                                     seen ? ro + 16 * (n32 ^ vswz(r)) : kNoRow, 0, 0, 0);
-        }
+    // this wave's 16 rows of tile t from the page of `entry`; past the last tile: an empty range
+    const auto tile_rows = [&](const void* pool, int t, int entry) {
+        const int kg = wg_lo + t * KT + 16 * wave;
+        return page_rows(a.t, pool, entry, kg, t < t1 ? kv_hi : kg, rowg / 2, kh * HD);
     };
+    // DMA j of a wave's eight for a tile: two rows. swz: K's or V's chunk places
+    const auto dma = [&](rsrc_t rp, char* dst, int j, int off) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (__attribute__((address_space(3))) void*)(dst + (16 * wave + 2 * j) * ROWB),
+                                                 16, off, 0, 0, 0);
+    };
+    const auto k_off = [&](int j) { return (2 * j + h) * rowg + 16 * (n32 ^ ((16 * wave + 2 * j + h) & 31)); };
+    const auto v_off = [&](int j) { return (2 * j + h) * rowg + 16 * (n32 ^ vswz(2 * j + h)); };
+    const auto tile_k = [&](int t) { return lds + (t & 1) * 2 * TILEB; };
+    const auto tile_v = [&](int t) { return lds + (t & 1) * 2 * TILEB + TILEB; };
 
     // ---- q: lane (column, h) holds dims 16s + 8h + i (s < 16, i < 8), the B operand of the 32x32x16
     // MFMA. Wave w DMAs the f16 q rows of its own 32 columns (two 512-byte rows an instruction, chunk
     // n32 of a row from logical chunk n32 ^ (row % 32)) into the LDS stage that tile t0 + 1 takes over
     // later, then reads them back in that layout; rows past the block's last token read as zeros.
     half8 qf[16];
+    int entry1, gone0, gone1 = 0;  // tile t + 1's page, the 16-row groups of tiles t and t + 1 without one
     {
         const rsrc_t rq = make_rsrc(a.q16 + ((size_t)row0 + qb * BQ) * a.n_q_heads * HD, (uint32_t)min(BQ, S - qb * BQ) * a.n_q_heads * ROWB);
         char* qs = lds + ((t0 + 1) & 1) * 2 * TILEB;
@@ -437,12 +463,18 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(qs + (32 * wave + 2 * j) * ROWB),
                                                      16, qo, 0, 0, 0);
         }
-        if (t0 < t1) {
-            issue(t0, t0 & 1);
-            asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // the 16 q DMAs, issued before tile t0's 16
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        entry1 = __builtin_amdgcn_readlane(pages.entry, 0);
+        gone0 = __builtin_amdgcn_readlane(pages.gone, 0);
+        if (t0 < t1) {  // tile t0: of the block's first tile, rows in front of the first attended key read as zeros
+            const rsrc_t rk = tile_rows(a.kc, t0, entry1), rv = tile_rows(a.vc, t0, entry1);
+            const int skip = first - (wg_lo + t0 * KT + 16 * wave);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                dma(rk, tile_k(t0), j, 2 * j + h < skip ? kNoRow : k_off(j));
+                dma(rv, tile_v(t0), j, 2 * j + h < skip ? kNoRow : v_off(j));
+            }
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const char* qrow = qs + c * ROWB;
 #pragma unroll
         for (int s = 0; s < 16; ++s) qf[s] = *reinterpret_cast<const half8*>(qrow + 16 * ((2 * s + h) ^ n32));
@@ -460,12 +492,13 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
     // ---- key ranges: this wave [w_lo, wp1], this column [col_lo, pos]
     const int wp0 = p0 + (32 * wave) / G;
     const int wp1 = min(p0 + (32 * wave + 31) / G, T_total - 1);
-    const int w_lo = a.window > 0 ? max(0, wp0 + 1 - a.window) : 0;
     const int col_lo = a.window > 0 ? pos + 1 - a.window : 0;
 
     float16v oacc[8];  // O^T[32dt + 8(r/4) + 4h + r%4][column]
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) oacc[dt] = float16v{};
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) asm volatile("" : "+a"(oacc[dt]));
     float m_use = kNegInf, l_run = 0.0f;
     bool started = false;
 
@@ -477,74 +510,52 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
     const int vb0 = 8 * (m16 & 1);                   // byte within the chunk
     const int vsw = vswz(vr0);                        // rows 16u + vr0 (+8) share r % 4
 
-    for (int t = t0; t < t1; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of tile t is in LDS
-        __syncthreads();                                    // all parts; tile t-1 fully consumed
-        const int gone = __builtin_amdgcn_readlane(pages.gone, (t - t0) & 63);  // 16-row groups without a page
-        if (((t + 1 - t0) & 63) == 0) pages.load(a.t, wu.b, wg_lo + (t + 1) * KT, wave, lane);
-        if (t + 1 < t1) issue(t + 1, (t + 1) & 1);
+    // A tile's scores, S^T = K . Q^T: two 32-key sub-tiles, 16 k-steps of 16 dims, the two accumulator
+    // chains in turn (a chain of dependent MFMAs issues at half rate).
+    // Masks of tile t's scores: key kb + 4h + 32kt + 8(r/4) + r%4 of this lane's column; tiles inside every
+    // column's range skip it.
+    auto mask = [&](int t, int gone, float16v (&sc)[2]) {
         const int kb = wg_lo + t * KT;
-        if (kb > wp1 || kb + KT - 1 < w_lo) continue;  // no key of this tile for this wave
-        const char* K = lds + (t & 1) * 2 * TILEB;
-        const char* V = K + TILEB;
-
-        // S^T = K . Q^T: two 32-key sub-tiles, 16 k-steps of 16 dims. The two accumulator
-        // chains alternate (a chain of dependent MFMAs issues at half rate), and the A
-        // operands are read in batches ahead of their MFMAs.
-        float16v sacc[2] = {float16v{}, float16v{}};
-        {
-            const char* krow0 = K + n32 * ROWB;
-            const char* krow1 = K + (32 + n32) * ROWB;
-#pragma unroll
-            for (int s0 = 0; s0 < 16; s0 += 4) {
-                half8 kv0[4], kv1[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const int cb = 16 * ((2 * (s0 + s) + h) ^ n32);
-                    kv0[s] = *reinterpret_cast<const half8*>(krow0 + cb);
-                    kv1[s] = *reinterpret_cast<const half8*>(krow1 + cb);
-                }
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    sacc[0] = mfma32(kv0[s], qf[s0 + s], sacc[0]);
-                    sacc[1] = mfma32(kv1[s], qf[s0 + s], sacc[1]);
-                }
-            }
-            // keep kQkAhead LDS reads ahead of the score MFMAs (masks: 0x100 DS read, 0x008 MFMA)
-            __builtin_amdgcn_sched_group_barrier(0x100, kQkAhead, 0);
-#pragma unroll
-            for (int i = 0; i < 32 - kQkAhead; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, kQkAhead, 0);
-        }
-
-        // scores of this lane: key kb + 4h + 32kt + 8(r/4) + r%4 of its column, log2 domain;
-        // tiles inside every column's range skip the per-element mask
-        const bool masked = (kb + KT - 1 > wp0) || (a.window > 0 && kb < wp1 + 1 - a.window);
-        if (masked) {
+        if ((kb + KT - 1 > wp0) || (a.window > 0 && kb < wp1 + 1 - a.window)) {
             const int rel_hi = pos - (kb + 4 * h), rel_lo = col_lo - (kb + 4 * h);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int o = 32 * kt + 8 * (r >> 2) + (r & 3);
-                    sacc[kt][r] = (o <= rel_hi && o >= rel_lo) ? sacc[kt][r] : kNegInf;
+                    sc[kt][r] = (o <= rel_hi && o >= rel_lo) ? sc[kt][r] : kNegInf;
                 }
         }
         if (gone) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) sacc[kt][r] = gone >> (2 * kt + (r >> 3)) & 1 ? kNegInf : sacc[kt][r];
+                for (int r = 0; r < 16; ++r) sc[kt][r] = gone >> (2 * kt + (r >> 3)) & 1 ? kNegInf : sc[kt][r];
         }
-        float mloc = kNegInf;  // max of the raw scores, scaled once (scale > 0)
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mloc = fmaxf(mloc, sacc[kt][r]);
-        mloc = max32(mloc) * a.scale_log2;  // the column's other half sits in lane ^ 32
+    };
+
+    // One tile. A wave has its SIMD to itself, so what is to overlap has to be interleaved in its own
+    // instruction stream (the order below is kept by the sched_barriers):
+    //   * the 32 score MFMAs of tile t + 1 with the exponentials of tile t -- a step's two MFMAs take the
+    //     matrix unit 64 cycles, in which two exponentials of three stages (argument, exp2, sum and
+    //     rounding of the step before) and the operand reads two steps ahead issue -- and with the DMAs
+    //     of V(t + 1) and K(t + 2), which issue one a step: all 16 at once hold the wave up while the
+    //     CU's four waves queue for the 64 B/clk path into LDS (1190 of 5300 cycles a tile);
+    //   * the 32 P.V MFMAs of tile t with the maxima of tile t + 1.
+    // So K is fetched two tiles ahead, V one: K(t + 2) into the buffer of K(t), whose scores are done,
+    // V(t + 1) into that of V(t - 1).
+    float mnext = kNegInf;  // this lane's maximum of the scores of the next tile
+    auto tile = [&](int t, float16v (&sacc)[2], float16v (&snext)[2]) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of V(t) and K(t + 1) is in LDS
+        __syncthreads();                                    // all parts; K(t) and V(t - 1) fully consumed
+        const int gone = gone1, entry = entry1;             // of tile t + 1
+        {
+            const int j = (t + 2 - t0) & 63;
+            if (j == 0) pages.load(a.t, wu.b, wg_lo + (t + 2) * KT, wave, lane);
+            entry1 = __builtin_amdgcn_readlane(pages.entry, j);
+            gone1 = __builtin_amdgcn_readlane(pages.gone, j);
+        }
+        const float mloc = max32(mnext) * a.scale_log2;  // the column's other half sits in lane ^ 32 (scale > 0)
         // move the running maxima only when a score passes one by more than 2^kMaxLag
         const bool bump = mloc > m_use + kMaxLag;
         if (__any(bump)) {
@@ -552,8 +563,20 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
             const float corr = m_use == kNegInf ? 0.0f : fexp2(m_use - m_new);
             l_run *= corr;
             if (started) {
+                // one 16-register tile at a time: copied to VGPRs, scaled, pinned back into
+                // AGPRs (left to itself the compiler moves all of them at once)
+                asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"  // the last MFMA's writes, as in the epilogue
+                             : "+a"(oacc[0]), "+a"(oacc[1]), "+a"(oacc[2]), "+a"(oacc[3]), "+a"(oacc[4]),
+                               "+a"(oacc[5]), "+a"(oacc[6]), "+a"(oacc[7]));
 #pragma unroll
-                for (int dt = 0; dt < 8; ++dt) oacc[dt] *= corr;
+                for (int dt = 0; dt < 8; ++dt) {
+                    float16v x = oacc[dt];
+                    asm volatile("" : "+v"(x));
+                    x *= corr;
+                    asm volatile("" : "+v"(x));
+                    oacc[dt] = x;
+                    asm volatile("" : "+a"(oacc[dt]));
+                }
             }
             m_use = m_new;
         }
@@ -561,43 +584,116 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
         const float msub = m_use == kNegInf ? 0.0f : m_use;
         half8 pb[4];
         float ps = 0.0f;
+        {
+            const char* krow0 = tile_k(t + 1) + n32 * ROWB;
+            const char* krow1 = krow0 + 32 * ROWB;
+            half8 kr[3][2];
+            auto read_k = [&](int s) {
+                const int cb = 16 * ((2 * s + h) ^ n32);
+                kr[s % 3][0] = *reinterpret_cast<const half8*>(krow0 + cb);
+                kr[s % 3][1] = *reinterpret_cast<const half8*>(krow1 + cb);
+            };
+            // exponential v of the lane's 32 in three stages
+            float ex[2][2], ev[2][2];
+            auto arg = [&](int v) { ex[(v >> 1) & 1][v & 1] = __builtin_fmaf(sacc[v >> 4][v & 15], a.scale_log2, -msub); };
+            auto expo = [&](int v) { ev[(v >> 1) & 1][v & 1] = fexp2(ex[(v >> 1) & 1][v & 1]); };
+            auto take = [&](int v) {
+                const float e = ev[(v >> 1) & 1][v & 1];
+                ps += e;
+                pb[v >> 3][v & 7] = (half_t)e;
+            };
+            read_k(0);
+            read_k(1);
+            arg(0);
+            arg(1);
+            const rsrc_t rv = tile_rows(a.vc, t + 1, entry), rk = tile_rows(a.kc, t + 2, entry1);
+            snext[0] = snext[1] = float16v{};
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float pv = fexp2(__builtin_fmaf(sacc[u >> 1][8 * (u & 1) + i], a.scale_log2, -msub));
-                ps += pv;
-                pb[u][i] = (half_t)pv;
+            for (int s = 0; s < 16; ++s) {
+                if (s + 2 < 16) read_k(s + 2);
+                snext[0] = mfma32(kr[s % 3][0], qf[s], snext[0]);
+                expo(2 * s);
+                expo(2 * s + 1);
+                if (s > 0) {
+                    take(2 * s - 2);
+                    take(2 * s - 1);
+                }
+                snext[1] = mfma32(kr[s % 3][1], qf[s], snext[1]);
+                if (s < 15) {
+                    arg(2 * s + 2);
+                    arg(2 * s + 3);
+                }
+                if (s < 8) dma(rv, tile_v(t + 1), s, v_off(s));
+                else dma(rk, tile_k(t + 2), s - 8, k_off(s - 8));
+                __builtin_amdgcn_sched_barrier(0);
             }
+            take(30);
+            take(31);
+        }
         l_run += ps;
+        // (here, not where they are used behind the masks' branches: the compiler would sink them there)
+        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(pb[2]), "+v"(pb[3]), "+v"(l_run));
+        if (t + 1 < t1) mask(t + 1, gone, snext);
 
-        // O^T += V^T . P^T over four 16-key steps; k-slot i < 4 is key 16u + 4h + i,
-        // i >= 4 is key 16u + 8 + 4h + i - 4, matching the S^T accumulator rows in pb
+        // O^T += V^T . P^T over four 16-key steps; k-slot i < 4 is key 16u + 4h + i, i >= 4 is key
+        // 16u + 8 + 4h + i - 4, matching the S^T accumulator rows in pb. Transposed V reads (two an
+        // MFMA) kPvAhead MFMAs ahead.
+        {
+            const char* V = tile_v(t);
+            half8 av[kPvAhead + 1];
+            auto read_v = [&](int i) {
+                const int u = i >> 3, ch = 4 * (i & 7) + vc0;
+                const char* vp = V + (16 * u + vr0) * ROWB + 16 * (ch ^ vsw) + vb0;
+                const half4 lo = lds_tr16(reinterpret_cast<const half_t*>(vp));
+                const half4 hi = lds_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
+                av[i % (kPvAhead + 1)] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            mnext = kNegInf;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int ra = 16 * u + vr0, rb = ra + 8;
-            half8 av[8];
+            for (int i = 0; i < kPvAhead; ++i) read_v(i);
 #pragma unroll
-            for (int dt = 0; dt < 8; ++dt) {
-                const int ch = 4 * dt + vc0;
-                const half4 lo = lds_tr16(reinterpret_cast<const half_t*>(V + ra * ROWB + 16 * (ch ^ vsw) + vb0));
-                const half4 hi = lds_tr16(reinterpret_cast<const half_t*>(V + rb * ROWB + 16 * (ch ^ vsw) + vb0));
-                av[dt] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            for (int i = 0; i < 32; ++i) {
+                if (i + kPvAhead < 32) read_v(i + kPvAhead);
+                mfma32_acc(oacc[i & 7], av[i % (kPvAhead + 1)], pb[i >> 3]);
+                if (i >= 8 && i < 24) mnext = fmaxf(mnext, fmaxf(snext[(i - 8) >> 3][2 * (i & 7)], snext[(i - 8) >> 3][2 * (i & 7) + 1]));
+                __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt) oacc[dt] = mfma32(av[dt], pb[u], oacc[dt]);
+            asm volatile("" : "+v"(mnext));
         }
-        // transposed V reads kept kPvAhead MFMAs ahead of the P.V MFMAs, two reads per MFMA
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * kPvAhead, 0);
+    };
+    if (t0 < t1) {
+        float16v sa[2] = {float16v{}, float16v{}}, sb[2];
+        __syncthreads();  // K(t0), V(t0); every wave has its q
+        entry1 = __builtin_amdgcn_readlane(pages.entry, 1);
+        gone1 = __builtin_amdgcn_readlane(pages.gone, 1);
+        const rsrc_t rk = tile_rows(a.kc, t0 + 1, entry1);
 #pragma unroll
-        for (int i = 0; i < 32 - kPvAhead; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        for (int j = 0; j < 8; ++j) dma(rk, tile_k(t0 + 1), j, k_off(j));
+        const char* krow0 = tile_k(t0) + n32 * ROWB;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+            const int cb = 16 * ((2 * s + h) ^ n32);
+            sa[0] = mfma32(*reinterpret_cast<const half8*>(krow0 + cb), qf[s], sa[0]);
+            sa[1] = mfma32(*reinterpret_cast<const half8*>(krow0 + 32 * ROWB + cb), qf[s], sa[1]);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, kPvAhead, 0);
+        mask(t0, gone0, sa);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mnext = fmaxf(mnext, fmaxf(sa[0][r], sa[1][r]));
+        for (int t = t0;;) {  // the two score sets change roles every tile
+            tile(t, sa, sb);
+            if (++t >= t1) break;
+            tile(t, sb, sa);
+            if (++t >= t1) break;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last tile's (empty) DMAs, before LDS is used again
     }
 
     // ---- epilogue: column sum over both halves, normalise, srq, store 4 dims at a time
+    // (the accumulators must not be read within 18 wait states of the last MFMA writing them, which the
+    // compiler does not see)
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
+                 : "+a"(oacc[0]), "+a"(oacc[1]), "+a"(oacc[2]), "+a"(oacc[3]), "+a"(oacc[4]), "+a"(oacc[5]),
+                   "+a"(oacc[6]), "+a"(oacc[7]));
     const float l_tot = add32(l_run);
     if (n_pieces > 1) {  // a piece of a split query block: O / l and (m, l)
         const float inv_p = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
