@@ -45,6 +45,14 @@ class AttnConfig:
         return G4ACfg(self.n_q_heads, self.n_kv_heads, self.head_dim, self.window, flags,
                       self.scale, self.eps, self.out_q)
 
+    def c_ref(self, flags: int):
+        """c(flags) as a ctypes argument, made once per flags (the instance is frozen; the library only
+        reads it)."""
+        ref = self.__dict__.get(flags)
+        if ref is None:
+            ref = self.__dict__[flags] = ctypes.byref(self.c(flags))
+        return ref
+
 
 # The short calls are bound by this layer, not by their kernels, so it wraps and unwraps nothing
 # that ctypes converts by itself: pointers and streams go as whole numbers, torch's raw stream

@@ -30,46 +30,72 @@ import torch
 
 from . import _lib
 from ._lib import G4APaged, check
-from .attention import AttnConfig, DecodeWorkspace, _need, _ptr
+from .attention import AttnConfig, DecodeWorkspace
 
 __all__ = ["paged_write", "paged_decode", "paged_decode_ws_bytes", "paged_prefill", "paged_prefill_ws_bytes"]
 
 _F32, _F16, _I32 = torch.float32, torch.float16, torch.int32
+_HALF_OR_FLOAT = (_F16, _F32)
+_EWORKSPACE = -3
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the other operands on {dev}")
+# A decode step of short sequences is bound by this layer, not by its kernels: the checks below touch each
+# tensor a few times, whole numbers go to ctypes as they are, and the workspace's size is only asked for
+# when the library finds it too small (one sequence of 300 keys 19.2 -> 13 us a call).
+def _refuse(name, t, dev, dtype):
+    """What is wrong with a tensor that _t found unfit."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the other operands on cuda:{dev}")
+    if t.dtype is not dtype and not (isinstance(dtype, tuple) and t.dtype in dtype):
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    raise ValueError(f"{name} must be contiguous")
 
 
-def _on_device(dev, fn, *args):
-    """fn(*args, stream) with dev current: the kernels launch on the current device."""
-    if dev.index == torch.cuda.current_device():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+def _t(name, t, dev, dtype):
+    """Address of a contiguous tensor of dtype on GPU dev; None stays None."""
+    if t is None:
+        return None
+    if t.get_device() != dev or t.dtype is not dtype or not t.is_contiguous():
+        _refuse(name, t, dev, dtype)
+    return t.data_ptr()
+
+
+def _gpu(name, t):
+    """The GPU that a call's first tensor is on: every other operand has to be there."""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name} must be a device tensor")
+    return dev
+
+
+def _launch(dev, fn, *args):
+    """fn(*args, stream) with GPU dev current (the kernels launch there), on its current stream."""
+    if dev == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     with torch.cuda.device(dev):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin) -> G4APaged:
-    """The checked g4a_paged of a call."""
-    if k_pages.dim() != 4 or k_pages.shape[2:] != (cfg.n_kv_heads, cfg.head_dim) or v_pages.shape != k_pages.shape:
+def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin):
+    """The checked g4a_paged of a call, and the addresses of the RoPE tables."""
+    shape, kv = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape[2] != cfg.n_kv_heads or shape[3] != cfg.head_dim or v_pages.shape != shape:
         raise ValueError(f"k_pages / v_pages must be [n_pages][page_size][{cfg.n_kv_heads}][{cfg.head_dim}], got "
-                         f"{tuple(k_pages.shape)} and {tuple(v_pages.shape)}")
-    if k_pages.dtype != v_pages.dtype or k_pages.dtype not in (_F16, _F32):
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    if kv not in _HALF_OR_FLOAT or v_pages.dtype is not kv:
         raise ValueError("k/v pages must both be float16 or both float32")
-    _need(k_pages, "k_pages")
-    _need(v_pages, "v_pages")
-    if not page_table.is_cuda or page_table.dtype is not _I32 or page_table.dim() != 2 or page_table.stride(1) != 1:
-        raise ValueError("page_table must be an int32 device tensor [n_seq][cols] with adjacent columns")
+    if page_table.get_device() != dev or page_table.dtype is not _I32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+        raise ValueError(f"page_table must be an int32 tensor [n_seq][cols] on cuda:{dev} with adjacent columns")
     n_seq, cols = page_table.shape
     stride = page_table.stride(0) if n_seq > 1 else cols
     if stride < cols:
         raise ValueError("page_table rows must not overlap")
-    _need(key_len, "key_len", _I32)
+    lens = _t("key_len", key_len, dev, _I32)
     if key_len.numel() != n_seq:
         raise ValueError(f"key_len must have one entry per row of page_table ({n_seq}), got {key_len.numel()}")
-    page = k_pages.shape[1]
+    page = shape[1]
     if max_key_len is None:
         max_key_len = cols * page
         if rope_cos is not None:
@@ -78,24 +104,47 @@ def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_co
         raise ValueError(f"max_key_len must be in [1, {cols * page}], what the page table's columns hold")
     if (rope_cos is None) != (rope_sin is None):
         raise ValueError("rope_cos and rope_sin go together")
+    rc = rs = None
     if rope_cos is not None:
-        _need(rope_cos, "rope_cos", _F32)
-        _need(rope_sin, "rope_sin", _F32)
-        if rope_cos.dim() != 2 or rope_cos.shape[1] != cfg.head_dim // 2 or rope_cos.shape[0] < max_key_len or (
-                rope_sin.shape != rope_cos.shape):
+        rc, rs = _t("rope_cos", rope_cos, dev, _F32), _t("rope_sin", rope_sin, dev, _F32)
+        rows = rope_cos.shape
+        if len(rows) != 2 or rows[0] < max_key_len or rows[1] * 2 != cfg.head_dim or rope_sin.shape != rows:
             raise ValueError(f"rope tables must be [>= max_key_len ({max_key_len})][head_dim/2], got "
-                             f"{tuple(rope_cos.shape)} and {tuple(rope_sin.shape)}")
-    _same_device(dev, k_pages=k_pages, v_pages=v_pages, page_table=page_table, key_len=key_len, rope_cos=rope_cos,
-                 rope_sin=rope_sin)
-    return G4APaged(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), key_len.data_ptr(), k_pages.shape[0],
-                    page, n_seq, cols, stride, int(max_key_len))
+                             f"{tuple(rows)} and {tuple(rope_sin.shape)}")
+    return G4APaged(_t("k_pages", k_pages, dev, kv), _t("v_pages", v_pages, dev, kv), page_table.data_ptr(), lens, shape[0],
+                    page, n_seq, cols, stride, int(max_key_len)), rc, rs
 
 
 def _cu(cu_q, n_seq, dev):
-    _need(cu_q, "cu_q", _I32)
+    at = _t("cu_q", cu_q, dev, _I32)
     if cu_q.numel() != n_seq + 1:
         raise ValueError(f"cu_q must have n_seq + 1 = {n_seq + 1} entries, got {cu_q.numel()}")
-    _same_device(dev, cu_q=cu_q)
+    return at
+
+
+def _scratch(workspace, dev, nbytes):
+    """A workspace of at least nbytes on GPU dev."""
+    ws = (workspace if workspace is not None else DecodeWorkspace(torch.device("cuda", dev))).get(nbytes)
+    if ws.get_device() != dev:
+        raise ValueError(f"workspace is on {ws.device}, the other operands on cuda:{dev}")
+    return ws
+
+
+def _with_scratch(workspace, dev, ws_bytes, call):
+    """call(address, bytes) on the workspace's buffer; only a call that finds it too small asks for the size."""
+    buf = workspace.buf if workspace is not None else None
+    if buf is not None:
+        if buf.get_device() != dev:
+            raise ValueError(f"workspace is on {buf.device}, the other operands on cuda:{dev}")
+        rc = call(buf.data_ptr(), buf.numel())
+        if rc != _EWORKSPACE:
+            check(rc)
+            return
+    need = ws_bytes()
+    if need == 0:
+        check(-1)
+    ws = _scratch(workspace, dev, need)
+    check(call(ws.data_ptr(), ws.numel()))
 
 
 def paged_write(k, v, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConfig, *, k_gain=None, rope_cos=None,
@@ -107,32 +156,34 @@ def paged_write(k, v, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConf
     k RMSNorm * k_gain and RoPE at its position, v RMSNorm."""
     if k.dim() != 3 or k.shape[1:] != (cfg.n_kv_heads, cfg.head_dim) or v.shape != k.shape or k.dtype != v.dtype:
         raise ValueError(f"k/v shape {tuple(k.shape)} does not match {cfg}")
-    _need(k, "k", (_F16, _F32))
-    _need(v, "v", (_F16, _F32))
-    _need(k_gain, "k_gain", _F32)
-    dev = k.device
-    pg = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
-    _cu(cu_q, pg.n_seq, dev)
-    _same_device(dev, v=v, k_gain=k_gain)
-    c = cfg.c((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.IN_F16 if k.dtype is _F16 else 0) |
-              (0 if v_norm else _lib.NO_V_NORM))
-    check(_on_device(dev, _lib.load().g4a_paged_write, ctypes.byref(c), ctypes.byref(pg), k.shape[0], _ptr(cu_q), _ptr(k),
-                     _ptr(v), float(k_in_q), float(v_in_q), _ptr(k_gain), _ptr(rope_cos), _ptr(rope_sin)))
+    dev, rows = _gpu("k", k), k.dtype
+    if rows not in _HALF_OR_FLOAT:
+        raise ValueError(f"k and v must be float16 or float32, got {rows}")
+    pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
+    c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.IN_F16 if rows is _F16 else 0) |
+                  (0 if v_norm else _lib.NO_V_NORM))
+    check(_launch(dev, _lib.load().g4a_paged_write, c, ctypes.byref(pg), k.shape[0], _cu(cu_q, pg.n_seq, dev),
+                  _t("k", k, dev, rows), _t("v", v, dev, rows), k_in_q, v_in_q, _t("k_gain", k_gain, dev, _F32), rc, rs))
 
 
-def _out(out, q, out_dtype):
+def _out(out, q, out_dtype, dev):
     if out is None:
-        return torch.empty(q.shape, dtype=out_dtype, device=q.device)
-    if out.shape != q.shape:
+        if out_dtype not in _HALF_OR_FLOAT:
+            raise ValueError(f"out_dtype must be float16 or float32, got {out_dtype}")
+        out = torch.empty_like(q, dtype=out_dtype)
+    elif out.shape != q.shape:
         raise ValueError(f"out must be shaped like q {tuple(q.shape)}, got {tuple(out.shape)}")
+    elif out.get_device() != dev or out.dtype not in _HALF_OR_FLOAT or not out.is_contiguous():
+        _refuse("out", out, dev, _HALF_OR_FLOAT)
     return out
 
 
 def _q(q, cfg, q_gain):
-    if q.dim() != 3 or q.shape[1:] != (cfg.n_q_heads, cfg.head_dim):
-        raise ValueError(f"q shape {tuple(q.shape)} does not match {cfg}")
-    _need(q, "q", _F32)
-    _need(q_gain, "q_gain", _F32)
+    shape = q.shape
+    if len(shape) != 3 or shape[1] != cfg.n_q_heads or shape[2] != cfg.head_dim:
+        raise ValueError(f"q shape {tuple(shape)} does not match {cfg}")
+    dev = _gpu("q", q)
+    return dev, _t("q", q, dev, _F32), _t("q_gain", q_gain, dev, _F32)
 
 
 def _sizes(n_pages, page_size, n_seq, cols, max_key_len) -> G4APaged:
@@ -160,32 +211,23 @@ def paged_decode(q, k_pages, v_pages, page_table, key_len, cfg: AttnConfig, *, w
     prepared as ``kv_write`` prepares them and appended at position key_len - 1 by the same call
     before they are attended. Returns out [n_seq][nH][hd] (f16 by default); an idle sequence's
     rows are zeros. `workspace`: the caller's scratch (paged_decode_ws_bytes)."""
-    _q(q, cfg, q_gain)
-    dev = q.device
-    pg = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
+    dev, qp, qg = _q(q, cfg, q_gain)
+    pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
     if q.shape[0] != pg.n_seq:
         raise ValueError(f"q holds {q.shape[0]} tokens, page_table {pg.n_seq} sequences")
+    kn = vn = kg = None
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new go together")
-    for name, x in (("k_new", k_new), ("v_new", v_new)):
-        _need(x, name, _F32)
-        if x is not None and x.shape != (pg.n_seq, cfg.n_kv_heads, cfg.head_dim):
-            raise ValueError(f"{name} must be [{pg.n_seq}][{cfg.n_kv_heads}][{cfg.head_dim}]")
-    _need(k_gain, "k_gain", _F32)
-    out = _out(out, q, out_dtype)
-    _need(out, "out", (_F16, _F32))
-    _same_device(dev, q_gain=q_gain, k_new=k_new, v_new=v_new, k_gain=k_gain, out=out)
-    c = cfg.c((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0) |
-              (0 if v_norm else _lib.NO_V_NORM))
-    lib = _lib.load()
-    ws_bytes = lib.g4a_paged_decode_ws_bytes(ctypes.byref(c), ctypes.byref(pg))
-    if ws_bytes == 0:
-        check(-1)
-    ws = (workspace or DecodeWorkspace(dev)).get(ws_bytes)
-    _same_device(dev, workspace=ws)
-    check(_on_device(dev, lib.g4a_paged_decode, ctypes.byref(c), ctypes.byref(pg), _ptr(q), _ptr(q_gain), _ptr(rope_cos),
-                     _ptr(rope_sin), _ptr(k_new), _ptr(v_new), float(k_in_q), float(v_in_q), _ptr(k_gain), _ptr(out),
-                     _ptr(ws), ws_bytes))
+    if k_new is not None:
+        kn, vn, kg = _t("k_new", k_new, dev, _F32), _t("v_new", v_new, dev, _F32), _t("k_gain", k_gain, dev, _F32)
+        if k_new.shape != (pg.n_seq, cfg.n_kv_heads, cfg.head_dim) or v_new.shape != k_new.shape:
+            raise ValueError(f"k_new and v_new must be [{pg.n_seq}][{cfg.n_kv_heads}][{cfg.head_dim}]")
+    out = _out(out, q, out_dtype, dev)
+    c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0) |
+                  (0 if v_norm else _lib.NO_V_NORM))
+    lib, at, p = _lib.load(), out.data_ptr(), ctypes.byref(pg)
+    _with_scratch(workspace, dev, lambda: lib.g4a_paged_decode_ws_bytes(c, p),
+                  lambda ws, n: _launch(dev, lib.g4a_paged_decode, c, p, qp, qg, rc, rs, kn, vn, k_in_q, v_in_q, kg, at, ws, n))
     return out
 
 
@@ -208,20 +250,12 @@ def paged_prefill(q, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConfi
     q f32 [T][nH][hd] raw; the normalised, rotated q is rounded to f16 (as ``prefill`` without
     q_hilo). Returns out [T][nH][hd] (f16 by default). f32 caches are converted to f16 in the
     workspace. `workspace`: the caller's scratch (paged_prefill_ws_bytes)."""
-    _q(q, cfg, q_gain)
-    dev = q.device
-    pg = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
-    _cu(cu_q, pg.n_seq, dev)
-    out = _out(out, q, out_dtype)
-    _need(out, "out", (_F16, _F32))
-    _same_device(dev, q_gain=q_gain, out=out)
-    c = cfg.c((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0))
-    lib = _lib.load()
-    ws_bytes = lib.g4a_paged_prefill_ws_bytes(ctypes.byref(c), ctypes.byref(pg), q.shape[0])
-    if ws_bytes == 0:
-        check(-1)
-    ws = workspace.get(ws_bytes)
-    _same_device(dev, workspace=ws)
-    check(_on_device(dev, lib.g4a_paged_prefill, ctypes.byref(c), ctypes.byref(pg), q.shape[0], _ptr(cu_q), _ptr(q),
-                     _ptr(q_gain), _ptr(rope_cos), _ptr(rope_sin), _ptr(out), _ptr(ws), ws_bytes))
+    dev, qp, qg = _q(q, cfg, q_gain)
+    pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
+    cu, n = _cu(cu_q, pg.n_seq, dev), q.shape[0]
+    out = _out(out, q, out_dtype, dev)
+    c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0))
+    lib, at, p = _lib.load(), out.data_ptr(), ctypes.byref(pg)
+    _with_scratch(workspace, dev, lambda: lib.g4a_paged_prefill_ws_bytes(c, p, n),
+                  lambda ws, nb: _launch(dev, lib.g4a_paged_prefill, c, p, n, cu, qp, qg, rc, rs, at, ws, nb))
     return out
