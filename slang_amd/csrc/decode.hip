@@ -256,6 +256,50 @@ __device__ __forceinline__ ListUnit list_unit(const A& a, int chunk, int act0, i
     }
     return ListUnit{-1, 0, 0, 0};
 }
+
+// The plan over a paged cache: the same chunk and units from DPP sums and reciprocals, with no LDS
+// crossbar and no integer division (4 sequences of 300 keys 11.0 -> 10.5 us a call, 8 of up to 8200 at hd 512 25.5 -> 24.9).
+// n / d rounded up for n < 2^30 and quotients far below 2^22, whose f32 estimate is off by at most one.
+__device__ __forceinline__ int ceil_div_near(int n, int d, float rd) {
+    int q = (int)((float)n * rd);
+    q -= (q - 1) * d >= n ? 1 : 0;
+    q += q * d < n ? 1 : 0;
+    return q + (q * d < n ? 1 : 0);
+}
+__device__ __forceinline__ int list_chunk(const PagedDecodeArgs& a, int& act0) {
+    const int lane = threadIdx.x & 63;
+    float tot = 0.0f;
+    act0 = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        const int s = s0 + lane;
+        const int act = s < a.n_seq ? active_keys(a, seq_len(a, s)) : 0;
+        if (s0 == 0) act0 = act;
+        tot += (float)act;
+    }
+    // 2^-10 more than the share, which the f32 sum may have missed: the grid must hold every unit
+    const float share = wave_sum(tot) * (float)a.n_kv_heads * __builtin_amdgcn_rcpf((float)a.list_target) * (1.0f + 0x1p-10f);
+    const int c = ((int)fminf(share, 0x1p30f) + 16) & ~15;
+    return __builtin_amdgcn_readfirstlane(max(c, a.chunk));
+}
+__device__ __forceinline__ ListUnit list_unit(const PagedDecodeArgs& a, int chunk, int act0, int L) {
+    const float rc = __builtin_amdgcn_rcpf((float)chunk);
+    int base = 0;  // units of the sequences before this group of 64
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        const int sp = ceil_div_near(list_active(a, s0, act0, a.n_seq), chunk, rc);
+        const int incl = wave_scan(sp * a.n_kv_heads);
+        const unsigned long long past = __ballot(base + incl > L);
+        if (past) {
+            const int j = __builtin_ctzll(past);
+            const int splits = __builtin_amdgcn_readlane(sp, j);
+            const int r = L - (base + __builtin_amdgcn_readlane(incl, j) - splits * a.n_kv_heads);
+            // kh = r / splits, from ceil((r + 1) / splits) - 1
+            const int kh = __builtin_amdgcn_readfirstlane(ceil_div_near(r + 1, splits, __builtin_amdgcn_rcpf((float)splits)) - 1);
+            return ListUnit{s0 + j, kh, r - kh * splits, splits};
+        }
+        base += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return ListUnit{-1, 0, 0, 0};
+}
 // QP consecutive f32 (QP = 2 or 4) from a buffer
 template <int QP>
 __device__ __forceinline__ void bload_q(rsrc_t r, int off, float (&x)[QP]) {
@@ -825,6 +869,9 @@ static long longest_active(const g4a_cfg* cfg, int max_key_len, bool paged) {
 static int decode_chunk(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
     const long pairs = (long)n_seq * cfg->n_kv_heads;
     const long max_active = longest_active(cfg, max_key_len, paged);
+    // paged: few keys in one split per pair, without a merge (us a call, one split / many; kvH 2: 1 x 100 keys
+    // 7.4 / 8.2, 64 x 100 8.2 / 12.2, 1 x 300 11.4 / 8.2; kvH 1: 64 x 300 14.5 / 18.0, 64 x 512 19.9 / 20.0)
+    if (paged && (max_active <= 128 || (max_active <= 320 && pairs >= 64))) return (int)((max_active + 15) & ~15L);
     const long target = kDecodeTargetWgs;
     const long min_chunk = kDecodeMinChunk;
     const long kp = max_active * pairs;
@@ -956,7 +1003,7 @@ static int decode_setup(DecodeArgs& a, const g4a_cfg* cfg, int n_seq, int max_ke
         // byte offsets stay within 32 bits
         a.max_splits = 0;
         a.chunk = 64;
-        a.chunk_cap = (int)(((0x7fffffff / row_bytes) - 64) & ~15LL);
+        a.chunk_cap = paged ? 1 << 30 : (int)(((0x7fffffff / row_bytes) - 64) & ~15LL);  // (paged: offsets within a block)
         if (a.chunk_cap < a.chunk) {
             set_error("cache rows too large for 32-bit buffer offsets");
             return G4A_EINVAL;

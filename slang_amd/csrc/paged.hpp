@@ -25,6 +25,18 @@ __device__ __forceinline__ int page_at(const PageTab& t, int b, int p) {
     return t.table[(size_t)b * t.stride + (p >> t.shift)];
 }
 
+// Inclusive prefix sum over the 64 lanes on DPP row shifts and broadcasts (wave_prefix_sum without its six
+// trips through the LDS crossbar).
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    return x;
+}
+
 // rows of a 16-key block that lie in front of its end, n = end - block start, wave-uniform. (The clamp
 // is a vector instruction; left in a vector register it would make the buffer resource it enters look
 // divergent, and every load through it a loop over lanes.)

@@ -53,17 +53,6 @@ struct PagedPrefillArgs {
 };
 
 // ---------------------------------------------------------------- the work list
-// Inclusive prefix sum over the 64 lanes on DPP row shifts and broadcasts.
-__device__ __forceinline__ int wave_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);  // row_shr:1
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
-    return x;
-}
-
 // Key tiles of query block qb: keys [first & ~15, min(p0 + bq, start + S)).
 __device__ __forceinline__ int block_tiles(const PagedPrefillArgs& a, int start, int S, int qb) {
     const int p0 = start + qb * a.bq, hi = min(p0 + a.bq, start + S);
