@@ -16,6 +16,7 @@
 // f32 caches are first converted to f16 pages in the workspace (the rounding of prefill.hip's form
 // without G4A_Q_HILO), with a table of their own.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
 #include "prefill_tiles.hpp"
@@ -29,7 +30,9 @@ constexpr int kCus = 256;      // compute units of the MI355X; the kernels run o
 struct PagedUnit {
     int b, qb, kh, n_pieces;   // sequence, query block, kv head; pieces of the block
     int slot, t0, t1, row0;    // partial block of this piece (merge list: of the first); key tiles; packed row of the
-    int S, start, pad0, pad1;  // sequence's first token, its tokens in this call, the position of the first
+    int S, start;              // sequence's first token, its tokens in this call, the position of the first
+    int page[4];               // table entries of the first tile's 16-row groups
+    int pad0, pad1;
 };
 
 struct PagedPrefillArgs {
@@ -240,23 +243,30 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
     __syncthreads();
     for_blocks([&](int b, int s, int qb, int nt) {
         const int np = pieces(nt);
-        int at = atomicAdd(&s_bin[bin_of(nt, np)], np * a.n_kv_heads), slot = 0, mg = 0;
+        const int at = atomicAdd(&s_bin[bin_of(nt, np)], np * a.n_kv_heads);
+        int slot = 0, mg = 0;
         if (np > 1) {
             slot = atomicAdd(&s_slot, np * a.n_kv_heads);
             mg = atomicAdd(&s_merge, a.n_kv_heads);
         }
-        PagedUnit u{b, qb, 0, np, 0, 0, 0, s_lo[s], s_S[s], s_start[s], 0, 0};
-        for (int kh = 0; kh < a.n_kv_heads; ++kh) {
-            u.kh = kh;
-            for (int p = 0; p < np; ++p, ++at) {
-                u.slot = slot + kh * np + p;
-                u.t0 = (p * nt + np - 1) / np;
-                u.t1 = ((p + 1) * nt + np - 1) / np;
-                // (offsets out of order could list more blocks than there are packed rows: cut to the room)
-                if (at < a.max_units) a.units[at] = u;
+        PagedUnit u{b, qb, 0, np, 0, 0, 0, s_lo[s], s_S[s], s_start[s], {-1, -1, -1, -1}, 0, 0};
+        const int p0 = s_start[s] + qb * a.bq, key0 = a.window > 0 ? max(0, p0 + 1 - a.window) & ~15 : 0;
+        for (int p = 0; p < np; ++p) {
+            u.t0 = (p * nt + np - 1) / np;
+            u.t1 = ((p + 1) * nt + np - 1) / np;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // (a group past the table's columns has no rows)
+                const int col = (key0 + u.t0 * a.kt + 16 * i) >> a.t.shift;
+                u.page[i] = nt > 0 && col < a.t.cols ? a.t.table[(size_t)b * a.t.stride + col] : -1;
             }
-            u.slot = slot + kh * np;
-            if (np > 1) a.merges[mg + kh] = u;
+            for (int kh = 0; kh < a.n_kv_heads; ++kh) {
+                u.kh = kh;
+                u.slot = slot + kh * np + p;
+                const int i = at + kh * np + p;
+                // (offsets out of order could list more blocks than there are packed rows: cut to the room)
+                if (i < a.max_units) a.units[i] = u;
+                if (np > 1 && p == 0) a.merges[mg + kh] = u;
+            }
         }
     });
     __syncthreads();
@@ -451,8 +461,13 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(qs + (32 * wave + 2 * j) * ROWB),
                                                      16, qo, 0, 0, 0);
         }
-        entry1 = __builtin_amdgcn_readlane(pages.entry, 0);
-        gone0 = __builtin_amdgcn_readlane(pages.gone, 0);
+        entry1 = wu.page[0];  // this wave's group
+        gone0 = 0;
+#pragma unroll
+        for (int i = 0; i < KT / 16; ++i) {
+            entry1 = i == wave ? wu.page[i] : entry1;
+            gone0 |= page_ok(a.t, wu.page[i]) ? 0 : 1 << i;
+        }
         if (t0 < t1) {  // tile t0: of the block's first tile, rows in front of the first attended key read as zeros
             const rsrc_t rk = tile_rows(a.kc, t0, entry1), rv = tile_rows(a.vc, t0, entry1);
             const int skip = first - (wg_lo + t0 * KT + 16 * wave);
@@ -699,14 +714,18 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
         constexpr int OSTR = HD * 2 + 16;
         __syncthreads();  // every wave is done with the last tile's K/V
         char* ost = lds + wave * 32 * OSTR;
+        auto stage = [&](auto quantise) {  // (one test of the step for all of them)
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt)
+            for (int dt = 0; dt < 8; ++dt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2],
-                                          oacc[dt][4 * j + 3]} * inv;
-                store4(reinterpret_cast<half_t*>(ost + n32 * OSTR) + 32 * dt + 8 * j + 4 * h, srq4(v, a.out_q));
-            }
+                for (int j = 0; j < 4; ++j) {
+                    float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]} * inv;
+                    if constexpr (decltype(quantise)::value) v = srq4(v, a.out_q);
+                    store4(reinterpret_cast<half_t*>(ost + n32 * OSTR) + 32 * dt + 8 * j + 4 * h, v);
+                }
+        };
+        if (a.out_q == 0.0f) stage(std::false_type{});
+        else stage(std::true_type{});
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int rr = 2 * i + h, cc = 32 * wave + rr;  // lanes 32h..: the wave's row rr
@@ -774,7 +793,7 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
         int ln = lane;
         asm volatile("" : "+v"(ln));
         const int kg = wg_lo + t * KT + 16 * (wave >> 1);  // the 16 rows that this wave's 8 belong to
-        const int entry = __builtin_amdgcn_readlane(pages.entry, (t - t0) & 63);
+        const int entry = t == t0 ? (wave >> 1 ? wu.page[1] : wu.page[0]) : __builtin_amdgcn_readlane(pages.entry, (t - t0) & 63);
         const rsrc_t pk = page_rows(a.t, a.kc, entry, kg, kv_hi, rowg / 2, kh * HD);
         const rsrc_t pv = page_rows(a.t, a.vc, entry, kg, kv_hi, rowg / 2, kh * HD);
 #pragma unroll
@@ -995,14 +1014,18 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
         // an instruction
         __syncthreads();  // every wave is done with the last tile's K/V
         char* ost = lds + wave * 32 * OSTR;
+        auto stage = [&](auto quantise) {  // (one test of the step for all of them)
 #pragma unroll
-        for (int dt = 0; dt < 16; ++dt)
+            for (int dt = 0; dt < 16; ++dt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2],
-                                          oacc[dt][4 * j + 3]} * inv;
-                store4(reinterpret_cast<half_t*>(ost + n32 * OSTR) + 32 * dt + 8 * j + 4 * h, srq4(v, a.out_q));
-            }
+                for (int j = 0; j < 4; ++j) {
+                    float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]} * inv;
+                    if constexpr (decltype(quantise)::value) v = srq4(v, a.out_q);
+                    store4(reinterpret_cast<half_t*>(ost + n32 * OSTR) + 32 * dt + 8 * j + 4 * h, v);
+                }
+        };
+        if (a.out_q == 0.0f) stage(std::false_type{});
+        else stage(std::true_type{});
 #pragma unroll
         for (int rr = 0; rr < 32; ++rr) {
             const int cc = 32 * wave + rr, so = qb * BQ + cc / G;
@@ -1245,19 +1268,18 @@ extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_
         k.window = a.window;
         hipLaunchKernelGGL(paged_kv16_kernel, dim3((unsigned)((pg->max_key_len + 15) / 16), pg->n_seq), dim3(256), 0, stream, k);
         if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged cache conversion launch");
-    }
-    const int64_t rows = (int64_t)n_tokens * ((a.n_q_heads + 3) / 4);  // waves, each four heads of a token
-    const dim3 pgrid((unsigned)((rows + 3) / 4 + 1));
-    if (HD == 256) hipLaunchKernelGGL(paged_prep_kernel<256>, pgrid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(paged_prep_kernel<512>, pgrid, dim3(256), 0, stream, a);
-    if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged prefill preparation launch");
-    if (cfg->flags & G4A_KV_F32) {  // from here on the f16 copy
+        // from here on the f16 copy and its table
         a.kc = w + p.k16;
         a.vc = w + p.v16;
         a.t.table = (const int32_t*)(w + p.tab16);
         a.t.cols = a.t.stride = p.cols16;
         a.t.n_pages = pg->n_seq * p.cols16;
     }
+    const int64_t rows = (int64_t)n_tokens * ((a.n_q_heads + 3) / 4);  // waves, each four heads of a token
+    const dim3 pgrid((unsigned)((rows + 3) / 4 + 1));
+    if (HD == 256) hipLaunchKernelGGL(paged_prep_kernel<256>, pgrid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(paged_prep_kernel<512>, pgrid, dim3(256), 0, stream, a);
+    if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged prefill preparation launch");
     const bool out32 = (cfg->flags & G4A_OUT_F32) != 0;
     const paged_prefill_fn fn = pick_paged(HD, G, out32);
     if (!fn) {
