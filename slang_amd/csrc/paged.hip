@@ -76,20 +76,25 @@ __global__ __launch_bounds__(HD / 2) void paged_write_kernel(PagedWriteArgs a) {
     constexpr int HALF = HD / 2, NW = HALF / 64;
     __shared__ float red[2 * NW];
     const int t = threadIdx.x, tok = blockIdx.x, kh = blockIdx.y;
-    // the raw row first: it depends on nothing, so its trip to memory runs beside the search's
+    int b = tok, p;  // without cu, row b is sequence b's last key
+    if (a.cu) {
+        b = seq_of_row(a.cu, a.t.n_seq, tok);
+        if (b >= a.t.n_seq) return;
+        const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
+        if (tok < r.lo || tok >= r.hi) return;
+        p = r.keys - r.hi + tok;
+    } else {
+        p = paged_len(a.t, b) - 1;
+    }
+    if (p < 0) return;
+    const int page = page_at(a.t, b, p);
+    if (!page_ok(a.t, page)) return;
     const size_t row = ((size_t)tok * a.n_kv_heads + kh) * HD;
     const IT* kin = reinterpret_cast<const IT*>(a.k) + row;
     const IT* vin = reinterpret_cast<const IT*>(a.v) + row;
-    const IT kr0 = kin[t], kr1 = kin[t + HALF], vr0 = vin[t], vr1 = vin[t + HALF];
-    // without cu, row b is sequence b's last key
-    const TokenAt at = a.cu ? token_at(a.t, a.cu, a.n_tokens, tok) : TokenAt{tok, paged_len(a.t, tok) - 1};
-    const int p = at.p;
-    if (at.b < 0 || p < 0) return;
-    const int page = page_at(a.t, at.b, p);
-    float k0 = (float)kr0, k1 = (float)kr1, v0 = (float)vr0, v1 = (float)vr1;
+    float k0 = (float)kin[t], k1 = (float)kin[t + HALF], v0 = (float)vin[t], v1 = (float)vin[t + HALF];
     kv_pair_prep<HD>(k0, k1, v0, v1, a.k_gain, a.rcos ? a.rcos + (size_t)p * HALF : nullptr,
                      a.rsin ? a.rsin + (size_t)p * HALF : nullptr, a.v_norm != 0, a.eps, a.k_in_q, a.v_in_q, red, t);
-    if (!page_ok(a.t, page)) return;
     const size_t crow = paged_row(a.t, page, p, a.n_kv_heads * HD) + (size_t)kh * HD;
     CT* kc = reinterpret_cast<CT*>(a.kc) + crow;
     CT* vc = reinterpret_cast<CT*>(a.vc) + crow;

@@ -60,31 +60,18 @@ __device__ __forceinline__ SeqRows seq_rows(const PageTab& t, const int32_t* cu,
     return r;
 }
 
-// The sequence and position of packed row `tok` (b < 0: a row of nobody): b is how many sequences end at or
-// before it (cu ascends), 64 offsets and lengths a load, so one memory round trip finds both for up to
-// 64 sequences. Every lane of the wave must call it; the result is wave-uniform.
-struct TokenAt {
-    int b, p;
-};
-__device__ __forceinline__ TokenAt token_at(const PageTab& t, const int32_t* cu, int n_tokens, int tok) {
+// The sequence of packed row `tok`: how many sequences end at or before it, 64 offsets a load
+// (cu ascends). n_seq: a row behind the last sequence. Every lane of the wave must call it.
+__device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int tok) {
     const int lane = threadIdx.x & 63;
-    int before = cu[0];  // offset of the first sequence of this group of 64
-    for (int s0 = 0; s0 < t.n_seq; s0 += 64) {
-        const int s = min(s0 + lane, t.n_seq - 1);
-        const int end = cu[s + 1], len = t.key_len[s];
-        const unsigned long long later = __ballot(s0 + lane < t.n_seq && end > tok);
-        if (later) {
-            const int j = __builtin_ctzll(later);
-            const int lo = j > 0 ? __builtin_amdgcn_readlane(end, j > 0 ? j - 1 : 0) : before;
-            const int hi = __builtin_amdgcn_readlane(end, j), keys = __builtin_amdgcn_readlane(len, j);
-            // seq_rows' bounds
-            const int l = min(max(lo, 0), n_tokens), h = min(max(hi, l), n_tokens);
-            if (tok < l || tok >= h) return TokenAt{-1, 0};
-            return TokenAt{s0 + j, min(max(keys, 0), t.max_len) - h + tok};
-        }
-        before = __builtin_amdgcn_readlane(end, 63);
+    int b = 0;
+    for (int s0 = 0; s0 < n_seq; s0 += 64) {
+        const int s = s0 + lane;
+        const unsigned long long m = __ballot(s < n_seq && cu[s < n_seq ? s + 1 : 0] <= tok);
+        b += __builtin_popcountll(m);
+        if (m != ~0ull) break;
     }
-    return TokenAt{-1, 0};
+    return b;
 }
 
 // checks of a g4a_paged and the config that goes with it; 0 or the error code (g4a_last_error set)

@@ -294,9 +294,10 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(PagedPrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < NH; ++i) x[i] = *reinterpret_cast<const vec_t*>(qr + (h0 + i < a.n_q_heads ? i * HD : 0));
     if (a.q_gain) gv = *reinterpret_cast<const vec_t*>(a.q_gain + E * lane);
-    const TokenAt at = token_at(a.t, a.cu, a.n_tokens, tok);
-    if (at.b < 0) return;  // a row of nobody
-    const int p = max(at.p, 0);
+    const int b = seq_of_row(a.cu, a.t.n_seq, tok);
+    if (b >= a.t.n_seq) return;  // a row of nobody
+    const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
+    const int p = max(r.keys - r.hi + tok, 0);
     vec_t c, sn;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
