@@ -214,7 +214,7 @@ int g4a_kv_write(const g4a_cfg* cfg, int S, int start_pos, const void* k, const 
  *               table_cols * page_size; sizes the workspaces and the grids.
  * Packed tokens: sequence b's rows of the packed inputs are cu_q[b] .. cu_q[b + 1] - 1 (cu_q
  * int32 [n_seq + 1], device, ascending from 0), at positions key_len[b] - (cu_q[b + 1] - cu_q[b])
- * .. key_len[b] - 1. Rows from cu_q[n_seq] on belong to nobody: they are not read, and their
+ * .. key_len[b] - 1. Rows from cu_q[n_seq] on belong to nobody: nothing is stored for them, and their
  * outputs are left as they were. A token at a position below zero attends nothing (zeros).
  * RoPE tables: f32 [max_key_len][head_dim / 2] at least, indexed by absolute position.
  * Two rows of one call that map to the same cache row (a page listed twice) must not be written.

@@ -11,7 +11,7 @@ sequences of unknown length keeps their rows in pages instead:
     its positions are neither written nor attended (-1 for pages behind a sliding window);
   * ``key_len`` int32 [n_seq]: the keys of each sequence, this call's tokens included; 0 = idle;
   * ``cu_q`` int32 [n_seq + 1]: packed rows cu_q[b] .. cu_q[b+1]-1 are sequence b's tokens, its last
-    ones. Rows from cu_q[n_seq] on belong to nobody: not read, their outputs left as they were;
+    ones. Rows from cu_q[n_seq] on belong to nobody: nothing is stored for them, their outputs stay;
   * ``rope_cos`` / ``rope_sin`` f32 [>= max_key_len][hd/2]: ``rope_tables`` over absolute positions.
 
 All of these live on one GPU, so lengths and tables can change between replays of a captured
