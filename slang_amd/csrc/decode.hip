@@ -1227,9 +1227,20 @@ extern "C" int g4a_decode_noalloc(const g4a_cfg* cfg, int n_seq, int max_key_len
 }
 
 // ---------------------------------------------------------------- a paged cache
+// A server reserves one workspace for its largest batch and runs smaller ones in it, so the size must not
+// fall with n_seq or max_key_len, as the plan's own slots do (8 times at worst): no plan has more than
+// kDecodeTargetWgs + pairs of them (the list's max(resident, resident / 2 + pairs), one sequence's
+// n_kv_heads * splits).
+static size_t paged_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg) {
+    const size_t pairs = (size_t)pg->n_seq * cfg->n_kv_heads, G = cfg->n_q_heads / cfg->n_kv_heads;
+    const size_t rows = (kDecodeTargetWgs + pairs) * G;
+    auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    return al(rows * sizeof(float2)) + al(rows * cfg->head_dim * sizeof(float)) + pairs * sizeof(int2);
+}
+
 extern "C" size_t g4a_paged_decode_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg) {
     if (check_paged(cfg, pg, true)) return 0;
-    return ws_layout(cfg, pg->n_seq, pg->max_key_len, true).total;
+    return paged_ws_bytes(cfg, pg);
 }
 
 extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, const float* q_gain,
@@ -1251,7 +1262,7 @@ extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const f
         set_error("k_new, v_new and k_gain must be 16-byte aligned");
         return G4A_EINVAL;
     }
-    const size_t need = ws_layout(cfg, pg->n_seq, pg->max_key_len, true).total;
+    const size_t need = paged_ws_bytes(cfg, pg);
     if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
         set_error("paged decode workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
         return G4A_EWORKSPACE;

@@ -1145,7 +1145,9 @@ static paged_prefill_fn pick_paged_merge(int HD, bool out32) {
 }
 
 // What the host can bound: query blocks (each sequence's last one may be short), units and partials; and
-// the workspace [counts][units][merges][q16][partials][(m, l)][K16][V16][table16].
+// the workspace [counts][units][merges][q16][partials][(m, l)][K16][V16][table16]. A server reserves one
+// for its largest call and runs smaller ones in it, so every part grows with n_tokens, n_seq and
+// max_key_len: there is room for partials also in a call too large to split.
 struct PagedPlan {
     int bq, kt, max_units, max_slots, cols16;
     size_t units, merges, q16, part_o, part_ml, k16, v16, tab16, total;
@@ -1163,7 +1165,8 @@ static bool paged_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, Pa
     const double longest = (double)((keys + p.kt - 1) / p.kt) + pc.unit;
     const double load = (double)(n_tokens / p.bq) * (double)kvh * (1.0 + pc.unit) / kCus;
     const bool split = longest > load;
-    p.max_slots = split ? (int)std::min<int64_t>(blocks * kvh * kMaxPieces, kMaxSlots) : 0;
+    const int slots = (int)std::min<int64_t>(blocks * kvh * kMaxPieces, kMaxSlots);
+    p.max_slots = split ? slots : 0;
     const int64_t units = blocks * kvh + p.max_slots;
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     size_t at = 256;
@@ -1173,11 +1176,11 @@ static bool paged_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, Pa
         return x;
     };
     p.max_units = (int)units;
-    p.units = part((size_t)units * sizeof(PagedUnit));
-    p.merges = part((size_t)p.max_slots * sizeof(PagedUnit));
+    p.units = part((size_t)(blocks * kvh + slots) * sizeof(PagedUnit));
+    p.merges = part((size_t)slots * sizeof(PagedUnit));
     p.q16 = part((size_t)n_tokens * cfg->n_q_heads * HD * sizeof(half_t));
-    p.part_o = part((size_t)p.max_slots * 128 * HD * 3);
-    p.part_ml = part((size_t)p.max_slots * 128 * sizeof(float2));
+    p.part_o = part((size_t)slots * 128 * HD * 3);
+    p.part_ml = part((size_t)slots * 128 * sizeof(float2));
     p.k16 = p.v16 = p.tab16 = at;
     p.cols16 = 0;
     int64_t pages16 = 0;

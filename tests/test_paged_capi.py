@@ -134,6 +134,19 @@ def test_workspace_sizes(lib):
         sa.paged_prefill_ws_bytes(0, 16, 4096, c, page_size=64)
 
 
+@pytest.mark.parametrize("kvh,hd,window", [(1, 256, 512), (2, 256, 0), (8, 256, 0), (2, 512, 0), (1, 512, 4096)])
+@pytest.mark.parametrize("kv_f32", [False, True])
+def test_a_workspace_holds_every_smaller_call(kvh, hd, window, kv_f32):
+    """Sizes grow with tokens, sequences and the bound of the keys: one reserved for the largest call does."""
+    c, kw = sa.AttnConfig(8, kvh, hd, window), dict(page_size=16, kv_f32=kv_f32)
+    seqs, keys = [1, 2, 3, 7, 16, 33, 64, 65, 200, 300, 1000, 4000], [1, 16, 128, 129, 320, 321, 600, 4096, 8192, 30000, 131072]
+    tokens = [1, 5, 33, 100, 1000, 3000, 10000, 30000, 100000]
+    dec = np.array([[sa.paged_decode_ws_bytes(n, k, c, **kw) for k in keys] for n in seqs])
+    assert (np.diff(dec, axis=0) >= 0).all() and (np.diff(dec, axis=1) >= 0).all()
+    pre = np.array([[[sa.paged_prefill_ws_bytes(t, n, k, c, **kw) for k in keys] for n in seqs] for t in tokens])
+    assert all((np.diff(pre, axis=i) >= 0).all() for i in range(3))
+
+
 def test_oracle_keys():
     """The definition's attended positions: window, missing pages, positions below zero."""
     table = np.array([[3, -1, 7, 100]], np.int32)
