@@ -16,7 +16,7 @@ host: when libg4attn.so is missing, the first call raises.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 
 import numpy as np
 import torch
@@ -52,6 +52,9 @@ class AttnConfig:
         if ref is None:
             ref = self.__dict__[flags] = ctypes.byref(self.c(flags))
         return ref
+
+    def __getstate__(self):  # the fields alone: a ctypes reference can be neither copied nor pickled
+        return {f.name: getattr(self, f.name) for f in fields(self)}
 
 
 # The short calls are bound by this layer, not by their kernels, so it wraps and unwraps nothing

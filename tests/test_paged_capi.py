@@ -1,5 +1,8 @@
 """CPU checks of the paged cache's entry points: struct layout, refusals before anything runs."""
+import copy
 import ctypes
+import dataclasses
+import pickle
 
 import numpy as np
 import pytest
@@ -121,6 +124,14 @@ def test_host_refusals_without_a_gpu():
                  lambda: sa.paged_decode(q[:, :4], pages, pages, tab, kl, c)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_used_configs_are_copied_and_pickled():
+    c = sa.AttnConfig(8, 2, 256, window=100, scale=0.5)
+    c.c_ref(3)
+    for x in (copy.copy(c), copy.deepcopy(c), pickle.loads(pickle.dumps(c)), dataclasses.replace(c)):
+        assert x == c and hash(x) == hash(c) and x.c(3).window == 100
+        assert ctypes.cast(x.c_ref(3), ctypes.POINTER(G4ACfg)).contents.scale == 0.5
 
 
 def test_workspace_sizes(lib):
