@@ -86,9 +86,11 @@ def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_co
                          f"{tuple(shape)} and {tuple(v_pages.shape)}")
     if kv not in _HALF_OR_FLOAT or v_pages.dtype is not kv:
         raise ValueError("k/v pages must both be float16 or both float32")
-    if page_table.get_device() != dev or page_table.dtype is not _I32 or page_table.dim() != 2 or page_table.stride(1) != 1:
-        raise ValueError(f"page_table must be an int32 tensor [n_seq][cols] on cuda:{dev} with adjacent columns")
+    if page_table.get_device() != dev or page_table.dtype is not _I32 or page_table.dim() != 2:
+        raise ValueError(f"page_table must be an int32 tensor [n_seq][cols] on cuda:{dev}")
     n_seq, cols = page_table.shape
+    if cols > 1 and page_table.stride(1) != 1:
+        raise ValueError("page_table's columns must be adjacent")
     stride = page_table.stride(0) if n_seq > 1 else cols
     if stride < cols:
         raise ValueError("page_table rows must not overlap")
@@ -163,7 +165,7 @@ def paged_write(k, v, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConf
     c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.IN_F16 if rows is _F16 else 0) |
                   (0 if v_norm else _lib.NO_V_NORM))
     check(_launch(dev, _lib.load().g4a_paged_write, c, ctypes.byref(pg), k.shape[0], _cu(cu_q, pg.n_seq, dev),
-                  _t("k", k, dev, rows), _t("v", v, dev, rows), k_in_q, v_in_q, _t("k_gain", k_gain, dev, _F32), rc, rs))
+                  _t("k", k, dev, rows), _t("v", v, dev, rows), float(k_in_q), float(v_in_q), _t("k_gain", k_gain, dev, _F32), rc, rs))
 
 
 def _out(out, q, out_dtype, dev):
@@ -223,6 +225,7 @@ def paged_decode(q, k_pages, v_pages, page_table, key_len, cfg: AttnConfig, *, w
         if k_new.shape != (pg.n_seq, cfg.n_kv_heads, cfg.head_dim) or v_new.shape != k_new.shape:
             raise ValueError(f"k_new and v_new must be [{pg.n_seq}][{cfg.n_kv_heads}][{cfg.head_dim}]")
     out = _out(out, q, out_dtype, dev)
+    k_in_q, v_in_q = float(k_in_q), float(v_in_q)
     c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0) |
                   (0 if v_norm else _lib.NO_V_NORM))
     lib, at, p = _lib.load(), out.data_ptr(), ctypes.byref(pg)

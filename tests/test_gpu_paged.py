@@ -363,6 +363,21 @@ def test_table_rows_apart():
     check(prefill(b, d).cpu().numpy(), out, bound(out, A, S, q16=True, kv32=False, out16=True))
 
 
+def test_numbers_and_tables_of_other_kinds():
+    """Steps as numpy numbers; a single column taken out of a transposed table."""
+    b = Batch([80, 50], [1, 1], page=128, extra_cols=0)
+    d, ref = b.dev(), b.dev()
+    column = torch.stack([ref["table"][:, 0], ref["table"][:, 0]]).t()[:, :1]
+    assert column.shape == (2, 1) and column.stride(1) != 1
+    steps = dict(k_in_q=np.float32(0.03), v_in_q=np.float32(0.05))
+    plain = {n: float(v) for n, v in steps.items()}
+    write(b, dict(d, table=column), **steps)
+    write(b, ref, **plain)
+    assert np.array_equal(bits(d["k_pages"]), bits(ref["k_pages"])) and np.array_equal(bits(d["v_pages"]), bits(ref["v_pages"]))
+    assert torch.equal(decode(b, dict(d, table=column), True, **steps), decode(b, ref, True, **plain))
+    assert torch.equal(prefill(b, dict(d, table=column)), prefill(b, ref))
+
+
 @pytest.mark.parametrize("hd,kvh", [(256, 2), (512, 1)])
 def test_captured_steps(hd, kvh):
     """Write, prefill and decode captured once and replayed on new lengths, tables and rows, with
