@@ -475,9 +475,9 @@ void decode_kernel(A a) {
             const size_t at = paged_row(a.t, ok ? blk_page : 0, blk, (int)rstride) + (size_t)kh * HD;
             const rsrc_t pk = make_rsrc(reinterpret_cast<const KVT*>(a.kc) + at, bytes);
             const rsrc_t pv = make_rsrc(reinterpret_cast<const KVT*>(a.vc) + at, bytes);
-            // rows in front of the first attended key: an offset past every range (and with room for
-            // the second half of an f32 load)
-            const auto off = [&](int row, int o) { return blk + row < key_lo ? 0x7fffff00 : o; };
+            // rows in front of the first attended key: an offset past every range (128 MiB at most), with
+            // room for the second half of an f32 load
+            const auto off = [&](int row, int o) { return blk + row < key_lo ? 0x7fff0000 : o; };
             if constexpr (KROW) {
 #pragma unroll
                 for (int i = 0; i < VLOADS; ++i) krow[i] = bload_h8_nt(pk, off(VROWS * i + vrow, VROWS * i * rsb + voff));

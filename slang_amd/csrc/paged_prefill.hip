@@ -390,7 +390,7 @@ __device__ __forceinline__ rsrc_t page_rows(const PageTab& t, const void* pool, 
     const uint32_t bytes = ok ? (uint32_t)(clamp16(kv_hi - k0) * row * 2) : 0u;
     return make_rsrc(reinterpret_cast<const half_t*>(pool) + paged_row(t, ok ? entry : 0, k0, row) + kh_off, bytes);
 }
-constexpr int kNoRow = 0x7fffff00;  // an offset past every such range, with room for a row's own bytes
+constexpr int kNoRow = 0x7fff0000;  // an offset past every such range (64 MiB at most), with room for a row's own bytes
 
 // ---------------------------------------------------------------- hd 256
 // 32 query columns a wave, 128 a workgroup, key tiles of 64 moved straight into LDS and double
@@ -800,7 +800,7 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int r = 8 * wave + j, rg = 8 * (wave & 1) + j;
-            const int so = kg + rg >= first ? rg * rowg : kNoRow;  // (past the range: lanes add 1 KiB at most)
+            const int so = kg + rg >= first ? rg * rowg : kNoRow;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(pk, (__attribute__((address_space(3))) void*)(kdst + r * ROWB), 16,
                                                      so + 16 * (ln ^ (r & 31)), 0, 0, 0);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(pv, (__attribute__((address_space(3))) void*)(kdst + TILEB + r * ROWB),
