@@ -48,7 +48,7 @@ __device__ __forceinline__ size_t paged_row(const PageTab& t, int page, int p, i
 }
 
 // the packed rows [lo, hi) of sequence b and its keys: row lo + i is the token at position
-// keys - (hi - lo) + i. Offsets outside [0, n_tokens] or out of order are cut to it.
+// keys - (hi - lo) + i. Offsets outside [0, n_tokens] are cut to it, one below its predecessor to that.
 struct SeqRows {
     int lo, hi, keys;
 };

@@ -109,11 +109,15 @@ __device__ __forceinline__ void ramp_sums(SplitSums& t, float u, float v, float 
 __device__ void plan_units(const PagedPrefillArgs& a) {
     __shared__ int s_lo[kPlanThreads], s_S[kPlanThreads], s_start[kPlanThreads], s_blk[kPlanThreads + 1];
     __shared__ int s_wave[kPlanThreads / 64], s_max, s_cut, s_bin[kBins], s_slot, s_merge;
+    __shared__ float s_blocks;
     __shared__ float s_sum[kMaxPieces + 1][7];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int chunks = (a.t.n_seq + kPlanThreads - 1) / kPlanThreads;
     if (tid < kBins) s_bin[tid] = 0;
-    if (tid == 0) s_max = s_cut = s_slot = s_merge = 0;
+    if (tid == 0) {
+        s_max = s_cut = s_slot = s_merge = 0;
+        s_blocks = 0.0f;
+    }
 
     // the sequences c * kPlanThreads .. into LDS, with the prefix sum of their query blocks
     auto load_chunk = [&](int c) {
@@ -159,9 +163,19 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
         if (nb > 0) mx = block_tiles(a, s_start[tid], s_S[tid], nb - 1);
         if (nb > 1) mx = max(mx, block_tiles(a, s_start[tid], s_S[tid], nb - 2));
         mx = (int)wave_max((float)mx);  // (at most 2^25 tiles)
-        if (lane == 0) atomicMax(&s_max, mx);
+        const float blocks = wave_sum((float)((s_S[tid] + a.bq - 1) / a.bq));
+        if (lane == 0) {
+            atomicMax(&s_max, mx);
+            atomicAdd(&s_blocks, blocks);
+        }
     }
     __syncthreads();
+    // Ascending offsets make no more blocks than this. Others can list the packed rows once a sequence, more
+    // than the sums below can count: no block runs then
+    if (s_blocks > 1.01f * ((float)a.n_tokens / (float)a.bq + (float)a.t.n_seq) + 64.0f) {
+        if (tid == 0) a.counts[0] = a.counts[1] = 0;
+        return;
+    }
     const int longest = s_max;
     const int st_min = a.kt == 64 ? 2 : 4;  // tiles a piece at least
     const auto cut = [&](int k) { return max((longest + k - 1) / k, k == 1 ? 1 : st_min); };

@@ -263,6 +263,23 @@ def test_prefill_more_rows_than_keys():
     check(got2.cpu().numpy(), out, bound(out, A, S, q16=True, kv32=False, out16=True))
 
 
+@pytest.mark.parametrize("hd", [256, 512])
+@pytest.mark.parametrize("n_seq", [3, 300])
+def test_prefill_offsets_that_do_not_ascend(hd, n_seq):
+    """Whatever the offsets, the cache stays, rows behind the packed ones stay, and a later call is right."""
+    b = Batch([700, 640], [640, 20], hd=hd, kvh=1, pad=9)
+    d = b.dev()
+    cu = [0] + [(660, 0)[i % 2] for i in range(n_seq)]
+    o = torch.full((b.T + 4, 8, hd), 7.25, dtype=torch.float16, device="cuda")
+    w = ws()
+    prefill(b, dict(d, table=d["table"][:1].repeat(n_seq, 1), key_len=d["key_len"][:1].repeat(n_seq),
+                    cu=torch.tensor(cu, dtype=torch.int32, device="cuda")), out=o[:b.T], workspace=w)
+    assert np.array_equal(bits(d["k_pages"]).reshape(-1), b.k_pages.reshape(-1).view(np.uint8))
+    assert (o[660:] == 7.25).all()
+    out, A, S = b.oracle()
+    check(prefill(b, d, workspace=w).cpu().numpy()[:660], out[:660], bound(out, A, S, q16=True, kv32=False, out16=True)[:660])
+
+
 def test_prefill_options():
     b = Batch([60, 33], [60, 9], kvh=4)
     out, A, S = b.oracle(gain=False, rope=False, scale=0.0625)
