@@ -1262,6 +1262,14 @@ extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const f
         set_error("k_new, v_new and k_gain must be 16-byte aligned");
         return G4A_EINVAL;
     }
+    // a pair's output may be written before another's row is read
+    const size_t rows = (size_t)pg->n_seq * cfg->head_dim, osz = (cfg->flags & G4A_OUT_F32) ? 4 : 2;
+    for (const float* x : {k_new, v_new})
+        if (x && (uintptr_t)x < (uintptr_t)out + rows * cfg->n_q_heads * osz &&
+            (uintptr_t)out < (uintptr_t)x + rows * cfg->n_kv_heads * sizeof(float)) {
+            set_error("out must not overlap k_new or v_new");
+            return G4A_EINVAL;
+        }
     const size_t need = paged_ws_bytes(cfg, pg);
     if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
         set_error("paged decode workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);

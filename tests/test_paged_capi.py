@@ -96,6 +96,9 @@ def test_decode_refusals(lib):
     assert decode(lib, kn=FAKE, vn=FAKE, ks=-0.5) == E
     assert decode(lib, c=cfg(flags=_lib.IN_F16)) == U
     assert decode(lib, out=FAKE) == E  # over q
+    far = 0x8000000
+    assert decode(lib, q=far, kn=0x4000000, vn=far + 0x10000) == E and decode(lib, q=far, kn=far + 0x10000, vn=0x4000100) == E
+    assert b"k_new" in lib.g4a_last_error()
     assert decode(lib, ws=None) == W and decode(lib, ws=FAKE + 16) == W and decode(lib, n=16) == W
     assert b"workspace" in lib.g4a_last_error()
     assert lib.g4a_paged_decode_ws_bytes(ctypes.byref(cfg()), ctypes.byref(paged())) > 0
