@@ -463,6 +463,126 @@ def test_two_streams():
             check(x.cpu().numpy(), out, bound(out, A, S, q16=True, kv32=False, out16=True))
 
 
+def test_two_graphs_share_a_workspace():
+    """A prefill and a decode captured over one workspace, replayed in turn."""
+    b = Batch([1300, 60], [40, 60])
+    d = b.dev()
+    w = sa.Workspace().reserve(max(sa.paged_decode_ws_bytes(2, MAX, b.cfg(), page_size=16),
+                                   sa.paged_prefill_ws_bytes(b.T, 2, MAX, b.cfg(), page_size=16)))
+    qd = d["q"][:2].contiguous()
+    outs = [torch.zeros(b.T, 8, 256, dtype=torch.float16, device="cuda"), torch.zeros(2, 8, 256, dtype=torch.float16, device="cuda")]
+    calls = [lambda: prefill(b, d, workspace=w, out=outs[0]), lambda: decode(b, dict(d, q=qd), workspace=w, out=outs[1])]
+    graphs, stream = [torch.cuda.CUDAGraph() for _ in calls], torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        for g, call in zip(graphs, calls):
+            call()
+            stream.synchronize()
+            with torch.cuda.graph(g, stream=stream):
+                call()
+        want = []
+        for call, o in zip(calls, outs):
+            call()
+            want.append(o.clone())
+        for i in range(6):
+            for o in outs:
+                o.zero_()
+            for g in graphs[::1 if i % 2 else -1]:
+                g.replay()
+            stream.synchronize()
+            assert all(torch.equal(o, x) for o, x in zip(outs, want)), f"replay {i}"
+
+
+# ---------------------------------------------------------------- many sequences, long ones
+def sparse_oracle(b, rows, **kw):
+    """The oracle at some of the packed rows, and those rows."""
+    toks = [t if i in rows else None for i, t in enumerate(b.tokens())]
+    out, A, S = b.oracle(tokens=toks, **kw)
+    return [x[list(rows)] for x in (out, A, S)]
+
+
+@pytest.mark.parametrize("hd,keys", [(256, 40000), (512, 24000)])
+def test_prefill_history_of_many_tiles(hd, keys):
+    """A piece of a block walks more than 64 key tiles. (scale 0.25: weights within 2^13 of each other, so
+    that no weight is subnormal and the bound's terms hold for any number of keys.)"""
+    b = Batch([keys, 70], [37, 70], hd=hd, kvh=1, page=64, missing=[(0, 5), (0, keys // 64 - 30)])
+    rows = (0, 1, 17, 36, 37, 106)
+    out, A, S = sparse_oracle(b, rows, rope=False, scale=0.25)
+    got = prefill(b, b.dev(), rope_cos=None, rope_sin=None, cfg=b.cfg(scale=0.25)).cpu().numpy()[list(rows)]
+    check(got, out, bound(out, A, S, q16=True, kv32=False, out16=True))
+
+
+@pytest.mark.parametrize("hd", [256, 512])
+def test_prefill_blocks_of_many_tiles(hd):
+    """So many tokens that no block is cut: the longest walk more than 64 tiles whole."""
+    kt = 64 if hd == 256 else 32
+    n, new = 30, 4000
+    b = Batch([70 * kt], [1], hd=hd, kvh=1, page=64)
+    q = torch.randn(n * new, 8, hd, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    key_len = torch.tensor([70 * kt - i for i in range(n)], dtype=torch.int32, device="cuda")
+    new_i = [min(new, int(k)) for k in key_len]
+    cu = np.concatenate([[0], np.cumsum(new_i)]).astype(np.int32)
+    d = b.dev()
+    out = prefill(b, dict(d, q=q, table=d["table"].repeat(n, 1), key_len=key_len, cu=torch.from_numpy(cu).cuda()),
+                  rope_cos=None, rope_sin=None, cfg=b.cfg(scale=0.25))
+    rows = [int(cu[s + 1]) - back for s in (0, 13, n - 1) for back in (1, 2, 700, new_i[s])]
+    toks = [(0, int(key_len[s]) - back) for s in (0, 13, n - 1) for back in (1, 2, 700, new_i[s])]
+    want, A, S = b.oracle(q=q[rows].cpu().numpy(), tokens=toks, rope=False, scale=0.25)
+    check(out[rows].cpu().numpy(), want, bound(want, A, S, q16=True, kv32=False, out16=True))
+
+
+@pytest.mark.parametrize("hd,window", [(512, 0), (512, 14000), (256, 0)])
+def test_decode_splits_of_many_blocks(hd, window):
+    """Enough keys for splits of more than 4096: a wave reloads its table entries."""
+    keys, n = (16000, 64) if hd == 512 else (20000, 128)
+    b = Batch([keys], [1], hd=hd, kvh=1, page=16, window=0, missing=[(0, 300), (0, keys // 16 - 9)])
+    b.window = window
+    q = torch.randn(n, 8, hd, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    key_len = torch.tensor([keys - 17 * i for i in range(n)], dtype=torch.int32, device="cuda")
+    d = b.dev()
+    got = decode(b, dict(d, q=q, table=d["table"].repeat(n, 1), key_len=key_len), rope_cos=None, rope_sin=None, cfg=b.cfg(scale=0.25))
+    rows = [0, 1, 33, n - 1]
+    want, A, S = b.oracle(q=q[rows].cpu().numpy(), tokens=[(0, int(key_len[i]) - 1) for i in rows], rope=False, scale=0.25)
+    check(got[rows].cpu().numpy(), want, bound(want, A, S, q16=False, kv32=False, out16=True))
+
+
+@pytest.mark.parametrize("n_seq", [65, 150])
+@pytest.mark.parametrize("hd,kvh", [(256, 2), (512, 1)])
+def test_decode_many_sequences(hd, kvh, n_seq):
+    """More sequences than lanes, of every length; every fifth idle."""
+    r = np.random.default_rng(n_seq)
+    keys = [0 if i % 5 == 4 else int(x) for i, x in enumerate(r.integers(1, 700, n_seq))]
+    b = Batch(keys, [1] * n_seq, hd=hd, kvh=kvh)
+    out, A, S = b.oracle()
+    check(decode(b, b.dev()).cpu().numpy(), out, bound(out, A, S, q16=False, kv32=False, out16=True))
+
+
+@pytest.mark.parametrize("hd,kvh,kv", [(256, 2, np.float16), (512, 1, np.float16), (256, 1, np.float32)])
+@pytest.mark.parametrize("n_seq", [65, 300])
+def test_prefill_many_sequences(hd, kvh, kv, n_seq):
+    """More sequences than lanes and than the plan takes at a time, short ones beside two long ones; rows
+    written by the call before."""
+    r = np.random.default_rng(n_seq)
+    keys = [int(x) for x in r.integers(0, 40, n_seq)]
+    new = [int(r.integers(0, 6)) if k > 6 else k for k in keys]
+    for i, (k, m) in {3: (1500, 70), n_seq - 1: (1100, 3)}.items():
+        keys[i], new[i] = k, m
+    b = Batch(keys, new, hd=hd, kvh=kvh, kv=kv, pad=2)
+    ref = b.dev()
+    write(b, ref)
+    d = b.dev()
+    rows = torch.zeros(2, b.T, kvh, hd, dtype=d["k_pages"].dtype, device="cuda")
+    pos = torch.tensor([0 if x is None else x[1] for x in b.tokens()], device="cuda")
+    sa.kv_write(d["k_new"], d["v_new"], rows[0], rows[1], 0, sa.AttnConfig(kvh, kvh, hd), k_gain=d["k_gain"],
+                rope_cos=d["cos"][pos].contiguous(), rope_sin=d["sin"][pos].contiguous())
+    for i, x in enumerate(b.tokens()):
+        if x is not None:
+            row = OP.keys_of(b.table, x[0], x[1], b.page, b.n_pages, 1)[1][0]
+            b.k_pages.reshape(-1, kvh, hd)[row], b.v_pages.reshape(-1, kvh, hd)[row] = rows[0, i].cpu().numpy(), rows[1, i].cpu().numpy()
+    assert np.array_equal(bits(ref["k_pages"]).reshape(-1), b.k_pages.reshape(-1).view(np.uint8))
+    assert np.array_equal(bits(ref["v_pages"]).reshape(-1), b.v_pages.reshape(-1).view(np.uint8))
+    run_prefill(b, kv32=kv is np.float32, dts=(torch.float16,))
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     b = Batch([40, 20], [1, 1])
