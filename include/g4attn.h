@@ -264,7 +264,9 @@ int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, co
 /*
  * Causal attention of n_tokens packed tokens, prompts or pieces of them, over the cache that
  * already holds their own rows (g4a_paged_write): the token at position p attends keys
- * [max(0, p + 1 - W), p] whose pages are there.
+ * [max(0, p + 1 - W), p] whose pages are there. (As in any masked product of weights and V, a V row that
+ * is not finite also reaches tokens it is masked for, those of the 128 / G positions handled together if
+ * one of them attends it. Masked K rows, and all rows that no such token attends, may hold anything.)
  *   q           f32 [n_tokens][n_q_heads][head_dim] raw; q_gain and RoPE are applied and the
  *               result rounded to f16, as g4a_prefill does without G4A_Q_HILO (refused here).
  *   out         [n_tokens][n_q_heads][head_dim], f16, or f32 with G4A_OUT_F32; srq'd with out_q.

@@ -250,6 +250,23 @@ def test_prefill_missing_pages(hd):
     assert (got[60:108] == 0).all()
 
 
+@pytest.mark.parametrize("hd", [256, 512])
+@pytest.mark.parametrize("window", [0, 50])
+def test_prefill_masked_keys_may_be_anything(hd, window):
+    """K rows that a token does not attend (later tokens' ones, ones its window has left) do not reach it,
+    whatever they hold; with V rows of the type's lowest value beside them."""
+    b = Batch([150], [150], hd=hd, kvh=1, window=window)
+    out, A, S = b.oracle()
+    k, v = b.k_pages.copy(), b.v_pages.copy()
+    at = b.table[0, 100 // 16], 100 % 16
+    v[at] = -65504.0
+    tokens = [i for i in range(150) if i < 100 or (window and i >= 100 + window)]
+    for junk in (np.inf, -np.inf, np.nan, 65504.0):
+        k[at] = junk
+        got = prefill(b, b.dev(k_pages=torch.from_numpy(k).cuda(), v_pages=torch.from_numpy(v).cuda())).cpu().numpy()
+        check(got[tokens], out[tokens], bound(out, A, S, q16=True, kv32=False, out16=True)[tokens], f"{junk}")
+
+
 def test_prefill_more_rows_than_keys():
     """Tokens at positions below zero attend nothing; offsets out of range are cut."""
     b = Batch([30, 20], [30, 20])
