@@ -407,6 +407,11 @@ __device__ __forceinline__ rsrc_t page_rows(const PageTab& t, const void* pool, 
 }
 constexpr int kNoRow = 0x7fff0000;  // an offset past every such range (64 MiB at most), with room for a row's own bytes
 
+// A transposed read that does not wait for the DMAs in flight. The compiler cannot tell that those fill other
+// tiles and would wait for all of them (vmcnt 0) before the first read of a tile's V; the __restrict puts the
+// read in an alias scope of its own. The tile loop's own wait and barrier order it behind the DMAs of its tile.
+__device__ __forceinline__ half4 read_tr16(const half_t* __restrict p) { return lds_tr16(p); }
+
 // ---------------------------------------------------------------- hd 256
 // 32 query columns a wave, 128 a workgroup, key tiles of 64 moved straight into LDS and double
 // buffered: the LDS layout and swizzles of prefill_kernel_w32, its tile loop pipelined by hand (below).
@@ -667,8 +672,8 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
             auto read_v = [&](int i) {
                 const int u = i >> 3, ch = 4 * (i & 7) + vc0;
                 const char* vp = V + (16 * u + vr0) * ROWB + 16 * (ch ^ vsw) + vb0;
-                const half4 lo = lds_tr16(reinterpret_cast<const half_t*>(vp));
-                const half4 hi = lds_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
+                const half4 lo = read_tr16(reinterpret_cast<const half_t*>(vp));
+                const half4 hi = read_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
                 av[i % (kPvAhead + 1)] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             };
             mnext = kNegInf;
