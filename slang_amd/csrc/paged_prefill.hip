@@ -65,7 +65,7 @@ __device__ __forceinline__ int block_tiles(const PagedPrefillArgs& a, int start,
 
 // Cost of the units, in key tiles: a unit's own beside its tiles (q, epilogue), a partial's store and
 // merge (its 3 bytes a value go to memory and back at a CU's share of the bandwidth, 20 GB/s), and
-// the merge launch. A tile takes about 2.1 us at hd 256 and 2.6 us at hd 512.
+// the merge launch. A tile takes about 1.9 us at hd 256 and 2.4 us at hd 512.
 struct PlanCost {
     float unit, part, merge;
 };
@@ -415,10 +415,10 @@ __device__ __forceinline__ half4 read_tr16(const half_t* __restrict p) { return 
 // ---------------------------------------------------------------- hd 256
 // 32 query columns a wave, 128 a workgroup, key tiles of 64 moved straight into LDS and double
 // buffered: the LDS layout and swizzles of prefill_kernel_w32, its tile loop pipelined by hand (below).
-// 7856 tokens, kvH 2, up to 3000 keys: 118 us = 730 TFLOP/s (123 us with the plain loop). A tile takes about
-// 4300 cycles, of them 2200 MFMA and about 3500 LDS: K rows 1024, V's transposed reads
-// 1490, the DMAs' writes 1024; beside the tiles a unit takes about 9 us (its page entries, q, the first
-// scores, the epilogue), which bounds short prompts and windows (15252 tokens, window 512: 125 us).
+// 7856 tokens, kvH 2, up to 3000 keys: 111 us = 780 TFLOP/s (123 us with the plain loop, 118 waiting for the
+// DMAs at V's first read). A tile takes 2200 cycles of MFMA and about 3500 of LDS: K rows 1024, V's
+// transposed reads 1490, the DMAs' writes 1024; beside the tiles a unit takes about 9 us (its page entries,
+// q, the first scores, the epilogue), which bounds short prompts and windows (15252 tokens, window 512: 120 us).
 template <int G, typename OUTT>
 __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs a) {
     constexpr int HD = 256, KT = 64, NCOL = 128, BQ = NCOL / G;
@@ -774,10 +774,10 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
 }
 
 // ---------------------------------------------------------------- hd 512
-// Every wave holds all 512 dims of its 32 columns, key tiles of 32: the tile loop, LDS layout and
-// register placement (O^T in AGPRs, q in VGPRs) of prefill_kernel_w32h. 13500 tokens in three prompts:
-// 864 us = 808 TFLOP/s at the 1.7 GHz that the card's power allows; LDS is busy 3700 of a tile's 4500
-// cycles. Interleaved as the hd-256 loop it ran 860 us, within the noise of a call.
+// Every wave holds all 512 dims of its 32 columns, key tiles of 32: the LDS layout and register placement
+// (O^T in AGPRs, q in VGPRs) of prefill_kernel_w32h, the tile loop interleaved as at hd 256. 13500 tokens in
+// three prompts: 811 us = 860 TFLOP/s at the 1.7 GHz that the card's power allows (873 us with the plain
+// loop, 867 interleaved but waiting for its DMAs at V's first read); LDS is busy 3700 cycles a tile.
 template <int G, typename OUTT>
 __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs a) {
     constexpr int HD = 512, KT = 32, NCOL = 128, BQ = NCOL / G;
@@ -811,28 +811,27 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
     const int pos = start_pos + s_idx;
 
     // K/V rows: wave w moves rows 8w .. 8w + 7 of a tile, one 1 KiB row an instruction. (The lane index
-    // passes through an empty asm each time, so the source offsets are formed per tile rather than
-    // held in registers across the loop.)
+    // passes through an empty asm each time, so the source offsets are formed where they are used rather
+    // than held in registers across the loop.)
     const int rowg = a.n_kv_heads * HD * 2;
     TilePages<KT> pages;
-    auto issue = [&](int t, int buf) {
-        char* kdst = lds + buf * 2 * TILEB;
+    // the 16 rows of tile t that this wave's 8 belong to, from the page of `entry`; past the last tile: an
+    // empty range
+    const auto tile_rows = [&](const void* pool, int t, int entry) {
+        const int kg = wg_lo + t * KT + 16 * (wave >> 1);
+        return page_rows(a.t, pool, entry, kg, t < t1 ? kv_hi : kg, rowg / 2, kh * HD);
+    };
+    const auto dma = [&](rsrc_t rp, char* dst, int j, int row_off, int swz) {
         int ln = lane;
         asm volatile("" : "+v"(ln));
-        const int kg = wg_lo + t * KT + 16 * (wave >> 1);  // the 16 rows that this wave's 8 belong to
-        const int entry = t == t0 ? (wave >> 1 ? wu.page[1] : wu.page[0]) : __builtin_amdgcn_readlane(pages.entry, (t - t0) & 63);
-        const rsrc_t pk = page_rows(a.t, a.kc, entry, kg, kv_hi, rowg / 2, kh * HD);
-        const rsrc_t pv = page_rows(a.t, a.vc, entry, kg, kv_hi, rowg / 2, kh * HD);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int r = 8 * wave + j, rg = 8 * (wave & 1) + j;
-            const int so = kg + rg >= first ? rg * rowg : kNoRow;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pk, (__attribute__((address_space(3))) void*)(kdst + r * ROWB), 16,
-                                                     so + 16 * (ln ^ (r & 31)), 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(pv, (__attribute__((address_space(3))) void*)(kdst + TILEB + r * ROWB),
-                                                     16, so + 16 * (ln ^ vswz(r)), 0, 0, 0);
-        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (__attribute__((address_space(3))) void*)(dst + (8 * wave + j) * ROWB), 16,
+                                                 row_off + 16 * (ln ^ swz), 0, 0, 0);
     };
+    const auto row_off = [&](int j) { return (8 * (wave & 1) + j) * rowg; };
+    const auto k_swz = [&](int j) { return (8 * wave + j) & 31; };
+    const auto v_swz = [&](int j) { return vswz(j); };
+    const auto tile_k = [&](int t) { return lds + (t & 1) * 2 * TILEB; };
+    const auto tile_v = [&](int t) { return lds + (t & 1) * 2 * TILEB + TILEB; };
 
     // ---- q: lane (column c, half h) holds dims 16s + 8h .. +7 (s < 32), the B operand layout. Wave w
     // DMAs the f16 q rows of its 32 columns, whole 1 KiB rows (chunk n of a row from logical chunk
@@ -840,6 +839,9 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
     // rounds of 16 rows, and reads each round back in that layout; tile t0's DMA goes out after the
     // first round's. Rows past the block's last token read as zeros.
     half8 qf[32];
+    int entry1 = wave >> 1 ? wu.page[1] : wu.page[0];  // tile t + 1's page
+    // the 16-row groups of tiles t and t + 1 without one
+    int gone0 = (page_ok(a.t, wu.page[0]) ? 0 : 1) | (page_ok(a.t, wu.page[1]) ? 0 : 2), gone1 = 0;
     {
         const rsrc_t rq = make_rsrc(a.q16 + ((size_t)row0 + qb * BQ) * a.n_q_heads * HD, (uint32_t)min(BQ, S - qb * BQ) * a.n_q_heads * ROWB);
         pages.load(a.t, wu.b, wg_lo + t0 * KT, wave >> 1, lane);
@@ -856,7 +858,15 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
                                                          16, qo, 0, 0, 0);
             }
             if (r == 0 && t0 < t1) {
-                issue(t0, t0 & 1);
+                // of the block's first tile, rows in front of the first attended key read as zeros
+                const rsrc_t rk = tile_rows(a.kc, t0, entry1), rv = tile_rows(a.vc, t0, entry1);
+                const int skip = first - (wg_lo + t0 * KT + 16 * (wave >> 1));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int ro = 8 * (wave & 1) + j < skip ? kNoRow : row_off(j);
+                    dma(rk, tile_k(t0), j, ro, k_swz(j));
+                    dma(rv, tile_v(t0), j, ro, v_swz(j));
+                }
                 asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // the 16 q DMAs before tile t0's
             } else {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -877,7 +887,6 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
     // ---- key ranges: this wave [w_lo, wp1], this column [col_lo, pos]
     const int wp0 = p0 + (32 * wave) / G;
     const int wp1 = min(p0 + (32 * wave + 31) / G, T_total - 1);
-    const int w_lo = a.window > 0 ? max(0, wp0 + 1 - a.window) : 0;
     const int col_lo = a.window > 0 ? pos + 1 - a.window : 0;
 
     // LDS read offsets. K operand k-step s of this lane: row n32, chunk (2s + h) ^ n32, i.e.
@@ -900,60 +909,41 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
     for (int dt = 0; dt < 16; ++dt) asm volatile("" : "+a"(oacc[dt]));
     float m_use = kNegInf, l_run = 0.0f;
     bool started = false;
-    for (int t = t0; t < t1; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of tile t are in LDS
-        __syncthreads();                                    // all rows; tile t-1 consumed
-        const int gone = __builtin_amdgcn_readlane(pages.gone, (t - t0) & 63);  // 16-row groups without a page
-        if (((t + 1 - t0) & 63) == 0) pages.load(a.t, wu.b, wg_lo + (t + 1) * KT, wave >> 1, lane);
-        if (t + 1 < t1) issue(t + 1, (t + 1) & 1);
+    // Masks of tile t's scores: key kb + 4h + 8(r/4) + r%4 of this lane's column; tiles inside every column's
+    // range skip it.
+    auto mask = [&](int t, int gone, float16v& sc) {
         const int kb = wg_lo + t * KT;
-        if (kb > wp1 || kb + KT - 1 < w_lo) continue;  // no key of this tile for this wave
-        int kofs = (t & 1) * 2 * TILEB + kofs0, vofs = (t & 1) * 2 * TILEB + TILEB + vofs0;
-        asm volatile("" : "+v"(kofs), "+v"(vofs));
-
-        // S^T = K . Q^T over 32 k-steps of 16 dims, even and odd steps in two chains
-        float16v se = float16v{}, so = float16v{};
-        {
-#pragma unroll
-            for (int s0 = 0; s0 < 32; s0 += 4) {
-                half8 kv[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) kv[s] = *reinterpret_cast<const half8*>(lds + (kofs ^ (32 * (s0 + s))));
-#pragma unroll
-                for (int s = 0; s < 4; s += 2) {
-                    se = mfma32(kv[s], qf[s0 + s], se);
-                    so = mfma32(kv[s + 1], qf[s0 + s + 1], so);
-                }
-            }
-            __builtin_amdgcn_sched_group_barrier(0x100, kQkAhead, 0);
-#pragma unroll
-            for (int i = 0; i < 32 - kQkAhead; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-            __builtin_amdgcn_sched_group_barrier(0x008, kQkAhead, 0);
-        }
-        float sacc[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sacc[r] = se[r] + so[r];
-        // scores of this lane: key kb + 4h + 8(r/4) + r%4 of its column, log2 domain
-        const bool masked = (kb + KT - 1 > wp0) || (a.window > 0 && kb < wp1 + 1 - a.window);
-        if (masked) {
+        if ((kb + KT - 1 > wp0) || (a.window > 0 && kb < wp1 + 1 - a.window)) {
             const int rel_hi = pos - (kb + 4 * h), rel_lo = col_lo - (kb + 4 * h);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int o = 8 * (r >> 2) + (r & 3);
-                sacc[r] = (o <= rel_hi && o >= rel_lo) ? sacc[r] : kNegInf;
+                sc[r] = (o <= rel_hi && o >= rel_lo) ? sc[r] : kNegInf;
             }
         }
         if (gone) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sacc[r] = gone >> (r >> 3) & 1 ? kNegInf : sacc[r];
+            for (int r = 0; r < 16; ++r) sc[r] = gone >> (r >> 3) & 1 ? kNegInf : sc[r];
         }
-        float mloc = kNegInf;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mloc = fmaxf(mloc, sacc[r]);
-        mloc = max32(mloc) * a.scale_log2;
+    };
+
+    // One tile, interleaved as in the hd-256 kernel: the 32 score MFMAs of tile t + 1 (even and odd k-steps
+    // in two chains, added at the end) with the 16 exponentials of tile t and the DMAs of V(t + 1) and
+    // K(t + 2); the 32 P.V MFMAs of tile t with the maxima of tile t + 1. On entry sacc holds tile t's
+    // scores, on return tile t + 1's.
+    float16v sacc = float16v{};
+    float mnext = kNegInf;  // this lane's maximum of them
+    auto tile = [&](int t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of V(t) and K(t + 1) are in LDS
+        __syncthreads();
+        const int gone = gone1, entry = entry1;             // of tile t + 1
+        {
+            const int j = (t + 2 - t0) & 63;
+            if (j == 0) pages.load(a.t, wu.b, wg_lo + (t + 2) * KT, wave >> 1, lane);
+            entry1 = __builtin_amdgcn_readlane(pages.entry, j);
+            gone1 = __builtin_amdgcn_readlane(pages.gone, j);
+        }
+        const float mloc = max32(mnext) * a.scale_log2;
         const bool bump = mloc > m_use + kMaxLag;  // the running maxima move only past 2^kMaxLag
         if (__any(bump)) {
             const float m_new = fmaxf(m_use, mloc);
@@ -983,40 +973,91 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs
         const float msub = m_use == kNegInf ? 0.0f : m_use;
         half8 pb[2];
         float ps = 0.0f;
+        float16v se = float16v{}, so = float16v{};
+        {
+            int kofs = ((t + 1) & 1) * 2 * TILEB + kofs0;
+            asm volatile("" : "+v"(kofs));
+            half8 kr[3][2];
+            auto read_k = [&](int s) {
+                kr[s % 3][0] = *reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s)));
+                kr[s % 3][1] = *reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s + 32)));
+            };
+            // exponential v of the lane's 16 in three stages
+            float ex[2], ev[2];
+            auto arg = [&](int v) { ex[v & 1] = __builtin_fmaf(sacc[v], a.scale_log2, -msub); };
+            auto take = [&](int v) {
+                ps += ev[v & 1];
+                pb[v >> 3][v & 7] = (half_t)ev[v & 1];
+            };
+            read_k(0);
+            read_k(1);
+            arg(0);
+            const rsrc_t rv = tile_rows(a.vc, t + 1, entry), rk = tile_rows(a.kc, t + 2, entry1);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float pv = fexp2(__builtin_fmaf(sacc[8 * u + i], a.scale_log2, -msub));
-                ps += pv;
-                pb[u][i] = (half_t)pv;
+            for (int s = 0; s < 16; ++s) {
+                if (s + 2 < 16) read_k(s + 2);
+                se = mfma32(kr[s % 3][0], qf[2 * s], se);
+                ev[s & 1] = fexp2(ex[s & 1]);
+                if (s > 0) take(s - 1);
+                so = mfma32(kr[s % 3][1], qf[2 * s + 1], so);
+                if (s < 15) arg(s + 1);
+                if (s < 8) dma(rv, tile_v(t + 1), s, row_off(s), v_swz(s));
+                else dma(rk, tile_k(t + 2), s - 8, row_off(s - 8), k_swz(s - 8));
+                __builtin_amdgcn_sched_barrier(0);
             }
+            take(15);
+        }
         l_run += ps;
+        sacc = se + so;
+        // (here, not where they are used behind the masks' branches: the compiler would sink them there)
+        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(l_run), "+v"(sacc));
+        if (t + 1 < t1) mask(t + 1, gone, sacc);
 
-        // O^T += V^T . P^T over two 16-key steps, 16 dims tiles each
+        // O^T += V^T . P^T over two 16-key steps, 16 dims tiles each; transposed V reads (two an MFMA) kPvAhead
+        // MFMAs ahead
+        {
+            int vofs = (t & 1) * 2 * TILEB + TILEB + vofs0;
+            asm volatile("" : "+v"(vofs));
+            half8 av[kPvAhead + 1];
+            auto read_v = [&](int i) {
+                const char* vp = lds + (vofs ^ (64 * (i & 15))) + 16 * (i >> 4) * ROWB;
+                const half4 lo = read_tr16(reinterpret_cast<const half_t*>(vp));
+                const half4 hi = read_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
+                av[i % (kPvAhead + 1)] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            mnext = kNegInf;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+            for (int i = 0; i < kPvAhead; ++i) read_v(i);
 #pragma unroll
-            for (int d0 = 0; d0 < 16; d0 += 4) {
-                half8 av[4];
-#pragma unroll
-                for (int dd = 0; dd < 4; ++dd) {
-                    const char* vp = lds + (vofs ^ (64 * (d0 + dd))) + 16 * u * ROWB;
-                    const half4 lo = lds_tr16(reinterpret_cast<const half_t*>(vp));
-                    const half4 hi = lds_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
-                    av[dd] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                }
-#pragma unroll
-                for (int dd = 0; dd < 4; ++dd) mfma32_acc(oacc[d0 + dd], av[dd], pb[u]);
+            for (int i = 0; i < 32; ++i) {
+                if (i + kPvAhead < 32) read_v(i + kPvAhead);
+                mfma32_acc(oacc[i & 15], av[i % (kPvAhead + 1)], pb[i >> 4]);
+                if (i >= 8 && i < 16) mnext = fmaxf(mnext, fmaxf(sacc[2 * (i - 8)], sacc[2 * (i - 8) + 1]));
+                __builtin_amdgcn_sched_barrier(0);
             }
+            asm volatile("" : "+v"(mnext));
         }
-        __builtin_amdgcn_sched_group_barrier(0x100, 2 * kPvAhead, 0);
+    };
+    if (t0 < t1) {
+        __syncthreads();  // K(t0), V(t0); every wave has its q
+        entry1 = __builtin_amdgcn_readlane(pages.entry, 1);
+        gone1 = __builtin_amdgcn_readlane(pages.gone, 1);
+        const rsrc_t rk = tile_rows(a.kc, t0 + 1, entry1);
 #pragma unroll
-        for (int i = 0; i < 32 - kPvAhead; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        for (int j = 0; j < 8; ++j) dma(rk, tile_k(t0 + 1), j, row_off(j), k_swz(j));
+        float16v se = float16v{}, so = float16v{};
+        const int kofs = (t0 & 1) * 2 * TILEB + kofs0;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+            se = mfma32(*reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s))), qf[2 * s], se);
+            so = mfma32(*reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s + 32))), qf[2 * s + 1], so);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, kPvAhead, 0);
+        sacc = se + so;
+        mask(t0, gone0, sacc);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mnext = fmaxf(mnext, sacc[r]);
+        for (int t = t0; t < t1; ++t) tile(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last tile's (empty) DMAs, before LDS is used again
     }
 
     // ---- epilogue: the 512 dims of this wave's 32 columns. The accumulators are read by
