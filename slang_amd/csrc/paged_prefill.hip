@@ -430,7 +430,7 @@ __device__ __forceinline__ half4 read_tr16(const half_t* __restrict p) { return 
 // ---------------------------------------------------------------- hd 256
 // 32 query columns a wave, 128 a workgroup, key tiles of 64 moved straight into LDS and double
 // buffered: the LDS layout and swizzles of prefill_kernel_w32, its tile loop pipelined by hand (below).
-// 7856 tokens, kvH 2, up to 3000 keys: 111 us = 780 TFLOP/s (123 us with the plain loop, 118 waiting for the
+// 7856 tokens, kvH 2, up to 3000 keys: 112 us = 770 TFLOP/s (123 us with the plain loop, 118 waiting for the
 // DMAs at V's first read). A tile takes 2200 cycles of MFMA and about 3500 of LDS: K rows 1024, V's
 // transposed reads 1490, the DMAs' writes 1024; beside the tiles a unit takes about 9 us (its page entries,
 // q, the first scores, the epilogue), which bounds short prompts and windows (15252 tokens, window 512: 120 us).
@@ -791,7 +791,7 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
 // ---------------------------------------------------------------- hd 512
 // Every wave holds all 512 dims of its 32 columns, key tiles of 32: the LDS layout and register placement
 // (O^T in AGPRs, q in VGPRs) of prefill_kernel_w32h, the tile loop interleaved as at hd 256. 13500 tokens in
-// three prompts: 811 us = 860 TFLOP/s at the 1.7 GHz that the card's power allows (873 us with the plain
+// three prompts: 800 to 820 us = 850 to 870 TFLOP/s at the 1.7 GHz that the card's power allows (873 us with the plain
 // loop, 867 interleaved but waiting for its DMAs at V's first read); LDS is busy 3700 cycles a tile.
 template <int G, typename OUTT>
 __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs a) {
