@@ -304,7 +304,7 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
 
 // q of packed rows to f16: RMSNorm * gain, then RoPE at the row's position (qprep_row512_kernel's
 // arithmetic). A wave takes four heads of a token; lane l holds dims E l .. E l + E - 1, whose RoPE
-// partners sit in lane l ^ 32. The first workgroup writes the work list meanwhile (6.7 us, what a call of few
+// partners sit in lane l ^ 32. The first workgroup writes the work list meanwhile (about 7 us, what a call of few
 // tokens waits for). Many tokens: the bytes (15252 of 8 x 256, 187 MB: 35 us = 5.3 TB/s, a copy's rate).
 template <int HD>
 __global__ __launch_bounds__(256) void paged_prep_kernel(PagedPrefillArgs a) {
