@@ -88,8 +88,8 @@ __global__ __launch_bounds__(HD / 2) void paged_write_kernel(PagedWriteArgs a) {
         b = seq_of_row(a.cu, a.t.n_seq, tok);
         if (b >= a.t.n_seq) return;
         const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
-        if (tok < r.lo || tok >= r.hi) return;
-        p = r.keys - r.hi + tok;
+        if (!holds(r, tok)) return;
+        p = row_position(r, tok);
     } else {
         p = paged_len(a.t, b) - 1;
     }

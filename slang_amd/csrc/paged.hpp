@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "paged_rows.hpp"
 
 namespace g4a {
 
@@ -47,21 +48,12 @@ __device__ __forceinline__ size_t paged_row(const PageTab& t, int page, int p, i
     return (((size_t)page << t.shift) + (size_t)(p & ((1 << t.shift) - 1))) * (size_t)row;
 }
 
-// the packed rows [lo, hi) of sequence b and its keys: row lo + i is the token at position
-// keys - (hi - lo) + i. Offsets outside [0, n_tokens] are cut to it, one below its predecessor to that.
-struct SeqRows {
-    int lo, hi, keys;
-};
 __device__ __forceinline__ SeqRows seq_rows(const PageTab& t, const int32_t* cu, int n_tokens, int b) {
-    SeqRows r;
-    r.lo = min(max(cu[b], 0), n_tokens);
-    r.hi = min(max(cu[b + 1], r.lo), n_tokens);
-    r.keys = paged_len(t, b);
-    return r;
+    return cut_rows(cu[b], cu[b + 1], n_tokens, paged_len(t, b));
 }
 
 // The sequence of packed row `tok`: how many sequences end at or before it, 64 offsets a load
-// (cu ascends). n_seq: a row behind the last sequence. Every lane of the wave must call it.
+// (cu ascends; if it does not, any sequence). n_seq: a row behind the last sequence. Every lane of the wave must call it.
 __device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int tok) {
     const int lane = threadIdx.x & 63;
     int b = 0;

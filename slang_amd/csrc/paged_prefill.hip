@@ -327,7 +327,8 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(PagedPrefillArgs a) {
     const int b = seq_of_row(a.cu, a.t.n_seq, tok);
     if (b >= a.t.n_seq) return;  // a row of nobody
     const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
-    const int p = max(r.keys - r.hi + tok, 0);
+    if (!holds(r, tok)) return;  // offsets that do not ascend
+    const int p = max(row_position(r, tok), 0);
     vec_t c, sn;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
