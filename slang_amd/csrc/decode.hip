@@ -708,7 +708,7 @@ void decode_kernel(A a) {
             o += *reinterpret_cast<const float4v*>(&lds[w * G * HD + e]) * wt;
         }
         if (single) {
-            const float inv = PAGED && !(L > 0.0f) ? 0.0f : 1.0f / L;  // paged: perhaps no page is there
+            const float inv = PAGED && L == 0.0f ? 0.0f : 1.0f / L;  // paged: perhaps no page is there
             float4v r;
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = srq(o[i] * inv, a.out_q);
@@ -727,8 +727,16 @@ void decode_kernel(A a) {
 // of the max_splits slots holds a partial or a weightless marker, so all loads are issued
 // at entry. Thread (split group sg, dim d) reads splits sg, sg+4, .. of its output element
 // (NB batches of 64; slots past max_splits read as zeros through the buffer range), thread
-// t reads (m, l) of split t. A slot of weight 0 is dropped by a select, never multiplied
-// in: a marker slot's o holds whatever an earlier call left there.
+// t reads (m, l) of split t. A slot with l = 0 (no attended key: a marker, whose o holds whatever
+// an earlier call left there) is dropped by a select, never multiplied in. All others are
+// multiplied in, whatever their weight, so that a key, value or query that is not finite gives NaN
+// however the keys were split, as in one softmax over all of them.
+// Weight of a split's partial (m, l) at the maximum M; below zero: nothing to add. A split whose
+// scores are all NaN has m = -inf, as a maximum passes NaN over, but l = NaN.
+__device__ __forceinline__ float split_weight(float m, float l, float M) {
+    if (l == 0.0f) return -1.0f;
+    return l != l ? l : fexp2(m - M);
+}
 template <typename A>
 __device__ __forceinline__ void store_merged(const A& a, size_t at, float v) {
     if constexpr (std::is_same_v<A, PagedDecodeArgs>) {
@@ -760,16 +768,16 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(A a) {
     if (lane == 0) s_red[sg] = mloc;
     __syncthreads();
     const float M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float w = mt == kNegInf ? 0.0f : fexp2(mt - M);
+    const float w = split_weight(mt, mlt.y, M);
     wts[tid] = w;
-    const float lw = wave_sum(w == 0.0f ? 0.0f : w * mlt.y);
+    const float lw = wave_sum(w < 0.0f ? 0.0f : w * mlt.y);
     if (lane == 0) s_red2[sg] = lw;
     __syncthreads();
     float o = 0.0f;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
         const float wc = wts[sg + 4 * u];
-        o = wc != 0.0f ? fmaf(wc, v[u], o) : o;
+        o = wc < 0.0f ? o : fmaf(wc, v[u], o);
     }
     red[sg][lane] = o;
     __syncthreads();
@@ -777,7 +785,7 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(A a) {
         const float L = (s_red2[0] + s_red2[1]) + (s_red2[2] + s_red2[3]);
         const float t = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
         // L = 0 only when the sequence attends no key: defined output of zeros
-        store_merged(a, ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e, L > 0.0f ? srq(t * (1.0f / L), a.out_q) : 0.0f);
+        store_merged(a, ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e, L == 0.0f ? 0.0f : srq(t * (1.0f / L), a.out_q));
     }
 }
 
@@ -812,7 +820,7 @@ __global__ __launch_bounds__(256) void decode_merge_list_kernel(A a) {
             const size_t u = (size_t)u0 + (s < splits ? s : s0);
             ml[j] = a.part_ml[u * G + hh];
             o[j] = a.part_o[u * E + e];
-            if (s >= splits) ml[j].x = kNegInf;
+            if (s >= splits) ml[j] = make_float2(kNegInf, 0.0f);
         }
         float bm = M;
 #pragma unroll
@@ -823,9 +831,9 @@ __global__ __launch_bounds__(256) void decode_merge_list_kernel(A a) {
         O *= c;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float w = ml[j].x == kNegInf ? 0.0f : fexp2(ml[j].x - bm);
-            Ls = w != 0.0f ? fmaf(w, ml[j].y, Ls) : Ls;
-            O = w != 0.0f ? fmaf(w, o[j], O) : O;
+            const float w = split_weight(ml[j].x, ml[j].y, bm);
+            Ls = w < 0.0f ? Ls : fmaf(w, ml[j].y, Ls);
+            O = w < 0.0f ? O : fmaf(w, o[j], O);
         }
         M = bm;
     }
@@ -838,12 +846,12 @@ __global__ __launch_bounds__(256) void decode_merge_list_kernel(A a) {
         float L = 0.0f, t = 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float w = sm[k][lane] == kNegInf ? 0.0f : fexp2(sm[k][lane] - Mx);
-            L = w != 0.0f ? fmaf(w, sl[k][lane], L) : L;
-            t = w != 0.0f ? fmaf(w, so[k][lane], t) : t;
+            const float w = split_weight(sm[k][lane], sl[k][lane], Mx);
+            L = w < 0.0f ? L : fmaf(w, sl[k][lane], L);
+            t = w < 0.0f ? t : fmaf(w, so[k][lane], t);
         }
         // L = 0 only when the sequence attends no key: defined output of zeros
-        store_merged(a, ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e, L > 0.0f ? srq(t * (1.0f / L), a.out_q) : 0.0f);
+        store_merged(a, ((size_t)b * a.n_q_heads + (size_t)kh * G) * HD + e, L == 0.0f ? 0.0f : srq(t * (1.0f / L), a.out_q));
     }
 }
 

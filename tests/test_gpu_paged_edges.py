@@ -38,3 +38,60 @@ def test_prefill_offsets_out_of_order_stay_in_the_rope_tables(hd, cu):
     want, A, S = b.oracle()
     got = prefill(b, d, rope_cos=tables[0], rope_sin=tables[1], max_key_len=keys, workspace=w)
     check(got.cpu().numpy(), want, bound(want, A, S, q16=True, kv32=False, out16=True))
+
+
+# ---------------------------------------------------------------- rows that are not finite
+@pytest.mark.parametrize("keys", [[100], [1500], [20, 1500, 700, 0, 90]])  # one split; splits; a work list
+@pytest.mark.parametrize("hd,kvh,kv", [(256, 2, np.float16), (512, 1, np.float16), (256, 1, np.float32)])
+@pytest.mark.parametrize("what", ["q", "q inf", "k", "v"])
+def test_decode_shows_what_is_not_finite(hd, kvh, kv, keys, what):
+    """A query head, or an attended K row or V value, that is not finite makes its outputs NaN and no other,
+    however the keys are split: through pages and over contiguous caches."""
+    b = Batch(keys, [min(1, k) for k in keys], hd=hd, kvh=kvh, kv=kv, extra_cols=0)
+    n, G, s = len(keys), 8 // kvh, int(np.argmax(keys))
+    b.q = np.random.default_rng(1).standard_normal((n, 8, hd)).astype(np.float32)
+    tokens = [(i, k - 1) for i, k in enumerate(keys)]
+    out, A, S = b.oracle(tokens=tokens)
+    tol = bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True)
+    bad = np.zeros(out.shape, bool)
+    if what[0] == "q":
+        b.q[s, 3, 7] = np.nan if what == "q" else np.inf
+        bad[s, 3] = True
+    else:
+        p = keys[s] // 3
+        pool = b.k_pages if what == "k" else b.v_pages
+        pool[b.table[s, p // b.page], p % b.page, kvh - 1, 5] = np.nan
+        bad[s, G * (kvh - 1):, slice(None) if what == "k" else 5] = True
+    d = b.dev()
+    got = [decode(b, d)]
+    longest = max(keys)
+    dense = [torch.zeros(n, longest, kvh, hd, dtype=d["k_pages"].dtype, device="cuda") for _ in range(2)]
+    for i, k in enumerate(keys):
+        at = [b.table[i, p // b.page] * b.page + p % b.page for p in range(k)]
+        for x, pool in zip(dense, (d["k_pages"], d["v_pages"])):
+            x[i, :k] = pool.view(-1, kvh, hd)[at]
+    pos = torch.tensor([max(0, k - 1) for k in keys], device="cuda")
+    got.append(sa.decode(d["q"], *dense, i32(keys), b.cfg(), q_gain=d["gain"], rope_cos=d["cos"][pos].contiguous(),
+                         rope_sin=d["sin"][pos].contiguous(), workspace=ws()))
+    for x, name in zip(got, ("paged", "contiguous")):
+        x = x.float().cpu().numpy()
+        assert np.isnan(x[bad]).all(), f"{name}: {np.isnan(x[bad]).sum()} of {bad.sum()} NaN, {(x[bad] == 0).sum()} zeros"
+        assert (np.abs(x - out)[~bad] <= tol[~bad]).all(), name
+
+
+@pytest.mark.parametrize("hd", [256, 512])
+@pytest.mark.parametrize("keys,new", [([300, 90], [40, 20]), ([2000, 90], [10, 20])])  # whole blocks; pieces
+def test_prefill_shows_what_is_not_finite(hd, keys, new):
+    """A query head of one token, and a K row that every later token attends."""
+    b = Batch(keys, new, hd=hd, kvh=1)
+    out, A, S = (x.copy() for x in b.oracle())
+    tol = bound(out, A, S, q16=True, kv32=False, out16=True)
+    bad = np.zeros(out.shape, bool)
+    b.q[2, 3, 7] = np.nan
+    bad[2, 3] = True
+    p = keys[1] - new[1] + 5  # row 5 of the second sequence's tokens
+    b.k_pages[b.table[1, p // b.page], p % b.page, 0, 9] = np.nan
+    bad[new[0] + 5:] = True
+    got = prefill(b, b.dev()).float().cpu().numpy()
+    assert np.isnan(got[bad]).all(), f"{np.isnan(got[bad]).sum()} of {bad.sum()} NaN"
+    assert (np.abs(got - out)[~bad] <= tol[~bad]).all()
