@@ -598,10 +598,15 @@ void decode_kernel(A a) {
     for (; blk < k1; blk += 64) {
         // the block holding the new key: its row comes from the prepared copy, whatever
         // the load (issued before the store) returned
-        const bool patch = owns_new && p_new >= blk && p_new < blk + 16;  // wave-uniform
-        // paged: the block's keys [lo_i, hi_i) attend, none if its page is not there
+        bool patch = owns_new && p_new >= blk && p_new < blk + 16;  // wave-uniform
+        // paged: the block's keys [lo_i, k1) attend, none if its page is not there; nor is a new row there
+        // then (its weight of 0 would not keep out values that are not finite)
         int lo_i = 0;
-        if constexpr (PAGED) lo_i = page_ok(a.t, blk_page) ? key_lo : k1;
+        if constexpr (PAGED) {
+            const bool there = page_ok(a.t, blk_page);
+            lo_i = there ? key_lo : k1;
+            patch = patch && there;
+        }
         float4v c4 = float4v{0, 0, 0, 0};
         if constexpr (KROW) {
             // K and V rows into this wave's LDS blocks (the new key's row over whatever its

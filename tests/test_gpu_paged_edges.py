@@ -95,3 +95,18 @@ def test_prefill_shows_what_is_not_finite(hd, keys, new):
     got = prefill(b, b.dev()).float().cpu().numpy()
     assert np.isnan(got[bad]).all(), f"{np.isnan(got[bad]).sum()} of {bad.sum()} NaN"
     assert (np.abs(got - out)[~bad] <= tol[~bad]).all()
+
+
+@pytest.mark.parametrize("hd,kvh,kv", [(256, 2, np.float16), (512, 1, np.float16), (256, 1, np.float32), (512, 1, np.float32)])
+@pytest.mark.parametrize("keys", [[40, 90], [1000, 90]])  # one split; a work list
+def test_decode_row_for_a_missing_page_may_hold_anything(hd, kvh, kv, keys):
+    """A step's row whose page is not there is neither stored nor attended, whatever it holds."""
+    b = Batch(keys, [1, 1], hd=hd, kvh=kvh, kv=kv, missing=[(0, (keys[0] - 1) // 16)])
+    out, A, S = b.oracle()
+    for junk in (np.nan, np.inf, -np.inf):
+        d = b.dev()
+        k, v = d["k_new"].clone(), d["v_new"].clone()
+        k[0] = v[0] = float(junk)
+        got = decode(b, dict(d, k_new=k, v_new=v), append=True, v_norm=False)[:1]
+        check(got.cpu().numpy(), out[:1], bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True)[:1], f"{junk}")
+        assert not torch.isfinite(d["k_pages"]).all()  # the poison of the rows that nobody attends is still there
