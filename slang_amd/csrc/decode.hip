@@ -38,6 +38,7 @@
 // resources of their own; everything else, the merge included, is shared. 16 sequences of 1 K to 32 K keys
 // (hd 256, kvH 2, 554 MB in pages of 64): 85-88 us + merge 4.6, 6.3 TB/s, as fast as contiguous caches; 64 of
 // 20 to 4097 keys under a window of 512 (26 MB): 11.4 + 4.6 us, two dependent kernels at their latency.
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -900,6 +901,7 @@ static int decode_chunk(const g4a_cfg* cfg, int n_seq, int max_key_len, bool pag
         chunk = (((max_active + s - 1) / s) + 15) & ~15L;
     }
     if ((max_active + chunk - 1) / chunk > 256) chunk = (max_active + 255) / 256;
+    chunk = std::min(chunk, max_active);  // (the share of many pairs passes it, and could pass 32 bits)
     return (int)((chunk + 15) & ~15L);
 }
 

@@ -169,3 +169,14 @@ def test_oracle_keys():
     t, _ = OP.keys_of(table, 0, 60, 16, 8, 30)
     assert t.tolist() == list(range(32, 48))
     assert len(OP.keys_of(table, 0, -1, 16, 8, 0)[0]) == 0
+
+
+@pytest.mark.parametrize("kvh,hd", [(1, 256), (8, 512), (64, 512)])
+def test_plans_of_the_largest_batches(lib, kvh, hd):
+    """The share of a key split stays within 32 bits, whatever the number of sequences and of keys."""
+    for n_seq in (1, 2, 64, 1000, 1024):
+        for keys in (1, 1000, 131072, 1 << 20, 1 << 24, 1 << 26, (1 << 30) - 1, 1 << 30):
+            for window in (0, 512):
+                c = cfg(n_q_heads=8 * kvh, n_kv_heads=kvh, head_dim=hd, window=window)
+                need = lib.g4a_decode_ws_bytes(ctypes.byref(c), n_seq, keys)
+                assert 0 < need <= (512 + 2 * n_seq * kvh) * 8 * (hd * 4 + 8 + 8) + 1024, (n_seq, keys, window)
