@@ -998,16 +998,11 @@ static decode_fn<A> pick_merge(int G, int splits) {
     return nullptr;
 }
 
-// what decode_impl and g4a_paged_decode set alike: the plan, the workspace's parts and the config
-static int decode_setup(DecodeArgs& a, const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged, void* ws) {
+// what decode_impl and g4a_paged_decode set alike: the plan and the config ...
+static int decode_setup(DecodeArgs& a, const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged) {
     const int HD = (int)cfg->head_dim;
     const size_t esz = (cfg->flags & G4A_KV_F32) != 0 ? 4 : 2;
     const ListPlan lp = list_plan(cfg, n_seq, max_key_len, paged);
-    const WsLayout L = ws_layout(cfg, n_seq, max_key_len, paged);
-    char* w = (char*)ws;
-    a.part_ml = (float2*)(w + L.ml);
-    a.part_o = (float*)(w + L.o);
-    a.list_tab = (int2*)(w + L.tab);
     a.n_q_heads = (int)cfg->n_q_heads;
     a.n_kv_heads = (int)cfg->n_kv_heads;
     a.window = (int)cfg->window;
@@ -1029,7 +1024,7 @@ static int decode_setup(DecodeArgs& a, const g4a_cfg* cfg, int n_seq, int max_ke
         a.max_splits = decode_splits(cfg, n_seq, max_key_len, paged);
         a.chunk = decode_chunk(cfg, n_seq, max_key_len, paged);
         a.chunk_cap = 0;
-        if ((int64_t)(a.chunk + 64) * row_bytes > 0x7fffffff) {
+        if (!paged && (int64_t)(a.chunk + 64) * row_bytes > 0x7fffffff) {
             set_error("keys per split too large for 32-bit buffer offsets");
             return G4A_EINVAL;
         }
@@ -1039,6 +1034,13 @@ static int decode_setup(DecodeArgs& a, const g4a_cfg* cfg, int n_seq, int max_ke
     a.out_q = cfg->out_q;
     a.v_norm = (cfg->flags & G4A_NO_V_NORM) ? 0 : 1;
     return G4A_OK;
+}
+// ... and the parts of the workspace
+static void decode_parts(DecodeArgs& a, const WsLayout& L, void* ws) {
+    char* w = (char*)ws;
+    a.part_ml = (float2*)(w + L.ml);
+    a.part_o = (float*)(w + L.o);
+    a.list_tab = (int2*)(w + L.tab);
 }
 
 // the decode kernel of `a` and, unless one split holds every key, the merge
@@ -1134,7 +1136,8 @@ static int decode_impl(const g4a_cfg* cfg, int n_seq, int max_key_len, const int
     a.vc = v_cache;
     a.seq_stride = seq_stride;
     a.out = out;
-    if (const int rc = decode_setup(a, cfg, n_seq, max_key_len, false, ws)) return rc;
+    if (const int rc = decode_setup(a, cfg, n_seq, max_key_len, false)) return rc;
+    decode_parts(a, L, ws);
     a.k_new = kvn ? kvn->k : nullptr;
     a.v_new = kvn ? kvn->v : nullptr;
     a.k_gain = kvn ? kvn->k_gain : nullptr;
@@ -1287,12 +1290,13 @@ extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const f
             set_error("out must not overlap k_new or v_new");
             return G4A_EINVAL;
         }
+    PagedDecodeArgs a{};
+    if (const int rc = decode_setup(a, cfg, pg->n_seq, pg->max_key_len, true)) return rc;
     const size_t need = paged_ws_bytes(cfg, pg);
     if (!ws || (uintptr_t)ws % 256 || ws_bytes < need) {
         set_error("paged decode workspace needs %zu bytes (256-byte aligned), got %zu", need, ws ? ws_bytes : (size_t)0);
         return G4A_EWORKSPACE;
     }
-    PagedDecodeArgs a{};
     a.t = page_tab(pg);
     a.q = q;
     a.q_gain = q_gain;
@@ -1302,7 +1306,7 @@ extern "C" int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const f
     a.vc = a.vc_out = pg->v_pages;
     a.out = (float*)out;
     a.out16 = (cfg->flags & G4A_OUT_F32) == 0;
-    if (const int rc = decode_setup(a, cfg, pg->n_seq, pg->max_key_len, true, ws)) return rc;
+    decode_parts(a, ws_layout(cfg, pg->n_seq, pg->max_key_len, true), ws);
     a.k_new = k_new;
     a.v_new = v_new;
     a.k_gain = k_gain;

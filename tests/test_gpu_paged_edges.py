@@ -110,3 +110,17 @@ def test_decode_row_for_a_missing_page_may_hold_anything(hd, kvh, kv, keys):
         got = decode(b, dict(d, k_new=k, v_new=v), append=True, v_norm=False)[:1]
         check(got.cpu().numpy(), out[:1], bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True)[:1], f"{junk}")
         assert not torch.isfinite(d["k_pages"]).all()  # the poison of the rows that nobody attends is still there
+
+
+# ---------------------------------------------------------------- long bounds, large batches
+@pytest.mark.parametrize("hd,kvh,kv,page,bound_keys,n", [(512, 8, np.float32, 16, 131072, 64), (512, 8, np.float16, 64, 1 << 18, 70),
+                                                         (256, 1, np.float16, 32768, 1 << 30, 1), (256, 2, np.float16, 32768, 1 << 30, 3)])
+def test_decode_long_bounds(hd, kvh, kv, page, bound_keys, n):
+    """Short sequences under a bound whose rows pass 32-bit offsets."""
+    keys = [1 + 13 * i % 90 for i in range(n)]
+    b = Batch(keys, [1] * n, hd=hd, kvh=kvh, kv=kv, page=page, spare=1, extra_cols=0)
+    table = np.full((n, bound_keys // page), -1, np.int32)
+    table[:, :b.cols] = b.table
+    out, A, S = b.oracle(rope=False)
+    got = decode(b, b.dev(table=torch.from_numpy(table).cuda()), rope_cos=None, rope_sin=None, max_key_len=bound_keys)
+    check(got.cpu().numpy(), out, bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True))

@@ -180,3 +180,17 @@ def test_plans_of_the_largest_batches(lib, kvh, hd):
                 c = cfg(n_q_heads=8 * kvh, n_kv_heads=kvh, head_dim=hd, window=window)
                 need = lib.g4a_decode_ws_bytes(ctypes.byref(c), n_seq, keys)
                 assert 0 < need <= (512 + 2 * n_seq * kvh) * 8 * (hd * 4 + 8 + 8) + 1024, (n_seq, keys, window)
+
+
+@pytest.mark.parametrize("flags", [0, _lib.KV_F32])
+@pytest.mark.parametrize("kvh,hd", [(1, 256), (8, 512), (64, 512), (512, 512)])
+def test_long_bounds_are_not_refused(lib, kvh, hd, flags):
+    """A decode call whose workspace has a size is not refused for its max_key_len: with no workspace, that
+    is all that is wrong with it."""
+    for n_seq in (1, 2, 64, 100):
+        for keys in (1000, 131072, 1 << 20, 1 << 26, 1 << 30):
+            c, pg = cfg(n_q_heads=8 * kvh, n_kv_heads=kvh, head_dim=hd, flags=flags), paged(
+                n_seq=n_seq, page_size=65536, table_cols=1 << 14, table_stride=1 << 14, max_key_len=keys)
+            assert lib.g4a_paged_decode_ws_bytes(ctypes.byref(c), ctypes.byref(pg)) > 0
+            far = 1 << 44
+            assert decode(lib, c=c, pg=pg, q=far, out=2 * far, ws=None) == W, (n_seq, keys, lib.g4a_last_error())
