@@ -124,3 +124,33 @@ def test_decode_long_bounds(hd, kvh, kv, page, bound_keys, n):
     out, A, S = b.oracle(rope=False)
     got = decode(b, b.dev(table=torch.from_numpy(table).cuda()), rope_cos=None, rope_sin=None, max_key_len=bound_keys)
     check(got.cpu().numpy(), out, bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True))
+
+
+@pytest.mark.parametrize("n,kvh,hd,kv,longest", [(33, 8, 256, np.float16, 3100), (65, 4, 256, np.float16, 3900), (300, 2, 256, np.float16, 10000),
+                                                 (264, 1, 512, np.float16, 4500), (280, 1, 256, np.float32, 4700)])
+@pytest.mark.parametrize("append", [False, True])
+def test_decode_one_long_sequence_among_many(n, kvh, hd, kv, longest, append):
+    """More pairs than workgroups that run at once, one long sequence and idle ones: the work list, whose
+    partials show in the workspace. (scale 0.25: no weight is subnormal in f16.)"""
+    keys = [1 + 29 * i % 70 for i in range(n)]
+    keys[n // 2], keys[n - 1], keys[3] = longest, 0, 0
+    b = Batch(keys, [1] * n, hd=hd, kvh=kvh, kv=kv, page=64)
+    b.q = np.random.default_rng(1).standard_normal((n, 8, hd)).astype(np.float32)
+    d = b.dev()
+    w = ws().reserve(sa.paged_decode_ws_bytes(n, 1 << 16, b.cfg(), page_size=64, kv_f32=kv is np.float32))
+    w.buf.zero_()
+    new = {}
+    if append:
+        new = dict(k_new=torch.randn(n, kvh, hd, device="cuda"), v_new=torch.randn(n, kvh, hd, device="cuda"), v_norm=False)
+    got = decode(b, d, rope_cos=None, rope_sin=None, cfg=b.cfg(scale=0.25), workspace=w, **new)
+    assert w.buf.any()
+    rows = [0, 3, n // 2, n // 2 + 1, n - 2, n - 1]
+    want, A, S = b.oracle(q=b.q[rows], tokens=[(i, keys[i] - 1) for i in rows], rope=False, scale=0.25,
+                          k_pages=d["k_pages"].cpu().numpy(), v_pages=d["v_pages"].cpu().numpy())
+    check(got.cpu().numpy()[rows], want, bound(want, A, S, q16=False, kv32=kv is np.float32, out16=True))
+    for i in rows:
+        if append and keys[i]:
+            p = keys[i] - 1
+            at = int(b.table[i, p // 64]), p % 64
+            assert torch.equal(d["k_pages"][at], new["k_new"][i].to(d["k_pages"].dtype))
+            assert torch.equal(d["v_pages"][at], new["v_new"][i].to(d["v_pages"].dtype))
