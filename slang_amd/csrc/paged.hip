@@ -83,16 +83,11 @@ __global__ __launch_bounds__(HD / 2) void paged_write_kernel(PagedWriteArgs a) {
     constexpr int HALF = HD / 2, NW = HALF / 64;
     __shared__ float red[2 * NW];
     const int t = threadIdx.x, tok = blockIdx.x, kh = blockIdx.y;
-    int b = tok, p;  // without cu, row b is sequence b's last key
-    if (a.cu) {
-        b = seq_of_row(a.cu, a.t.n_seq, tok);
-        if (b >= a.t.n_seq) return;
-        const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
-        if (!holds(r, tok)) return;
-        p = row_position(r, tok);
-    } else {
-        p = paged_len(a.t, b) - 1;
-    }
+    const int b = seq_of_row(a.cu, a.t.n_seq, tok);
+    if (b >= a.t.n_seq) return;
+    const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
+    if (!holds(r, tok)) return;
+    const int p = row_position(r, tok);
     if (p < 0) return;
     const int page = page_at(a.t, b, p);
     if (!page_ok(a.t, page)) return;

@@ -1214,14 +1214,13 @@ static paged_prefill_fn pick_out(int HD, bool out32) {
     if (HD == 256) return out32 ? paged_prefill_kernel_256<G, float> : paged_prefill_kernel_256<G, half_t>;
     return out32 ? paged_prefill_kernel_512<G, float> : paged_prefill_kernel_512<G, half_t>;
 }
-static paged_prefill_fn pick_paged(int HD, int G, bool out32) {
+static paged_prefill_fn pick_paged(int HD, int G, bool out32) {  // G: 1, 2, 4 or 8 (check_cfg)
     switch (G) {
         case 1: return pick_out<1>(HD, out32);
         case 2: return pick_out<2>(HD, out32);
         case 4: return pick_out<4>(HD, out32);
-        case 8: return pick_out<8>(HD, out32);
+        default: return pick_out<8>(HD, out32);
     }
-    return nullptr;
 }
 static paged_prefill_fn pick_paged_merge(int HD, bool out32) {
     if (HD == 256) return out32 ? paged_merge_kernel<float, 256> : paged_merge_kernel<half_t, 256>;
@@ -1372,12 +1371,7 @@ extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_
     else hipLaunchKernelGGL(paged_prep_kernel<512>, pgrid, dim3(256), 0, stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged prefill preparation launch");
     const bool out32 = (cfg->flags & G4A_OUT_F32) != 0;
-    const paged_prefill_fn fn = pick_paged(HD, G, out32);
-    if (!fn) {
-        set_error("no prefill kernel for group size %d", G);
-        return G4A_EUNSUPPORTED;
-    }
-    hipLaunchKernelGGL(fn, dim3((unsigned)p.max_units), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(pick_paged(HD, G, out32), dim3((unsigned)p.max_units), dim3(256), 0, stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged prefill launch");
     if (p.max_slots > 0) {  // a block of the merge list has two slots at least
         hipLaunchKernelGGL(pick_paged_merge(HD, out32), dim3((unsigned)p.max_slots / 2, 4 * (HD / 256)), dim3(256), 0, stream, a);

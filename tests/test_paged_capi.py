@@ -194,3 +194,13 @@ def test_long_bounds_are_not_refused(lib, kvh, hd, flags):
             assert lib.g4a_paged_decode_ws_bytes(ctypes.byref(c), ctypes.byref(pg)) > 0
             far = 1 << 44
             assert decode(lib, c=c, pg=pg, q=far, out=2 * far, ws=None) == W, (n_seq, keys, lib.g4a_last_error())
+
+
+@pytest.mark.parametrize("groups", [3, 5, 6, 7, 12, 16])
+def test_group_sizes_without_a_kernel(lib, groups):
+    """Refused before anything is launched, with the sizes that are taken named."""
+    c = cfg(n_q_heads=2 * groups, n_kv_heads=2)
+    for call in (decode, prefill):
+        assert call(lib, c=c) == E and b"1, 2, 4 or 8" in lib.g4a_last_error()
+    assert lib.g4a_paged_decode_ws_bytes(ctypes.byref(c), ctypes.byref(paged())) == 0
+    assert lib.g4a_paged_prefill_ws_bytes(ctypes.byref(c), ctypes.byref(paged()), 8) == 0
