@@ -33,6 +33,7 @@ __all__ = [
 @dataclass(frozen=True)
 class AttnConfig:
     """Per-layer attention constants (the reference bakes them into kernel consts)."""
+    __slots__ = ("__dict__", "__weakref__", "_refs")  # c_ref's cache beside the fields: vars() is the fields alone
     n_q_heads: int
     n_kv_heads: int
     head_dim: int
@@ -48,9 +49,13 @@ class AttnConfig:
     def c_ref(self, flags: int):
         """c(flags) as a ctypes argument, made once per flags (the instance is frozen; the library only
         reads it)."""
-        ref = self.__dict__.get(flags)
-        if ref is None:
-            ref = self.__dict__[flags] = ctypes.byref(self.c(flags))
+        try:
+            return self._refs[flags]
+        except AttributeError:
+            object.__setattr__(self, "_refs", {})
+        except KeyError:
+            pass
+        ref = self._refs[flags] = ctypes.byref(self.c(flags))
         return ref
 
     def __getstate__(self):  # the fields alone: a ctypes reference can be neither copied nor pickled

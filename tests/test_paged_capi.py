@@ -3,6 +3,7 @@ import copy
 import ctypes
 import dataclasses
 import pickle
+import weakref
 
 import numpy as np
 import pytest
@@ -204,3 +205,24 @@ def test_group_sizes_without_a_kernel(lib, groups):
         assert call(lib, c=c) == E and b"1, 2, 4 or 8" in lib.g4a_last_error()
     assert lib.g4a_paged_decode_ws_bytes(ctypes.byref(c), ctypes.byref(paged())) == 0
     assert lib.g4a_paged_prefill_ws_bytes(ctypes.byref(c), ctypes.byref(paged()), 8) == 0
+
+
+def test_used_configs_are_their_fields():
+    """What a call keeps of a config stays out of vars(), copies and pickles of every protocol."""
+    @dataclasses.dataclass(frozen=True)
+    class Named(sa.AttnConfig):
+        name: str = "x"
+    for c in (sa.AttnConfig(8, 2, 256, window=100), Named(8, 2, 256, name="y")):
+        names = {f.name for f in dataclasses.fields(c)}
+        for flags in (0, 3, 3):
+            got = ctypes.cast(c.c_ref(flags), ctypes.POINTER(G4ACfg)).contents
+            assert (got.n_kv_heads, got.flags) == (2, flags)
+        assert c.c_ref(3) is c.c_ref(3)
+        assert set(vars(c)) == names and type(c)(**vars(c)) == c and dataclasses.asdict(c) == vars(c)
+        with pytest.raises(dataclasses.FrozenInstanceError):
+            c.window = 3
+        assert copy.copy(c) == c and copy.deepcopy(c) == c and weakref.ref(c)() is c
+    c = sa.AttnConfig(8, 2, 256)
+    c.c_ref(0)
+    for protocol in range(pickle.HIGHEST_PROTOCOL + 1):
+        assert pickle.loads(pickle.dumps(c, protocol)) == c
