@@ -217,6 +217,7 @@ int g4a_kv_write(const g4a_cfg* cfg, int S, int start_pos, const void* k, const 
  * .. key_len[b] - 1. Rows from cu_q[n_seq] on belong to nobody: nothing is stored for them, and their
  * outputs are left as they were. A token at a position below zero attends nothing (zeros). Offsets that
  * do not ascend: no memory but the call's own is touched, what it holds is undefined.
+ * n_tokens is at least 1.
  * RoPE tables: f32 [max_key_len][head_dim / 2] at least, indexed by absolute position.
  * Two rows of one call that map to the same cache row (a page listed twice) must not be written.
  * Zero-initialise the struct: later versions may take over its reserved words.

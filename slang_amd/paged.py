@@ -11,7 +11,8 @@ sequences of unknown length keeps their rows in pages instead:
     its positions are neither written nor attended (-1 for pages behind a sliding window);
   * ``key_len`` int32 [n_seq]: the keys of each sequence, this call's tokens included; 0 = idle;
   * ``cu_q`` int32 [n_seq + 1]: packed rows cu_q[b] .. cu_q[b+1]-1 are sequence b's tokens, its last
-    ones. Rows from cu_q[n_seq] on belong to nobody: nothing is stored for them, their outputs stay;
+    ones. Rows from cu_q[n_seq] on belong to nobody: nothing is stored for them, their outputs stay. A call
+    of no packed rows, or no sequences, has nothing to do (its operands are checked all the same);
   * ``rope_cos`` / ``rope_sin`` f32 [>= max_key_len][hd/2]: ``rope_tables`` over absolute positions.
 
 All of these live on one GPU, so lengths and tables can change between replays of a captured
@@ -162,10 +163,13 @@ def paged_write(k, v, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConf
     if rows not in _HALF_OR_FLOAT:
         raise ValueError(f"k and v must be float16 or float32, got {rows}")
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
+    cu, kp, vp, kg = _cu(cu_q, pg.n_seq, dev), _t("k", k, dev, rows), _t("v", v, dev, rows), _t("k_gain", k_gain, dev, _F32)
+    if k.shape[0] == 0:
+        return
     c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.IN_F16 if rows is _F16 else 0) |
                   (0 if v_norm else _lib.NO_V_NORM))
-    check(_launch(dev, _lib.load().g4a_paged_write, c, ctypes.byref(pg), k.shape[0], _cu(cu_q, pg.n_seq, dev),
-                  _t("k", k, dev, rows), _t("v", v, dev, rows), float(k_in_q), float(v_in_q), _t("k_gain", k_gain, dev, _F32), rc, rs))
+    check(_launch(dev, _lib.load().g4a_paged_write, c, ctypes.byref(pg), k.shape[0], cu, kp, vp, float(k_in_q), float(v_in_q),
+                  kg, rc, rs))
 
 
 def _out(out, q, out_dtype, dev):
@@ -225,6 +229,8 @@ def paged_decode(q, k_pages, v_pages, page_table, key_len, cfg: AttnConfig, *, w
         if k_new.shape != (pg.n_seq, cfg.n_kv_heads, cfg.head_dim) or v_new.shape != k_new.shape:
             raise ValueError(f"k_new and v_new must be [{pg.n_seq}][{cfg.n_kv_heads}][{cfg.head_dim}]")
     out = _out(out, q, out_dtype, dev)
+    if pg.n_seq == 0:
+        return out
     k_in_q, v_in_q = float(k_in_q), float(v_in_q)
     c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0) |
                   (0 if v_norm else _lib.NO_V_NORM))
@@ -257,6 +263,8 @@ def paged_prefill(q, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConfi
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
     cu, n = _cu(cu_q, pg.n_seq, dev), q.shape[0]
     out = _out(out, q, out_dtype, dev)
+    if n == 0:
+        return out
     c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.OUT_F32 if out.dtype is _F32 else 0))
     lib, at, p = _lib.load(), out.data_ptr(), ctypes.byref(pg)
     _with_scratch(workspace, dev, lambda: lib.g4a_paged_prefill_ws_bytes(c, p, n),

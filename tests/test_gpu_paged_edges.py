@@ -154,3 +154,31 @@ def test_decode_one_long_sequence_among_many(n, kvh, hd, kv, longest, append):
             at = int(b.table[i, p // 64]), p % 64
             assert torch.equal(d["k_pages"][at], new["k_new"][i].to(d["k_pages"].dtype))
             assert torch.equal(d["v_pages"][at], new["v_new"][i].to(d["v_pages"].dtype))
+
+
+# ---------------------------------------------------------------- empty calls
+@pytest.mark.parametrize("kv", [np.float16, np.float32])
+def test_calls_without_tokens(kv):
+    """A step that brings no prompt: nothing is written, the outputs are empty, wrong operands are refused."""
+    b = Batch([40, 0], [0, 0], kv=kv)
+    d = b.dev()
+    none = dict(d, q=d["q"][:0], k_new=d["k_new"][:0], v_new=d["v_new"][:0])
+    write(b, none)
+    write(b, none, rows=(none["k_new"].half(), none["v_new"].half()))
+    w = ws()
+    got = prefill(b, none, workspace=w)
+    assert got.shape == (0, 8, 256) and got.dtype is torch.float16 and w.buf is None
+    out = torch.empty(0, 8, 256, device="cuda")
+    assert prefill(b, none, workspace=w, out=out) is out
+    for name in ("k_pages", "v_pages"):
+        assert np.array_equal(bits(d[name]), getattr(b, name).reshape(-1).view(np.uint8).reshape(bits(d[name]).shape))
+    with pytest.raises(ValueError):
+        write(b, dict(none, cu=d["cu"][:2].contiguous()))
+    with pytest.raises(ValueError):
+        prefill(b, none, out=torch.empty(1, 8, 256, device="cuda"))
+    with pytest.raises(ValueError):
+        prefill(b, dict(none, q=none["q"].half()))
+    empty = dict(none, table=d["table"][:0], key_len=d["key_len"][:0], cu=d["cu"][:1].contiguous())
+    write(b, empty)
+    for got in (decode(b, empty), decode(b, empty, append=True), prefill(b, empty)):
+        assert got.shape == (0, 8, 256)
