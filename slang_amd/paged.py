@@ -63,6 +63,15 @@ def _t(name, t, dev, dtype):
     return t.data_ptr()
 
 
+def _gain(name, t, dev, cfg):
+    """Address of a norm's gains, one per dim: the kernels read head_dim of them."""
+    if t is None:
+        return None
+    if t.numel() != cfg.head_dim:
+        raise ValueError(f"{name} must hold head_dim ({cfg.head_dim}) gains, got {tuple(t.shape)}")
+    return _t(name, t, dev, _F32)
+
+
 def _gpu(name, t):
     """The GPU that a call's first tensor is on: every other operand has to be there."""
     dev = t.get_device()
@@ -163,7 +172,7 @@ def paged_write(k, v, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConf
     if rows not in _HALF_OR_FLOAT:
         raise ValueError(f"k and v must be float16 or float32, got {rows}")
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
-    cu, kp, vp, kg = _cu(cu_q, pg.n_seq, dev), _t("k", k, dev, rows), _t("v", v, dev, rows), _t("k_gain", k_gain, dev, _F32)
+    cu, kp, vp, kg = _cu(cu_q, pg.n_seq, dev), _t("k", k, dev, rows), _t("v", v, dev, rows), _gain("k_gain", k_gain, dev, cfg)
     if k.shape[0] == 0:
         return
     c = cfg.c_ref((_lib.KV_F32 if k_pages.dtype is _F32 else 0) | (_lib.IN_F16 if rows is _F16 else 0) |
@@ -189,7 +198,7 @@ def _q(q, cfg, q_gain):
     if len(shape) != 3 or shape[1] != cfg.n_q_heads or shape[2] != cfg.head_dim:
         raise ValueError(f"q shape {tuple(shape)} does not match {cfg}")
     dev = _gpu("q", q)
-    return dev, _t("q", q, dev, _F32), _t("q_gain", q_gain, dev, _F32)
+    return dev, _t("q", q, dev, _F32), _gain("q_gain", q_gain, dev, cfg)
 
 
 def _sizes(n_pages, page_size, n_seq, cols, max_key_len) -> G4APaged:
@@ -225,7 +234,7 @@ def paged_decode(q, k_pages, v_pages, page_table, key_len, cfg: AttnConfig, *, w
     if (k_new is None) != (v_new is None):
         raise ValueError("k_new and v_new go together")
     if k_new is not None:
-        kn, vn, kg = _t("k_new", k_new, dev, _F32), _t("v_new", v_new, dev, _F32), _t("k_gain", k_gain, dev, _F32)
+        kn, vn, kg = _t("k_new", k_new, dev, _F32), _t("v_new", v_new, dev, _F32), _gain("k_gain", k_gain, dev, cfg)
         if k_new.shape != (pg.n_seq, cfg.n_kv_heads, cfg.head_dim) or v_new.shape != k_new.shape:
             raise ValueError(f"k_new and v_new must be [{pg.n_seq}][{cfg.n_kv_heads}][{cfg.head_dim}]")
     out = _out(out, q, out_dtype, dev)

@@ -182,3 +182,17 @@ def test_calls_without_tokens(kv):
     write(b, empty)
     for got in (decode(b, empty), decode(b, empty, append=True), prefill(b, empty)):
         assert got.shape == (0, 8, 256)
+
+
+# ---------------------------------------------------------------- refusals of what would be read past its end
+def test_gains_of_another_length_are_refused():
+    b = Batch([40, 20], [1, 1])
+    d = b.dev()
+    for bad in (d["gain"][:255].contiguous(), d["gain"][:1], torch.ones(512, device="cuda"), torch.ones(2, 256, device="cuda")):
+        for call in (lambda: decode(b, dict(d, gain=bad)), lambda: prefill(b, dict(d, gain=bad)),
+                     lambda: write(b, dict(d, k_gain=bad)), lambda: decode(b, dict(d, k_gain=bad), append=True)):
+            with pytest.raises(ValueError):
+                call()
+    out, A, S = b.oracle()
+    got = decode(b, dict(d, gain=d["gain"].view(1, 256)))
+    check(got.cpu().numpy(), out, bound(out, A, S, q16=False, kv32=False, out16=True))
