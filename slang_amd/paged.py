@@ -37,7 +37,7 @@ __all__ = ["paged_write", "paged_decode", "paged_decode_ws_bytes", "paged_prefil
 
 _F32, _F16, _I32 = torch.float32, torch.float16, torch.int32
 _HALF_OR_FLOAT = (_F16, _F32)
-_EWORKSPACE = -3
+_EWORKSPACE, _I32_MAX = -3, 2 ** 31 - 1
 
 
 # A decode step of short sequences is bound by this layer, not by its kernels: the checks below touch each
@@ -104,6 +104,8 @@ def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_co
     stride = page_table.stride(0) if n_seq > 1 else cols
     if stride < cols:
         raise ValueError("page_table rows must not overlap")
+    if stride > _I32_MAX or n_seq > _I32_MAX:  # the library's struct holds 32 bits
+        raise ValueError(f"page_table's rows lie too far apart, or are too many ({n_seq} rows, {stride} entries apart)")
     lens = _t("key_len", key_len, dev, _I32)
     if key_len.numel() != n_seq:
         raise ValueError(f"key_len must have one entry per row of page_table ({n_seq}), got {key_len.numel()}")

@@ -196,3 +196,15 @@ def test_gains_of_another_length_are_refused():
     out, A, S = b.oracle()
     got = decode(b, dict(d, gain=d["gain"].view(1, 256)))
     check(got.cpu().numpy(), out, bound(out, A, S, q16=False, kv32=False, out16=True))
+
+
+def test_table_rows_too_far_apart_are_refused():
+    """A row stride past 32 bits, which cut to them would read other entries."""
+    b = Batch([40, 20], [1, 1], extra_cols=0)
+    wide = torch.empty(2 ** 32 + 2 * b.cols, dtype=torch.int32, device="cuda")
+    table = wide.as_strided((2, b.cols), (2 ** 32 + b.cols, 1))
+    table.copy_(torch.from_numpy(b.table))
+    d = b.dev(table=table)
+    for call in (lambda: decode(b, d), lambda: prefill(b, d), lambda: write(b, d)):
+        with pytest.raises(ValueError):
+            call()
