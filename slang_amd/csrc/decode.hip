@@ -738,11 +738,9 @@ void decode_kernel(A a) {
 // multiplied in, whatever their weight, so that a key, value or query that is not finite gives NaN
 // however the keys were split, as in one softmax over all of them.
 // Weight of a split's partial (m, l) at the maximum M; below zero: nothing to add. A split whose
-// scores are all NaN has m = -inf, as a maximum passes NaN over, but l = NaN.
-__device__ __forceinline__ float split_weight(float m, float l, float M) {
-    if (l == 0.0f) return -1.0f;
-    return l != l ? l : fexp2(m - M);
-}
+// scores are all NaN has m = -inf, as a maximum passes NaN over, but l = NaN and o = NaN, which no
+// weight hides.
+__device__ __forceinline__ float split_weight(float m, float l, float M) { return l == 0.0f ? -1.0f : fexp2(m - M); }
 template <typename A>
 __device__ __forceinline__ void store_merged(const A& a, size_t at, float v) {
     if constexpr (std::is_same_v<A, PagedDecodeArgs>) {
