@@ -56,11 +56,8 @@ struct PagedPrefillArgs {
 };
 
 // ---------------------------------------------------------------- the work list
-// Key tiles of query block qb: keys [first & ~15, min(p0 + bq, start + S)).
 __device__ __forceinline__ int block_tiles(const PagedPrefillArgs& a, int start, int S, int qb) {
-    const int p0 = start + qb * a.bq, hi = min(p0 + a.bq, start + S);
-    const int first = a.window > 0 ? max(0, p0 + 1 - a.window) : 0;
-    return max(0, (hi - (first & ~15) + a.kt - 1) / a.kt);
+    return key_tiles(start, S, qb, a.bq, a.kt, a.window);
 }
 
 // Cost of the units, in key tiles: a unit's own beside its tiles (q, epilogue), a partial's store and
@@ -167,7 +164,7 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
         int mx = 0;
         if (nb > 0) mx = block_tiles(a, s_start[tid], s_S[tid], nb - 1);
         if (nb > 1) mx = max(mx, block_tiles(a, s_start[tid], s_S[tid], nb - 2));
-        mx = (int)wave_max((float)mx);  // (at most 2^25 tiles)
+        mx = (int)wave_max((float)mx);
         const float blocks = wave_sum((float)((s_S[tid] + a.bq - 1) / a.bq));
         if (lane == 0) {
             atomicMax(&s_max, mx);
@@ -181,7 +178,7 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
         if (tid == 0) a.counts[0] = a.counts[1] = 0;
         return;
     }
-    const int longest = s_max;
+    const int longest = tiles_at_least(s_max);
     const int st_min = a.kt == 64 ? 2 : 4;  // tiles a piece at least
     const auto cut = [&](int k) { return max((longest + k - 1) / k, k == 1 ? 1 : st_min); };
     int st = cut(1);

@@ -20,4 +20,16 @@ constexpr SeqRows cut_rows(int begin, int end, int n_tokens, int keys) {
 constexpr bool holds(const SeqRows& r, int tok) { return tok >= r.lo && tok < r.hi; }
 constexpr int row_position(const SeqRows& r, int tok) { return r.keys - r.hi + tok; }  // below keys if r holds tok
 
+// Key tiles of query block qb of a sequence whose S tokens start at position `start`: keys
+// [first & ~15, min(p0 + bq, start + S)), first the first one that the block attends.
+constexpr int key_tiles(int start, int S, int qb, int bq, int kt, int window) {
+    const int p0 = start + qb * bq, hi = p0 + bq < start + S ? p0 + bq : start + S;
+    const int front = p0 + 1 - window, first = window > 0 ? (front > 0 ? front : 0) : 0;
+    const int n = (hi - (first & ~15) + kt - 1) / kt;
+    return n > 0 ? n : 0;
+}
+// A bound of a count (2^25 at most) that went through a 32-bit float, which above 2^24 may have made it one
+// less: a longest block taken for shorter than it is would be cut where no partial has room.
+constexpr int tiles_at_least(int rounded) { return rounded + (rounded >> 24); }
+
 }  // namespace g4a

@@ -107,3 +107,40 @@ constexpr bool all() {
 }
 static_assert(all(), "a row of another sequence");
 """)
+
+
+def test_tiles_of_the_longest_blocks(tmp_path):
+    """Up to 2^30 keys: no step of the count, of a size class (63 classes of tiles) or of a piece's range (8 pieces)
+    overflows, and a count that went through a 32-bit float is not taken for less than it is."""
+    holds(tmp_path, """
+constexpr int kMost = 1 << 30;
+constexpr bool fits(int keys, int S, int bq, int kt, int window) {
+    const int nb = (S + bq - 1) / bq;
+    for (int qb : {0, nb / 2, nb - 1}) {
+        const int64_t p0 = (int64_t)keys - S + (int64_t)qb * bq, hi = p0 + bq < keys ? p0 + bq : keys;
+        const int64_t first = window > 0 && p0 + 1 > window ? p0 + 1 - window : 0, span = hi - first / 16 * 16;
+        const int64_t want = span > 0 ? (span + kt - 1) / kt : 0;
+        const int n = key_tiles(keys - S, S, qb, bq, kt, window);
+        if (n != want || (int64_t)n * 63 > 0x7fffffff || (int64_t)n * 8 > 0x7fffffff) return false;
+    }
+    return true;
+}
+constexpr bool all() {
+    for (int keys : {1, 15, 16, 17, 1000, kMost - 33, kMost - 1, kMost})
+        for (int S : {1, 16, 100, 4000, 1 << 26})
+            for (int bq : {16, 32, 64, 128})
+                for (int kt : {32, 64})
+                    for (int window : {0, 1, 16, 512, kMost})
+                        if (!fits(keys, S, bq, kt, window)) return false;
+    return true;
+}
+static_assert(all(), "a count that overflows");
+constexpr bool bounded() {
+    for (int n = 1; n < 1 << 25; n += n < 1 << 23 ? n / 8 + 1 : 997)
+        if (tiles_at_least((int)(float)n) < n || (n <= 1 << 24 && n != 1 << 24 && tiles_at_least((int)(float)n) != n)) return false;
+    return tiles_at_least((int)(float)(1 << 25)) >= 1 << 25;
+}
+static_assert(bounded(), "a count taken for less");
+constexpr int n = key_tiles(32 * ((1 << 24) + 1) - 1, 1, 0, 16, 32, 0);
+static_assert(n > 1 << 24 && (int)(float)n < n && tiles_at_least((int)(float)n) >= n, "");
+""")
