@@ -84,6 +84,12 @@ struct PagedDecodeArgs : DecodeArgs {
     int out16;  // f16 output
 };
 
+// P enters an f16 product, whose normal range ends at 2^-14. Over a paged cache the running maxima are held
+// this many powers of two below the scores', so that P reaches 2^15 and a key keeps all bits down to 2^-29 of
+// the largest weight (2^-14 without; zero below 2^-25, where l still counts it: 20000 keys of 2^-26 beside a
+// large one were lost). m, l and o share the factor, which the division takes out.
+constexpr float kDecodeLift = 15.0f;
+
 template <int HD, int G>
 struct DecodeShape {
     static constexpr int KSTEPS = HD / 32;         // score MFMA k-steps per 16-key block
@@ -658,6 +664,7 @@ void decode_kernel(A a) {
             mloc = fmaxf(mloc, sc[i]);
         }
         mloc = max32(max16(mloc));
+        if constexpr (PAGED) mloc -= kDecodeLift;
         // finite for heads, as key blk is valid (but for a paged block without an attended key)
         const float m_new = fmaxf(m_run, mloc);
         const float m_use = (m_new == kNegInf) ? 0.0f : m_new;  // such columns and the padding's stay at zero

@@ -208,3 +208,69 @@ def test_table_rows_too_far_apart_are_refused():
     for call in (lambda: decode(b, d), lambda: prefill(b, d), lambda: write(b, d)):
         with pytest.raises(ValueError):
             call()
+
+
+# ---------------------------------------------------------------- long contexts at scale 1
+def long_tables(b, keys):
+    c, s = sa.rope_tables(np.arange(keys), b.hd, 1e6, device="cpu")
+    b.cos, b.sin = c.numpy(), s.numpy()
+
+
+@pytest.mark.parametrize("hd,keys", [(256, 33000), (512, 20000)])
+def test_prefill_long_history_at_scale_1(hd, keys):
+    b = Batch([keys, 70], [37, 70], hd=hd, kvh=1, page=64)
+    long_tables(b, keys)
+    rows = [0, 17, 36, 37, 106]
+    out, A, S = (x[rows] for x in b.oracle(tokens=[t if i in rows else None for i, t in enumerate(b.tokens())]))
+    got = prefill(b, b.dev())
+    check(got.cpu().numpy()[rows], out, bound(out, A, S, q16=True, kv32=False, out16=True))
+
+
+@pytest.mark.parametrize("hd,kv,n", [(256, np.float16, 1), (256, np.float16, 128), (512, np.float16, 64), (256, np.float32, 128)])
+def test_decode_long_context_at_scale_1(hd, kv, n):
+    keys = 20000
+    b = Batch([keys], [1], hd=hd, kvh=1, page=64, kv=kv)
+    long_tables(b, keys)
+    d = b.dev()
+    q = np.random.default_rng(2).standard_normal((n, 8, hd)).astype(np.float32)
+    lens = [keys - 17 * i for i in range(n)]
+    got = decode(b, dict(d, q=torch.from_numpy(q).cuda(), table=d["table"].repeat(n, 1), key_len=i32(lens)))
+    rows = sorted({0, n // 3, n - 1})
+    want, A, S = b.oracle(q=q[rows], tokens=[(0, lens[i] - 1) for i in rows])
+    check(got.cpu().numpy()[rows], want, bound(want, A, S, q16=False, kv32=kv is np.float32, out16=True))
+
+
+@pytest.mark.parametrize("hd", [256, 512])
+@pytest.mark.parametrize("kv", [np.float16, np.float32])
+@pytest.mark.parametrize("call", ["decode", "prefill"])
+def test_many_weak_keys_beside_a_strong_one(hd, kv, call):
+    """Weights of 2^-26 of the largest, below f16's smallest number, whose values are all that the output
+    holds: a strong key at the front of every 2048, one in each wave's blocks, with a value of zero."""
+    keys, n, new = 16000, 64, 20
+    b = Batch([keys], [1 if call == "decode" else new], hd=hd, kvh=1, page=64, kv=kv)
+    p = np.arange(keys)
+    strong = (p % 2048 < 64) & (p % 16 == 0)
+    k, v = np.zeros((keys, 1, hd)), np.full((keys, 1, hd), 1024.0)
+    k[strong, 0, 0], v[strong] = 1.0, 0.0
+    at = b.table[0, p // 64] * 64 + p % 64
+    b.k_pages.reshape(-1, 1, hd)[at], b.v_pages.reshape(-1, 1, hd)[at] = k, v
+    b.q = np.zeros((n if call == "decode" else new, 8, hd), np.float32)
+    b.q[..., 0] = 18.0
+    d = b.dev()
+    off = dict(q_gain=None, rope_cos=None, rope_sin=None)
+    if call == "decode":
+        lens = [keys - i for i in range(n)]
+        got = decode(b, dict(d, table=d["table"].repeat(n, 1), key_len=i32(lens)), out_dtype=torch.float32, **off)
+        tokens = [(0, x - 1) for x in lens]
+    else:
+        got, tokens = prefill(b, d, out_dtype=torch.float32, **off), b.tokens()
+    rows = [0, 7, len(tokens) - 1]
+    want, A, S = b.oracle(q=b.q[rows], tokens=[tokens[i] for i in rows], gain=False, rope=False)
+    assert want.min() > 0.005
+    tol = bound(want, A, S, q16=call == "prefill", kv32=kv is np.float32, out16=False, k16=call == "prefill" and kv is np.float32)
+    if call == "prefill":
+        # P of a key is off by at most 2^-25, where the largest is 2^4 or more: 2^-29 sum |v| / sum_t exp(s_t - max s)
+        most = np.array([strong[:tokens[i][1] + 1].sum() for i in rows])
+        tol = tol + (2.0 ** -29 * 1024 * keys / most)[:, None, None]
+        assert (tol < want / 4).all()
+    check(got.cpu().numpy()[rows], want, tol)
