@@ -890,9 +890,16 @@ static long longest_active(const g4a_cfg* cfg, int max_key_len, bool paged) {
 static int decode_chunk(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
     const long pairs = (long)n_seq * cfg->n_kv_heads;
     const long max_active = longest_active(cfg, max_key_len, paged);
-    // paged: few keys in one split per pair, without a merge (us a call, one split / many; kvH 2: 1 x 100 keys
-    // 7.4 / 8.2, 64 x 100 8.2 / 12.2, 1 x 300 11.4 / 8.2; kvH 1: 64 x 300 14.5 / 18.0, 64 x 512 19.9 / 20.0)
-    if (paged && (max_active <= 128 || (max_active <= 320 && pairs >= 64))) return (int)((max_active + 15) & ~15L);
+    // paged: few keys in one split per pair, without a merge. What a split saves is the walk over its rows, so
+    // the bounds of few pairs are in 512-byte rows; of 128 pairs and more, which fill the card, in keys. us a
+    // call, one split / many (pairs x keys): hd 256 f16 2 x 128 9.9 / 10.8, 64 x 320 16.6 / 19.8, 128 x 320 16.0 / 20.2;
+    // hd 512 f16 2 x 64 11.1 / 13.4, 2 x 128 15.2 / 13.1, 64 x 128 15.7 / 16.6, 64 x 320 24.3 / 21.8, 128 x 320
+    // 25.4 / 31.1; hd 256 f32 2 x 64 11.5 / 12.1, 2 x 128 16.5 / 12.4, 64 x 320 30.8 / 21.3, 128 x 320 32.2 / 36.2; hd 512 f32
+    // 8 x 64 30.0 / 31.8, 2 x 64 29.0 / 26.8, 2 x 128 55 / 27, 64 x 320 139 / 66, 128 x 320 149 / 142, 200 x 320 147 / 153.
+    if (paged) {
+        const long rows = max_active * cfg->head_dim * ((cfg->flags & G4A_KV_F32) ? 4 : 2) / 512;
+        if (rows <= 128 || (rows <= 320 && pairs >= 64) || (max_active <= 320 && pairs >= 128)) return (int)((max_active + 15) & ~15L);
+    }
     const long target = kDecodeTargetWgs;
     const long min_chunk = kDecodeMinChunk;
     const long kp = max_active * pairs;

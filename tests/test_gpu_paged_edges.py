@@ -274,3 +274,21 @@ def test_many_weak_keys_beside_a_strong_one(hd, kv, call):
         tol = tol + (2.0 ** -29 * 1024 * keys / most)[:, None, None]
         assert (tol < want / 4).all()
     check(got.cpu().numpy()[rows], want, tol)
+
+
+# ---------------------------------------------------------------- one split or many
+@pytest.mark.parametrize("hd,kv,n,kvh,keys,one", [
+    (256, np.float16, 1, 2, 128, True), (256, np.float16, 1, 2, 129, False), (256, np.float16, 64, 1, 320, True), (256, np.float16, 64, 1, 321, False),
+    (512, np.float16, 1, 2, 64, True), (512, np.float16, 1, 2, 65, False), (512, np.float16, 32, 2, 161, False), (512, np.float16, 64, 2, 320, True),
+    (256, np.float32, 1, 2, 64, True), (256, np.float32, 1, 2, 65, False), (256, np.float32, 64, 1, 160, True), (256, np.float32, 64, 1, 200, False),
+    (512, np.float32, 1, 2, 32, True), (512, np.float32, 1, 2, 33, False), (512, np.float32, 32, 2, 81, False), (512, np.float32, 64, 2, 320, True)])
+def test_decode_few_keys(hd, kv, n, kvh, keys, one):
+    """Either side of the bounds below which a pair's keys are one split (no partials in the workspace), by
+    the bytes of a row."""
+    b = Batch([keys - i % 3 for i in range(n)], [1] * n, hd=hd, kvh=kvh, kv=kv)
+    w = ws().reserve(sa.paged_decode_ws_bytes(n, keys, b.cfg(), page_size=16, kv_f32=kv is np.float32))
+    w.buf.zero_()
+    got = decode(b, b.dev(), workspace=w, max_key_len=keys)
+    assert bool(w.buf.any()) != one
+    out, A, S = b.oracle()
+    check(got.cpu().numpy(), out, bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True))
