@@ -9,6 +9,7 @@ from paged_cases import Batch, bound, check
 from test_gpu_paged import bits, decode, prefill, write, ws
 
 pytestmark = pytest.mark.gpu
+MAX_KEYS = 2048
 
 
 def i32(x):
@@ -292,3 +293,104 @@ def test_decode_few_keys(hd, kv, n, kvh, keys, one):
     assert bool(w.buf.any()) != one
     out, A, S = b.oracle()
     check(got.cpu().numpy(), out, bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True))
+
+
+# ---------------------------------------------------------------- calls that the documents allow
+@pytest.mark.parametrize("hd,kvh", [(256, 2), (512, 1)])
+@pytest.mark.parametrize("window", [0, 60])
+def test_f32_prefill_missing_and_shared_pages(hd, kvh, window):
+    """f32 caches: pages that are not there, a prefix shared by two sequences, idle sequences, a loose bound."""
+    b = Batch([100, 48, 150, 0, 90], [60, 48, 20, 0, 33], hd=hd, kvh=kvh, kv=np.float32, window=window, pad=3,
+              missing=[(0, 0), (0, 4), (1, 0), (1, 1), (1, 2), (2, 6), (2, 9)])
+    b.table[4, :2] = b.table[2, :2]
+    k, v = b.k_pages.copy(), b.v_pages.copy()  # the shared pages hold rows for both sequences' windows
+    r = np.random.default_rng(5)
+    for pool in (k, v):
+        pool[b.table[2, :2]] = r.standard_normal((2, 16, kvh, hd)) * (0.4 if pool is k else 1)
+    out, A, S = b.oracle(k_pages=k, v_pages=v)
+    live = np.array([t is not None for t in b.tokens()])
+    table = np.pad(b.table, ((0, 0), (0, 20)), constant_values=-1)
+    for max_key_len in (150, 300):
+        got = prefill(b, b.dev(table=torch.from_numpy(table).cuda(), k_pages=torch.from_numpy(k).cuda(), v_pages=torch.from_numpy(v).cuda()),
+                      max_key_len=max_key_len).cpu().numpy()
+        check(got[live], out[live], bound(out, A, S, q16=True, kv32=True, out16=True, k16=True)[live])
+
+
+@pytest.mark.parametrize("hd", [256, 512])
+@pytest.mark.parametrize("keys,new", [([70, 200], [70, 33]), ([1900, 40], [9, 40])])  # whole blocks; pieces
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_prefill_quantised_outputs(hd, keys, new, dt):
+    b = Batch(keys, new, hd=hd, kvh=2)
+    out, A, S = b.oracle()
+    step = 0.015625
+    got = prefill(b, b.dev(), cfg=b.cfg(out_q=step), out_dtype=dt).float().cpu().numpy()
+    k = got / step
+    assert (k == np.round(k)).all() and k.min() >= -128 and k.max() <= 127  # a step of 2^-6: exact in both types
+    exact = np.clip(out, -128 * step, 127 * step)
+    check(got, exact, bound(out, A, S, q16=True, kv32=False, out16=False) + step / 2)
+
+
+@pytest.mark.parametrize("hd,kvh,kv", [(256, 2, np.float16), (512, 1, np.float32)])
+def test_captured_appends(hd, kvh, kv):
+    """Steps that append, captured once and replayed: each replay adds the next row, as the eager calls do."""
+    keys, steps = [150, 1, 900], 4
+    b = Batch([k + steps + 1 for k in keys], [1] * 3, hd=hd, kvh=kvh, kv=kv)
+    rows = [torch.randn(steps + 1, 3, h, hd, device="cuda") for h in (8, kvh, kvh)]
+    eager, graphed = b.dev(), b.dev()
+    for d in (eager, graphed):
+        d["key_len"] = i32(keys)
+        d["q"], d["k_new"], d["v_new"] = (x[0].clone() for x in rows)
+    w = ws().reserve(sa.paged_decode_ws_bytes(3, MAX_KEYS, b.cfg(), page_size=16, kv_f32=kv is np.float32))
+    out = torch.zeros(3, 8, hd, dtype=torch.float16, device="cuda")
+    decode(b, graphed, append=True, workspace=w, out=out)
+    g, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        decode(b, graphed, append=True, workspace=w, out=out)
+    decode(b, eager, append=True)
+    for i in range(1, steps + 1):
+        for d in (eager, graphed):
+            d["key_len"].add_(1)
+            for name, x in zip(("q", "k_new", "v_new"), rows):
+                d[name].copy_(x[i])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            g.replay()
+        torch.cuda.synchronize()
+        want = decode(b, eager, append=True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), f"step {i}"
+        for name in ("k_pages", "v_pages"):
+            assert np.array_equal(bits(eager[name]), bits(graphed[name])), f"step {i}: {name}"
+
+
+def test_calls_from_two_threads():
+    """Two threads, a stream and a workspace each, one config: the outputs are the calls' own."""
+    import threading
+    bs = [Batch([300 + 400 * s, 90], [3, 1], seed=s) for s in (0, 1)]
+    cfg, outs, errors = bs[0].cfg(), [[], []], []
+    ds = [b.dev() for b in bs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                w, dd = ws(), dict(ds[i], q=ds[i]["q"][2:4].contiguous())
+                for _ in range(20):
+                    outs[i].append((prefill(bs[i], ds[i], workspace=w, cfg=cfg), decode(bs[i], dd, workspace=w, cfg=cfg)))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for b, o in zip(bs, outs):
+        out, A, S = b.oracle()
+        tol = bound(out, A, S, q16=True, kv32=False, out16=True)
+        for x, y in o:
+            check(x.cpu().numpy(), out, tol)
+            check(y.cpu().numpy(), out[2:4], tol[2:4])
