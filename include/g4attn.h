@@ -252,7 +252,10 @@ int g4a_paged_write(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const
  *   k_new/v_new f32 [n_seq][n_kv_heads][head_dim] or both NULL: the step's raw rows, prepared and
  *               stored at position key_len[b] - 1 first, as g4a_decode_kv does (k_in_q, v_in_q and
  *               k_gain are theirs).
- *   out         [n_seq][n_q_heads][head_dim], f16, or f32 with G4A_OUT_F32; srq'd with out_q.
+ *   out         [n_seq][n_q_heads][head_dim], f16, or f32 with G4A_OUT_F32; srq'd with out_q. A query, or an
+ *               attended row, that is not finite gives NaN.
+ * q, and K of f32 caches, enter the products as f16 pairs (f32 accuracy); V of f32 caches and the weights
+ * are rounded to f16, so values of V beyond 65504 are infinite there.
  *   ws          at least g4a_paged_decode_ws_bytes() bytes, 256-byte aligned, uninitialised;
  *               concurrent calls need distinct ones.
  */
@@ -273,7 +276,7 @@ int g4a_paged_decode(const g4a_cfg* cfg, const g4a_paged* pg, const float* q, co
  *   out         [n_tokens][n_q_heads][head_dim], f16, or f32 with G4A_OUT_F32; srq'd with out_q.
  *   ws          at least g4a_paged_prefill_ws_bytes() bytes, 256-byte aligned, uninitialised;
  *               concurrent calls need distinct ones. f32 caches are converted to f16 in it
- *               (n_seq * max_key_len rows of K and V).
+ *               (n_seq * max_key_len rows of K and V; values beyond 65504 become infinite).
  */
 size_t g4a_paged_prefill_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens);
 int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q, const float* q,

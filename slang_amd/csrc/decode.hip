@@ -36,8 +36,9 @@
 // A paged cache (g4a_paged_decode) runs the same kernels with PagedDecodeArgs: a 16-key block lies
 // in one page, so splits start at multiples of 16 and each block's rows come through buffer
 // resources of their own; everything else, the merge included, is shared. 16 sequences of 1 K to 32 K keys
-// (hd 256, kvH 2, 554 MB in pages of 64): 85-88 us + merge 4.6, 6.3 TB/s, as fast as contiguous caches; 64 of
-// 20 to 4097 keys under a window of 512 (26 MB): 11.4 + 4.6 us, two dependent kernels at their latency.
+// (hd 256, kvH 2, 554 MB in pages of 64): 87 us + merge 4.6, 6.3 TB/s, as fast as contiguous caches; 64 of
+// 20 to 4097 keys under a window of 512 (26 MB): 12.6 + 5.5 us, two dependent kernels at their latency (medians
+// of a trace).
 #include <algorithm>
 #include <mutex>
 #include <type_traits>

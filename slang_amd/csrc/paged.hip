@@ -75,9 +75,9 @@ struct PagedWriteArgs {
 // workgroup of HD / 2 threads takes one (token, kv head), as kv_write's does, and through the same
 // kv_pair_prep, so that the rows are kv_write's to the bit. Few rows: the chain of loads cu -> key_len -> table
 // -> row (3.1 us for 16 rows, of which a launch is most). Many: vector instructions, the steps' divisions and
-// the sums' shuffles, ahead of the bytes (13501 tokens of 2 x 256, f16 rows into an f32 cache, 83 MB: 20.8 us =
-// 4.0 TB/s, where a copy reaches 5.2). 4 or 8 rows a workgroup took 24.6 / 26.5 us, the steps through a
-// refined reciprocal 22.0, the raw rows fetched before the position is known 22.3.
+// the sums' shuffles, ahead of the bytes (13501 tokens of 2 x 256, f16 rows into an f32 cache, 83 MB: 21 us =
+// 4.0 TB/s, where a copy reaches 5.2). Against 20.8 then, 4 or 8 rows a workgroup took 24.6 / 26.5 us, the steps
+// through a refined reciprocal 22.0, the raw rows fetched before the position is known 22.3.
 template <int HD, typename IT, typename CT>
 __global__ __launch_bounds__(HD / 2) void paged_write_kernel(PagedWriteArgs a) {
     constexpr int HALF = HD / 2, NW = HALF / 64;

@@ -1,8 +1,12 @@
 // Causal attention of packed prompts over a paged K/V cache, for gfx950 on f16 MFMA.
 //
 // The mathematics is prefill.hip's: per query column an online softmax over key tiles, scores formed
-// transposed (S^T = K . Q^T), so that they are the B operand of O^T += V^T . P^T, P and q rounded to
-// f16, all sums in f32. What differs is what a server's batch brings:
+// transposed (S^T = K . Q^T), so that they are the B operand of O^T += V^T . P^T, all sums in f32. q and P
+// are rounded to f16, and f32 caches too, because the matrix units take f16 operands at 16 times
+// the rate of f32 ones: half a step (2^-11) of a query, key, weight or value, which puts outputs 4 to 5e-4 of
+// the largest off where 32-bit products with an f16 output are 2e-4 off. Partials of split blocks keep 24
+// bits, half a step of which is 2^-16, and move three quarters of the bytes. What differs from prefill.hip is what
+// a server's batch brings:
 //   * Lengths are device data, so nothing can be planned on the host. One launch prepares q in f16 and,
 //     in its first workgroup, writes the work list: a unit is a query block (128 columns: the G heads
 //     of a kv head x 128/G positions) of one sequence and kv head, or a piece of its keys. A list
@@ -310,7 +314,7 @@ __device__ void plan_units(const PagedPrefillArgs& a) {
 // q of packed rows to f16: RMSNorm * gain, then RoPE at the row's position (qprep_row512_kernel's
 // arithmetic). A wave takes four heads of a token; lane l holds dims E l .. E l + E - 1, whose RoPE
 // partners sit in lane l ^ 32. The first workgroup writes the work list meanwhile (about 7 us, what a call of few
-// tokens waits for). Many tokens: the bytes (15252 of 8 x 256, 187 MB: 35 us = 5.3 TB/s, a copy's rate).
+// tokens waits for). Many tokens: the bytes (15252 of 8 x 256, 187 MB: 36 us = 5.2 TB/s, a copy's rate).
 template <int HD>
 __global__ __launch_bounds__(256) void paged_prep_kernel(PagedPrefillArgs a) {
     if (blockIdx.x == 0) {
@@ -439,7 +443,7 @@ __device__ __forceinline__ half4 read_tr16(const half_t* __restrict p) { return 
 // 7856 tokens, kvH 2, up to 3000 keys: 112 us = 770 TFLOP/s (123 us with the plain loop, 118 waiting for the
 // DMAs at V's first read). A tile takes 2200 cycles of MFMA and about 3500 of LDS: K rows 1024, V's
 // transposed reads 1490, the DMAs' writes 1024; beside the tiles a unit takes about 9 us (its page entries,
-// q, the first scores, the epilogue), which bounds short prompts and windows (15252 tokens, window 512: 120 us).
+// q, the first scores, the epilogue), which bounds short prompts and windows (15252 tokens, window 512: 121 us).
 template <int G, typename OUTT>
 __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs a) {
     constexpr int HD = 256, KT = 64, NCOL = 128, BQ = NCOL / G;
@@ -797,8 +801,9 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(PagedPrefillArgs
 // ---------------------------------------------------------------- hd 512
 // Every wave holds all 512 dims of its 32 columns, key tiles of 32: the LDS layout and register placement
 // (O^T in AGPRs, q in VGPRs) of prefill_kernel_w32h, the tile loop interleaved as at hd 256. 13500 tokens in
-// three prompts: 800 to 820 us = 850 to 870 TFLOP/s at the 1.7 GHz that the card's power allows (873 us with the plain
-// loop, 867 interleaved but waiting for its DMAs at V's first read); LDS is busy 3700 cycles a tile.
+// three prompts: 831 us = 840 TFLOP/s at the 1.7 GHz that the card's power allows (before kPagedLift 800 to 820, and
+// then 873 us with the plain loop, 867 interleaved but waiting for its DMAs at V's first read); LDS is busy
+// 3700 cycles a tile. Times at hd 256 and here are the least of 12 in a trace; the median here is 914.
 template <int G, typename OUTT>
 __global__ __launch_bounds__(256) void paged_prefill_kernel_512(PagedPrefillArgs a) {
     constexpr int HD = 512, KT = 32, NCOL = 128, BQ = NCOL / G;

@@ -12,7 +12,7 @@ typedef unsigned v2u32 __attribute__((ext_vector_type(2)));
 // Most a column's running maximum lags its true maximum by (log2 units): P <= 2^15 < 65504
 constexpr float kMaxLag = 15.0f;
 
-// f32 values rounded to their upper 24 bits (a 16-bit mantissa, 2^-17 relative; an infinity and
+// f32 values rounded to their upper 24 bits (a 16-bit mantissa, half a step 2^-16; an infinity and
 // the NaNs that f16 operands make keep their bits), eight at a time: the upper halves, and the
 // third bytes.
 struct Part24 {

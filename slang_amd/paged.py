@@ -16,8 +16,8 @@ sequences of unknown length keeps their rows in pages instead:
   * ``rope_cos`` / ``rope_sin`` f32 [>= max_key_len][hd/2]: ``rope_tables`` over absolute positions.
 
 All of these live on one GPU, so lengths and tables can change between replays of a captured
-graph. ``max_key_len`` is the host's bound of key_len (default: all that the table's columns
-hold); it sizes grids and workspaces, and a longer key_len is taken as max_key_len.
+graph. ``max_key_len`` is the host's bound of key_len (default: all that the table's columns and
+the RoPE tables hold); it sizes grids and workspaces, and a longer key_len is taken as max_key_len.
 
 A step of such a server, per layer: ``paged_write`` the prompts' k/v rows, then ``paged_prefill``
 their queries; then one ``paged_decode`` per generated token, which appends the token's own row.
@@ -42,7 +42,7 @@ _EWORKSPACE, _I32_MAX = -3, 2 ** 31 - 1
 
 # A decode step of short sequences is bound by this layer, not by its kernels: the checks below touch each
 # tensor a few times, whole numbers go to ctypes as they are, and the workspace's size is only asked for
-# when the library finds it too small (one sequence of 300 keys 19.2 -> 13 us a call).
+# when the library finds it too small (one sequence of 300 keys 19.2 -> 15 us a call).
 def _refuse(name, t, dev, dtype):
     """What is wrong with a tensor that _t found unfit."""
     if not t.is_cuda:
@@ -227,7 +227,9 @@ def paged_decode(q, k_pages, v_pages, page_table, key_len, cfg: AttnConfig, *, w
     q f32 [n_seq][nH][hd] raw. With k_new / v_new (f32 [n_seq][kvH][hd]) the step's rows are
     prepared as ``kv_write`` prepares them and appended at position key_len - 1 by the same call
     before they are attended. Returns out [n_seq][nH][hd] (f16 by default); an idle sequence's
-    rows are zeros. `workspace`: the caller's scratch (paged_decode_ws_bytes)."""
+    rows are zeros. q, and K of f32 caches, keep f32 accuracy (f16 pairs); V of f32 caches is
+    rounded to f16 for its product, so values beyond 65504 are infinite there.
+    `workspace`: the caller's scratch (paged_decode_ws_bytes)."""
     dev, qp, qg = _q(q, cfg, q_gain)
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
     if q.shape[0] != pg.n_seq:
@@ -269,7 +271,8 @@ def paged_prefill(q, k_pages, v_pages, page_table, key_len, cu_q, cfg: AttnConfi
 
     q f32 [T][nH][hd] raw; the normalised, rotated q is rounded to f16 (as ``prefill`` without
     q_hilo). Returns out [T][nH][hd] (f16 by default). f32 caches are converted to f16 in the
-    workspace. `workspace`: the caller's scratch (paged_prefill_ws_bytes)."""
+    workspace (values beyond 65504 become infinite). `workspace`: the caller's scratch
+    (paged_prefill_ws_bytes)."""
     dev, qp, qg = _q(q, cfg, q_gain)
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
     cu, n = _cu(cu_q, pg.n_seq, dev), q.shape[0]
