@@ -934,7 +934,8 @@ struct ListPlan {
 };
 // Many pairs take one split each if every sequence is as long as the bound, but a server's bound is loose and
 // its batch ragged: one long sequence would run on one CU a kv head. A 512-byte row of a pair takes about 18 ns
-// there; the list takes 4 us for the merge and 0.045 us a sequence for the plan. It is taken where the bound's
+// there; the list takes 4 us for the merge and 0.045 us a sequence for the plan, which every workgroup makes
+// (so a term in the sequences times the pairs: 4000 x 1 240 us, 16000 x 1 2550). It is taken where the bound's
 // longest walk is ten times that, so that a loose bound costs short batches little. us a call, one split /
 // list (hd 256, f16): one of 32768 keys among 300s, 64 x 8 kv heads 620 / 100, 300 x 2 629 / 69, 1000 x 1
 // 603 / 121; 64 x 8 of 300 each under a bound of 32768 31 / 35, 300 x 2 39 / 53, 1000 x 1 59 / 104; all of 4096,
@@ -942,7 +943,8 @@ struct ListPlan {
 // 65 x 8, one of 32768 1360 / 205, all of 4096 788 / 797; 520 x 1 of 128 to 4096 335 / 374.)
 static bool long_walk(const g4a_cfg* cfg, int n_seq, int max_key_len) {
     const int64_t esz = (cfg->flags & G4A_KV_F32) ? 4 : 2;
-    return (int64_t)longest_active(cfg, max_key_len, true) * cfg->head_dim * esz >= (2200 + 25 * (int64_t)n_seq) * 512;
+    const int64_t n = n_seq, cost = 2200 + 25 * n + n * n * cfg->n_kv_heads / 600;  // ten times, in 512-byte rows
+    return (int64_t)longest_active(cfg, max_key_len, true) * cfg->head_dim * esz >= cost * 512;
 }
 static ListPlan list_plan(const g4a_cfg* cfg, int n_seq, int max_key_len, bool paged = false) {
     ListPlan p{0, 0};
