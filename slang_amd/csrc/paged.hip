@@ -53,7 +53,9 @@ int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8) {
 }
 
 PageTab page_tab(const g4a_paged* pg) {
-    return PageTab{pg->page_table, pg->key_len, pg->n_seq, pg->table_stride, pg->table_cols, pg->n_pages,
+    // the columns that max_key_len keys use: 2^26 at most, whose bytes a buffer range holds
+    const int cols = (pg->max_key_len + pg->page_size - 1) / pg->page_size;
+    return PageTab{pg->page_table, pg->key_len, pg->n_seq, pg->table_stride, cols, pg->n_pages,
                    __builtin_ctz((unsigned)pg->page_size), pg->max_key_len};
 }
 

@@ -394,3 +394,22 @@ def test_calls_from_two_threads():
         for x, y in o:
             check(x.cpu().numpy(), out, tol)
             check(y.cpu().numpy(), out[2:4], tol[2:4])
+
+
+@pytest.mark.parametrize("kv", [np.float16, np.float32])
+def test_table_of_more_columns_than_a_buffer_range_holds(kv):
+    """2^30 columns, of whose bytes 32 bits keep none: the entries are still the sequence's."""
+    b = Batch([200], [33], kv=kv)
+    assert b.table[0, 0] != 0
+    table = torch.full((1, 2 ** 30), -1, dtype=torch.int32, device="cuda")
+    table[:, :b.cols] = torch.from_numpy(b.table)
+    d = b.dev(table=table)
+    out, A, S = b.oracle()
+    got = prefill(b, d, max_key_len=1000)
+    check(got.cpu().numpy(), out, bound(out, A, S, q16=True, kv32=kv is np.float32, out16=True, k16=kv is np.float32))
+    got = decode(b, dict(d, q=d["q"][32:33].contiguous()), max_key_len=1000)
+    check(got.cpu().numpy(), out[32:], bound(out, A, S, q16=False, kv32=kv is np.float32, out16=True)[32:])
+    ref = b.dev()
+    write(b, d, max_key_len=1000)
+    write(b, ref)
+    assert np.array_equal(bits(d["k_pages"]), bits(ref["k_pages"])) and np.array_equal(bits(d["v_pages"]), bits(ref["v_pages"]))
