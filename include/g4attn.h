@@ -35,10 +35,11 @@ extern "C" {
 
 /* cfg.flags */
 #define G4A_KV_F32    0x1u /* caches hold f32 (the reference's own cache type); default f16 */
-#define G4A_IN_F16    0x2u /* g4a_kv_write, g4a_paged_write: k/v inputs are f16 (kvnorm_b); default f32 (kvnorm) */
+#define G4A_IN_F16    0x2u /* g4a_kv_write, g4a_paged_write, g4a_paged_tree: k/v inputs are f16 (kvnorm_b); default
+                              f32 (kvnorm) */
 #define G4A_NO_V_NORM 0x4u /* g4a_kv_write, g4a_decode_kv, g4a_paged_*: store v as given instead of RMSNorm(v) */
-#define G4A_OUT_F32   0x8u /* g4a_prefill, g4a_paged_decode, g4a_paged_prefill: f32 output (attn_prefill's
-                              "out"); default f16 (attnh) */
+#define G4A_OUT_F32   0x8u /* g4a_prefill, g4a_paged_decode, g4a_paged_prefill, g4a_paged_tree: f32 output
+                              (attn_prefill's "out"); default f16 (attnh) */
 #define G4A_Q_HILO    0x10u /* g4a_prefill: keep q at f32 accuracy (f16 hi + lo MFMA operands),
                                as attn_prefill's f32 q (kernels_dsl.py:2007-2014); default rounds
                                q to f16 as qprep_b does (kernels_dsl.py:1872-1873) */
@@ -282,6 +283,32 @@ size_t g4a_paged_prefill_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n
 int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q, const float* q,
                       const float* q_gain, const float* rope_cos, const float* rope_sin, void* out, void* ws,
                       size_t ws_bytes, void* stream);
+
+/*
+ * ---- Generation that branches, over a paged cache -----------------------------------------
+ * Drafted trees (several continuations of a sequence checked in one step) and beams. No counterpart in the
+ * reference.
+ *
+ * Attention of drafted trees. The packed tokens of a sequence are one tree, at most G4A_TREE_MAX of them (those
+ * behind are rows of nobody): token i, at row start + i of its sequence (start = key_len - its tokens), continues token
+ * parents[i] < i of the same tree, or, with any other value (-1), the last key in front of the tree. It stands at
+ * position start + depth(i), which is its row of the RoPE tables, and attends the keys t < start with position - t < W
+ * and, of the tree, itself and the ancestors whose depth is less than W below its own, all on pages that are there.
+ * (A V row that is not finite reaches other tokens of the tree as in g4a_paged_prefill. Masked K rows may hold anything.)
+ *   parents     int32 [n_tokens], device, indices within the tree.
+ *   q, out      as g4a_paged_prefill (q rounded to f16, G4A_Q_HILO refused).
+ *   k_new/v_new [n_tokens][n_kv_heads][head_dim], f32, or f16 with G4A_IN_F16, or both NULL (the cache holds the rows):
+ *               prepared as g4a_kv_write prepares rows at the tokens' positions, to the bit, and stored at rows
+ *               start + i before they are attended (k_in_q, v_in_q, k_gain as there).
+ *   ws          at least g4a_paged_tree_ws_bytes() bytes, 256-byte aligned, uninitialised; concurrent calls need
+ *               distinct ones. f32 caches are converted to f16 in it, as in g4a_paged_prefill.
+ */
+#define G4A_TREE_MAX 1024
+size_t g4a_paged_tree_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens);
+int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const int32_t* cu_q, const int32_t* parents,
+                   const float* q, const float* q_gain, const float* rope_cos, const float* rope_sin, const void* k_new,
+                   const void* v_new, float k_in_q, float v_in_q, const float* k_gain, void* out, void* ws,
+                   size_t ws_bytes, void* stream);
 
 /*
  * ---- The q/k/v producer: projections with QAT weights --------------------------------

@@ -29,6 +29,7 @@ EXPORTS = (
     "g4a_prefill_ws_bytes", "g4a_prefill", "g4a_qprep",
     "g4a_kv_write",
     "g4a_paged_write", "g4a_paged_decode_ws_bytes", "g4a_paged_decode", "g4a_paged_prefill_ws_bytes", "g4a_paged_prefill",
+    "g4a_paged_tree_ws_bytes", "g4a_paged_tree",
     "g4a_dequant", "g4a_qkv_gemv", "g4a_qkv_gemv_norm", "g4a_srqh", "g4a_gemm16",
     "g4a_gemm16_ws_bytes", "g4a_gemm16_ws", "g4a_gemm16_geglu",
     "g4a_qgemv", "g4a_qgemv_geglu", "g4a_qgemv_gelu_mul", "g4a_gemv_f16", "g4a_rms_norm", "g4a_geglu",
@@ -39,6 +40,9 @@ EXPORTS = (
 
 # g4a_gemm16_ws: the workspace's leading ticket words (g4attn.h)
 GEMM_TICKET_BYTES = 2048
+
+# most tokens of a drafted tree (G4A_TREE_MAX)
+TREE_MAX = 1024
 
 # g4a_rows_tail modes (g4attn.h)
 TAIL_NONE, TAIL_SRQ, TAIL_NORM, TAIL_NORM16 = 0, 1, 2, 3
@@ -163,6 +167,10 @@ def load() -> ctypes.CDLL:
     lib.g4a_paged_prefill_ws_bytes.argtypes = [cfgp, pgp, i]
     lib.g4a_paged_prefill.restype = ctypes.c_int
     lib.g4a_paged_prefill.argtypes = [cfgp, pgp, i, P, P, P, P, P, P, P, zp, P]
+    lib.g4a_paged_tree_ws_bytes.restype = zp
+    lib.g4a_paged_tree_ws_bytes.argtypes = [cfgp, pgp, i]
+    lib.g4a_paged_tree.restype = ctypes.c_int
+    lib.g4a_paged_tree.argtypes = [cfgp, pgp, i, P, P, P, P, P, P, P, P, f, f, P, P, P, zp, P]
     lib.g4a_dequant.restype = ctypes.c_int
     lib.g4a_dequant.argtypes = [i, i, i, P, P, P, P]
     lib.g4a_qkv_gemv.restype = ctypes.c_int

@@ -1,0 +1,887 @@
+// The attention of packed rows over a paged K/V cache on f16 MFMA: one work unit, a block of 128 query columns
+// (the G heads of a kv head x 128/G tokens) times the key tiles of a piece. paged_prefill.hip runs it over
+// prompts, whose tokens attend every earlier row, paged_tree.hip over drafted trees, whose tokens attend their
+// ancestors among the rows of the call (bits of a row per token, and per 64 keys a word).
+#pragma once
+
+#include <type_traits>
+
+#include "paged.hpp"
+#include "prefill_tiles.hpp"
+
+namespace g4a {
+
+// P, rounded to f16 for its product, is at most 2^kMaxLag. A maximum that moves is set this many powers of two
+// below the score, so that a key keeps all bits down to 2^-18 of the largest weight and is zero only below
+// 2^-29 (2^-14 and 2^-25 without, while the sum still counts it: 32768 such keys are 2^-10 of it), and it moves
+// again when a score passes the largest so far by 2^11. Each move rescales O^T: 0 / 2 / 4 / 8 powers took
+// prefill_hd512 824 / 831 / 840 / 900 us, prefill_mixed 128 / 128 / 128 / 135.
+constexpr float kPagedLift = 4.0f;
+constexpr int kCus = 256;      // compute units of the MI355X; the kernels run one workgroup a CU
+
+struct PagedUnit {
+    int b, qb, kh, n_pieces;   // sequence, query block, kv head; pieces of the block
+    int slot, t0, t1, row0;    // partial block of this piece (merge list: of the first); key tiles; packed row of the
+    int S, start;              // sequence's first token, its tokens in this call, the position of the first
+    int page[4];               // table entries of the first tile's 16-row groups
+    int pad0, pad1;
+};
+
+struct PagedPrefillArgs {
+    PageTab t;
+    const int32_t* cu;
+    const float* q;
+    const float* q_gain;
+    const float* rcos;
+    const float* rsin;
+    const void* kc;  // f16 pages
+    const void* vc;
+    void* out;
+    half_t* q16;
+    PagedUnit* units;
+    PagedUnit* merges;
+    int* counts;  // units, merges
+    void* part_o;
+    float2* part_ml;
+    int n_tokens, n_q_heads, n_kv_heads, window, max_units, max_slots, bq, kt;
+    float scale_log2, eps, out_q;
+};
+
+// What a call over drafted trees has beside that. Bit k of a packed row's words is the row's answer for key
+// (start & ~63) + k of its sequence (start: the row of the first token): attended or not, its ancestors and itself among
+// the rows of the call, and the history in front of them in the same 64.
+struct PagedTreeArgs : PagedPrefillArgs {
+    const int32_t* parents;
+    unsigned long long* bits;  // [n_tokens][words]
+    int32_t* depth;            // [n_tokens]: the token's position is start + depth
+    int words;
+};
+
+// The rows of f32 pages that the call attends, as f16 pages of the workspace: page i of sequence b is
+// page b * cols + i of ko / vo, and the table written to tab names it if the cache's own is there.
+struct PagedKv16Args {
+    PageTab t;
+    const int32_t* cu;
+    const float* kc;
+    const float* vc;
+    half_t* ko;
+    half_t* vo;
+    int32_t* tab;
+    int n_tokens, row, cols, window;
+};
+int launch_kv16(const PagedKv16Args& k, const g4a_paged* pg, hipStream_t stream);
+
+// ---------------------------------------------------------------- pages of a workgroup's tiles
+// Lane j holds, for tile t0 + j (64 at a time), the table entry of the 16 rows that its wave moves and a
+// bit for each 16 rows of the tile whose page is not there.
+template <int KT>
+struct TilePages {
+    int entry = -1, gone = 0;
+    __device__ __forceinline__ void load(const PageTab& t, int b, int key0, int own, int lane) {
+        const rsrc_t rt = make_rsrc(t.table + (size_t)b * t.stride, (uint32_t)t.cols * 4);
+        int e[KT / 16];
+#pragma unroll
+        for (int i = 0; i < KT / 16; ++i)
+            e[i] = __builtin_amdgcn_raw_buffer_load_b32(rt, ((key0 + KT * lane + 16 * i) >> t.shift) * 4, 0, 0);
+        gone = 0;
+#pragma unroll
+        for (int i = 0; i < KT / 16; ++i) {
+            entry = i == own ? e[i] : entry;
+            gone |= page_ok(t, e[i]) ? 0 : 1 << i;
+        }
+    }
+};
+// the 16 rows of keys k0 .. of a page as a buffer resource: rows at or past kv_hi, and all of a page that
+// is not there, read as zeros
+__device__ __forceinline__ rsrc_t page_rows(const PageTab& t, const void* pool, int entry, int k0, int kv_hi, int row,
+                                            int kh_off) {
+    const bool ok = page_ok(t, entry);
+    const uint32_t bytes = ok ? (uint32_t)(clamp16(kv_hi - k0) * row * 2) : 0u;
+    return make_rsrc(reinterpret_cast<const half_t*>(pool) + paged_row(t, ok ? entry : 0, k0, row) + kh_off, bytes);
+}
+constexpr int kNoRow = 0x7fff0000;  // an offset past every such range (64 MiB at most), with room for a row's own bytes
+
+// A transposed read that does not wait for the DMAs in flight. The compiler cannot tell that those fill other
+// tiles and would wait for all of them (vmcnt 0) before the first read of a tile's V; the __restrict puts the
+// read in an alias scope of its own. The tile loop's own wait and barrier order it behind the DMAs of its tile.
+__device__ __forceinline__ half4 read_tr16(const half_t* __restrict p) { return lds_tr16(p); }
+
+// ---------------------------------------------------------------- hd 256
+// 32 query columns a wave, 128 a workgroup, key tiles of 64 moved straight into LDS and double
+// buffered: the LDS layout and swizzles of prefill_kernel_w32, its tile loop pipelined by hand (below).
+// 7856 tokens, kvH 2, up to 3000 keys: 112 us = 770 TFLOP/s (123 us with the plain loop, 118 waiting for the
+// DMAs at V's first read). A tile takes 2200 cycles of MFMA and about 3500 of LDS: K rows 1024, V's
+// transposed reads 1490, the DMAs' writes 1024; beside the tiles a unit takes about 9 us (its page entries,
+// q, the first scores, the epilogue), which bounds short prompts and windows (15252 tokens, window 512: 121 us).
+template <int G, typename OUTT, typename ARGS = PagedPrefillArgs>
+__global__ __launch_bounds__(256) void paged_prefill_kernel_256(ARGS a) {
+    constexpr bool TREE = std::is_same<ARGS, PagedTreeArgs>::value;
+    constexpr int HD = 256, KT = 64, NCOL = 128, BQ = NCOL / G;
+    constexpr int ROWB = HD * 2;      // bytes per LDS tile row
+    constexpr int TILEB = KT * ROWB;  // one K or V tile
+    __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILEB];  // [buffer][K, V]
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n32 = lane & 31, h = lane >> 5;
+    if ((int)blockIdx.x >= a.counts[0]) return;  // past the work list
+    const PagedUnit wu = a.units[blockIdx.x];
+    const int start_pos = wu.start, S = wu.S, row0 = wu.row0;
+    const int T_total = start_pos + S;
+    const int kh = wu.kh, qb = wu.qb, n_pieces = wu.n_pieces;
+
+    // ---- key range of the workgroup [wg_lo, kv_hi) in tiles; with a key split this
+    // workgroup takes tiles [t0, t1) of its query block
+    const int p0 = start_pos + qb * BQ;
+    const int kv_hi = min(p0 + BQ, T_total);
+    // first attended key (of a tree: by a root)
+    const int first = a.window > 0 ? max(0, (TREE ? start_pos : p0) + 1 - a.window) : 0;
+    const int wg_lo = first & (TREE ? ~(KT - 1) : ~15);
+    const int t0 = wu.t0, t1 = wu.t1;
+
+    // ---- this lane's query column (head hh, position offset pl) and 8-dim half h
+    const int c = 32 * wave + n32;
+    const int hh = c % G, pl = c / G;
+    const int s_raw = qb * BQ + pl;
+    const bool col_ok = s_raw < S;
+    const int s_idx = col_ok ? s_raw : S - 1;
+    int pos = start_pos + s_idx;
+    if constexpr (TREE) pos = start_pos + a.depth[row0 + s_idx];
+
+    // K/V rows of this kv head; wave w moves rows 16w .. 16w + 15 of a tile, two rows (1 KiB) an instruction
+    const int rowg = a.n_kv_heads * HD * 2;  // bytes per cache row
+    TilePages<KT> pages;
+    // this wave's 16 rows of tile t from the page of `entry`; past the last tile: an empty range
+    const auto tile_rows = [&](const void* pool, int t, int entry) {
+        const int kg = wg_lo + t * KT + 16 * wave;
+        return page_rows(a.t, pool, entry, kg, t < t1 ? kv_hi : kg, rowg / 2, kh * HD);
+    };
+    // DMA j of a wave's eight for a tile: two rows. swz: K's or V's chunk places
+    const auto dma = [&](rsrc_t rp, char* dst, int j, int off) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (__attribute__((address_space(3))) void*)(dst + (16 * wave + 2 * j) * ROWB),
+                                                 16, off, 0, 0, 0);
+    };
+    const auto k_off = [&](int j) { return (2 * j + h) * rowg + 16 * (n32 ^ ((16 * wave + 2 * j + h) & 31)); };
+    const auto v_off = [&](int j) { return (2 * j + h) * rowg + 16 * (n32 ^ vswz(2 * j + h)); };
+    const auto tile_k = [&](int t) { return lds + (t & 1) * 2 * TILEB; };
+    const auto tile_v = [&](int t) { return lds + (t & 1) * 2 * TILEB + TILEB; };
+
+    // ---- q: lane (column, h) holds dims 16s + 8h + i (s < 16, i < 8), the B operand of the 32x32x16
+    // MFMA. Wave w DMAs the f16 q rows of its own 32 columns (two 512-byte rows an instruction, chunk
+    // n32 of a row from logical chunk n32 ^ (row % 32)) into the LDS stage that tile t0 + 1 takes over
+    // later, then reads them back in that layout; rows past the block's last token read as zeros.
+    half8 qf[16];
+    int entry1, gone0, gone1 = 0;  // tile t + 1's page, the 16-row groups of tiles t and t + 1 without one
+    {
+        const rsrc_t rq = make_rsrc(a.q16 + ((size_t)row0 + qb * BQ) * a.n_q_heads * HD, (uint32_t)min(BQ, S - qb * BQ) * a.n_q_heads * ROWB);
+        char* qs = lds + ((t0 + 1) & 1) * 2 * TILEB;
+        pages.load(a.t, wu.b, wg_lo + t0 * KT, wave, lane);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int r = 32 * wave + 2 * j + h;  // column of the row this lane moves
+            const int qo = ((r / G) * a.n_q_heads + kh * G + r % G) * ROWB + 16 * (n32 ^ (r & 31));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(qs + (32 * wave + 2 * j) * ROWB),
+                                                     16, qo, 0, 0, 0);
+        }
+        entry1 = wu.page[0];  // this wave's group
+        gone0 = 0;
+#pragma unroll
+        for (int i = 0; i < KT / 16; ++i) {
+            entry1 = i == wave ? wu.page[i] : entry1;
+            gone0 |= page_ok(a.t, wu.page[i]) ? 0 : 1 << i;
+        }
+        if (t0 < t1) {  // tile t0: of the block's first tile, rows in front of the first attended key read as zeros
+            const rsrc_t rk = tile_rows(a.kc, t0, entry1), rv = tile_rows(a.vc, t0, entry1);
+            const int skip = first - (wg_lo + t0 * KT + 16 * wave);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                dma(rk, tile_k(t0), j, 2 * j + h < skip ? kNoRow : k_off(j));
+                dma(rv, tile_v(t0), j, 2 * j + h < skip ? kNoRow : v_off(j));
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const char* qrow = qs + c * ROWB;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) qf[s] = *reinterpret_cast<const half8*>(qrow + 16 * ((2 * s + h) ^ n32));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // stage free for tile t0 + 1's DMA
+        if (!col_ok) {
+#pragma unroll
+            for (int s = 0; s < 16; ++s) qf[s] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+        // q is only ever an MFMA B operand, which may sit in AGPRs: that leaves the VGPRs to
+        // the O^T accumulators, the scores and the LDS operand batches
+#pragma unroll
+        for (int s = 0; s < 16; ++s) asm volatile("" : "+a"(qf[s]));
+    }
+
+    // ---- key ranges: this wave [w_lo, wp1], this column [col_lo, pos]
+    const int wp0 = p0 + (32 * wave) / G;
+    const int wp1 = min(p0 + (32 * wave + 31) / G, T_total - 1);
+    const int col_lo = a.window > 0 ? pos + 1 - a.window : 0;
+    int lo_max = 0;  // tree: the last column's first attended key of the history
+    if constexpr (TREE) {
+        lo_max = col_lo;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) lo_max = max(lo_max, __shfl_xor(lo_max, d));
+        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    }
+    // tree: the word of tile t for this lane's column, if the tile holds rows of the call
+    const auto tree_word = [&](int t) {
+        unsigned long long w = ~0ull;
+        if constexpr (TREE) {
+            const int kb = wg_lo + t * KT;
+            if (t < t1 && kb + KT > start_pos) {
+                const unsigned long long* row = a.bits + (size_t)(row0 + s_idx) * a.words;
+                if constexpr (KT == 64) w = row[(kb - (start_pos & ~63)) >> 6];
+                else w = reinterpret_cast<const uint32_t*>(row)[(kb - (start_pos & ~63)) >> 5];
+            }
+        }
+        return w;
+    };
+
+    float16v oacc[8];  // O^T[32dt + 8(r/4) + 4h + r%4][column]
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) oacc[dt] = float16v{};
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) asm volatile("" : "+a"(oacc[dt]));
+    float m_use = kNegInf, l_run = 0.0f;
+    bool started = false;
+
+    // transposed V reads: 16-lane group (h, half16), lane m supplies row 4h + m/4 (+8, +16u),
+    // dims 32dt + 16 half16 + 4(m%4) .. +3
+    const int m16 = lane & 15, half16 = (lane >> 4) & 1;
+    const int vr0 = 4 * h + (m16 >> 2);
+    const int vc0 = 2 * half16 + ((m16 & 3) >> 1);  // chunk within a 32-dim tile
+    const int vb0 = 8 * (m16 & 1);                   // byte within the chunk
+    const int vsw = vswz(vr0);                        // rows 16u + vr0 (+8) share r % 4
+
+    // A tile's scores, S^T = K . Q^T: two 32-key sub-tiles, 16 k-steps of 16 dims, the two accumulator
+    // chains in turn (a chain of dependent MFMAs issues at half rate).
+    // Masks of tile t's scores: key kb + 4h + 32kt + 8(r/4) + r%4 of this lane's column; tiles inside every
+    // column's range skip it.
+    auto mask = [&](int t, int gone, unsigned long long word, float16v (&sc)[2]) {
+        const int kb = wg_lo + t * KT;
+        if constexpr (TREE) {
+            if (kb + KT > start_pos) {
+                const uint32_t w[2] = {(uint32_t)word >> (4 * h), (uint32_t)(word >> 32) >> (4 * h)};
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[kt][r] = w[kt] >> (8 * (r >> 2) + (r & 3)) & 1 ? sc[kt][r] : kNegInf;
+            } else if (a.window > 0 && kb < lo_max) {
+                const int rel_lo = col_lo - (kb + 4 * h);
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) sc[kt][r] = 32 * kt + 8 * (r >> 2) + (r & 3) >= rel_lo ? sc[kt][r] : kNegInf;
+            }
+        } else if ((kb + KT - 1 > wp0) || (a.window > 0 && kb < wp1 + 1 - a.window)) {
+            const int rel_hi = pos - (kb + 4 * h), rel_lo = col_lo - (kb + 4 * h);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int o = 32 * kt + 8 * (r >> 2) + (r & 3);
+                    sc[kt][r] = (o <= rel_hi && o >= rel_lo) ? sc[kt][r] : kNegInf;
+                }
+        }
+        if (gone) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[kt][r] = gone >> (2 * kt + (r >> 3)) & 1 ? kNegInf : sc[kt][r];
+        }
+    };
+
+    // One tile. A wave has its SIMD to itself, so what is to overlap has to be interleaved in its own
+    // instruction stream (the order below is kept by the sched_barriers):
+    //   * the 32 score MFMAs of tile t + 1 with the exponentials of tile t -- a step's two MFMAs take the
+    //     matrix unit 64 cycles, in which two exponentials of three stages (argument, exp2, sum and
+    //     rounding of the step before) and the operand reads two steps ahead issue -- and with the DMAs
+    //     of V(t + 1) and K(t + 2), which issue one a step: all 16 at once hold the wave up while the
+    //     CU's four waves queue for the 64 B/clk path into LDS (1190 of 5300 cycles a tile);
+    //   * the 32 P.V MFMAs of tile t with the maxima of tile t + 1.
+    // So K is fetched two tiles ahead, V one: K(t + 2) into the buffer of K(t), whose scores are done,
+    // V(t + 1) into that of V(t - 1).
+    float mnext = kNegInf;  // this lane's maximum of the scores of the next tile
+    auto tile = [&](int t, float16v (&sacc)[2], float16v (&snext)[2]) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of V(t) and K(t + 1) is in LDS
+        __syncthreads();                                    // all parts; K(t) and V(t - 1) fully consumed
+        const int gone = gone1, entry = entry1;             // of tile t + 1
+        const unsigned long long word = tree_word(t + 1);
+        {
+            const int j = (t + 2 - t0) & 63;
+            if (j == 0) pages.load(a.t, wu.b, wg_lo + (t + 2) * KT, wave, lane);
+            entry1 = __builtin_amdgcn_readlane(pages.entry, j);
+            gone1 = __builtin_amdgcn_readlane(pages.gone, j);
+        }
+        const float mloc = max32(mnext) * a.scale_log2;  // the column's other half sits in lane ^ 32 (scale > 0)
+        // move the running maxima only when a score passes one by more than 2^kMaxLag
+        const bool bump = mloc > m_use + kMaxLag;
+        if (__any(bump)) {
+            const float m_new = fmaxf(m_use, mloc - kPagedLift);
+            const float corr = m_use == kNegInf ? 0.0f : fexp2(m_use - m_new);
+            l_run *= corr;
+            if (started) {
+                // one 16-register tile at a time: copied to VGPRs, scaled, pinned back into
+                // AGPRs (left to itself the compiler moves all of them at once)
+                asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"  // the last MFMA's writes, as in the epilogue
+                             : "+a"(oacc[0]), "+a"(oacc[1]), "+a"(oacc[2]), "+a"(oacc[3]), "+a"(oacc[4]),
+                               "+a"(oacc[5]), "+a"(oacc[6]), "+a"(oacc[7]));
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt) {
+                    float16v x = oacc[dt];
+                    asm volatile("" : "+v"(x));
+                    x *= corr;
+                    asm volatile("" : "+v"(x));
+                    oacc[dt] = x;
+                    asm volatile("" : "+a"(oacc[dt]));
+                }
+            }
+            m_use = m_new;
+        }
+        started = true;
+        const float msub = m_use == kNegInf ? 0.0f : m_use;
+        half8 pb[4];
+        float ps = 0.0f;
+        {
+            const char* krow0 = tile_k(t + 1) + n32 * ROWB;
+            const char* krow1 = krow0 + 32 * ROWB;
+            half8 kr[3][2];
+            auto read_k = [&](int s) {
+                const int cb = 16 * ((2 * s + h) ^ n32);
+                kr[s % 3][0] = *reinterpret_cast<const half8*>(krow0 + cb);
+                kr[s % 3][1] = *reinterpret_cast<const half8*>(krow1 + cb);
+            };
+            // exponential v of the lane's 32 in three stages
+            float ex[2][2], ev[2][2];
+            auto arg = [&](int v) { ex[(v >> 1) & 1][v & 1] = __builtin_fmaf(sacc[v >> 4][v & 15], a.scale_log2, -msub); };
+            auto expo = [&](int v) { ev[(v >> 1) & 1][v & 1] = fexp2(ex[(v >> 1) & 1][v & 1]); };
+            auto take = [&](int v) {
+                const float e = ev[(v >> 1) & 1][v & 1];
+                ps += e;
+                pb[v >> 3][v & 7] = (half_t)e;
+            };
+            read_k(0);
+            read_k(1);
+            arg(0);
+            arg(1);
+            const rsrc_t rv = tile_rows(a.vc, t + 1, entry), rk = tile_rows(a.kc, t + 2, entry1);
+            snext[0] = snext[1] = float16v{};
+#pragma unroll
+            for (int s = 0; s < 16; ++s) {
+                if (s + 2 < 16) read_k(s + 2);
+                snext[0] = mfma32(kr[s % 3][0], qf[s], snext[0]);
+                expo(2 * s);
+                expo(2 * s + 1);
+                if (s > 0) {
+                    take(2 * s - 2);
+                    take(2 * s - 1);
+                }
+                snext[1] = mfma32(kr[s % 3][1], qf[s], snext[1]);
+                if (s < 15) {
+                    arg(2 * s + 2);
+                    arg(2 * s + 3);
+                }
+                if (s < 8) dma(rv, tile_v(t + 1), s, v_off(s));
+                else dma(rk, tile_k(t + 2), s - 8, k_off(s - 8));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            take(30);
+            take(31);
+        }
+        l_run += ps;
+        // (here, not where they are used behind the masks' branches: the compiler would sink them there)
+        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(pb[2]), "+v"(pb[3]), "+v"(l_run));
+        if (t + 1 < t1) mask(t + 1, gone, word, snext);
+
+        // O^T += V^T . P^T over four 16-key steps; k-slot i < 4 is key 16u + 4h + i, i >= 4 is key
+        // 16u + 8 + 4h + i - 4, matching the S^T accumulator rows in pb. Transposed V reads (two an
+        // MFMA) kPvAhead MFMAs ahead.
+        {
+            const char* V = tile_v(t);
+            half8 av[kPvAhead + 1];
+            auto read_v = [&](int i) {
+                const int u = i >> 3, ch = 4 * (i & 7) + vc0;
+                const char* vp = V + (16 * u + vr0) * ROWB + 16 * (ch ^ vsw) + vb0;
+                const half4 lo = read_tr16(reinterpret_cast<const half_t*>(vp));
+                const half4 hi = read_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
+                av[i % (kPvAhead + 1)] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            mnext = kNegInf;
+#pragma unroll
+            for (int i = 0; i < kPvAhead; ++i) read_v(i);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if (i + kPvAhead < 32) read_v(i + kPvAhead);
+                mfma32_acc(oacc[i & 7], av[i % (kPvAhead + 1)], pb[i >> 3]);
+                if (i >= 8 && i < 24) mnext = fmaxf(mnext, fmaxf(snext[(i - 8) >> 3][2 * (i & 7)], snext[(i - 8) >> 3][2 * (i & 7) + 1]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("" : "+v"(mnext));
+        }
+    };
+    if (t0 < t1) {
+        float16v sa[2] = {float16v{}, float16v{}}, sb[2];
+        __syncthreads();  // K(t0), V(t0); every wave has its q
+        entry1 = __builtin_amdgcn_readlane(pages.entry, 1);
+        gone1 = __builtin_amdgcn_readlane(pages.gone, 1);
+        const rsrc_t rk = tile_rows(a.kc, t0 + 1, entry1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dma(rk, tile_k(t0 + 1), j, k_off(j));
+        const char* krow0 = tile_k(t0) + n32 * ROWB;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+            const int cb = 16 * ((2 * s + h) ^ n32);
+            sa[0] = mfma32(*reinterpret_cast<const half8*>(krow0 + cb), qf[s], sa[0]);
+            sa[1] = mfma32(*reinterpret_cast<const half8*>(krow0 + 32 * ROWB + cb), qf[s], sa[1]);
+        }
+        mask(t0, gone0, tree_word(t0), sa);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mnext = fmaxf(mnext, fmaxf(sa[0][r], sa[1][r]));
+        for (int t = t0;;) {  // the two score sets change roles every tile
+            tile(t, sa, sb);
+            if (++t >= t1) break;
+            tile(t, sb, sa);
+            if (++t >= t1) break;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last tile's (empty) DMAs, before LDS is used again
+    }
+
+    // ---- epilogue: column sum over both halves, normalise, srq, store 4 dims at a time
+    // (the accumulators must not be read within 18 wait states of the last MFMA writing them, which the
+    // compiler does not see)
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
+                 : "+a"(oacc[0]), "+a"(oacc[1]), "+a"(oacc[2]), "+a"(oacc[3]), "+a"(oacc[4]), "+a"(oacc[5]),
+                   "+a"(oacc[6]), "+a"(oacc[7]));
+    const float l_tot = add32(l_run);
+    if (n_pieces > 1) {  // a piece of a split query block: O / l and (m, l)
+        if (TREE && !col_ok) return;  // few tokens: columns of none move no bytes
+        const float inv_p = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) store_part<true, HD, NCOL * HD>(a.part_o, true, wu.slot, wave, dt, lane, oacc[dt], inv_p);
+        if (h == 0) a.part_ml[(size_t)wu.slot * NCOL + c] = make_float2(m_use, l_tot);
+        return;
+    }
+    const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+    if constexpr (sizeof(OUTT) == 2) {
+        // f16 rows through LDS: each wave stages its 32 output rows (528-byte stride: the
+        // 8-byte writes of a store instruction fall on distinct banks), then stores two whole
+        // 512-byte rows an instruction. Written straight from the accumulator layout, every
+        // store instruction put 16 bytes into each of 32 rows.
+        constexpr int OSTR = HD * 2 + 16;
+        __syncthreads();  // every wave is done with the last tile's K/V
+        char* ost = lds + wave * 32 * OSTR;
+        auto stage = [&](auto quantise) {  // (one test of the step for all of them)
+#pragma unroll
+            for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]} * inv;
+                    if constexpr (decltype(quantise)::value) v = srq4(v, a.out_q);
+                    store4(reinterpret_cast<half_t*>(ost + n32 * OSTR) + 32 * dt + 8 * j + 4 * h, v);
+                }
+        };
+        if (a.out_q == 0.0f) stage(std::false_type{});
+        else stage(std::true_type{});
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int rr = 2 * i + h, cc = 32 * wave + rr;  // lanes 32h..: the wave's row rr
+            const int so = qb * BQ + cc / G;
+            const half8 val = *reinterpret_cast<const half8*>(ost + rr * OSTR + 16 * n32);
+            if (so < S)
+                *reinterpret_cast<half8*>(reinterpret_cast<half_t*>(a.out) +
+                                          ((size_t)(row0 + so) * a.n_q_heads + kh * G + cc % G) * HD + 8 * n32) = val;
+        }
+    } else if (col_ok) {
+        OUTT* orow = reinterpret_cast<OUTT*>(a.out) + ((size_t)(row0 + s_idx) * a.n_q_heads + kh * G + hh) * HD;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2],
+                                          oacc[dt][4 * j + 3]} * inv;
+                store4(orow + 32 * dt + 8 * j + 4 * h, srq4(v, a.out_q));
+            }
+    }
+}
+
+// ---------------------------------------------------------------- hd 512
+// Every wave holds all 512 dims of its 32 columns, key tiles of 32: the LDS layout and register placement
+// (O^T in AGPRs, q in VGPRs) of prefill_kernel_w32h, the tile loop interleaved as at hd 256. 13500 tokens in
+// three prompts: 831 us = 840 TFLOP/s at the 1.7 GHz that the card's power allows (before kPagedLift 800 to 820, and
+// then 873 us with the plain loop, 867 interleaved but waiting for its DMAs at V's first read); LDS is busy
+// 3700 cycles a tile. Times at hd 256 and here are the least of 12 in a trace; the median here is 914.
+template <int G, typename OUTT, typename ARGS = PagedPrefillArgs>
+__global__ __launch_bounds__(256) void paged_prefill_kernel_512(ARGS a) {
+    constexpr bool TREE = std::is_same<ARGS, PagedTreeArgs>::value;
+    constexpr int HD = 512, KT = 32, NCOL = 128, BQ = NCOL / G;
+    constexpr int ROWB = HD * 2;       // 1 KiB rows
+    constexpr int TILEB = KT * ROWB;   // one K or V tile: 32 KiB
+    constexpr int OSTR = HD * 2 + 16;  // the epilogue's staged f16 output rows (1040 B apart)
+    constexpr int LDS_BYTES = 2 * 2 * TILEB > 4 * 32 * OSTR ? 2 * 2 * TILEB : 4 * 32 * OSTR;
+    __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES];  // [buffer][K, V]; output rows
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n32 = lane & 31, h = lane >> 5;
+    if ((int)blockIdx.x >= a.counts[0]) return;  // past the work list
+    const PagedUnit wu = a.units[blockIdx.x];
+    const int start_pos = wu.start, S = wu.S, row0 = wu.row0;
+    const int T_total = start_pos + S;
+    const int kh = wu.kh, qb = wu.qb, n_pieces = wu.n_pieces;
+
+    const int p0 = start_pos + qb * BQ;
+    const int kv_hi = min(p0 + BQ, T_total);
+    // first attended key (of a tree: by a root)
+    const int first = a.window > 0 ? max(0, (TREE ? start_pos : p0) + 1 - a.window) : 0;
+    const int wg_lo = first & (TREE ? ~(KT - 1) : ~15);
+    const int t0 = wu.t0, t1 = wu.t1;
+
+    // ---- this lane's query column (head hh, position offset pl) and 8-dim half h
+    const int c = 32 * wave + n32;
+    const int hh = c % G, pl = c / G;
+    const int s_raw = qb * BQ + pl;
+    const bool col_ok = s_raw < S;
+    const int s_idx = col_ok ? s_raw : S - 1;
+    int pos = start_pos + s_idx;
+    if constexpr (TREE) pos = start_pos + a.depth[row0 + s_idx];
+
+    // K/V rows: wave w moves rows 8w .. 8w + 7 of a tile, one 1 KiB row an instruction. (The lane index
+    // passes through an empty asm each time, so the source offsets are formed where they are used rather
+    // than held in registers across the loop.)
+    const int rowg = a.n_kv_heads * HD * 2;
+    TilePages<KT> pages;
+    // the 16 rows of tile t that this wave's 8 belong to, from the page of `entry`; past the last tile: an
+    // empty range
+    const auto tile_rows = [&](const void* pool, int t, int entry) {
+        const int kg = wg_lo + t * KT + 16 * (wave >> 1);
+        return page_rows(a.t, pool, entry, kg, t < t1 ? kv_hi : kg, rowg / 2, kh * HD);
+    };
+    const auto dma = [&](rsrc_t rp, char* dst, int j, int row_off, int swz) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rp, (__attribute__((address_space(3))) void*)(dst + (8 * wave + j) * ROWB), 16,
+                                                 row_off + 16 * (ln ^ swz), 0, 0, 0);
+    };
+    const auto row_off = [&](int j) { return (8 * (wave & 1) + j) * rowg; };
+    const auto k_swz = [&](int j) { return (8 * wave + j) & 31; };
+    const auto v_swz = [&](int j) { return vswz(j); };
+    const auto tile_k = [&](int t) { return lds + (t & 1) * 2 * TILEB; };
+    const auto tile_v = [&](int t) { return lds + (t & 1) * 2 * TILEB + TILEB; };
+
+    // ---- q: lane (column c, half h) holds dims 16s + 8h .. +7 (s < 32), the B operand layout. Wave w
+    // DMAs the f16 q rows of its 32 columns, whole 1 KiB rows (chunk n of a row from logical chunk
+    // n ^ (column % 32)), into its 16 KiB of the LDS stage that tile t0 + 1 takes over later, in two
+    // rounds of 16 rows, and reads each round back in that layout; tile t0's DMA goes out after the
+    // first round's. Rows past the block's last token read as zeros.
+    half8 qf[32];
+    int entry1 = wave >> 1 ? wu.page[1] : wu.page[0];  // tile t + 1's page
+    // the 16-row groups of tiles t and t + 1 without one
+    int gone0 = (page_ok(a.t, wu.page[0]) ? 0 : 1) | (page_ok(a.t, wu.page[1]) ? 0 : 2), gone1 = 0;
+    {
+        const rsrc_t rq = make_rsrc(a.q16 + ((size_t)row0 + qb * BQ) * a.n_q_heads * HD, (uint32_t)min(BQ, S - qb * BQ) * a.n_q_heads * ROWB);
+        pages.load(a.t, wu.b, wg_lo + t0 * KT, wave >> 1, lane);
+        char* qs = lds + ((t0 + 1) & 1) * 2 * TILEB + wave * 16 * ROWB;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int cj = 32 * wave + 16 * r + j;  // the column whose row this DMA moves
+                const int qo = ((cj / G) * a.n_q_heads + kh * G + cj % G) * ROWB + 16 * (ln ^ (16 * r + j));
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rq, (__attribute__((address_space(3))) void*)(qs + j * ROWB),
+                                                         16, qo, 0, 0, 0);
+            }
+            if (r == 0 && t0 < t1) {
+                // of the block's first tile, rows in front of the first attended key read as zeros
+                const rsrc_t rk = tile_rows(a.kc, t0, entry1), rv = tile_rows(a.vc, t0, entry1);
+                const int skip = first - (wg_lo + t0 * KT + 16 * (wave >> 1));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int ro = 8 * (wave & 1) + j < skip ? kNoRow : row_off(j);
+                    dma(rk, tile_k(t0), j, ro, k_swz(j));
+                    dma(rv, tile_v(t0), j, ro, v_swz(j));
+                }
+                asm volatile("s_waitcnt vmcnt(16)" ::: "memory");  // the 16 q DMAs before tile t0's
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            }
+            if ((n32 >> 4) == r) {
+                const char* qrow = qs + (n32 & 15) * ROWB;
+#pragma unroll
+                for (int s = 0; s < 32; ++s) qf[s] = *reinterpret_cast<const half8*>(qrow + 16 * ((2 * s + h) ^ n32));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's 16 KiB free again
+        }
+        if (!col_ok) {
+#pragma unroll
+            for (int s = 0; s < 32; ++s) qf[s] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+        }
+    }
+
+    // ---- key ranges: this wave [w_lo, wp1], this column [col_lo, pos]
+    const int wp0 = p0 + (32 * wave) / G;
+    const int wp1 = min(p0 + (32 * wave + 31) / G, T_total - 1);
+    const int col_lo = a.window > 0 ? pos + 1 - a.window : 0;
+    int lo_max = 0;  // tree: the last column's first attended key of the history
+    if constexpr (TREE) {
+        lo_max = col_lo;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) lo_max = max(lo_max, __shfl_xor(lo_max, d));
+        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    }
+    // tree: the word of tile t for this lane's column, if the tile holds rows of the call
+    const auto tree_word = [&](int t) {
+        unsigned long long w = ~0ull;
+        if constexpr (TREE) {
+            const int kb = wg_lo + t * KT;
+            if (t < t1 && kb + KT > start_pos) {
+                const unsigned long long* row = a.bits + (size_t)(row0 + s_idx) * a.words;
+                if constexpr (KT == 64) w = row[(kb - (start_pos & ~63)) >> 6];
+                else w = reinterpret_cast<const uint32_t*>(row)[(kb - (start_pos & ~63)) >> 5];
+            }
+        }
+        return w;
+    };
+
+    // LDS read offsets. K operand k-step s of this lane: row n32, chunk (2s + h) ^ n32, i.e.
+    // byte kofs ^ 32s with kofs = 1024 n32 + 16 (h ^ n32). Transposed V reads (as
+    // prefill_kernel_w32's): row 16u + 8i + vr0, chunk (4dt + vc0) ^ vsw, i.e. byte
+    // (vofs ^ 64dt) + 1024 (16u + 8i) with vofs = 1024 vr0 + 16 (vc0 ^ vsw) + vb0. Both offsets
+    // pass through an empty asm every tile, so the compiler forms the 32 + 16 XORs in the
+    // loop instead of holding 48 hoisted addresses.
+    const int m16 = lane & 15, half16 = (lane >> 4) & 1;
+    const int vr0 = 4 * h + (m16 >> 2);
+    const int vc0 = 2 * half16 + ((m16 & 3) >> 1);
+    const int vb0 = 8 * (m16 & 1);
+    const int kofs0 = 1024 * n32 + 16 * (h ^ n32);
+    const int vofs0 = 1024 * vr0 + 16 * (vc0 ^ vswz(vr0)) + vb0;
+
+    float16v oacc[16];  // O^T[32dt + 8(r/4) + 4h + r%4][column]
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt) oacc[dt] = float16v{};
+#pragma unroll
+    for (int dt = 0; dt < 16; ++dt) asm volatile("" : "+a"(oacc[dt]));
+    float m_use = kNegInf, l_run = 0.0f;
+    bool started = false;
+    // Masks of tile t's scores: key kb + 4h + 8(r/4) + r%4 of this lane's column; tiles inside every column's
+    // range skip it.
+    auto mask = [&](int t, int gone, unsigned long long word, float16v& sc) {
+        const int kb = wg_lo + t * KT;
+        if constexpr (TREE) {
+            if (kb + KT > start_pos) {
+                const uint32_t w = (uint32_t)word >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[r] = w >> (8 * (r >> 2) + (r & 3)) & 1 ? sc[r] : kNegInf;
+            } else if (a.window > 0 && kb < lo_max) {
+                const int rel_lo = col_lo - (kb + 4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[r] = 8 * (r >> 2) + (r & 3) >= rel_lo ? sc[r] : kNegInf;
+            }
+        } else if ((kb + KT - 1 > wp0) || (a.window > 0 && kb < wp1 + 1 - a.window)) {
+            const int rel_hi = pos - (kb + 4 * h), rel_lo = col_lo - (kb + 4 * h);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int o = 8 * (r >> 2) + (r & 3);
+                sc[r] = (o <= rel_hi && o >= rel_lo) ? sc[r] : kNegInf;
+            }
+        }
+        if (gone) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = gone >> (r >> 3) & 1 ? kNegInf : sc[r];
+        }
+    };
+
+    // One tile, interleaved as in the hd-256 kernel: the 32 score MFMAs of tile t + 1 (even and odd k-steps
+    // in two chains, added at the end) with the 16 exponentials of tile t and the DMAs of V(t + 1) and
+    // K(t + 2); the 32 P.V MFMAs of tile t with the maxima of tile t + 1. On entry sacc holds tile t's
+    // scores, on return tile t + 1's.
+    float16v sacc = float16v{};
+    float mnext = kNegInf;  // this lane's maximum of them
+    auto tile = [&](int t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of V(t) and K(t + 1) are in LDS
+        __syncthreads();
+        const int gone = gone1, entry = entry1;             // of tile t + 1
+        const unsigned long long word = tree_word(t + 1);
+        {
+            const int j = (t + 2 - t0) & 63;
+            if (j == 0) pages.load(a.t, wu.b, wg_lo + (t + 2) * KT, wave >> 1, lane);
+            entry1 = __builtin_amdgcn_readlane(pages.entry, j);
+            gone1 = __builtin_amdgcn_readlane(pages.gone, j);
+        }
+        const float mloc = max32(mnext) * a.scale_log2;
+        const bool bump = mloc > m_use + kMaxLag;  // the running maxima move only past 2^kMaxLag
+        if (__any(bump)) {
+            const float m_new = fmaxf(m_use, mloc - kPagedLift);
+            const float corr = m_use == kNegInf ? 0.0f : fexp2(m_use - m_new);
+            l_run *= corr;
+            if (started) {
+                // one 16-register tile at a time: copied to VGPRs, scaled, pinned back into
+                // AGPRs (left to itself the compiler moves all 256 through VGPRs and spills)
+                asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"  // the last MFMA's writes, as in the epilogue
+                             : "+a"(oacc[0]), "+a"(oacc[1]), "+a"(oacc[2]), "+a"(oacc[3]), "+a"(oacc[4]),
+                               "+a"(oacc[5]), "+a"(oacc[6]), "+a"(oacc[7]), "+a"(oacc[8]), "+a"(oacc[9]),
+                               "+a"(oacc[10]), "+a"(oacc[11]), "+a"(oacc[12]), "+a"(oacc[13]), "+a"(oacc[14]),
+                               "+a"(oacc[15]));
+#pragma unroll
+                for (int dt = 0; dt < 16; ++dt) {
+                    float16v x = oacc[dt];
+                    asm volatile("" : "+v"(x));
+                    x *= corr;
+                    asm volatile("" : "+v"(x));
+                    oacc[dt] = x;
+                    asm volatile("" : "+a"(oacc[dt]));
+                }
+            }
+            m_use = m_new;
+        }
+        started = true;
+        const float msub = m_use == kNegInf ? 0.0f : m_use;
+        half8 pb[2];
+        float ps = 0.0f;
+        float16v se = float16v{}, so = float16v{};
+        {
+            int kofs = ((t + 1) & 1) * 2 * TILEB + kofs0;
+            asm volatile("" : "+v"(kofs));
+            half8 kr[3][2];
+            auto read_k = [&](int s) {
+                kr[s % 3][0] = *reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s)));
+                kr[s % 3][1] = *reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s + 32)));
+            };
+            // exponential v of the lane's 16 in three stages
+            float ex[2], ev[2];
+            auto arg = [&](int v) { ex[v & 1] = __builtin_fmaf(sacc[v], a.scale_log2, -msub); };
+            auto take = [&](int v) {
+                ps += ev[v & 1];
+                pb[v >> 3][v & 7] = (half_t)ev[v & 1];
+            };
+            read_k(0);
+            read_k(1);
+            arg(0);
+            const rsrc_t rv = tile_rows(a.vc, t + 1, entry), rk = tile_rows(a.kc, t + 2, entry1);
+#pragma unroll
+            for (int s = 0; s < 16; ++s) {
+                if (s + 2 < 16) read_k(s + 2);
+                se = mfma32(kr[s % 3][0], qf[2 * s], se);
+                ev[s & 1] = fexp2(ex[s & 1]);
+                if (s > 0) take(s - 1);
+                so = mfma32(kr[s % 3][1], qf[2 * s + 1], so);
+                if (s < 15) arg(s + 1);
+                if (s < 8) dma(rv, tile_v(t + 1), s, row_off(s), v_swz(s));
+                else dma(rk, tile_k(t + 2), s - 8, row_off(s - 8), k_swz(s - 8));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            take(15);
+        }
+        l_run += ps;
+        sacc = se + so;
+        // (here, not where they are used behind the masks' branches: the compiler would sink them there)
+        asm volatile("" : "+v"(pb[0]), "+v"(pb[1]), "+v"(l_run), "+v"(sacc));
+        if (t + 1 < t1) mask(t + 1, gone, word, sacc);
+
+        // O^T += V^T . P^T over two 16-key steps, 16 dims tiles each; transposed V reads (two an MFMA) kPvAhead
+        // MFMAs ahead
+        {
+            int vofs = (t & 1) * 2 * TILEB + TILEB + vofs0;
+            asm volatile("" : "+v"(vofs));
+            half8 av[kPvAhead + 1];
+            auto read_v = [&](int i) {
+                const char* vp = lds + (vofs ^ (64 * (i & 15))) + 16 * (i >> 4) * ROWB;
+                const half4 lo = read_tr16(reinterpret_cast<const half_t*>(vp));
+                const half4 hi = read_tr16(reinterpret_cast<const half_t*>(vp + 8 * ROWB));
+                av[i % (kPvAhead + 1)] = half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            mnext = kNegInf;
+#pragma unroll
+            for (int i = 0; i < kPvAhead; ++i) read_v(i);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                if (i + kPvAhead < 32) read_v(i + kPvAhead);
+                mfma32_acc(oacc[i & 15], av[i % (kPvAhead + 1)], pb[i >> 4]);
+                if (i >= 8 && i < 16) mnext = fmaxf(mnext, fmaxf(sacc[2 * (i - 8)], sacc[2 * (i - 8) + 1]));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            asm volatile("" : "+v"(mnext));
+        }
+    };
+    if (t0 < t1) {
+        __syncthreads();  // K(t0), V(t0); every wave has its q
+        entry1 = __builtin_amdgcn_readlane(pages.entry, 1);
+        gone1 = __builtin_amdgcn_readlane(pages.gone, 1);
+        const rsrc_t rk = tile_rows(a.kc, t0 + 1, entry1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dma(rk, tile_k(t0 + 1), j, row_off(j), k_swz(j));
+        float16v se = float16v{}, so = float16v{};
+        const int kofs = (t0 & 1) * 2 * TILEB + kofs0;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+            se = mfma32(*reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s))), qf[2 * s], se);
+            so = mfma32(*reinterpret_cast<const half8*>(lds + (kofs ^ (64 * s + 32))), qf[2 * s + 1], so);
+        }
+        sacc = se + so;
+        mask(t0, gone0, tree_word(t0), sacc);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mnext = fmaxf(mnext, sacc[r]);
+        for (int t = t0; t < t1; ++t) tile(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the last tile's (empty) DMAs, before LDS is used again
+    }
+
+    // ---- epilogue: the 512 dims of this wave's 32 columns. The accumulators are read by
+    // VALU instructions below, which must not issue within 18 wait states of the last MFMA
+    // writing them (the compiler does not see the asm MFMAs); the asm also orders every read
+    // after the wait, since each accumulator passes through it.
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
+                 : "+a"(oacc[0]), "+a"(oacc[1]), "+a"(oacc[2]), "+a"(oacc[3]), "+a"(oacc[4]), "+a"(oacc[5]),
+                   "+a"(oacc[6]), "+a"(oacc[7]), "+a"(oacc[8]), "+a"(oacc[9]), "+a"(oacc[10]), "+a"(oacc[11]),
+                   "+a"(oacc[12]), "+a"(oacc[13]), "+a"(oacc[14]), "+a"(oacc[15]));
+    const float l_tot = add32(l_run);
+    if (n_pieces > 1) {  // a piece of a split query block: O / l and (m, l)
+        if (TREE && !col_ok) return;  // few tokens: columns of none move no bytes
+        const float inv_p = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) store_part<false, HD, NCOL * HD>(a.part_o, true, wu.slot, wave, dt, lane, oacc[dt], inv_p);
+        if (h == 0) a.part_ml[(size_t)wu.slot * NCOL + c] = make_float2(m_use, l_tot);
+        return;
+    }
+    const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+    if constexpr (sizeof(OUTT) == 2) {
+        // f16 rows through LDS: each wave stages its 32 output rows, then stores one whole 1 KiB row
+        // an instruction
+        __syncthreads();  // every wave is done with the last tile's K/V
+        char* ost = lds + wave * 32 * OSTR;
+        auto stage = [&](auto quantise) {  // (one test of the step for all of them)
+#pragma unroll
+            for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2], oacc[dt][4 * j + 3]} * inv;
+                    if constexpr (decltype(quantise)::value) v = srq4(v, a.out_q);
+                    store4(reinterpret_cast<half_t*>(ost + n32 * OSTR) + 32 * dt + 8 * j + 4 * h, v);
+                }
+        };
+        if (a.out_q == 0.0f) stage(std::false_type{});
+        else stage(std::true_type{});
+#pragma unroll
+        for (int rr = 0; rr < 32; ++rr) {
+            const int cc = 32 * wave + rr, so = qb * BQ + cc / G;
+            const half8 val = *reinterpret_cast<const half8*>(ost + rr * OSTR + 16 * lane);
+            if (so < S)
+                *reinterpret_cast<half8*>(reinterpret_cast<half_t*>(a.out) +
+                                          ((size_t)(row0 + so) * a.n_q_heads + kh * G + cc % G) * HD + 8 * lane) = val;
+        }
+    } else if (col_ok) {
+        OUTT* orow = reinterpret_cast<OUTT*>(a.out) + ((size_t)(row0 + s_idx) * a.n_q_heads + kh * G + hh) * HD;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4v v = float4v{oacc[dt][4 * j], oacc[dt][4 * j + 1], oacc[dt][4 * j + 2],
+                                          oacc[dt][4 * j + 3]} * inv;
+                store4(orow + 32 * dt + 8 * j + 4 * h, srq4(v, a.out_q));
+            }
+    }
+}
+
+}  // namespace g4a
