@@ -311,6 +311,76 @@ int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, const 
                    size_t ws_bytes, void* stream);
 
 /*
+ * Greedy verification of drafted trees. drafts[t] is packed token t, targets[t] the token that the model puts behind it.
+ * A sequence's path is its token 0 and then, while there is one, the child of lowest index of the path's last token
+ * whose draft is that token's target.
+ *   path        int32 [n_seq][max_path]: the path's indices within the tree (max_path of them at most), then -1.
+ *   n_path      int32 [n_seq]: their number; 0 for a sequence without tokens.
+ *   next        int32 [n_seq]: the target of the path's last token, -1 without tokens.
+ *   kept        int32 [n_seq]: key_len - tokens + n_path, the keys that are left once g4a_paged_keep has run.
+ */
+int g4a_tree_accept(int n_tokens, int n_seq, const int32_t* cu_q, const int32_t* parents, const int32_t* drafts,
+                    const int32_t* targets, const int32_t* key_len, int max_path, int32_t* path, int32_t* n_path,
+                    int32_t* next, int32_t* kept, void* stream);
+
+/* Pages of one tensor of a cache (K or V of a layer): row r of page p at rows + (p * page_size + r) * row_bytes. */
+typedef struct g4a_pool {
+    void* rows;        /* 16-byte aligned */
+    int64_t row_bytes; /* a multiple of 16, at most 2^20 */
+} g4a_pool;
+#define G4A_POOLS_MAX 64
+
+/*
+ * Moves the rows of accepted paths up: row start + path[b][d] of sequence b to row start + d in every pool, for
+ * d < n_path[b] (start = key_len[b] - its tokens, key_len that of the tree's call; path ascends, as g4a_tree_accept writes
+ * it, and ends at an entry that does not or that is no token). A row whose page, or whose place's page, is not there stays.
+ * pg: its k_pages and v_pages are not used. Pools must not share memory.
+ */
+int g4a_paged_keep(const g4a_pool* pools, int n_pools, const g4a_paged* pg, int n_tokens, const int32_t* cu_q,
+                   const int32_t* path, int max_path, const int32_t* n_path, void* stream);
+
+/*
+ * The cache of beams that follow their parents: new row j continues row parent[j] of pg (a parent outside [0, n_seq): an
+ * idle row), so it has L = key_len[parent[j]] keys. pg holds every sequence that has pages of the pools; one that
+ * does not branch is a row whose parent is itself.
+ *   new_table   int32 [n_new][table_cols]. Columns below L / page_size are the parent's: pages shared by its heirs.
+ *               The columns behind, as many as L + room keys take, are ones that the row will write to: the first new
+ *               row that has its parent's page there keeps it, unless another row has it in a full column; every
+ *               other one gets a page off the end of the free list, into which the filled L % page_size rows are
+ *               copied in every pool. A filled page that is not there stays so. All other columns are -1.
+ *   new_len     int32 [n_new]: L.
+ *   free_pages  int32 [n_pages], n_free int32 [1], device: pages that no row holds. new_free is that list, with the
+ *               pages added in ascending order that some row of pg held and no new row does, less the ones taken
+ *               (in order of rows and columns), then -1; new_n_free its length. Without enough pages the last
+ *               columns that need one are -1. n_new * (2 + room / page_size) pages always suffice.
+ *   ws          at least g4a_paged_fork_ws_bytes() bytes, 256-byte aligned, uninitialised.
+ * The outputs must not overlap the inputs or each other.
+ */
+size_t g4a_paged_fork_ws_bytes(const g4a_paged* pg, int n_new);
+int g4a_paged_fork(const g4a_pool* pools, int n_pools, const g4a_paged* pg, int n_new, const int32_t* parent, int room,
+                   const int32_t* free_pages, const int32_t* n_free, int32_t* new_table, int32_t* new_len,
+                   int32_t* new_free, int32_t* new_n_free, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Beam search's selection. Beam w of group g has the logits x of row g * width + w and the score s; token t makes the
+ * candidate of score s + x'[t] - log sum exp x', x' = cap * tanh(x / cap) (cap 0: x' = x). Of a group's width * vocab
+ * candidates the n_out of highest score, best first, equal ones by beam and then by token.
+ *   logits      f32, or f16 with logits_f16, rows row_stride elements apart, 16-byte aligned. A token whose logit is -inf
+ *               or NaN is none: no weight, no candidate. +inf (without a cap) shares the weight with the row's other +inf.
+ *   done        uint8 [n_groups][width] or NULL: a beam that is done has one candidate, token pad at its own score.
+ *   out_score   f32, out_parent (the row of logits that the beam continues) and out_token int32 [n_groups][n_out]. A
+ *               candidate of score -inf or NaN is none: places without one hold -inf, -1, -1.
+ * Scores are formed in 64 bits from a row's sum in 32, and rounded once. Within a beam larger logits come first.
+ *   ws          at least g4a_beam_select_ws_bytes() bytes, 256-byte aligned, uninitialised.
+ * width and n_out are at most G4A_BEAMS_MAX.
+ */
+#define G4A_BEAMS_MAX 64
+size_t g4a_beam_select_ws_bytes(int n_groups, int width, int vocab, int n_out);
+int g4a_beam_select(int n_groups, int width, int vocab, int logits_f16, const void* logits, int64_t row_stride,
+                    const float* scores, const uint8_t* done, int pad, float cap, int n_out, float* out_score,
+                    int32_t* out_parent, int32_t* out_token, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * ---- The q/k/v producer: projections with QAT weights --------------------------------
  * Packed weights: row o of an [n_out][n_in] matrix is n_in*bits/32 uint32 words; value i
  * of the row sits at bit 8*(i/(8/bits)) + bits*(i%(8/bits)) of the row's bytes (byte-major,

@@ -29,7 +29,8 @@ EXPORTS = (
     "g4a_prefill_ws_bytes", "g4a_prefill", "g4a_qprep",
     "g4a_kv_write",
     "g4a_paged_write", "g4a_paged_decode_ws_bytes", "g4a_paged_decode", "g4a_paged_prefill_ws_bytes", "g4a_paged_prefill",
-    "g4a_paged_tree_ws_bytes", "g4a_paged_tree",
+    "g4a_paged_tree_ws_bytes", "g4a_paged_tree", "g4a_tree_accept", "g4a_paged_keep", "g4a_paged_fork_ws_bytes",
+    "g4a_paged_fork", "g4a_beam_select_ws_bytes", "g4a_beam_select",
     "g4a_dequant", "g4a_qkv_gemv", "g4a_qkv_gemv_norm", "g4a_srqh", "g4a_gemm16",
     "g4a_gemm16_ws_bytes", "g4a_gemm16_ws", "g4a_gemm16_geglu",
     "g4a_qgemv", "g4a_qgemv_geglu", "g4a_qgemv_gelu_mul", "g4a_gemv_f16", "g4a_rms_norm", "g4a_geglu",
@@ -43,6 +44,10 @@ GEMM_TICKET_BYTES = 2048
 
 # most tokens of a drafted tree (G4A_TREE_MAX)
 TREE_MAX = 1024
+
+# most pools of a call (G4A_POOLS_MAX), most beams of a group (G4A_BEAMS_MAX)
+POOLS_MAX = 64
+BEAMS_MAX = 64
 
 # g4a_rows_tail modes (g4attn.h)
 TAIL_NONE, TAIL_SRQ, TAIL_NORM, TAIL_NORM16 = 0, 1, 2, 3
@@ -87,6 +92,14 @@ class G4APaged(ctypes.Structure):
         ("table_stride", ctypes.c_int32),
         ("max_key_len", ctypes.c_int32),
         ("reserved", ctypes.c_int32 * 2),
+    ]
+
+
+class G4APool(ctypes.Structure):
+    """struct g4a_pool: the pages of one tensor of a cache."""
+    _fields_ = [
+        ("rows", ctypes.c_void_p),
+        ("row_bytes", ctypes.c_int64),
     ]
 
 
@@ -171,6 +184,19 @@ def load() -> ctypes.CDLL:
     lib.g4a_paged_tree_ws_bytes.argtypes = [cfgp, pgp, i]
     lib.g4a_paged_tree.restype = ctypes.c_int
     lib.g4a_paged_tree.argtypes = [cfgp, pgp, i, P, P, P, P, P, P, P, P, f, f, P, P, P, zp, P]
+    pools = ctypes.POINTER(G4APool)
+    lib.g4a_tree_accept.restype = ctypes.c_int
+    lib.g4a_tree_accept.argtypes = [i, i, P, P, P, P, P, i, P, P, P, P, P]
+    lib.g4a_paged_keep.restype = ctypes.c_int
+    lib.g4a_paged_keep.argtypes = [pools, i, pgp, i, P, P, i, P, P]
+    lib.g4a_paged_fork_ws_bytes.restype = zp
+    lib.g4a_paged_fork_ws_bytes.argtypes = [pgp, i]
+    lib.g4a_paged_fork.restype = ctypes.c_int
+    lib.g4a_paged_fork.argtypes = [pools, i, pgp, i, P, i, P, P, P, P, P, P, P, zp, P]
+    lib.g4a_beam_select_ws_bytes.restype = zp
+    lib.g4a_beam_select_ws_bytes.argtypes = [i, i, i, i]
+    lib.g4a_beam_select.restype = ctypes.c_int
+    lib.g4a_beam_select.argtypes = [i, i, i, i, P, ctypes.c_int64, P, P, i, f, i, P, P, P, P, zp, P]
     lib.g4a_dequant.restype = ctypes.c_int
     lib.g4a_dequant.argtypes = [i, i, i, P, P, P, P]
     lib.g4a_qkv_gemv.restype = ctypes.c_int

@@ -18,6 +18,24 @@ int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8) {
         set_error("k_pages and v_pages must be 16-byte aligned, page_table and key_len 4-byte aligned");
         return G4A_EINVAL;
     }
+    if (const int rc = check_table(pg)) return rc;
+    if (cfg->head_dim != 256 && cfg->head_dim != 512) {
+        set_error("head_dim %u not supported (256 or 512)", cfg->head_dim);
+        return G4A_EUNSUPPORTED;
+    }
+    if (cfg->n_kv_heads > 4096 || cfg->n_q_heads > 32768 || (int64_t)pg->n_seq * cfg->n_kv_heads > 65535) {
+        set_error("n_kv_heads (%u), n_q_heads (%u) or n_seq * n_kv_heads (n_seq %d) too large", cfg->n_kv_heads,
+                  cfg->n_q_heads, pg->n_seq);
+        return G4A_EINVAL;
+    }
+    if (cfg->window > 1u << 30) {
+        set_error("window (%u) must be at most 2^30", cfg->window);
+        return G4A_EINVAL;
+    }
+    return G4A_OK;
+}
+
+int check_table(const g4a_paged* pg) {
     const int ps = pg->page_size;
     if (ps < 16 || ps > 65536 || (ps & (ps - 1))) {
         set_error("page_size must be a power of two of 16 .. 65536 (got %d)", ps);
@@ -34,19 +52,6 @@ int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8) {
     }
     if (pg->reserved[0] || pg->reserved[1]) {
         set_error("g4a_paged's reserved words must be 0");
-        return G4A_EINVAL;
-    }
-    if (cfg->head_dim != 256 && cfg->head_dim != 512) {
-        set_error("head_dim %u not supported (256 or 512)", cfg->head_dim);
-        return G4A_EUNSUPPORTED;
-    }
-    if (cfg->n_kv_heads > 4096 || cfg->n_q_heads > 32768 || (int64_t)pg->n_seq * cfg->n_kv_heads > 65535) {
-        set_error("n_kv_heads (%u), n_q_heads (%u) or n_seq * n_kv_heads (n_seq %d) too large", cfg->n_kv_heads,
-                  cfg->n_q_heads, pg->n_seq);
-        return G4A_EINVAL;
-    }
-    if (cfg->window > 1u << 30) {
-        set_error("window (%u) must be at most 2^30", cfg->window);
         return G4A_EINVAL;
     }
     return G4A_OK;

@@ -68,6 +68,7 @@ __device__ __forceinline__ int seq_of_row(const int32_t* cu, int n_seq, int tok)
 
 // checks of a g4a_paged and the config that goes with it; 0 or the error code (g4a_last_error set)
 int check_paged(const g4a_cfg* cfg, const g4a_paged* pg, bool need_group_le8);
+int check_table(const g4a_paged* pg);  // of them the table's sizes alone
 // ... of the operands that paged decode and prefill share, n_tokens rows of q and out
 int check_paged_call(const g4a_cfg* cfg, int n_tokens, const float* q, const float* q_gain, const float* rcos,
                      const float* rsin, const void* out);

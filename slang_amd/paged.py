@@ -88,14 +88,8 @@ def _launch(dev, fn, *args):
         return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin):
-    """The checked g4a_paged of a call, and the addresses of the RoPE tables."""
-    shape, kv = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or shape[2] != cfg.n_kv_heads or shape[3] != cfg.head_dim or v_pages.shape != shape:
-        raise ValueError(f"k_pages / v_pages must be [n_pages][page_size][{cfg.n_kv_heads}][{cfg.head_dim}], got "
-                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
-    if kv not in _HALF_OR_FLOAT or v_pages.dtype is not kv:
-        raise ValueError("k/v pages must both be float16 or both float32")
+def _table(dev, page_table, key_len, n_pages, page, max_key_len, rope_cos=None):
+    """What g4a_paged holds behind the pages, of a call's checked table and lengths."""
     if page_table.get_device() != dev or page_table.dtype is not _I32 or page_table.dim() != 2:
         raise ValueError(f"page_table must be an int32 tensor [n_seq][cols] on cuda:{dev}")
     n_seq, cols = page_table.shape
@@ -109,13 +103,25 @@ def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_co
     lens = _t("key_len", key_len, dev, _I32)
     if key_len.numel() != n_seq:
         raise ValueError(f"key_len must have one entry per row of page_table ({n_seq}), got {key_len.numel()}")
-    page = shape[1]
     if max_key_len is None:
         max_key_len = cols * page
         if rope_cos is not None:
             max_key_len = min(max_key_len, rope_cos.shape[0])
     if not 0 < max_key_len <= cols * page:
         raise ValueError(f"max_key_len must be in [1, {cols * page}], what the page table's columns hold")
+    return page_table.data_ptr(), lens, n_pages, page, n_seq, cols, stride, int(max_key_len)
+
+
+def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin):
+    """The checked g4a_paged of a call, and the addresses of the RoPE tables."""
+    shape, kv = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or shape[2] != cfg.n_kv_heads or shape[3] != cfg.head_dim or v_pages.shape != shape:
+        raise ValueError(f"k_pages / v_pages must be [n_pages][page_size][{cfg.n_kv_heads}][{cfg.head_dim}], got "
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
+    if kv not in _HALF_OR_FLOAT or v_pages.dtype is not kv:
+        raise ValueError("k/v pages must both be float16 or both float32")
+    table = _table(dev, page_table, key_len, shape[0], shape[1], max_key_len, rope_cos)
+    max_key_len = table[-1]
     if (rope_cos is None) != (rope_sin is None):
         raise ValueError("rope_cos and rope_sin go together")
     rc = rs = None
@@ -125,8 +131,7 @@ def _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_co
         if len(rows) != 2 or rows[0] < max_key_len or rows[1] * 2 != cfg.head_dim or rope_sin.shape != rows:
             raise ValueError(f"rope tables must be [>= max_key_len ({max_key_len})][head_dim/2], got "
                              f"{tuple(rows)} and {tuple(rope_sin.shape)}")
-    return G4APaged(_t("k_pages", k_pages, dev, kv), _t("v_pages", v_pages, dev, kv), page_table.data_ptr(), lens, shape[0],
-                    page, n_seq, cols, stride, int(max_key_len)), rc, rs
+    return G4APaged(_t("k_pages", k_pages, dev, kv), _t("v_pages", v_pages, dev, kv), *table), rc, rs
 
 
 def _cu(cu_q, n_seq, dev):
