@@ -95,14 +95,6 @@ class G4APaged(ctypes.Structure):
     ]
 
 
-class G4APool(ctypes.Structure):
-    """struct g4a_pool: the pages of one tensor of a cache."""
-    _fields_ = [
-        ("rows", ctypes.c_void_p),
-        ("row_bytes", ctypes.c_int64),
-    ]
-
-
 class G4ANormIn(ctypes.Structure):
     """struct g4a_norm_in: the residual-add + norm prologue of the fused GEMVs."""
     _fields_ = [
@@ -184,15 +176,14 @@ def load() -> ctypes.CDLL:
     lib.g4a_paged_tree_ws_bytes.argtypes = [cfgp, pgp, i]
     lib.g4a_paged_tree.restype = ctypes.c_int
     lib.g4a_paged_tree.argtypes = [cfgp, pgp, i, P, P, P, P, P, P, P, P, f, f, P, P, P, zp, P]
-    pools = ctypes.POINTER(G4APool)
     lib.g4a_tree_accept.restype = ctypes.c_int
     lib.g4a_tree_accept.argtypes = [i, i, P, P, P, P, P, i, P, P, P, P, P]
     lib.g4a_paged_keep.restype = ctypes.c_int
-    lib.g4a_paged_keep.argtypes = [pools, i, pgp, i, P, P, i, P, P]
+    lib.g4a_paged_keep.argtypes = [P, i, pgp, i, P, P, i, P, P]
     lib.g4a_paged_fork_ws_bytes.restype = zp
     lib.g4a_paged_fork_ws_bytes.argtypes = [pgp, i]
     lib.g4a_paged_fork.restype = ctypes.c_int
-    lib.g4a_paged_fork.argtypes = [pools, i, pgp, i, P, i, P, P, P, P, P, P, P, zp, P]
+    lib.g4a_paged_fork.argtypes = [P, i, pgp, i, P, i, P, P, P, P, P, P, P, zp, P]
     lib.g4a_beam_select_ws_bytes.restype = zp
     lib.g4a_beam_select_ws_bytes.argtypes = [i, i, i, i]
     lib.g4a_beam_select.restype = ctypes.c_int

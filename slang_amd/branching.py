@@ -22,12 +22,14 @@ on new ones. Calls run on the current stream of the tensors' device.
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import math
 
 import torch
 
 from . import _lib
-from ._lib import G4APaged, G4APool, check
+from ._lib import G4APaged, check
 from .attention import AttnConfig, DecodeWorkspace
 from .paged import (_F16, _F32, _HALF_OR_FLOAT, _I32, _cache, _cu, _gain, _gpu, _launch, _out, _q, _refuse, _sizes, _t, _table,
                     _with_scratch)
@@ -42,21 +44,25 @@ class CachePools:
     list of tensors, which they then check anew each time."""
 
     def __init__(self, pools):
-        pools = list(pools)
+        pools = self.tensors = list(pools)
         if len(pools) > _lib.POOLS_MAX:
             raise ValueError(f"at most {_lib.POOLS_MAX} pools a call, got {len(pools)}")
-        self.tensors, self.dev, self.shape = pools, -1, (0, 0)
-        self.c = (G4APool * max(1, len(pools)))()
-        for i, p in enumerate(pools):
-            if p.dim() < 3:
-                raise ValueError(f"pool {i} must be [n_pages][page_size][...], got {tuple(p.shape)}")
-            if i == 0:
-                self.dev, self.shape = _gpu("pool 0", p), tuple(p.shape[:2])
+        self.dev, self.shape, at, like, kind, row = -1, (0, 0), [], None, None, 0
+        for p in pools:
+            if p.shape != like or p.dtype is not kind:  # layers are mostly alike
+                like, kind = p.shape, p.dtype
+                if len(like) < 3:
+                    raise ValueError(f"a pool must be [n_pages][page_size][...], got {tuple(like)}")
+                if not at:
+                    self.dev, self.shape = _gpu("a pool", p), tuple(like[:2])
+                if tuple(like[:2]) != self.shape:
+                    raise ValueError(f"a pool holds {tuple(like[:2])} pages and rows, the first one {self.shape}")
+                row = math.prod(like[2:]) * p.element_size()
             if p.get_device() != self.dev or not p.is_contiguous():
-                _refuse(f"pool {i}", p, self.dev, p.dtype)
-            if tuple(p.shape[:2]) != self.shape:
-                raise ValueError(f"pool {i} holds {tuple(p.shape[:2])} pages and rows, pool 0 {self.shape}")
-            self.c[i] = G4APool(p.data_ptr(), p[0, 0].numel() * p.element_size() if p.numel() else 0)
+                _refuse("a pool", p, self.dev, kind)
+            at += p.data_ptr(), row
+        self._c = array.array("q", at)  # struct g4a_pool [n]: an address, bytes of a row
+        self.c = self._c.buffer_info()[0]
 
     def __len__(self):
         return len(self.tensors)
@@ -129,7 +135,7 @@ def paged_tree(q, k_pages, v_pages, page_table, key_len, cu_q, parents, cfg: Att
 
 def _i32(name, t, dev, shape):
     at = _t(name, t, dev, _I32)
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be int32 {list(shape)}, got {tuple(t.shape)}")
     return at
 
@@ -146,23 +152,24 @@ def tree_accept(drafts, targets, parents, cu_q, key_len, *, max_path: int | None
     dev = _gpu("drafts", drafts)
     if drafts.dim() != 1:
         raise ValueError(f"drafts must hold one token per packed row, got {tuple(drafts.shape)}")
-    n = drafts.shape[0]
+    n, n_seq = drafts.shape[0], key_len.numel()
     dr, tg, par = _t("drafts", drafts, dev, _I32), _i32("targets", targets, dev, (n,)), _parents(parents, n, dev)
-    lens, n_seq = _t("key_len", key_len, dev, _I32), key_len.numel()
-    cu = _cu(cu_q, n_seq, dev)
-    if max_path is None:
-        max_path = max(1, min(n, _lib.TREE_MAX))
-    max_path = int(max_path)
-    if max_path < 1 or n_seq > 2 ** 31 - 1:
+    lens, cu = _t("key_len", key_len, dev, _I32), _cu(cu_q, n_seq, dev)
+    max_path = max(1, min(n, _lib.TREE_MAX)) if max_path is None else int(max_path)
+    if max_path < 1:
         raise ValueError(f"max_path must be positive, got {max_path}")
-    shapes = ((n_seq, max_path), (n_seq,), (n_seq,), (n_seq,))
     if out is None:
-        out = tuple(torch.empty(s, dtype=_I32, device=drafts.device) for s in shapes)
-    at = [_i32(name, t, dev, s) for name, t, s in zip(("path", "n_path", "next", "kept"), out, shapes)]
+        one = key_len if key_len.dim() == 1 else key_len.view(-1)
+        out = (torch.empty((n_seq, max_path), dtype=_I32, device=drafts.device), torch.empty_like(one), torch.empty_like(one),
+               torch.empty_like(one))
+        at = [t.data_ptr() for t in out]
+    else:
+        shapes = ((n_seq, max_path), (n_seq,), (n_seq,), (n_seq,))
+        at = [_i32(name, t, dev, s) for name, t, s in zip(("path", "n_path", "next", "kept"), out, shapes)]
     if n_seq == 0:
         return tuple(out)
     if n == 0:  # no sequence has a token
-        out[0].fill_(-1), out[1].zero_(), out[2].fill_(-1), out[3].copy_(key_len)
+        out[0].fill_(-1), out[1].zero_(), out[2].fill_(-1), out[3].copy_(key_len.view(-1))
         return tuple(out)
     check(_launch(dev, _lib.load().g4a_tree_accept, n, n_seq, cu, par, dr, tg, lens, max_path, *at))
     return tuple(out)
@@ -224,10 +231,13 @@ def paged_fork(pools, page_table, key_len, parent, free_pages, n_free, *, worksp
     room = int(room)
     if not 0 <= room <= 1 << 30:
         raise ValueError(f"room must be in [0, 2^30], got {room}")
-    shapes = ((n_new, pg.table_cols), (n_new,), (pg.n_pages,), (1,))
     if out is None:
-        out = tuple(torch.empty(s, dtype=_I32, device=page_table.device) for s in shapes)
-    at = [_i32(name, t, dev, s) for name, t, s in zip(("new table", "new key_len", "new free_pages", "new n_free"), out, shapes)]
+        out = (torch.empty((n_new, pg.table_cols), dtype=_I32, device=page_table.device), torch.empty_like(parent),
+               torch.empty_like(free_pages), torch.empty_like(n_free))
+        at = [t.data_ptr() for t in out]
+    else:
+        shapes = ((n_new, pg.table_cols), (n_new,), (pg.n_pages,), (1,))
+        at = [_i32(name, t, dev, s) for name, t, s in zip(("new table", "new key_len", "new free_pages", "new n_free"), out, shapes)]
     if pg.n_seq == 0 or n_new == 0:
         raise ValueError("paged_fork needs a row to follow and a row that follows")
     lib, p = _lib.load(), ctypes.byref(pg)
@@ -271,12 +281,18 @@ def beam_select(logits, scores, *, workspace: DecodeWorkspace, cap: float = 0.0,
             raise ValueError(f"done must be bool, shaped like scores {tuple(scores.shape)}, got {done.dtype} {tuple(done.shape)}")
         dn = _t("done", done, dev, done.dtype)
     if out is None:
-        out = tuple(torch.empty((groups, n_out), dtype=t, device=logits.device) for t in (_F32, _I32, _I32))
-    at = []
-    for name, t, kind in zip(("score", "parent", "token"), out, (_F32, _I32, _I32)):
-        at.append(_t(name, t, dev, kind))
-        if tuple(t.shape) != (groups, n_out):
-            raise ValueError(f"{name} must be [{groups}][{n_out}], got {tuple(t.shape)}")
+        where = logits.device
+        if n_out < 0:
+            raise ValueError(f"n_out must be positive, got {n_out}")
+        token = torch.empty((groups, n_out), dtype=_I32, device=where)
+        out = torch.empty((groups, n_out), dtype=_F32, device=where), torch.empty_like(token), token
+        at = [t.data_ptr() for t in out]
+    else:
+        at = []
+        for name, t, kind in zip(("score", "parent", "token"), out, (_F32, _I32, _I32)):
+            at.append(_t(name, t, dev, kind))
+            if tuple(t.shape) != (groups, n_out):
+                raise ValueError(f"{name} must be [{groups}][{n_out}], got {tuple(t.shape)}")
     if groups == 0:
         return tuple(out)
     lib, f16 = _lib.load(), int(logits.dtype is _F16)

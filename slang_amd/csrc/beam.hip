@@ -1,15 +1,15 @@
 // Beam search's selection over beams and vocabulary (g4a_beam_select).
 //
 // Scores within a beam are ordered as its logits, so a row's candidates are its n_out largest logits, and the sum of
-// exponentials is needed only to compare beams. One pass over the logits: a wave takes 64 * E of a row into registers and
-// writes its maximum, its sum and its n_out largest. A second launch joins a row's waves, and in the group's last row
-// the beams.
+// exponentials is needed only to compare beams. One pass over the logits: a wave walks a part of a row, 64 * E at a time
+// in registers while the next are on their way, and keeps the maximum, the sum relative to it and the n_out largest. A second
+// launch, a workgroup a group, joins each row's parts and then the beams.
 //
-// A logit's place in the order is a 64-bit key: its bits, made to ascend, over the complement of its token, so that
-// equal logits come lowest token first and no two keys are the same; 0 is no candidate (NaN and -inf are none).
+// Logits are ranked by 64-bit keys: a logit's bits, made to ascend, over the complement of its token, so that equal
+// logits come lowest token first and no two keys are the same; 0 is no candidate (NaN and -inf are none).
 #include <algorithm>
 
-#include "common.hpp"
+#include "paged.hpp"
 
 namespace g4a {
 
@@ -26,9 +26,7 @@ struct BeamArgs {
     int32_t* out_token;
     float2* sums;     // [rows][parts]: maximum, sum of 2^(log2e (x' - maximum))
     u64* keys;        // [rows][parts][n_out], largest first
-    u64* row_keys;    // [rows][n_out]
-    double2* row_sum;  // [rows]: the largest x', the logarithm of the sum of exp(x' - it)
-    int width, vocab, n_out, parts, pad;
+    int width, vocab, n_out, parts, steps, pad;  // a part is 64 * E * steps logits
     float cap;
 };
 
@@ -42,9 +40,15 @@ __device__ __forceinline__ float of_ascending(uint32_t u) {
 }
 __device__ __forceinline__ u64 key_of(float x, int token) { return (u64)ascending(x) << 32 | (uint32_t)~token; }
 
-// x' of a logit: cap tanh(x / cap) as cap - 2 cap / (1 + 2^(2 log2e x / cap)); up2 = 2 log2e / cap
-__device__ __forceinline__ float capped(float x, float cap, float up2) {
-    return cap == 0.0f ? x : __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + fexp2(x * up2)), cap);
+// x' log2e / unit of a logit: unit is log2e with a cap, cap tanh(x / cap) as cap - 2 cap / (1 + 2^(2 log2e x / cap)), and 1
+// without, so that the difference of two, which is exact where it matters, is rounded last. up2 = 2 log2e / cap
+template <bool CAP>
+__device__ __forceinline__ float capped(float x, float cap2, float up2) {
+    return CAP ? __builtin_fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + fexp2(x * up2)), cap2) : x;
+}
+// ... in 64 bits, where beams are compared (not by tanh(), whose 64 bits take a microsecond)
+__device__ __forceinline__ double capped64(float x, float cap) {
+    return cap == 0.0f ? (double)x : (double)cap - 2.0 * (double)cap / (1.0 + exp(2.0 * (double)x / (double)cap));
 }
 
 __device__ __forceinline__ u64 wave_max64(u64 k) {
@@ -56,220 +60,295 @@ __device__ __forceinline__ u64 wave_max64(u64 k) {
     return k;
 }
 
-// The wave's `want` largest of the keys x[0 .. N) of all its lanes, largest first, to out (0 behind the last). Fast: the
-// want-th largest of the lanes' own maxima bounds the want-th largest key from below; the few keys that pass it go to
-// `list` (kList keys of the wave's own LDS), where each counts the ones above it. More than kList pass where many are
-// equal: then one maximum after the other.
-constexpr int kList = 128;
-template <int N>
-__device__ __forceinline__ void wave_top(const u64 (&x)[N], int want, u64* list, u64* out, int lane) {
-    u64 mine = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) mine = x[i] > mine ? x[i] : mine;
-    // the largest bound that `want` lanes' maxima reach, by its bits from the top
+// The upper 16 bits of a value that `want` lanes' `top` reach (0: fewer do), found from the highest bit down. Where
+// `top` is the largest of a lane's values, at least `want` values reach it, and not many more do.
+__device__ __forceinline__ uint32_t wave_bound(uint32_t top, int want) {
     uint32_t bound = 0;
-    const uint32_t top = (uint32_t)(mine >> 32);
-    for (int b = 31; b >= 0; --b) {
+#pragma unroll
+    for (int b = 31; b >= 16; --b) {
         const uint32_t t = bound | 1u << b;
         if (__builtin_popcountll(__ballot(top >= t)) >= want) bound = t;
     }
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) n += x[i] != 0 && (uint32_t)(x[i] >> 32) >= bound;
-    int at = 0, total = 0;
-    {
-        int incl = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(incl, d);
-            if (lane >= d) incl += y;
-        }
-        at = incl - n;
-        total = __builtin_amdgcn_readlane(incl, 63);
-    }
-    if (total <= kList) {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (x[i] != 0 && (uint32_t)(x[i] >> 32) >= bound) list[at++] = x[i];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        for (int k = lane; k < total; k += 64) {
-            const u64 me = list[k];
-            int rank = 0;
-            for (int o = 0; o < total; ++o) rank += list[o] > me;
-            if (rank < want) out[rank] = me;
-        }
-        for (int k = total + lane; k < want; k += 64) out[k] = 0;
-        __builtin_amdgcn_wave_barrier();
-        return;
-    }
-    u64 last = ~0ull;
-    for (int k = 0; k < want; ++k) {
-        u64 best = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) best = x[i] < last && x[i] > best ? x[i] : best;
-        best = wave_max64(best);
-        if (lane == 0) out[k] = best;
-        last = best;
-    }
+    return bound;
 }
 
-// A wave's 64 * E logits of a row, E / VEC loads of 16 bytes a lane. Rows may begin anywhere: a part begins at a multiple of VEC
-// elements of the tensor, at or in front of the row's first.
-template <typename T, int E>
+// Sorts the `total` keys of the wave's list, largest first, and drops all behind the first `want`: each counts the ones
+// above it. Returns how many are left.
+constexpr int kList = 128;
+__device__ __forceinline__ int wave_rank(u64* list, int total, int want, int lane) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const u64 me = lane < total ? list[lane] : 0, far = 64 + lane < total ? list[64 + lane] : 0;
+    int rank = 0, far_rank = 0;
+    if (total <= 64) {
+#pragma unroll 4
+        for (int o = 0; o < total; ++o) rank += list[o] > me;
+    } else {
+#pragma unroll 4
+        for (int o = 0; o < total; ++o) {
+            rank += list[o] > me;
+            far_rank += list[o] > far;
+        }
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (me && rank < want) list[rank] = me;
+    if (far && far_rank < want) list[far_rank] = far;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return min(total, want);
+}
+
+// What a part's sum, relative to its own maximum, counts relative to M
+template <bool CAP>
+__device__ __forceinline__ float part_weight(float2 v, float M, float Mc, float cap2, float up2) {
+    const float d = capped<CAP>(v.x, cap2, up2) - Mc;
+    return v.x == M ? v.y : v.x > kNegInf ? v.y * fexp2(CAP ? d : d * kLog2e) : 0.0f;
+}
+
+// Rows may begin anywhere: a part begins at a multiple of VEC elements of the tensor, at or in front of the row's first.
+template <typename T, int E, bool CAP>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     typedef T vec_t __attribute__((ext_vector_type(VEC)));
     __shared__ u64 s_list[4][kList];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = blockIdx.y, part = blockIdx.x * 4 + wave;
+    const int row = blockIdx.y, part = blockIdx.x * 4 + wave, K = a.n_out;
     if (part >= a.parts) return;
+    u64* list = s_list[wave];
     const int64_t first = (int64_t)row * a.row_stride, base = first & ~(int64_t)(VEC - 1);
     const int skip = (int)(first - base);
     const T* p = reinterpret_cast<const T*>(a.logits) + base;
-    float x[E];
+    const int64_t wave0 = (int64_t)part * a.steps * (64 * E) - skip, part0 = wave0 + lane * VEC;  // tokens of the first values
+    const auto load = [&](int step, float (&x)[E]) {
+        const int64_t w0 = wave0 + (int64_t)step * (64 * E), o0 = part0 + (int64_t)step * (64 * E);
+        if (w0 >= 0 && w0 + 64 * E <= a.vocab) {  // wave-uniform
+            vec_t v[E / VEC];
 #pragma unroll
-    for (int i = 0; i < E / VEC; ++i) {
-        const int64_t o = (int64_t)part * (64 * E) + (i * 64 + lane) * VEC - skip;  // token of the first of VEC
-        if (o >= 0 && o + VEC <= a.vocab) {
-            const vec_t v = __builtin_nontemporal_load(reinterpret_cast<const vec_t*>(p + o + skip));
+            for (int i = 0; i < E / VEC; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const vec_t*>(p + o0 + skip) + i * 64);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) x[i * VEC + e] = (float)v[e];
-        } else {
+            for (int i = 0; i < E; ++i) x[i] = (float)v[i / VEC][i % VEC];
+        } else {  // a row's ends
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) x[i * VEC + e] = o + e >= 0 && o + e < a.vocab ? (float)p[o + e + skip] : kNegInf;
+            for (int i = 0; i < E; ++i) {
+                const int64_t o = o0 + (i / VEC) * 64 * VEC + i % VEC;
+                x[i] = o >= 0 && o < a.vocab ? (float)p[o + skip] : kNegInf;
+            }
+        }
+    };
+    const float cap2 = a.cap * kLog2e, up2 = CAP ? 2.0f * kLog2e / a.cap : 0.0f;
+    float m = kNegInf, s = 0.0f;
+    float least = -3.40282347e38f;  // what a logit has to reach to be a candidate: nothing below can be among the largest
+    int count = 0, sorted = 0;      // candidates in the list; of them in order and above all that came before them
+    float x[E], y[E];
+    load(0, y);
+    for (int step = 0; step < a.steps; ++step) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {  // (copied here, so that no wait below is for the loads that follow)
+            x[i] = y[i];
+            asm volatile("" : "+v"(x[i]));
+        }
+        if (step + 1 < a.steps) load(step + 1, y);
+        float mine = kNegInf, low = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {  // (both pass over NaN)
+            mine = fmaxf(mine, x[i]);
+            if (CAP) low = fminf(low, x[i]);
+        }
+        const float mx = wave_max(mine);
+        if (mx > m) {
+            const float d = capped<CAP>(m, cap2, up2) - capped<CAP>(mx, cap2, up2);
+            s = m == kNegInf ? 0.0f : s * fexp2(CAP ? d : d * kLog2e);
+            m = mx;
+        }
+        const float mc = capped<CAP>(m, cap2, up2);
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float d = capped<CAP>(x[i], cap2, up2) - mc;
+            sum += fexp2(CAP ? d : d * kLog2e);
+        }
+        // with -inf, which a cap would make finite, or NaN, which are no tokens, or +inf, which is all there is: with care
+        if (__ballot(!(sum < __builtin_huge_valf()) || (CAP && low == kNegInf))) {
+            sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                x[i] = fmaxf(x[i], kNegInf);
+                const float d = capped<CAP>(x[i], cap2, up2) - mc;
+                sum += x[i] == kNegInf ? 0.0f : x[i] == m ? 1.0f : fexp2(CAP ? d : d * kLog2e);
+            }
+        }
+        s += sum;
+        if (step == 0) least = fmaxf(least, of_ascending(wave_bound(ascending(mine), K)));  // (NaN: as it was)
+        if (__ballot(mine >= least)) {
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < E; ++i) n += x[i] >= least;
+            const int t0 = (int)(part0 + (int64_t)step * (64 * E));
+            int incl = wave_scan(n), total = __builtin_amdgcn_readlane(incl, 63);
+            if (count + total > kList) {
+                if (count > K) count = wave_rank(list, count, K, lane);
+                if (count + total > kList) {  // many are equal, or ascend: this step's largest, one after the other
+                    u64 last = ~0ull;
+                    for (int k = 0; k < K; ++k) {
+                        u64 best = 0;
+#pragma unroll
+                        for (int i = 0; i < E; ++i) {
+                            const u64 key = x[i] >= least ? key_of(x[i], t0 + (i / VEC) * 64 * VEC + i % VEC) : 0;
+                            best = key < last && key > best ? key : best;
+                        }
+                        last = wave_max64(best);
+                        if (last == 0) break;
+                        if (lane == 0) list[count] = last;
+                        ++count;
+                    }
+                    total = 0;
+                }
+            }
+            if (total > 0) {
+                int k = count + incl - n;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if (x[i] >= least) list[k++] = key_of(x[i], t0 + (i / VEC) * 64 * VEC + i % VEC);
+                count += total;
+            }
+            if (count >= K && (count > kList / 2 || step == 0) && step + 1 < a.steps) {
+                // of equal logits the earlier token is taken, so a later one has to be above the last
+                count = sorted = wave_rank(list, count, K, lane);
+                least = fmaxf(least, of_ascending((uint32_t)(list[K - 1] >> 32) + 1));
+            }
         }
     }
-    float m = kNegInf;
-#pragma unroll
-    for (int i = 0; i < E; ++i) m = fmaxf(m, x[i]);
-    m = wave_max(m);
-    const float up2 = 2.0f * kLog2e / a.cap, mc = capped(m, a.cap, up2);
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const float c = capped(x[i], a.cap, up2);
-        // (equal to the maximum: 1, for infinities too; NaN and what is no token: 0)
-        s += x[i] == m ? 1.0f : x[i] > kNegInf ? fexp2((c - mc) * kLog2e) : 0.0f;
-    }
-    s = wave_sum(m == kNegInf ? 0.0f : s);
-    u64 k[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int64_t t = (int64_t)part * (64 * E) + ((i / VEC) * 64 + lane) * VEC + i % VEC - skip;
-        k[i] = x[i] > kNegInf ? key_of(x[i], (int)t) : 0;  // (what is no token is -inf)
-    }
+    s = wave_sum(s);
     const size_t at = (size_t)row * a.parts + part;
     if (lane == 0) a.sums[at] = make_float2(m, s);
-    wave_top<E>(k, a.n_out, s_list[wave], a.keys + at * a.n_out, lane);
+    if (count != sorted) count = wave_rank(list, count, K, lane);
+    if (lane < K) a.keys[at * K + lane] = lane < count ? list[lane] : 0;
 }
 
-// A row: its parts' sums in 64 bits, its n_out largest keys.
-__global__ __launch_bounds__(256) void beam_row_kernel(BeamArgs a) {
-    __shared__ u64 s_top[4][kBeams], s_list[4][kList];
-    __shared__ float s_m[4];
-    __shared__ double s_s[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
-    const float2* sums = a.sums + (size_t)row * a.parts;
-    float m = kNegInf;
-    for (int i = tid; i < a.parts; i += 256) m = fmaxf(m, sums[i].x);
-    m = wave_max(m);
-    if (lane == 0) s_m[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const auto cap64 = [&](float x) { return a.cap == 0.0f ? (double)x : (double)a.cap * tanh((double)x / (double)a.cap); };
-    double s = 0.0;
-    for (int i = tid; i < a.parts; i += 256) {
-        const float2 v = sums[i];
-        if (v.x == m) s += (double)v.y;
-        else if (v.x > kNegInf) s += (double)v.y * exp(cap64(v.x) - cap64(m));
+// A group. A wave a row: its parts' sums, in 64 bits, and the n_out largest of its parts' keys, whose lists descend. Then a
+// candidate's place among the group's is its own place in its beam and, of each other beam, the number of candidates in
+// front of it, found by halving.
+constexpr int kGroupWaves = 16;
+__global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a) {
+    __shared__ u64 s_list[kGroupWaves][kList];
+    __shared__ union {
+        u64 key;
+        double score;
+    } s_cand[kBeams * kBeams];
+    __shared__ double s_final[kBeams * kBeams];
+    __shared__ int s_token[kBeams * kBeams], s_n[kBeams], s_done[kBeams];
+    __shared__ double s_score[kBeams];
+    __shared__ double s_log[kBeams], s_most[kBeams];  // of a row: log of the sum of exp(x' - the largest x'), and that x'
+    const int g = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, W = a.width, K = a.n_out;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (tid < W) {
+        s_n[tid] = 0;
+        s_score[tid] = (double)a.scores[g * W + tid];
+        s_done[tid] = a.done && a.done[g * W + tid];
     }
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    if (lane == 0) s_s[wave] = s;
-    // keys: 8 a lane at a time, the wave's best so far among them
-    const u64* keys = a.keys + (size_t)row * a.parts * a.n_out;
-    const int64_t n = (int64_t)a.parts * a.n_out;
-    for (int k = lane; k < a.n_out; k += 64) s_top[wave][k] = 0;
-    for (int64_t k0 = 0; k0 < n; k0 += 4 * 64 * 7) {
-        u64 x[8];
-#pragma unroll
-        for (int i = 0; i < 7; ++i) {
-            const int64_t k = k0 + (int64_t)(i * 4 + wave) * 64 + lane;
-            x[i] = k < n ? keys[k] : 0;
+    for (int w = wave; w < W; w += threads >> 6) {
+        const size_t row = (size_t)g * W + w;
+        const float2* sums = a.sums + row * a.parts;
+        const u64* keys = a.keys + row * a.parts * K;
+        float m = kNegInf;
+        uint32_t top = 0;
+        for (int i = lane; i < a.parts; i += 64) {
+            m = fmaxf(m, sums[i].x);
+            top = max(top, (uint32_t)(keys[(size_t)i * K] >> 32));
         }
-        __builtin_amdgcn_wave_barrier();
-        x[7] = lane < a.n_out ? s_top[wave][lane] : 0;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        wave_top<8>(x, a.n_out, s_list[wave], s_top[wave], lane);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-    __syncthreads();
-    if (wave > 0) return;
-    u64 x[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = lane < a.n_out ? s_top[i][lane] : 0;
-    wave_top<4>(x, a.n_out, s_list[0], a.row_keys + (size_t)row * a.n_out, lane);
-    if (lane == 0) a.row_sum[row] = make_double2(cap64(m), log(s_s[0] + s_s[1] + s_s[2] + s_s[3]));
-}
-
-// A group: candidate (beam, place) of score s + x' - lse; its place among the group's is its own place in its beam and, of
-// each other beam, the candidates in front of it, found by halving.
-__global__ __launch_bounds__(256) void beam_group_kernel(BeamArgs a) {
-    __shared__ double s_score[kBeams * kBeams];
-    __shared__ int s_token[kBeams * kBeams], s_n[kBeams];
-    const int g = blockIdx.x, tid = threadIdx.x, W = a.width, K = a.n_out;
-    for (int i = tid; i < W * K; i += 256) {
-        const int w = i / K, k = i - w * K, row = g * W + w;
-        const double at = (double)a.scores[row];
-        const bool done = a.done && a.done[row];
-        double score = (double)kNegInf;
-        int token = -1;
-        if (done) {
-            if (k == 0) {
-                score = at;
-                token = a.pad;
+        m = wave_max(m);
+        const bool cap = a.cap != 0.0f;
+        const float cap2 = a.cap * kLog2e, up2 = 2.0f * kLog2e / a.cap, mc = cap ? capped<true>(m, cap2, up2) : m;
+        const uint32_t bound = max(wave_bound(top, K), 1u);  // (0 is no key)
+        double s = 0.0;
+        int total = 0;
+        for (int i0 = 0; i0 < a.parts; i0 += 64) {  // wave-uniform
+            const int i = i0 + lane;
+            const float2 v = i < a.parts ? sums[i] : make_float2(kNegInf, 0.0f);
+            s += (double)(cap ? part_weight<true>(v, m, mc, cap2, up2) : part_weight<false>(v, m, mc, cap2, up2));
+            bool more = i < a.parts;
+            for (int k = 0; k < K; ++k) {
+                const u64 key = more ? keys[(size_t)i * K + k] : 0;
+                more = (uint32_t)(key >> 32) >= bound;
+                const unsigned long long in = __ballot(more);
+                if (!in) break;
+                const int at = total + __builtin_popcountll(in & ((1ull << lane) - 1));
+                if (more && at < kList) s_list[wave][at] = key;
+                total += __builtin_popcountll(in);
             }
-        } else if (const u64 key = a.row_keys[(size_t)row * K + k]) {
-            const float x = of_ascending((uint32_t)(key >> 32));
-            const double2 sum = a.row_sum[row];
-            const double c = a.cap == 0.0f ? (double)x : (double)a.cap * tanh((double)x / (double)a.cap);
-            score = at + ((c == sum.x ? 0.0 : c - sum.x) - sum.y);  // (the largest may be +inf)
-            token = ~(int)(uint32_t)key;
         }
-        if (!(score > (double)kNegInf)) score = (double)kNegInf;
-        s_score[i] = score;
-        s_token[i] = token;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+        if (lane == 0) s_log[w] = log(s);
+        if (total <= kList) {
+            total = wave_rank(s_list[wave], total, K, lane);
+            if (lane < K) s_cand[w * K + lane].key = lane < total ? s_list[wave][lane] : 0;
+        } else {  // many are equal: one after the other
+            u64 last = ~0ull;
+            for (int k = 0; k < K; ++k) {
+                u64 best = 0;
+                for (int i = lane; i < a.parts; i += 64)
+                    for (int j = 0; j < K; ++j) {
+                        const u64 key = keys[(size_t)i * K + j];
+                        if (key >= last) continue;
+                        best = key > best ? key : best;
+                        break;
+                    }
+                last = wave_max64(best);
+                if (lane == 0) s_cand[w * K + k].key = last;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    if (tid < W) {  // the beam's candidates: the ones that are there come first, and no rounding puts two out of order
-        int n = 0;
-        double least = (double)__builtin_huge_valf();
-        for (int k = 0; k < K; ++k) {
-            least = fmin(least, s_score[tid * K + k]);
-            s_score[tid * K + k] = least;
-            n += least > (double)kNegInf;
+    for (int i = tid; i < W * K; i += threads) {
+        const u64 key = s_cand[i].key;
+        const double c = capped64(of_ascending((uint32_t)(key >> 32)), a.cap);
+        s_token[i] = key ? ~(int)(uint32_t)key : -1;
+        s_cand[i].score = c;
+        if (i % K == 0) s_most[i / K] = c;
+    }
+    __syncthreads();
+    for (int i = tid; i < W * K; i += threads) {
+        const int w = i / K, k = i - w * K;
+        double score = (double)kNegInf;
+        if (s_done[w]) {
+            if (k == 0) {
+                score = s_score[w];
+                s_token[i] = a.pad;
+            }
+        } else if (s_token[i] >= 0) {
+            double c = s_cand[i].score;  // no rounding puts two of a beam out of order
+#pragma unroll 4
+            for (int j = 0; j < k; ++j) c = fmin(c, s_cand[i - 1 - j].score);
+            score = s_score[w] + ((c == s_most[w] ? 0.0 : c - s_most[w]) - s_log[w]);  // (the largest may be +inf)
         }
-        s_n[tid] = n;
+        s_final[i] = score > (double)kNegInf ? score : (double)kNegInf;
+        if (score > (double)kNegInf) atomicAdd(&s_n[w], 1);  // a beam's candidates come first
     }
     __syncthreads();
     int total = 0;
+#pragma unroll 4
     for (int w = 0; w < W; ++w) total += s_n[w];
-    for (int i = tid; i < W * K; i += 256) {
+    for (int i = tid; i < W * K; i += threads) {
         const int w = i / K, k = i - w * K;
         if (k >= s_n[w]) continue;
-        const double me = s_score[i];
+        const double me = s_final[i];
         int rank = k;
-        for (int o = 0; o < W && rank < K; ++o) {
-            if (o == w) continue;
-            int lo = 0, hi = s_n[o];  // candidates of beam o in front of this one: [0, lo)
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                const double s = s_score[o * K + mid];
-                if (s > me || (s == me && o < w)) lo = mid + 1;
-                else hi = mid;
+        for (int o0 = 0; o0 < W && rank < K; o0 += 4) {  // four beams' searches at once: LDS answers in 130 cycles
+            int front[4] = {}, n[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) n[u] = o0 + u < W && o0 + u != w ? s_n[o0 + u] : 0;
+            for (int step = kBeams; step; step >>= 1) {
+                if (step > K) continue;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int o = o0 + u, at = front[u] + step;
+                    const double s = s_final[at <= n[u] ? o * K + at - 1 : i];
+                    if (at <= n[u] && (s > me || (s == me && o < w))) front[u] = at;
+                }
             }
-            rank += lo;
+            rank += front[0] + front[1] + front[2] + front[3];
         }
         if (rank < K) {
             const size_t at = (size_t)g * K + rank;
@@ -278,30 +357,42 @@ __global__ __launch_bounds__(256) void beam_group_kernel(BeamArgs a) {
             a.out_token[at] = s_token[i];
         }
     }
-    for (int k = total + tid; k < K; k += 256) {
+    for (int k = total + tid; k < K; k += threads) {
         const size_t at = (size_t)g * K + k;
         a.out_score[at] = kNegInf;
         a.out_parent[at] = a.out_token[at] = -1;
     }
 }
 
-// Tokens that a wave takes: enough waves for the card first (four a SIMD), then long ones, whose lists are fewer.
-static int beam_each(int64_t rows, int64_t vocab) { return rows * vocab >= (int64_t)64 * 32 * 4096 ? 32 : 8; }
+typedef void (*beam_part_fn)(BeamArgs);
+template <typename T>
+static beam_part_fn pick_each(int each, bool cap) {
+    if (each == 32) return cap ? beam_part_kernel<T, 32, true> : beam_part_kernel<T, 32, false>;
+    return cap ? beam_part_kernel<T, 8, true> : beam_part_kernel<T, 8, false>;
+}
+static beam_part_fn pick_part(bool f16, int each, bool cap) { return f16 ? pick_each<half_t>(each, cap) : pick_each<float>(each, cap); }
 
+// Few logits: 512 a wave, one step, so that many waves share them. Many: steps of 2048, as many as leave the card kPartWaves
+// waves. A wave pays for its first step's bound and order, so longer walks are cheaper, and fewer waves hide less: 128 rows of
+// 262144 in f32 with a cap 35.4 us with 2 steps of 2048 (3.8 TB/s), 35.5 with 1, 37.6 with 4, 36.5 and 37.5 with 4 and 8
+// of 1024, 43 where the next step's loads were waited for; 30.7 without a cap. What bounds it: a logit with a cap takes two
+// exponentials, a reciprocal and six more instructions, about 72 cycles a wave of 64, 15 us of the card's VALU beside the 26
+// us that the bytes take, and a wave's first step's ballots and LDS trips.
+constexpr int kPartWaves = 8192;
 struct BeamPlan {
-    int each, parts;
-    size_t keys, row_keys, row_sum, total;
+    int each, steps, parts;
+    size_t keys, total;
 };
 static BeamPlan beam_plan(int n_groups, int width, int vocab, int n_out) {
     BeamPlan p;
-    const int64_t rows = (int64_t)n_groups * width;
-    p.each = beam_each(rows, vocab);
-    p.parts = (int)(((int64_t)vocab + 7 + 64 * p.each - 1) / (64 * p.each));  // a row may begin 7 behind its part
+    const int64_t rows = (int64_t)n_groups * width, span = (int64_t)vocab + 7;  // (a row may begin 7 behind its part)
+    p.each = rows * vocab >= (int64_t)64 * 16 * kPartWaves ? 32 : 8;
+    p.steps = p.each == 8 ? 1 : (int)std::min<int64_t>(std::max<int64_t>(rows * vocab / ((int64_t)64 * 32 * kPartWaves), 1), 64);
+    const int64_t part = (int64_t)64 * p.each * p.steps;
+    p.parts = (int)((span + part - 1) / part);
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.keys = al((size_t)rows * p.parts * sizeof(float2));
-    p.row_keys = p.keys + al((size_t)rows * p.parts * n_out * sizeof(u64));
-    p.row_sum = p.row_keys + al((size_t)rows * n_out * sizeof(u64));
-    p.total = p.row_sum + al((size_t)rows * sizeof(double2));
+    p.total = p.keys + al((size_t)rows * p.parts * n_out * sizeof(u64));
     return p;
 }
 
@@ -348,15 +439,12 @@ extern "C" int g4a_beam_select(int n_groups, int width, int vocab, int logits_f1
         return G4A_EWORKSPACE;
     }
     char* w = (char*)ws;
-    const BeamArgs a{logits, row_stride, scores, done, out_score, out_parent, out_token, (float2*)w, (u64*)(w + p.keys),
-                     (u64*)(w + p.row_keys), (double2*)(w + p.row_sum), width, vocab, n_out, p.parts, pad, cap};
+    const BeamArgs a{logits, row_stride, scores, done, out_score, out_parent, out_token, (float2*)w, (u64*)(w + p.keys), width, vocab, n_out,
+                     p.parts, p.steps, pad, cap};
     const hipStream_t stream = (hipStream_t)stream_;
     const dim3 grid((unsigned)((p.parts + 3) / 4), (unsigned)(n_groups * width));
-    void (*part)(BeamArgs) = logits_f16 ? (p.each == 32 ? beam_part_kernel<half_t, 32> : beam_part_kernel<half_t, 8>)
-                                        : (p.each == 32 ? beam_part_kernel<float, 32> : beam_part_kernel<float, 8>);
-    hipLaunchKernelGGL(part, grid, dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(beam_row_kernel, dim3((unsigned)(n_groups * width)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(beam_group_kernel, dim3((unsigned)n_groups), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(pick_part(logits_f16 != 0, p.each, cap > 0.0f), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(beam_group_kernel, dim3((unsigned)n_groups), dim3(64 * std::min(width, kGroupWaves)), 0, stream, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? G4A_OK : hip_error(e, "beam select launch");
 }

@@ -166,10 +166,6 @@ struct ForkArgs {
     int32_t* len;
     int32_t* free_out;
     int32_t* n_free_out;
-    int32_t* owner;    // [n_pages]: the first new row that has the page in a column it will write to
-    uint32_t* was;     // bitmaps of pages: some old row's;
-    uint32_t* held;    //   some new row's;
-    uint32_t* full;    //   some new row's in a column that is full
     int32_t* copy;     // [3][n_new]: a row's tail: from page, to page, rows
     int n_new, room, words;
 };
@@ -185,46 +181,35 @@ __device__ __forceinline__ int fork_end(const ForkArgs& a, int p, int L) {
 __device__ __forceinline__ bool bit(const uint32_t* map, int p) { return map[p >> 5] >> (p & 31) & 1; }
 __device__ __forceinline__ void set_bit(uint32_t* map, int p) { atomicOr(map + (p >> 5), 1u << (p & 31)); }
 
-__global__ __launch_bounds__(256) void fork_clear_kernel(ForkArgs a) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < a.t.n_pages) a.owner[i] = 0x7fffffff;
-    if (i < a.words) a.was[i] = a.held[i] = a.full[i] = 0;
+// The marks of a call's pages: in the workspace, or in LDS where one workgroup does all of it.
+struct ForkMarks {
+    int32_t* owner;   // the first new row that has the page in a column it will write to
+    uint32_t* was;    // bits: some old row has it;
+    uint32_t* held;   //   some new row has it;
+    uint32_t* full;   //   some new row has it in a column that is full
+};
+
+// Column c of new row j, whose parent has page x there: a full one is the parent's, one that the row will write to is
+// claimed
+__device__ __forceinline__ void mark_new(const ForkArgs& a, const ForkMarks& mk, int j, int full, int end, int c, int x) {
+    int e = -1;
+    if (c < end && page_ok(a.t, x)) {
+        if (c < full) {
+            set_bit(mk.held, x);
+            set_bit(mk.full, x);
+            e = x;
+        } else {
+            atomicMin(mk.owner + x, j);
+        }
+    }
+    a.table[(size_t)j * a.t.cols + c] = e;
 }
 
-// What the old rows hold, and the new rows' full columns; a workgroup per row of either
-__global__ __launch_bounds__(256) void fork_mark_kernel(ForkArgs a) {
-    const int row = blockIdx.x;
-    if (row < a.t.n_seq) {
-        for (int c = threadIdx.x; c < a.t.cols; c += 256) {
-            const int e = a.t.table[(size_t)row * a.t.stride + c];
-            if (page_ok(a.t, e)) set_bit(a.was, e);
-        }
-        return;
-    }
-    const int j = row - a.t.n_seq, p = a.parent[j], L = fork_len(a, p), full = L >> a.t.shift, end = fork_end(a, p, L);
-    for (int c = threadIdx.x; c < a.t.cols; c += 256) {
-        int e = -1;
-        if (c < end) {
-            const int x = a.t.table[(size_t)p * a.t.stride + c];
-            if (page_ok(a.t, x)) {
-                if (c < full) {
-                    set_bit(a.held, x);
-                    set_bit(a.full, x);
-                    e = x;
-                } else {
-                    atomicMin(a.owner + x, j);
-                }
-            }
-        }
-        a.table[(size_t)j * a.t.cols + c] = e;
-    }
-    if (threadIdx.x == 0) a.len[j] = L;
-}
-
-// The writable columns, in order of rows and columns, by one workgroup: a page that no other row holds stays, the others
-// take pages off the end of the free list, to which the pages that no row holds any more are added first.
+// The writable columns, in order of rows and columns, by one workgroup, once all is marked: a page that no other row holds
+// stays, the others take pages off the end of the free list, to which the pages that no row holds any more are added
+// first.
 constexpr int kForkThreads = 1024;
-__global__ __launch_bounds__(kForkThreads) void fork_pages_kernel(ForkArgs a) {
+__device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& mk) {
     __shared__ int s_wave[kForkThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // exclusive prefix of x over the workgroup, and the total
@@ -235,47 +220,48 @@ __global__ __launch_bounds__(kForkThreads) void fork_pages_kernel(ForkArgs a) {
         __syncthreads();
         int before = 0;
         total = 0;
+#pragma unroll
         for (int w = 0; w < kForkThreads / 64; ++w) {
             if (w < wave) before += s_wave[w];
             total += s_wave[w];
         }
         return before + incl - x;
     };
-    // f(column, the parent's page there or -1, whether the row keeps it, whether it needs another) over row j
-    auto columns = [&](int j, int& p, int& L, auto f) {
-        p = a.parent[j];
-        L = fork_len(a, p);
+    // f(column, the parent's page there or -1, whether the row keeps it, whether it needs another) over row j of parent p
+    auto columns = [&](int j, int p, int L, auto f) {
         const int end = fork_end(a, p, L);
         for (int c = L >> a.t.shift; c < end; ++c) {
             int x = a.t.table[(size_t)p * a.t.stride + c];
             if (!page_ok(a.t, x)) x = -1;
-            const bool keeps = x >= 0 && !bit(a.full, x) && a.owner[x] == j;
+            const bool keeps = x >= 0 && !bit(mk.full, x) && mk.owner[x] == j;
             // (keys whose page is not there stay lost: a new page there would make them rows of anything)
             f(c, x, keeps, !keeps && (x >= 0 || (int64_t)c << a.t.shift >= L));
         }
     };
     const int chunks = (a.n_new + kForkThreads - 1) / kForkThreads;
-    for (int ch = 0; ch < chunks; ++ch) {
-        const int j = ch * kForkThreads + tid;
-        int p, L;
-        if (j < a.n_new)
-            columns(j, p, L, [&](int c, int x, bool keeps, bool) {
-                if (keeps) {
-                    a.table[(size_t)j * a.t.cols + c] = x;
-                    set_bit(a.held, x);
-                }
-            });
-    }
-    __threadfence();
-    __syncthreads();
     const int had = min(max(a.n_free_in[0], 0), a.t.n_pages);
     for (int i = tid; i < had; i += kForkThreads) a.free_out[i] = a.free_in[i];
+    int p = -1, L = 0, need = 0;  // of this thread's row; of the only chunk, if there is one
+    for (int ch = 0; ch < chunks; ++ch) {
+        const int j = ch * kForkThreads + tid;
+        if (j >= a.n_new) break;
+        p = a.parent[j];
+        L = fork_len(a, p);
+        need = 0;
+        columns(j, p, L, [&](int c, int x, bool keeps, bool needs) {
+            need += needs;
+            if (keeps) {
+                a.table[(size_t)j * a.t.cols + c] = x;
+                set_bit(mk.held, x);
+            }
+        });
+    }
     __syncthreads();
     int m = had;
     for (int w0 = 0; w0 < a.words; w0 += kForkThreads) {
         const int w = w0 + tid;
-        uint32_t gone = w < a.words ? __hip_atomic_load(a.was + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) &
-                                          ~__hip_atomic_load(a.held + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+        uint32_t gone = w < a.words ? __hip_atomic_load(mk.was + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) &
+                                          ~__hip_atomic_load(mk.held + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
                                     : 0u;
         int total;
         int at = m + scan(__builtin_popcount(gone), total);
@@ -284,31 +270,35 @@ __global__ __launch_bounds__(kForkThreads) void fork_pages_kernel(ForkArgs a) {
         m += total;
     }
     m = min(m, a.t.n_pages);
-    __threadfence();
     __syncthreads();
     int taken = 0;
     for (int ch = 0; ch < chunks; ++ch) {
         const int j = ch * kForkThreads + tid;
-        int p, L, need = 0;
-        if (j < a.n_new) columns(j, p, L, [&](int, int, bool, bool needs) { need += needs; });
+        if (chunks > 1) {
+            need = 0;
+            p = j < a.n_new ? a.parent[j] : -1;
+            L = fork_len(a, p);
+            if (j < a.n_new) columns(j, p, L, [&](int, int, bool, bool needs) { need += needs; });
+        }
         int total;
         int k = taken + scan(need, total);
         if (j < a.n_new) {
             int from = -1, to = -1, rows = 0;
-            columns(j, p, L, [&](int c, int x, bool, bool needs) {
-                if (!needs) return;
-                const int at = m - 1 - k++;
-                int got = -1;
-                if (at >= 0) got = __hip_atomic_load(a.free_out + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                if (!page_ok(a.t, got)) got = -1;
-                a.table[(size_t)j * a.t.cols + c] = got;
-                const int fill = L - (c << a.t.shift);
-                if (fill > 0) {  // the parent's last page, partly filled
-                    from = x;
-                    to = got;
-                    rows = got >= 0 ? fill : 0;
-                }
-            });
+            if (need > 0)
+                columns(j, p, L, [&](int c, int x, bool, bool needs) {
+                    if (!needs) return;
+                    const int at = m - 1 - k++;
+                    int got = -1;
+                    if (at >= 0) got = a.free_out[at];
+                    if (!page_ok(a.t, got)) got = -1;
+                    a.table[(size_t)j * a.t.cols + c] = got;
+                    const int fill = L - (c << a.t.shift);
+                    if (fill > 0) {  // the parent's last page, partly filled
+                        from = x;
+                        to = got;
+                        rows = got >= 0 ? fill : 0;
+                    }
+                });
             a.copy[j] = from;
             a.copy[a.n_new + j] = to;
             a.copy[2 * a.n_new + j] = rows;
@@ -320,6 +310,69 @@ __global__ __launch_bounds__(kForkThreads) void fork_pages_kernel(ForkArgs a) {
     for (int i = left + tid; i < a.t.n_pages; i += kForkThreads) a.free_out[i] = -1;
     if (tid == 0) a.n_free_out[0] = left;
 }
+
+// All of it by one workgroup, the marks in LDS, where pages and table entries are few: three launches less.
+constexpr int kForkPages = 12288, kForkEntries = 1 << 15, kForkRows = 1024;
+__global__ __launch_bounds__(kForkThreads) void fork_small_kernel(ForkArgs a) {
+    __shared__ int32_t s_owner[kForkPages];
+    __shared__ uint32_t s_bits[3][kForkPages / 32];
+    const ForkMarks mk{s_owner, s_bits[0], s_bits[1], s_bits[2]};
+    __shared__ int s_parent[kForkRows], s_full[kForkRows], s_end[kForkRows];
+    constexpr int NW = kForkThreads / 64, U = 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, cols = a.t.cols;
+    if (tid < a.n_new) {
+        const int p = a.parent[tid], L = fork_len(a, p), end = fork_end(a, p, L);
+        a.len[tid] = L;
+        s_parent[tid] = end > 0 ? p : 0;  // (a row that is not read)
+        s_full[tid] = L >> a.t.shift;
+        s_end[tid] = end;
+    }
+    for (int i = tid; i < a.t.n_pages; i += kForkThreads) s_owner[i] = 0x7fffffff;
+    for (int i = tid; i < a.words; i += kForkThreads) s_bits[0][i] = s_bits[1][i] = s_bits[2][i] = 0;
+    __syncthreads();
+    for (int c0 = 0; c0 < cols; c0 += 64) {  // a wave a row, the entries of eight rows' loads at once
+        const int c = c0 + lane;
+        for (int r0 = wave; r0 < max(a.t.n_seq, a.n_new); r0 += NW * U) {
+            int was[U], heir[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + NW * u;
+                was[u] = r < a.t.n_seq && c < cols ? a.t.table[(size_t)r * a.t.stride + c] : -1;
+                heir[u] = r < a.n_new && c < s_end[r] ? a.t.table[(size_t)s_parent[r] * a.t.stride + c] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + NW * u;
+                if (page_ok(a.t, was[u])) set_bit(mk.was, was[u]);
+                if (r < a.n_new && c < cols) mark_new(a, mk, r, s_full[r], s_end[r], c, heir[u]);
+            }
+        }
+    }
+    __syncthreads();
+    fork_pages(a, mk);
+}
+
+__global__ __launch_bounds__(256) void fork_clear_kernel(ForkArgs a, ForkMarks mk) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < a.t.n_pages) mk.owner[i] = 0x7fffffff;
+    if (i < a.words) mk.was[i] = mk.held[i] = mk.full[i] = 0;
+}
+// A workgroup per row of either table
+__global__ __launch_bounds__(256) void fork_mark_kernel(ForkArgs a, ForkMarks mk) {
+    const int row = blockIdx.x;
+    if (row < a.t.n_seq) {
+        for (int c = threadIdx.x; c < a.t.cols; c += 256) {
+            const int e = a.t.table[(size_t)row * a.t.stride + c];
+            if (page_ok(a.t, e)) set_bit(mk.was, e);
+        }
+        return;
+    }
+    const int j = row - a.t.n_seq, p = a.parent[j], L = fork_len(a, p), end = fork_end(a, p, L);
+    for (int c = threadIdx.x; c < a.t.cols; c += 256)
+        mark_new(a, mk, j, L >> a.t.shift, end, c, c < end ? a.t.table[(size_t)p * a.t.stride + c] : -1);
+    if (threadIdx.x == 0) a.len[j] = L;
+}
+__global__ __launch_bounds__(kForkThreads) void fork_pages_kernel(ForkArgs a, ForkMarks mk) { fork_pages(a, mk); }
 
 // The filled rows of the pages that were replaced, in every pool: a workgroup per row, pool and 16 KB
 __global__ __launch_bounds__(256) void fork_copy_kernel(ForkArgs a, Pools pools) {
@@ -501,17 +554,19 @@ extern "C" int g4a_paged_fork(const g4a_pool* pools, int n_pools, const g4a_page
     a.len = new_len;
     a.free_out = new_free;
     a.n_free_out = new_n_free;
-    a.owner = (int32_t*)w;
-    a.was = (uint32_t*)(w + p.was);
-    a.held = (uint32_t*)(w + p.held);
-    a.full = (uint32_t*)(w + p.full);
     a.copy = (int32_t*)(w + p.copy);
     a.n_new = n_new;
     a.room = room;
     a.words = p.words;
-    hipLaunchKernelGGL(fork_clear_kernel, dim3((unsigned)((pg->n_pages + 255) / 256)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(fork_mark_kernel, dim3((unsigned)(pg->n_seq + n_new)), dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kForkThreads), 0, stream, a);
+    const int64_t entries = ((int64_t)pg->n_seq + n_new) * pg->table_cols;
+    if (pg->n_pages <= kForkPages && n_new <= kForkRows && entries <= kForkEntries) {
+        hipLaunchKernelGGL(fork_small_kernel, dim3(1), dim3(kForkThreads), 0, stream, a);
+    } else {
+        const ForkMarks mk{(int32_t*)w, (uint32_t*)(w + p.was), (uint32_t*)(w + p.held), (uint32_t*)(w + p.full)};
+        hipLaunchKernelGGL(fork_clear_kernel, dim3((unsigned)((pg->n_pages + 255) / 256)), dim3(256), 0, stream, a, mk);
+        hipLaunchKernelGGL(fork_mark_kernel, dim3((unsigned)(pg->n_seq + n_new)), dim3(256), 0, stream, a, mk);
+        hipLaunchKernelGGL(fork_pages_kernel, dim3(1), dim3(kForkThreads), 0, stream, a, mk);
+    }
     hipError_t e;
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged fork launch");
     if (n_pools > 0) {

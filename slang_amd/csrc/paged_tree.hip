@@ -322,13 +322,13 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
 // out = sum_p o_p l_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), M = max_p m_p, of a block's pieces (o_p = O_p / l_p). A
 // workgroup's item is a wave block of 32 columns x 256 dims of an entry of the merge list, and of its 16 runs of 8 values
 // x 64 lanes one, with few blocks to merge, so that many workgroups share the bytes, or four. Its four waves take every
-// fourth piece and add up through LDS.
-constexpr int kMergeGrid = 1024, kMergeFew = 64;
+// fourth piece, each relative to its own largest m so far, and join through LDS: one trip to memory for up to 16 pieces.
+constexpr int kMergeGrid = 2048, kMergeFew = 64;
 template <typename OUTT, int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
     constexpr int NCOL = 128, NV = NCOL * HD, BLK = NV * 3;  // values and bytes of a piece's block
     constexpr int NW = 4 * (HD / 256);                       // wave blocks
-    __shared__ float s_o[3][8][64], s_l[3][64];
+    __shared__ float s_o[4][8][64], s_l[4][64], s_m[4][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int merges = a.counts[1], G = a.n_q_heads / a.n_kv_heads, BQ = NCOL / G;
     const int nk = merges <= kMergeFew ? 1 : 4, per = 16 / nk;
@@ -340,18 +340,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
         const bool ok = s_idx < pu.S;
         const float2* ml = a.part_ml + (size_t)pu.slot * NCOL + c;
         const char* base = reinterpret_cast<const char*>(a.part_o) + (size_t)pu.slot * BLK;
-        float M = kNegInf;
-        for (int p = 0; p < n_pieces; p += 8) {
-            float m[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) m[e] = ok && p + e < n_pieces ? ml[(size_t)(p + e) * NCOL].x : kNegInf;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) M = fmaxf(M, m[e]);
-        }
         for (int k = item % per * nk; k < item % per * nk + nk; ++k) {
-            float o[8] = {}, L = 0.0f;
+            float o[8] = {}, L = 0.0f, M = kNegInf;
             const int run = w * (32 * 256) + k * 512 + 8 * lane;
-            // four pieces' loads at once; a piece with no attended key (l = 0) counts for nothing, whatever it holds
             for (int p0 = wave; p0 < n_pieces; p0 += 16) {
                 float2 mp[4];
                 v4u32 hi[4];
@@ -368,8 +359,16 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
                         lo[e] = *reinterpret_cast<const v2u32*>(base + (size_t)p * BLK + 2 * NV + run);
                     }
                 }
+                const float top = fmaxf(M, fmaxf(fmaxf(mp[0].x, mp[1].x), fmaxf(mp[2].x, mp[3].x)));
+                const float back = M == kNegInf ? 0.0f : fexp2(M - top);
+                M = top;
+                L *= back;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] *= back;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                    // a piece with no attended key (l = 0) counts for nothing, whatever it holds; one of NaN scores alone
+                    // (l NaN, m -inf) makes all NaN
                     const bool none = mp[e].y == 0.0f;
                     const float wt = none ? 0.0f : mp[e].y * fexp2(mp[e].x - M);
                     L += wt;
@@ -377,27 +376,30 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
                     for (int i = 0; i < 8; ++i) o[i] = __builtin_fmaf(none ? 0.0f : unpack24(hi[e], lo[e], i), wt, o[i]);
                 }
             }
-            if (wave > 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s_o[wave - 1][e][lane] = o[e];
-                s_l[wave - 1][lane] = L;
-            }
+            for (int e = 0; e < 8; ++e) s_o[wave][e][lane] = o[e];
+            s_l[wave][lane] = L;
+            s_m[wave][lane] = M;
             __syncthreads();
-            if (wave == 0 && ok) {
+            // wave w finishes values 2w and 2w + 1 of each run
+            if (ok) {
+                M = fmaxf(fmaxf(s_m[0][lane], s_m[1][lane]), fmaxf(s_m[2][lane], s_m[3][lane]));
+                float x = 0.0f, y = 0.0f;
+                L = 0.0f;
 #pragma unroll
-                for (int v = 0; v < 3; ++v) {
-                    L += s_l[v][lane];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] += s_o[v][e][lane];
+                for (int v = 0; v < 4; ++v) {
+                    const float l = s_l[v][lane], f = l == 0.0f ? 0.0f : fexp2(s_m[v][lane] - M);
+                    L += l * f;
+                    x = __builtin_fmaf(l == 0.0f ? 0.0f : s_o[v][2 * wave][lane], f, x);
+                    y = __builtin_fmaf(l == 0.0f ? 0.0f : s_o[v][2 * wave + 1][lane], f, y);
                 }
                 const float inv = L == 0.0f ? 0.0f : 1.0f / L;
                 OUTT* orow = reinterpret_cast<OUTT*>(a.out) + ((size_t)(pu.row0 + s_idx) * a.n_q_heads + kh * G + c % G) * HD +
                              (HD == 256 ? 0 : 256 * (w & 1));
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {  // run k: dims tile k/2, 4-row pair k%2
-                    const int d = 32 * (k >> 1) + 16 * (k & 1) + 8 * e + 4 * h;
-                    store4(orow + d, srq4(float4v{o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]} * inv, a.out_q));
-                }
+                // run k: dims tile k/2, 4-row pair k%2
+                OUTT* to = orow + 32 * (k >> 1) + 16 * (k & 1) + 8 * (wave >> 1) + 4 * h + 2 * (wave & 1);
+                store_elem(to, srq(x * inv, a.out_q));
+                store_elem(to + 1, srq(y * inv, a.out_q));
             }
             __syncthreads();
         }
