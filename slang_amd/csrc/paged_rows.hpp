@@ -43,7 +43,7 @@ constexpr int tree_first(int start, int window) {
 }
 constexpr int tree_tiles(int start, int S, int qb, int bq, int kt, int window) {
     const int p0 = start + qb * bq, hi = p0 + bq < start + S ? p0 + bq : start + S;
-    const int n = (hi - (tree_first(start, window) & ~(kt - 1)) + kt - 1) / kt;
+    const int span = hi - (tree_first(start, window) & ~(kt - 1)), n = kt == 64 ? (span + 63) / 64 : (span + 31) / 32;
     return n > 0 ? n : 0;
 }
 // 64-bit words of a row's bits: keys (start & ~63) .. start + S - 1

@@ -54,6 +54,7 @@ struct PagedTreeArgs : PagedPrefillArgs {
     const int32_t* parents;
     unsigned long long* bits;  // [n_tokens][words]
     int32_t* depth;            // [n_tokens]: the token's position is start + depth
+    half_t* q16_lo;            // hd 256: what f16 leaves of q, as q16
     int words;
 };
 
@@ -170,12 +171,19 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(ARGS a) {
     // MFMA. Wave w DMAs the f16 q rows of its own 32 columns (two 512-byte rows an instruction, chunk
     // n32 of a row from logical chunk n32 ^ (row % 32)) into the LDS stage that tile t0 + 1 takes over
     // later, then reads them back in that layout; rows past the block's last token read as zeros.
-    half8 qf[16];
+    // (A tree's q keeps a second operand, what f16 leaves of it: the loop waits for memory, so the twice as many score MFMAs
+    // fit in, and the outputs are those of 32-bit queries. Straight into registers, in the same trip.)
+    half8 qf[16], ql[TREE ? 16 : 1];
     int entry1, gone0, gone1 = 0;  // tile t + 1's page, the 16-row groups of tiles t and t + 1 without one
     {
         const rsrc_t rq = make_rsrc(a.q16 + ((size_t)row0 + qb * BQ) * a.n_q_heads * HD, (uint32_t)min(BQ, S - qb * BQ) * a.n_q_heads * ROWB);
         char* qs = lds + ((t0 + 1) & 1) * 2 * TILEB;
         pages.load(a.t, wu.b, wg_lo + t0 * KT, wave, lane);
+        if constexpr (TREE) {
+            const rsrc_t rl = make_rsrc(a.q16_lo + ((size_t)row0 + qb * BQ) * a.n_q_heads * HD, (uint32_t)min(BQ, S - qb * BQ) * a.n_q_heads * ROWB);
+#pragma unroll
+            for (int s = 0; s < 16; ++s) ql[s] = bload_h8(rl, (pl * a.n_q_heads + kh * G + hh) * ROWB + 32 * s + 16 * h);
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const int r = 32 * wave + 2 * j + h;  // column of the row this lane moves
@@ -204,6 +212,10 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(ARGS a) {
 #pragma unroll
         for (int s = 0; s < 16; ++s) qf[s] = *reinterpret_cast<const half8*>(qrow + 16 * ((2 * s + h) ^ n32));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // stage free for tile t0 + 1's DMA
+        if constexpr (TREE) {
+#pragma unroll
+            for (int s = 0; s < 16; ++s) asm volatile("" : "+v"(ql[s]));
+        }
         if (!col_ok) {
 #pragma unroll
             for (int s = 0; s < 16; ++s) qf[s] = half8{0, 0, 0, 0, 0, 0, 0, 0};
@@ -379,10 +391,12 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(ARGS a) {
                     take(2 * s - 1);
                 }
                 snext[1] = mfma32(kr[s % 3][1], qf[s], snext[1]);
+                if constexpr (TREE) snext[0] = mfma32(kr[s % 3][0], ql[s], snext[0]);
                 if (s < 15) {
                     arg(2 * s + 2);
                     arg(2 * s + 3);
                 }
+                if constexpr (TREE) snext[1] = mfma32(kr[s % 3][1], ql[s], snext[1]);
                 if (s < 8) dma(rv, tile_v(t + 1), s, v_off(s));
                 else dma(rk, tile_k(t + 2), s - 8, k_off(s - 8));
                 __builtin_amdgcn_sched_barrier(0);
@@ -421,6 +435,32 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(ARGS a) {
             asm volatile("" : "+v"(mnext));
         }
     };
+    // A wave without a token (trees are short) moves its rows and leaves LDS and the matrix units to the others.
+    if (TREE && qb * BQ + 32 * wave / G >= S) {
+        if (t0 < t1) {
+            __syncthreads();
+            for (int t = t0 - 1;;) {
+                const int j = t + 2 - t0;
+                if (j > 1 && (j & 63) == 0) pages.load(a.t, wu.b, wg_lo + (t + 2) * KT, wave, lane);
+                const int entry = __builtin_amdgcn_readlane(pages.entry, j & 63);
+                if (t >= t0) {
+                    const rsrc_t rv = tile_rows(a.vc, t + 1, entry1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dma(rv, tile_v(t + 1), i, v_off(i));
+                }
+                const rsrc_t rk = tile_rows(a.kc, t + 2, entry);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dma(rk, tile_k(t + 2), i, k_off(i));
+                entry1 = entry;
+                if (++t >= t1) break;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (sizeof(OUTT) == 2 && n_pieces == 1) __syncthreads();  // the epilogue's
+        return;
+    }
     if (t0 < t1) {
         float16v sa[2] = {float16v{}, float16v{}}, sb[2];
         __syncthreads();  // K(t0), V(t0); every wave has its q
@@ -435,6 +475,10 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_256(ARGS a) {
             const int cb = 16 * ((2 * s + h) ^ n32);
             sa[0] = mfma32(*reinterpret_cast<const half8*>(krow0 + cb), qf[s], sa[0]);
             sa[1] = mfma32(*reinterpret_cast<const half8*>(krow0 + 32 * ROWB + cb), qf[s], sa[1]);
+            if constexpr (TREE) {
+                sa[0] = mfma32(*reinterpret_cast<const half8*>(krow0 + cb), ql[s], sa[0]);
+                sa[1] = mfma32(*reinterpret_cast<const half8*>(krow0 + 32 * ROWB + cb), ql[s], sa[1]);
+            }
         }
         mask(t0, gone0, tree_word(t0), sa);
 #pragma unroll
@@ -806,6 +850,31 @@ __global__ __launch_bounds__(256) void paged_prefill_kernel_512(ARGS a) {
             asm volatile("" : "+v"(mnext));
         }
     };
+    if (TREE && qb * BQ + 32 * wave / G >= S) {  // a wave without a token, as at hd 256
+        if (t0 < t1) {
+            __syncthreads();
+            for (int t = t0 - 1;;) {
+                const int j = t + 2 - t0;
+                if (j > 1 && (j & 63) == 0) pages.load(a.t, wu.b, wg_lo + (t + 2) * KT, wave >> 1, lane);
+                const int entry = __builtin_amdgcn_readlane(pages.entry, j & 63);
+                if (t >= t0) {
+                    const rsrc_t rv = tile_rows(a.vc, t + 1, entry1);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dma(rv, tile_v(t + 1), i, row_off(i), v_swz(i));
+                }
+                const rsrc_t rk = tile_rows(a.kc, t + 2, entry);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dma(rk, tile_k(t + 2), i, row_off(i), k_swz(i));
+                entry1 = entry;
+                if (++t >= t1) break;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (sizeof(OUTT) == 2 && n_pieces == 1) __syncthreads();  // the epilogue's
+        return;
+    }
     if (t0 < t1) {
         __syncthreads();  // K(t0), V(t0); every wave has its q
         entry1 = __builtin_amdgcn_readlane(pages.entry, 1);

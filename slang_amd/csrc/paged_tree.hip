@@ -44,6 +44,23 @@ __device__ __forceinline__ TreeCost tree_cost(int kt) { return kt == 64 ? TreeCo
 // Pieces of the longest block in candidate c of 64: 1 .. 32, then every seventh up to 256.
 __device__ __forceinline__ int tree_candidate(int c) { return c < 32 ? c + 1 : 32 + 7 * (c - 31); }
 
+// floor(x / d) of x in [0, 2^31), r = 1 / d on the transcendental unit: the first product is off by 2^-22 of itself, the
+// second, of what is left, by less than one, which the remainder puts right. A division by an unknown d takes the
+// compiler some 35 dependent instructions, and the list is waited for by everything.
+struct Over {
+    int d;
+    float r;
+    __device__ __forceinline__ explicit Over(int d_) : d(d_), r(__builtin_amdgcn_rcpf((float)d_)) {}
+    __device__ __forceinline__ int operator()(int x) const {
+        int q = (int)((float)x * r), rest = x - q * d;
+        const int more = (int)((float)rest * r);
+        q += more;
+        rest -= more * d;
+        return q + (rest >= d ? 1 : rest < 0 ? -1 : 0);
+    }
+    __device__ __forceinline__ int up(int x) const { return (*this)(x + d - 1); }
+};
+
 // Written by one workgroup of kPlanThreads threads. A sequence's blocks all read its whole history, so they take the same
 // number of pieces, ceil(tiles of the last block / st) for one st, the tiles that a piece may have. Lane c of every
 // wave prices candidate c of st over a quarter of the sequences: units that all fit the card at once end with the longest
@@ -53,7 +70,7 @@ __device__ void plan_trees(const TreeRowArgs& a) {
     __shared__ int s_at[3][kPlanThreads + 1], s_wave[3][kPlanThreads / 64], s_long;
     __shared__ float s_sum[kPlanThreads / 64][3][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int chunks = (a.t.n_seq + kPlanThreads - 1) / kPlanThreads;
+    const int chunks = (a.t.n_seq + kPlanThreads - 1) / kPlanThreads, log_bq = 31 - __builtin_clz((unsigned)a.bq);
     if (tid == 0) s_long = 0;
     // the sequences c * kPlanThreads .. into LDS
     auto load_chunk = [&](int c) {
@@ -65,7 +82,7 @@ __device__ void plan_trees(const TreeRowArgs& a) {
         s_lo[tid] = r.lo;
         s_S[tid] = S;
         s_start[tid] = start;
-        s_nt[tid] = S > 0 ? tree_tiles(start, S, (S - 1) / a.bq, a.bq, a.kt, a.window) : 0;
+        s_nt[tid] = S > 0 ? tree_tiles(start, S, (S - 1) >> log_bq, a.bq, a.kt, a.window) : 0;
         __syncthreads();
     };
     load_chunk(0);
@@ -77,12 +94,13 @@ __device__ void plan_trees(const TreeRowArgs& a) {
     const int longest = max(s_long, 1);
     int st = longest;
     if (a.max_slots > 0 && longest > 1) {  // workgroup-uniform
-        const int my = max((longest + tree_candidate(lane) - 1) / tree_candidate(lane), 1);
+        const int my = max(Over(tree_candidate(lane)).up(longest), 1);
+        const Over per(my);
         float units = 0.0f, slots = 0.0f, tiles = 0.0f;
         for (int c = 0; c < chunks; ++c) {
             if (chunks > 1) load_chunk(c);
             for (int i = wave; i < min(kPlanThreads, a.t.n_seq - c * kPlanThreads); i += kPlanThreads / 64) {
-                const int nb = (s_S[i] + a.bq - 1) / a.bq, np = max((s_nt[i] + my - 1) / my, 1);
+                const int nb = (s_S[i] + a.bq - 1) >> log_bq, np = max(per.up(s_nt[i]), 1);
                 units += (float)(nb * np);  // exact up to 2^24, far above the slots that there are
                 slots += np > 1 ? (float)(nb * np) : 0.0f;
                 tiles += (float)nb * (float)s_nt[i];
@@ -112,14 +130,14 @@ __device__ void plan_trees(const TreeRowArgs& a) {
         const float best = -wave_max(-cost);
         const unsigned long long m = __ballot(cost == best);
         const int pick = __builtin_ctzll(m | 1ull << 63);
-        st = max((longest + tree_candidate(pick) - 1) / tree_candidate(pick), 1);
+        st = __builtin_amdgcn_readlane(my, pick);
         __syncthreads();
     }
+    const Over over_st(st), over_kvh(a.n_kv_heads);
     int at[3] = {0, 0, 0};  // units, slots, merges of the chunks before
     for (int c = 0; c < chunks; ++c) {
         if (chunks > 1) load_chunk(c);
-        const int nb = (s_S[tid] + a.bq - 1) / a.bq;
-        const int np = max((s_nt[tid] + st - 1) / st, 1);
+        const int nb = (s_S[tid] + a.bq - 1) >> log_bq, np = max(over_st.up(s_nt[tid]), 1);
         const int n[3] = {nb * np * a.n_kv_heads, np > 1 ? nb * np * a.n_kv_heads : 0, np > 1 ? nb * a.n_kv_heads : 0};
         int incl[3];
 #pragma unroll
@@ -137,18 +155,21 @@ __device__ void plan_trees(const TreeRowArgs& a) {
         __syncthreads();
         const int u0 = s_at[0][0], u1 = s_at[0][kPlanThreads];
         for (int u = u0 + tid; u < min(u1, a.max_units); u += kPlanThreads) {
-            int lo = 0, hi = kPlanThreads;  // s_at[0][lo] <= u < s_at[0][lo + 1]
+            int lo = 0, hi = min(kPlanThreads, a.t.n_seq - c * kPlanThreads);  // s_at[0][lo] <= u < s_at[0][lo + 1]
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (s_at[0][mid] <= u) lo = mid;
                 else hi = mid;
             }
-            const int pieces = max((s_nt[lo] + st - 1) / st, 1);
-            const int k = u - s_at[0][lo], p = k % pieces, kh = k / pieces % a.n_kv_heads, qb = k / pieces / a.n_kv_heads;
+            const int pieces = max(over_st.up(s_nt[lo]), 1);
+            const Over over_pieces(pieces);
+            const int k = u - s_at[0][lo], block = over_pieces(k), p = k - block * pieces;
+            const int qb = over_kvh(block), kh = block - qb * a.n_kv_heads;
             const int start = s_start[lo], S = s_S[lo], b = c * kPlanThreads + lo;
             const int nt = tree_tiles(start, S, qb, a.bq, a.kt, a.window);
-            PagedUnit w{b, qb, kh, pieces, 0, (p * nt + pieces - 1) / pieces, ((p + 1) * nt + pieces - 1) / pieces, s_lo[lo], S, start,
-                        {-1, -1, -1, -1}, 0, 0};
+            // (pieces of ceil(nt / pieces) tiles or one less, so that no product passes 32 bits)
+            const int each = over_pieces(nt), more = nt - each * pieces, t0 = p * each + min(p, more);
+            PagedUnit w{b, qb, kh, pieces, 0, t0, t0 + each + (p < more ? 1 : 0), s_lo[lo], S, start, {-1, -1, -1, -1}, 0, 0};
             const int key0 = (tree_first(start, a.window) & ~(a.kt - 1)) + w.t0 * a.kt;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // (a group past the table's columns has no rows)
@@ -269,14 +290,20 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) x[i][e] = x[i][e] * rs * gv[e];
                 }
-                hvec_t hv;
+                hvec_t hv, lo;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float2 pr = pair32(x[i][e]);  // (lane < 32: this lane's, its partner's), the same pair in both
                     const float y = lane < 32 ? pr.y : pr.x;
-                    hv[e] = (half_t)pin(lane < 32 ? __builtin_fmaf(x[i][e], c[e], -(y * sn[e])) : __builtin_fmaf(x[i][e], c[e], y * sn[e]));
+                    const float z = pin(lane < 32 ? __builtin_fmaf(x[i][e], c[e], -(y * sn[e])) : __builtin_fmaf(x[i][e], c[e], y * sn[e]));
+                    hv[e] = (half_t)z;
+                    lo[e] = (half_t)(z - (float)hv[e]);
                 }
-                if (h0 + i < a.n_q_heads) *reinterpret_cast<hvec_t*>(a.q16 + ((size_t)tok * a.n_q_heads + h0 + i) * HD + E * lane) = hv;
+                if (h0 + i < a.n_q_heads) {
+                    const size_t at = ((size_t)tok * a.n_q_heads + h0 + i) * HD + E * lane;
+                    *reinterpret_cast<hvec_t*>(a.q16 + at) = hv;
+                    if constexpr (HD == 256) *reinterpret_cast<hvec_t*>(a.q16_lo + at) = lo;
+                }
             }
             return;
         }
@@ -433,11 +460,11 @@ static tree_rows_fn pick_rows(bool in16, bool c32) {
     return c32 ? tree_rows_kernel<HD, float, float> : tree_rows_kernel<HD, float, half_t>;
 }
 
-// What the host can bound, and the workspace [counts][units][merges][depth][bits][q16][partials][(m, l)][K16][V16][table16].
+// What the host can bound, and the workspace [counts][units][merges][depth][bits][q16][its remainders][partials][(m, l)][K16][V16][table16].
 // Every part grows with n_tokens, n_seq and max_key_len, so that one reserved for the largest call holds all.
 struct TreePlan {
     int bq, kt, max_units, max_slots, words, cols16;
-    size_t units, merges, depth, bits, q16, part_o, part_ml, k16, v16, tab16, total;
+    size_t units, merges, depth, bits, q16, q16_lo, part_o, part_ml, k16, v16, tab16, total;
 };
 static bool tree_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, TreePlan& p) {
     const int HD = (int)cfg->head_dim, G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
@@ -464,6 +491,7 @@ static bool tree_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, Tre
     p.depth = part((size_t)n_tokens * sizeof(int32_t));
     p.bits = part((size_t)n_tokens * p.words * sizeof(unsigned long long));
     p.q16 = part((size_t)n_tokens * cfg->n_q_heads * HD * sizeof(half_t));
+    p.q16_lo = HD == 256 ? part((size_t)n_tokens * cfg->n_q_heads * HD * sizeof(half_t)) : p.q16;
     p.part_o = part((size_t)slots * 128 * HD * 3);
     p.part_ml = part((size_t)slots * 128 * sizeof(float2));
     p.k16 = p.v16 = p.tab16 = at;
@@ -558,6 +586,7 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
     a.parents = parents;
     a.bits = (unsigned long long*)(w + p.bits);
     a.depth = (int32_t*)(w + p.depth);
+    a.q16_lo = (half_t*)(w + p.q16_lo);
     a.words = p.words;
     a.k_new = k_new;
     a.v_new = v_new;
