@@ -333,25 +333,7 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(PagedPrefillArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void paged_kv16_kernel(PagedKv16Args a) {
-    const int b = blockIdx.y, k0 = 16 * blockIdx.x, ps = 1 << a.t.shift;
-    const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
-    const int page = k0 >> a.t.shift;
-    if (page >= a.cols) return;
-    const int first = a.window > 0 ? max(0, r.keys - (r.hi - r.lo) + 1 - a.window) & ~15 : 0;
-    const bool used = k0 < r.keys && r.hi > r.lo && (page + 1) << a.t.shift > first;
-    const int from = used ? page_at(a.t, b, k0) : -1;
-    const bool ok = page_ok(a.t, from);
-    const int to = b * a.cols + page;
-    if ((k0 & (ps - 1)) == 0 && threadIdx.x == 0 && blockIdx.z == 0) a.tab[to] = ok ? to : -1;
-    if (!ok || k0 < first) return;
-    const size_t src = paged_row(a.t, from, k0, a.row), dst = paged_row(a.t, to, k0, a.row);
-    const int n8 = min(16, r.keys - k0) * a.row / 8;
-    for (int i = threadIdx.x + 256 * blockIdx.z; i < n8; i += 256 * gridDim.z) {
-        *reinterpret_cast<half8*>(a.ko + dst + 8 * (size_t)i) = load8h(a.kc + src + 8 * (size_t)i);
-        *reinterpret_cast<half8*>(a.vo + dst + 8 * (size_t)i) = load8h(a.vc + src + 8 * (size_t)i);
-    }
-}
+__global__ __launch_bounds__(256) void paged_kv16_kernel(PagedKv16Args a) { kv16_rows(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z); }
 
 // Merge of the pieces of a split query block, as prefill_merge_kernel: with each piece holding
 // o_p = O_p / l_p, out = sum_p o_p l_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), M = max_p m_p. One workgroup
@@ -429,15 +411,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedPrefillArgs a) {
 
 
 // ---------------------------------------------------------------- host side
-int launch_kv16(const PagedKv16Args& k, const g4a_paged* pg, hipStream_t stream) {
-    // a workgroup per 16 rows, and per 512 elements of a row: four loads a thread (595 keys of 8 x 256: 11.4
-    // us with one workgroup per 16 rows, 5 so)
-    hipLaunchKernelGGL(paged_kv16_kernel, dim3((unsigned)((pg->max_key_len + 15) / 16), pg->n_seq, (unsigned)((k.row + 511) / 512)),
-                       dim3(256), 0, stream, k);
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? G4A_OK : hip_error(e, "paged cache conversion launch");
-}
-
 typedef void (*paged_prefill_fn)(PagedPrefillArgs);
 
 template <int G>
@@ -584,7 +557,12 @@ extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_
         k.row = (int)cfg->n_kv_heads * HD;
         k.cols = p.cols16;
         k.window = a.window;
-        if (const int rc = launch_kv16(k, pg, stream)) return rc;
+        k.rows_given = 0;
+        // a workgroup per 16 rows, and per 512 elements of a row: four loads a thread (595 keys of 8 x 256: 11.4
+        // us with one workgroup per 16 rows, 5 so)
+        hipLaunchKernelGGL(paged_kv16_kernel, dim3((unsigned)((pg->max_key_len + 15) / 16), pg->n_seq, (unsigned)((k.row + 511) / 512)),
+                           dim3(256), 0, stream, k);
+        if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged cache conversion launch");
         // from here on the f16 copy and its table
         a.kc = w + p.k16;
         a.vc = w + p.v16;

@@ -69,8 +69,29 @@ struct PagedKv16Args {
     half_t* vo;
     int32_t* tab;
     int n_tokens, row, cols, window;
+    int rows_given;  // the call's own rows are stored in both by whoever makes them
 };
-int launch_kv16(const PagedKv16Args& k, const g4a_paged* pg, hipStream_t stream);
+// rows 16 x .. of sequence b, part z of nz of their elements, by a workgroup of 256 threads
+__device__ __forceinline__ void kv16_rows(const PagedKv16Args& a, int x, int b, int z, int nz) {
+    const int k0 = 16 * x, ps = 1 << a.t.shift;
+    const SeqRows r = seq_rows(a.t, a.cu, a.n_tokens, b);
+    const int page = k0 >> a.t.shift;
+    if (page >= a.cols) return;
+    const int first = a.window > 0 ? max(0, r.keys - (r.hi - r.lo) + 1 - a.window) & ~15 : 0;
+    const bool used = k0 < r.keys && r.hi > r.lo && (page + 1) << a.t.shift > first;
+    const int from = used ? page_at(a.t, b, k0) : -1;
+    const bool ok = page_ok(a.t, from);
+    const int to = b * a.cols + page;
+    if ((k0 & (ps - 1)) == 0 && threadIdx.x == 0 && z == 0) a.tab[to] = ok ? to : -1;
+    if (!ok || k0 < first) return;
+    const size_t src = paged_row(a.t, from, k0, a.row), dst = paged_row(a.t, to, k0, a.row);
+    const int end = a.rows_given ? cut_tree(r).keys - (cut_tree(r).hi - r.lo) : r.keys;
+    const int n8 = min(16, end - k0) * a.row / 8;
+    for (int i = threadIdx.x + 256 * z; i < n8; i += 256 * nz) {
+        *reinterpret_cast<half8*>(a.ko + dst + 8 * (size_t)i) = load8h(a.kc + src + 8 * (size_t)i);
+        *reinterpret_cast<half8*>(a.vo + dst + 8 * (size_t)i) = load8h(a.vc + src + 8 * (size_t)i);
+    }
+}
 
 // ---------------------------------------------------------------- pages of a workgroup's tiles
 // Lane j holds, for tile t0 + j (64 at a time), the table entry of the 16 rows that its wave moves and a

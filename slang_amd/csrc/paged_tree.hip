@@ -26,7 +26,9 @@ struct TreeRowArgs : PagedTreeArgs {
     void* k_pages;
     void* v_pages;
     PageTab rows;  // the cache's own table (t is the f16 copy's where there is one)
-    int v_norm, q_groups, plan_and_q;  // q_groups: groups of four heads
+    PagedKv16Args conv;
+    int v_norm, q_groups;  // groups of four heads
+    int conv_x, conv_z;    // f32 caches: the conversion's workgroups a sequence and 16 rows; 0: none
     float k_in_q, v_in_q;
 };
 
@@ -174,7 +176,8 @@ __device__ void plan_trees(const TreeRowArgs& a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // (a group past the table's columns has no rows)
                 const int col = (key0 + 16 * i) >> a.t.shift;
-                w.page[i] = nt > 0 && col < a.t.cols ? a.t.table[(size_t)b * a.t.stride + col] : -1;
+                w.page[i] = nt > 0 && col < a.t.cols ? a.rows.table[(size_t)b * a.rows.stride + col] : -1;
+                if (a.conv_x) w.page[i] = page_ok(a.rows, w.page[i]) ? b * a.t.cols + col : -1;  // as the conversion names it
             }
             if (pieces > 1) {  // the prices have kept to max_slots
                 const int slot0 = s_at[1][lo] + (qb * a.n_kv_heads + kh) * pieces;
@@ -225,13 +228,14 @@ __device__ __forceinline__ int walk_up(const int32_t* par, int i, int* lds, int 
 
 // Workgroup 0: the work list. Then a wave per token and four heads: q to f16 as paged_prep_kernel makes it, at the token's
 // depth, and once a token its depth and bits. Then, with new rows, a workgroup per token and kv head: paged_write's row at
-// its own place, rotated by its depth.
+// its own place, rotated by its depth, in the cache and in an f32 cache's f16 copy. Then the copy's other rows, which need
+// none of that: one launch where rows, copy, q and list took three (tree_wide 74 -> 66 us a call).
 template <int HD, typename IT, typename CT>
 __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
     __shared__ int s_par[4][kTreeMax];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int blk = blockIdx.x;
-    if (a.plan_and_q) {
+    {
         if (blk == 0) {
             plan_trees(a);
             return;
@@ -309,7 +313,16 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
         }
         blk -= 1 + q_blocks;
     }
-    // one (token, kv head); blk < n_tokens * n_kv_heads by the grid, every exit is the whole workgroup's
+    const int row_blocks = a.k_new ? a.n_tokens * a.n_kv_heads : 0;
+    if (blk >= row_blocks) {
+        if constexpr (sizeof(CT) == 4) {
+            blk -= row_blocks;  // < conv_x * n_seq * conv_z by the grid
+            const int x = blk % a.conv_x, bz = blk / a.conv_x;
+            kv16_rows(a.conv, x, bz / a.conv_z, bz % a.conv_z, a.conv_z);
+        }
+        return;
+    }
+    // one (token, kv head); every exit is the whole workgroup's
     constexpr int HALF = HD / 2;
     __shared__ float red[2 * (HALF / 64)];
     const int t = threadIdx.x, tok = blk / a.n_kv_heads, kh = blk - tok * a.n_kv_heads;
@@ -343,6 +356,13 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
     store_elem(kc + t + HALF, k1);
     store_elem(vc + t, v0);
     store_elem(vc + t + HALF, v1);
+    if constexpr (sizeof(CT) == 4) {
+        const size_t copy = paged_row(a.rows, b * a.t.cols + (at >> a.rows.shift), at, a.n_kv_heads * HD) + (size_t)kh * HD;
+        a.conv.ko[copy + t] = (half_t)k0;
+        a.conv.ko[copy + t + HALF] = (half_t)k1;
+        a.conv.vo[copy + t] = (half_t)v0;
+        a.conv.vo[copy + t + HALF] = (half_t)v1;
+    }
 }
 
 // ---------------------------------------------------------------- merge
@@ -595,21 +615,15 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
     a.k_in_q = k_in_q;
     a.v_in_q = v_in_q;
     a.q_groups = (a.n_q_heads + 3) / 4;
-    a.plan_and_q = 1;
     const bool kv32 = (cfg->flags & G4A_KV_F32) != 0, in16 = (cfg->flags & G4A_IN_F16) != 0;
     const tree_rows_fn rows = HD == 256 ? pick_rows<256>(in16, kv32) : pick_rows<512>(in16, kv32);
-    unsigned row_blocks = k_new ? (unsigned)((int64_t)n_tokens * a.n_kv_heads) : 0u;
+    int64_t blocks = 1 + ((int64_t)n_tokens * a.q_groups + 3) / 4 + (k_new ? (int64_t)n_tokens * a.n_kv_heads : 0);
     hipError_t e;
+    a.conv = PagedKv16Args{};
+    a.conv_x = a.conv_z = 0;
     if (kv32) {
-        if (row_blocks) {  // the rows first: the conversion reads them
-            a.plan_and_q = 0;
-            hipLaunchKernelGGL(rows, dim3(row_blocks), dim3(256), 0, stream, a);
-            if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged tree rows launch");
-            a.plan_and_q = 1;
-            row_blocks = 0;
-        }
-        PagedKv16Args k;
-        k.t = a.t;
+        PagedKv16Args& k = a.conv;
+        k.t = a.rows;
         k.cu = cu_q;
         k.kc = (const float*)pg->k_pages;
         k.vc = (const float*)pg->v_pages;
@@ -620,16 +634,22 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
         k.row = a.n_kv_heads * HD;
         k.cols = p.cols16;
         k.window = a.window;
-        if (const int rc = launch_kv16(k, pg, stream)) return rc;
-        // from here on the f16 copy and its table
+        k.rows_given = k_new != nullptr;
+        a.conv_x = (pg->max_key_len + 15) / 16;
+        a.conv_z = (k.row + 511) / 512;
+        blocks += (int64_t)a.conv_x * pg->n_seq * a.conv_z;
+        // the units read the f16 copy by its own table
         a.kc = w + p.k16;
         a.vc = w + p.v16;
         a.t.table = (const int32_t*)(w + p.tab16);
         a.t.cols = a.t.stride = p.cols16;
         a.t.n_pages = pg->n_seq * p.cols16;
     }
-    const unsigned q_blocks = (unsigned)(((int64_t)n_tokens * a.q_groups + 3) / 4);
-    hipLaunchKernelGGL(rows, dim3(1 + q_blocks + row_blocks), dim3(256), 0, stream, a);
+    if (blocks > 0x7fffffff) {
+        set_error("n_tokens or n_seq * max_key_len too large");
+        return G4A_EINVAL;
+    }
+    hipLaunchKernelGGL(rows, dim3((unsigned)blocks), dim3(256), 0, stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged tree preparation launch");
     const bool out32 = (cfg->flags & G4A_OUT_F32) != 0;
     const PagedTreeArgs& t = a;
