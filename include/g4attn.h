@@ -296,7 +296,8 @@ int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, con
  * and, of the tree, itself and the ancestors whose depth is less than W below its own, all on pages that are there.
  * (A V row that is not finite reaches other tokens of the tree as in g4a_paged_prefill. Masked K rows may hold anything.)
  *   parents     int32 [n_tokens], device, indices within the tree.
- *   q, out      as g4a_paged_prefill (q rounded to f16, G4A_Q_HILO refused).
+ *   q, out      as g4a_paged_prefill, but that at head_dim 256 the prepared q enters the products as f16 pairs (f32
+ *               accuracy); at 512 it is rounded to f16 (G4A_Q_HILO refused).
  *   k_new/v_new [n_tokens][n_kv_heads][head_dim], f32, or f16 with G4A_IN_F16, or both NULL (the cache holds the rows):
  *               prepared as g4a_kv_write prepares rows at the tokens' positions, to the bit, and stored at rows
  *               start + i before they are attended (k_in_q, v_in_q, k_gain as there).

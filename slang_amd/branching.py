@@ -100,7 +100,8 @@ def paged_tree(q, k_pages, v_pages, page_table, key_len, cu_q, parents, cfg: Att
     """Attention of packed drafted trees, a tree per sequence, over the cache.
 
     A token attends its sequence's keys in front of the tree, its ancestors and itself, within cfg's window
-    of its position. q f32 [T][nH][hd] raw, rounded to f16 once normalised and rotated. With k_new / v_new ([T][kvH][hd],
+    of its position. q f32 [T][nH][hd] raw; normalised and rotated, it enters the products at f32 accuracy (f16 pairs) at
+    head_dim 256 and rounded to f16 at 512. With k_new / v_new ([T][kvH][hd],
     f32 or f16) the tokens' rows are prepared as ``kv_write`` prepares them, each at its position, and stored
     by the same call before they are attended; without, the cache holds them. A tree has at most 1024 tokens: rows
     behind are rows of nobody. Returns out [T][nH][hd] (f16 by default). f32 caches are converted to f16 in the
@@ -209,7 +210,7 @@ def paged_fork(pools, page_table, key_len, parent, free_pages, n_free, *, worksp
                n_pages: int | None = None, page_size: int | None = None, max_key_len: int | None = None):
     """The tables, lengths and free list of sequences that follow their parents (beams after a step's selection).
 
-    New row j continues row parent[j] of page_table [n_seq][cols], which lists every sequence that has pages of the pools
+    New row j continues row parent[j] (int32 [n_new], of any shape) of page_table [n_seq][cols], which lists every sequence that has pages of the pools
     (one that does not branch is its own parent; a parent outside [0, n_seq) makes an idle row). Full pages are shared;
     each page that a row will write to, for `room` more keys, becomes its own: the first heir keeps the parent's, the
     others get pages off the end of free_pages (int32 [n_pages], n_free int32 [1] of them in use), and the filled rows of a
@@ -224,15 +225,13 @@ def paged_fork(pools, page_table, key_len, parent, free_pages, n_free, *, worksp
     if None in shape or n_pages not in (None, shape[0]) or page_size not in (None, shape[1]):
         raise ValueError(f"n_pages ({n_pages}) and page_size ({page_size}) must be those of the pools, {tuple(shape)}")
     pg = G4APaged(None, None, *_table(dev, page_table, key_len, *shape, max_key_len))
-    if parent.dim() != 1:
-        raise ValueError(f"parent must hold one entry per new row, got {tuple(parent.shape)}")
-    n_new, par = parent.shape[0], _t("parent", parent, dev, _I32)
+    n_new, par = parent.numel(), _t("parent", parent, dev, _I32)
     fr, nf = _i32("free_pages", free_pages, dev, (pg.n_pages,)), _i32("n_free", n_free, dev, (1,))
     room = int(room)
     if not 0 <= room <= 1 << 30:
         raise ValueError(f"room must be in [0, 2^30], got {room}")
     if out is None:
-        out = (torch.empty((n_new, pg.table_cols), dtype=_I32, device=page_table.device), torch.empty_like(parent),
+        out = (torch.empty((n_new, pg.table_cols), dtype=_I32, device=page_table.device), torch.empty_like(parent.view(-1)),
                torch.empty_like(free_pages), torch.empty_like(n_free))
         at = [t.data_ptr() for t in out]
     else:

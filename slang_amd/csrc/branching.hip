@@ -241,6 +241,11 @@ __device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& m
     const int chunks = (a.n_new + kForkThreads - 1) / kForkThreads;
     const int had = min(max(a.n_free_in[0], 0), a.t.n_pages);
     for (int i = tid; i < had; i += kForkThreads) a.free_out[i] = a.free_in[i];
+    // a workgroup's barrier alone does not wait for stores and atomics to reach memory, where the others read them
+    auto reached = [] {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
     int p = -1, L = 0, need = 0;  // of this thread's row; of the only chunk, if there is one
     for (int ch = 0; ch < chunks; ++ch) {
         const int j = ch * kForkThreads + tid;
@@ -256,7 +261,7 @@ __device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& m
             }
         });
     }
-    __syncthreads();
+    reached();
     int m = had;
     for (int w0 = 0; w0 < a.words; w0 += kForkThreads) {
         const int w = w0 + tid;
@@ -270,7 +275,7 @@ __device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& m
         m += total;
     }
     m = min(m, a.t.n_pages);
-    __syncthreads();
+    reached();
     int taken = 0;
     for (int ch = 0; ch < chunks; ++ch) {
         const int j = ch * kForkThreads + tid;
@@ -305,7 +310,7 @@ __device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& m
         }
         taken += total;
     }
-    __syncthreads();
+    reached();
     const int left = max(m - taken, 0);
     for (int i = left + tid; i < a.t.n_pages; i += kForkThreads) a.free_out[i] = -1;
     if (tid == 0) a.n_free_out[0] = left;

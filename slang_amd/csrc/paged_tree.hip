@@ -235,84 +235,81 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
     __shared__ int s_par[4][kTreeMax];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int blk = blockIdx.x;
-    {
-        if (blk == 0) {
-            plan_trees(a);
-            return;
-        }
-        const int64_t waves = (int64_t)a.n_tokens * a.q_groups;
-        const int q_blocks = (int)((waves + 3) / 4);
-        if (blk <= q_blocks) {
-            constexpr int E = HD / 64, NH = 4;
-            typedef float vec_t __attribute__((ext_vector_type(E)));
-            typedef half_t hvec_t __attribute__((ext_vector_type(E)));
-            const int64_t w = (int64_t)(blk - 1) * 4 + wave;
-            if (w >= waves) return;
-            const int tok = (int)(w / a.q_groups), h0 = (int)(w - (int64_t)tok * a.q_groups) * NH;
-            vec_t x[NH], gv;
-            const float* qr = a.q + ((size_t)tok * a.n_q_heads + h0) * HD + E * lane;
+    if (blk == 0) {
+        plan_trees(a);
+        return;
+    }
+    const int waves = a.n_tokens * a.q_groups, q_blocks = (waves + 3) / 4;  // (n_tokens * n_q_heads fits 32 bits with room)
+    if (blk <= q_blocks) {
+        constexpr int E = HD / 64, NH = 4;
+        typedef float vec_t __attribute__((ext_vector_type(E)));
+        typedef half_t hvec_t __attribute__((ext_vector_type(E)));
+        const int w = (blk - 1) * 4 + wave;
+        if (w >= waves) return;
+        const int tok = w / a.q_groups, h0 = (w - tok * a.q_groups) * NH;
+        vec_t x[NH], gv;
+        const float* qr = a.q + ((size_t)tok * a.n_q_heads + h0) * HD + E * lane;
 #pragma unroll
-            for (int i = 0; i < NH; ++i) x[i] = *reinterpret_cast<const vec_t*>(qr + (h0 + i < a.n_q_heads ? i * HD : 0));
-            if (a.q_gain) gv = *reinterpret_cast<const vec_t*>(a.q_gain + E * lane);
-            const int b = seq_of_row(a.cu, a.t.n_seq, tok);
-            if (b >= a.t.n_seq) return;  // a row of nobody
-            const SeqRows r = tree_rows(a.t, a.cu, a.n_tokens, b);
-            if (!holds(r, tok)) return;  // offsets that do not ascend, or a row behind the tree's last
-            const int i0 = tok - r.lo, start = r.keys - (r.hi - r.lo), off = start & 63;
-            unsigned long long bits = 0;  // lane k: word k
-            const int depth = walk_up(a.parents + r.lo, i0, s_par[wave], lane, [&](int j, int d) {
-                if (lane == (off + j) >> 6 && (a.window == 0 || d < a.window)) bits |= 1ull << ((off + j) & 63);
-            });
-            const int pos = start + depth;
-            if (h0 == 0) {
-                // the history in the first word: keys start - off .. start - 1 that the window holds
-                if (lane == 0) {
-                    const int from = a.window > 0 ? min(max(pos + 1 - a.window - (start - off), 0), off) : 0;
-                    bits |= ((1ull << off) - 1) & ~((1ull << from) - 1);
-                    a.depth[tok] = depth;
-                }
-                if (lane < a.words) a.bits[(size_t)tok * a.words + lane] = bits;
+        for (int i = 0; i < NH; ++i) x[i] = *reinterpret_cast<const vec_t*>(qr + (h0 + i < a.n_q_heads ? i * HD : 0));
+        if (a.q_gain) gv = *reinterpret_cast<const vec_t*>(a.q_gain + E * lane);
+        const int b = seq_of_row(a.cu, a.t.n_seq, tok);
+        if (b >= a.t.n_seq) return;  // a row of nobody
+        const SeqRows r = tree_rows(a.t, a.cu, a.n_tokens, b);
+        if (!holds(r, tok)) return;  // offsets that do not ascend, or a row behind the tree's last
+        const int i0 = tok - r.lo, start = r.keys - (r.hi - r.lo), off = start & 63;
+        unsigned long long bits = 0;  // lane k: word k
+        const int depth = walk_up(a.parents + r.lo, i0, s_par[wave], lane, [&](int j, int d) {
+            if (lane == (off + j) >> 6 && (a.window == 0 || d < a.window)) bits |= 1ull << ((off + j) & 63);
+        });
+        const int pos = start + depth;
+        if (h0 == 0) {
+            // the history in the first word: keys start - off .. start - 1 that the window holds
+            if (lane == 0) {
+                const int from = a.window > 0 ? min(max(pos + 1 - a.window - (start - off), 0), off) : 0;
+                bits |= ((1ull << off) - 1) & ~((1ull << from) - 1);
+                a.depth[tok] = depth;
             }
-            const int p = max(pos, 0);
-            vec_t c, sn;
+            if (lane < a.words) a.bits[(size_t)tok * a.words + lane] = bits;
+        }
+        const int p = max(pos, 0);
+        vec_t c, sn;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            c[e] = 1.0f;
+            sn[e] = 0.0f;
+        }
+        if (a.rcos) {
+            c = *reinterpret_cast<const vec_t*>(a.rcos + (size_t)p * (HD / 2) + E * (lane & 31));
+            sn = *reinterpret_cast<const vec_t*>(a.rsin + (size_t)p * (HD / 2) + E * (lane & 31));
+        }
+#pragma unroll
+        for (int i = 0; i < NH; ++i) {
+            if (a.q_gain) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int e = 0; e < E; ++e) ss = __builtin_fmaf(x[i][e], x[i][e], ss);
+                const float rs = 1.0f / sqrtf(wave_sum(ss) / (float)HD + a.eps);
+#pragma unroll
+                for (int e = 0; e < E; ++e) x[i][e] = x[i][e] * rs * gv[e];
+            }
+            hvec_t hv, lo;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                c[e] = 1.0f;
-                sn[e] = 0.0f;
+                const float2 pr = pair32(x[i][e]);  // (lane < 32: this lane's, its partner's), the same pair in both
+                const float y = lane < 32 ? pr.y : pr.x;
+                const float z = pin(lane < 32 ? __builtin_fmaf(x[i][e], c[e], -(y * sn[e])) : __builtin_fmaf(x[i][e], c[e], y * sn[e]));
+                hv[e] = (half_t)z;
+                lo[e] = (half_t)(z - (float)hv[e]);
             }
-            if (a.rcos) {
-                c = *reinterpret_cast<const vec_t*>(a.rcos + (size_t)p * (HD / 2) + E * (lane & 31));
-                sn = *reinterpret_cast<const vec_t*>(a.rsin + (size_t)p * (HD / 2) + E * (lane & 31));
+            if (h0 + i < a.n_q_heads) {
+                const size_t at = ((size_t)tok * a.n_q_heads + h0 + i) * HD + E * lane;
+                *reinterpret_cast<hvec_t*>(a.q16 + at) = hv;
+                if constexpr (HD == 256) *reinterpret_cast<hvec_t*>(a.q16_lo + at) = lo;
             }
-#pragma unroll
-            for (int i = 0; i < NH; ++i) {
-                if (a.q_gain) {
-                    float ss = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) ss = __builtin_fmaf(x[i][e], x[i][e], ss);
-                    const float rs = 1.0f / sqrtf(wave_sum(ss) / (float)HD + a.eps);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) x[i][e] = x[i][e] * rs * gv[e];
-                }
-                hvec_t hv, lo;
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float2 pr = pair32(x[i][e]);  // (lane < 32: this lane's, its partner's), the same pair in both
-                    const float y = lane < 32 ? pr.y : pr.x;
-                    const float z = pin(lane < 32 ? __builtin_fmaf(x[i][e], c[e], -(y * sn[e])) : __builtin_fmaf(x[i][e], c[e], y * sn[e]));
-                    hv[e] = (half_t)z;
-                    lo[e] = (half_t)(z - (float)hv[e]);
-                }
-                if (h0 + i < a.n_q_heads) {
-                    const size_t at = ((size_t)tok * a.n_q_heads + h0 + i) * HD + E * lane;
-                    *reinterpret_cast<hvec_t*>(a.q16 + at) = hv;
-                    if constexpr (HD == 256) *reinterpret_cast<hvec_t*>(a.q16_lo + at) = lo;
-                }
-            }
-            return;
         }
-        blk -= 1 + q_blocks;
+        return;
     }
+    blk -= 1 + q_blocks;
     const int row_blocks = a.k_new ? a.n_tokens * a.n_kv_heads : 0;
     if (blk >= row_blocks) {
         if constexpr (sizeof(CT) == 4) {
@@ -564,7 +561,7 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
         return G4A_EINVAL;
     }
     if (cfg->flags & G4A_Q_HILO) {
-        set_error("g4a_paged_tree rounds q to f16 (G4A_Q_HILO not supported)");
+        set_error("g4a_paged_tree takes q as its head_dim allows (G4A_Q_HILO not supported)");
         return G4A_EUNSUPPORTED;
     }
     const int HD = (int)cfg->head_dim, G = (int)(cfg->n_q_heads / cfg->n_kv_heads);

@@ -285,7 +285,8 @@ def test_fork_refused():
     a = dict(pools=pools, page_table=dev(table), key_len=dev(keys), parent=dev([0, 0]), free_pages=dev(fr), n_free=dev([len(free)]),
              workspace=sa.Workspace())
     out = sa.paged_fork(**a)
-    for over in (dict(parent=a["parent"].long()), dict(parent=a["parent"].view(1, 2)), dict(free_pages=a["free_pages"][:-1]),
+    assert torch.equal(sa.paged_fork(**dict(a, parent=a["parent"].view(1, 2)))[0], out[0])
+    for over in (dict(parent=a["parent"].long()), dict(parent=a["parent"].cpu()), dict(free_pages=a["free_pages"][:-1]),
                  dict(n_free=dev([1, 2])), dict(room=-1), dict(room=2 ** 31), dict(out=[x[:1] for x in out]), dict(pools=[]),
                  dict(n_pages=3), dict(page_size=64), dict(parent=a["parent"][:0]), dict(key_len=a["key_len"][:1])):
         with pytest.raises(ValueError):

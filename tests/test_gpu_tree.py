@@ -92,6 +92,15 @@ def test_shapes_of_trees(kind, window):
     run(b, dts=(torch.float16,))
 
 
+@pytest.mark.parametrize("kvh", [1, 4])
+@pytest.mark.parametrize("keys", [[40, 130], [1500, 700]])
+def test_queries_keep_their_bits(kvh, keys):
+    """At head_dim 256 q is a pair of f16 operands: the error of its rounding is not there."""
+    b = Trees(keys, [20, 33], kvh=kvh, seed=7)
+    out, A, S = b.oracle()
+    check(tree(b, b.dev()).cpu().numpy(), out, bound(out, A, S, q16=False, kv32=False, out16=True))
+
+
 @pytest.mark.parametrize("hd,kvh", [(256, 2), (512, 1)])
 @pytest.mark.parametrize("window", [0, 300])
 def test_long_histories(hd, kvh, window):
