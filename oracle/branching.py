@@ -166,7 +166,8 @@ def select(logits, scores, cap, n_out, done=None, pad=0):
             if not len(t):
                 continue
             m = x.max()
-            lp = np.where(x == m, 0.0, x - m)
+            with np.errstate(invalid="ignore"):
+                lp = np.where(x == m, 0.0, x - m)
             lp = lp - np.log(np.exp(lp).sum())
             order = np.lexsort((t, -np.asarray(logits[b * W + w], np.float64)[t]))[:n_out]
             cand += [(-(at + lp[i]), w, k, int(t[i])) for k, i in enumerate(order)]

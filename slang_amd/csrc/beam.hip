@@ -372,12 +372,15 @@ static beam_part_fn pick_each(int each, bool cap) {
 }
 static beam_part_fn pick_part(bool f16, int each, bool cap) { return f16 ? pick_each<half_t>(each, cap) : pick_each<float>(each, cap); }
 
-// Few logits: 512 a wave, one step, so that many waves share them. Many: steps of 2048, as many as leave the card kPartWaves
-// waves. A wave pays for its first step's bound and order, so longer walks are cheaper, and fewer waves hide less: 128 rows of
-// 262144 in f32 with a cap 35.4 us with 2 steps of 2048 (3.8 TB/s), 35.5 with 1, 37.6 with 4, 36.5 and 37.5 with 4 and 8
-// of 1024, 43 where the next step's loads were waited for; 30.7 without a cap. What bounds it: a logit with a cap takes two
-// exponentials, a reciprocal and six more instructions, about 72 cycles a wave of 64, 15 us of the card's VALU beside the 26
-// us that the bytes take, and a wave's first step's ballots and LDS trips.
+// Few logits: 512 a wave, one step, so that many waves share them. Many, or rows so long that their parts would be many to
+// join: steps of 2048, as many as leave the card kPartWaves waves. A call in a graph with steps of 512 and of 2048: 4 rows
+// of 32000 10.6 and 14.3 us, of 100000 12.8 and 14.6, of 131072 12.9 and 12.3, of 262144 16.5 and 13.3; 128 rows of 50000
+// 17.5 and 18.6, of 65536 19.5 and 18.3, of 262144 48.0 and 36.9.
+// A wave pays for its first step's bound and order, so longer walks are cheaper, and fewer waves hide less: the kernel takes
+// 35.4 us for 128 rows of 262144 in f32 with a cap with 2 steps of 2048 (3.8 TB/s), 35.5 with 1, 37.6 with 4, 36.5 and 37.5
+// with 4 and 8 of 1024, 43 where the next step's loads were waited for; 30.7 without a cap. What bounds it: a logit with
+// a cap takes two exponentials, a reciprocal and six more instructions, about 72 cycles a wave of 64, 15 us of the card's
+// VALU beside the 26 us that the bytes take, and a wave's first step's ballots and LDS trips.
 constexpr int kPartWaves = 8192;
 struct BeamPlan {
     int each, steps, parts;
@@ -386,13 +389,15 @@ struct BeamPlan {
 static BeamPlan beam_plan(int n_groups, int width, int vocab, int n_out) {
     BeamPlan p;
     const int64_t rows = (int64_t)n_groups * width, span = (int64_t)vocab + 7;  // (a row may begin 7 behind its part)
-    p.each = rows * vocab >= (int64_t)64 * 16 * kPartWaves ? 32 : 8;
+    p.each = vocab >= 1 << 17 || rows * vocab >= (int64_t)64 * 16 * kPartWaves ? 32 : 8;
     p.steps = p.each == 8 ? 1 : (int)std::min<int64_t>(std::max<int64_t>(rows * vocab / ((int64_t)64 * 32 * kPartWaves), 1), 64);
     const int64_t part = (int64_t)64 * p.each * p.steps;
     p.parts = (int)((span + part - 1) / part);
     auto al = [](size_t x) { return (x + 255) & ~(size_t)255; };
     p.keys = al((size_t)rows * p.parts * sizeof(float2));
-    p.total = p.keys + al((size_t)rows * p.parts * n_out * sizeof(u64));
+    // (room for the parts that the shortest steps make, so that a workspace for the largest call holds every smaller one)
+    const size_t most = (size_t)rows * (size_t)((span + 511) / 512);
+    p.total = al(most * sizeof(float2)) + al(most * n_out * sizeof(u64));
     return p;
 }
 

@@ -316,8 +316,10 @@ __device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& m
     if (tid == 0) a.n_free_out[0] = left;
 }
 
-// All of it by one workgroup, the marks in LDS, where pages and table entries are few: three launches less.
-constexpr int kForkPages = 12288, kForkEntries = 1 << 15, kForkRows = 1024;
+// All of it by one workgroup, the marks in LDS, where pages and table entries are few. A call without copies, against the
+// three launches: 4 rows of 11 columns 5.6 and 9.2 us, 128 of 67 12.3 and 23.0, 256 of 67 18.5 and 28.5, 1024 of 23
+// 30.6 and 31.5, 512 of 66 (67584 entries) 29.8 and 32.3.
+constexpr int kForkPages = 12288, kForkEntries = 1 << 16, kForkRows = 1024;
 __global__ __launch_bounds__(kForkThreads) void fork_small_kernel(ForkArgs a) {
     __shared__ int32_t s_owner[kForkPages];
     __shared__ uint32_t s_bits[3][kForkPages / 32];

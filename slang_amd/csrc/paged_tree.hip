@@ -229,7 +229,7 @@ __device__ __forceinline__ int walk_up(const int32_t* par, int i, int* lds, int 
 // Workgroup 0: the work list. Then a wave per token and four heads: q to f16 as paged_prep_kernel makes it, at the token's
 // depth, and once a token its depth and bits. Then, with new rows, a workgroup per token and kv head: paged_write's row at
 // its own place, rotated by its depth, in the cache and in an f32 cache's f16 copy. Then the copy's other rows, which need
-// none of that: one launch where rows, copy, q and list took three (tree_wide 74 -> 66 us a call).
+// none of that: one launch where rows, copy, q and list took three (3 trees of 253, 123 and 60 after 500 to 5000 keys 74 -> 64 us a call).
 template <int HD, typename IT, typename CT>
 __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
     __shared__ int s_par[4][kTreeMax];
@@ -365,9 +365,10 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
 // ---------------------------------------------------------------- merge
 // out = sum_p o_p l_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), M = max_p m_p, of a block's pieces (o_p = O_p / l_p). A
 // workgroup's item is a wave block of 32 columns x 256 dims of an entry of the merge list, and of its 16 runs of 8 values
-// x 64 lanes one, with few blocks to merge, so that many workgroups share the bytes, or four. Its four waves take every
-// fourth piece, each relative to its own largest m so far, and join through LDS: one trip to memory for up to 16 pieces.
-constexpr int kMergeGrid = 2048, kMergeFew = 64;
+// x 64 lanes one, so that many workgroups share the bytes (four runs an item: 8 trees of 16 after 2000 keys 29 -> 35 us a
+// call, 64 after 3000 111 -> 116). Its four waves take every fourth piece, each relative to its own largest m so far, and
+// join through LDS: one trip to memory for up to 16 pieces.
+constexpr int kMergeGrid = 2048;
 template <typename OUTT, int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
     constexpr int NCOL = 128, NV = NCOL * HD, BLK = NV * 3;  // values and bytes of a piece's block
@@ -375,78 +376,75 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
     __shared__ float s_o[4][8][64], s_l[4][64], s_m[4][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int merges = a.counts[1], G = a.n_q_heads / a.n_kv_heads, BQ = NCOL / G;
-    const int nk = merges <= kMergeFew ? 1 : 4, per = 16 / nk;
-    for (int item = blockIdx.x; item < merges * NW * per; item += gridDim.x) {
-        const PagedUnit pu = a.merges[item / (NW * per)];
-        const int w = item / per % NW, qb = pu.qb, kh = pu.kh, n_pieces = pu.n_pieces, w32 = HD == 256 ? w : w >> 1;
+    for (int item = blockIdx.x; item < merges * NW * 16; item += gridDim.x) {
+        const PagedUnit pu = a.merges[item / (NW * 16)];
+        const int w = item / 16 % NW, k = item % 16, qb = pu.qb, kh = pu.kh, n_pieces = pu.n_pieces, w32 = HD == 256 ? w : w >> 1;
         if (qb * BQ + 32 * w32 / G >= pu.S) continue;  // no token in these 32 columns
         const int c = 32 * w32 + (lane & 31), s_idx = qb * BQ + c / G;
         const bool ok = s_idx < pu.S;
         const float2* ml = a.part_ml + (size_t)pu.slot * NCOL + c;
         const char* base = reinterpret_cast<const char*>(a.part_o) + (size_t)pu.slot * BLK;
-        for (int k = item % per * nk; k < item % per * nk + nk; ++k) {
-            float o[8] = {}, L = 0.0f, M = kNegInf;
-            const int run = w * (32 * 256) + k * 512 + 8 * lane;
-            for (int p0 = wave; p0 < n_pieces; p0 += 16) {
-                float2 mp[4];
-                v4u32 hi[4];
-                v2u32 lo[4];
+        float o[8] = {}, L = 0.0f, M = kNegInf;
+        const int run = w * (32 * 256) + k * 512 + 8 * lane;
+        for (int p0 = wave; p0 < n_pieces; p0 += 16) {
+            float2 mp[4];
+            v4u32 hi[4];
+            v2u32 lo[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int p = p0 + 4 * e;
-                    mp[e] = make_float2(kNegInf, 0.0f);
-                    hi[e] = v4u32{0, 0, 0, 0};
-                    lo[e] = v2u32{0, 0};
-                    if (ok && p < n_pieces) {
-                        mp[e] = ml[(size_t)p * NCOL];
-                        hi[e] = *reinterpret_cast<const v4u32*>(base + (size_t)p * BLK + 2 * run);
-                        lo[e] = *reinterpret_cast<const v2u32*>(base + (size_t)p * BLK + 2 * NV + run);
-                    }
-                }
-                const float top = fmaxf(M, fmaxf(fmaxf(mp[0].x, mp[1].x), fmaxf(mp[2].x, mp[3].x)));
-                const float back = M == kNegInf ? 0.0f : fexp2(M - top);
-                M = top;
-                L *= back;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o[i] *= back;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    // a piece with no attended key (l = 0) counts for nothing, whatever it holds; one of NaN scores alone
-                    // (l NaN, m -inf) makes all NaN
-                    const bool none = mp[e].y == 0.0f;
-                    const float wt = none ? 0.0f : mp[e].y * fexp2(mp[e].x - M);
-                    L += wt;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = __builtin_fmaf(none ? 0.0f : unpack24(hi[e], lo[e], i), wt, o[i]);
+            for (int e = 0; e < 4; ++e) {
+                const int p = p0 + 4 * e;
+                mp[e] = make_float2(kNegInf, 0.0f);
+                hi[e] = v4u32{0, 0, 0, 0};
+                lo[e] = v2u32{0, 0};
+                if (ok && p < n_pieces) {
+                    mp[e] = ml[(size_t)p * NCOL];
+                    hi[e] = *reinterpret_cast<const v4u32*>(base + (size_t)p * BLK + 2 * run);
+                    lo[e] = *reinterpret_cast<const v2u32*>(base + (size_t)p * BLK + 2 * NV + run);
                 }
             }
+            const float top = fmaxf(M, fmaxf(fmaxf(mp[0].x, mp[1].x), fmaxf(mp[2].x, mp[3].x)));
+            const float back = M == kNegInf ? 0.0f : fexp2(M - top);
+            M = top;
+            L *= back;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s_o[wave][e][lane] = o[e];
-            s_l[wave][lane] = L;
-            s_m[wave][lane] = M;
-            __syncthreads();
-            // wave w finishes values 2w and 2w + 1 of each run
-            if (ok) {
-                M = fmaxf(fmaxf(s_m[0][lane], s_m[1][lane]), fmaxf(s_m[2][lane], s_m[3][lane]));
-                float x = 0.0f, y = 0.0f;
-                L = 0.0f;
+            for (int i = 0; i < 8; ++i) o[i] *= back;
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    const float l = s_l[v][lane], f = l == 0.0f ? 0.0f : fexp2(s_m[v][lane] - M);
-                    L += l * f;
-                    x = __builtin_fmaf(l == 0.0f ? 0.0f : s_o[v][2 * wave][lane], f, x);
-                    y = __builtin_fmaf(l == 0.0f ? 0.0f : s_o[v][2 * wave + 1][lane], f, y);
-                }
-                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-                OUTT* orow = reinterpret_cast<OUTT*>(a.out) + ((size_t)(pu.row0 + s_idx) * a.n_q_heads + kh * G + c % G) * HD +
-                             (HD == 256 ? 0 : 256 * (w & 1));
-                // run k: dims tile k/2, 4-row pair k%2
-                OUTT* to = orow + 32 * (k >> 1) + 16 * (k & 1) + 8 * (wave >> 1) + 4 * h + 2 * (wave & 1);
-                store_elem(to, srq(x * inv, a.out_q));
-                store_elem(to + 1, srq(y * inv, a.out_q));
+            for (int e = 0; e < 4; ++e) {
+                // a piece with no attended key (l = 0) counts for nothing, whatever it holds; one of NaN scores alone
+                // (l NaN, m -inf) makes all NaN
+                const bool none = mp[e].y == 0.0f;
+                const float wt = none ? 0.0f : mp[e].y * fexp2(mp[e].x - M);
+                L += wt;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = __builtin_fmaf(none ? 0.0f : unpack24(hi[e], lo[e], i), wt, o[i]);
             }
-            __syncthreads();
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s_o[wave][e][lane] = o[e];
+        s_l[wave][lane] = L;
+        s_m[wave][lane] = M;
+        __syncthreads();
+        // wave w finishes values 2w and 2w + 1 of each run
+        if (ok) {
+            M = fmaxf(fmaxf(s_m[0][lane], s_m[1][lane]), fmaxf(s_m[2][lane], s_m[3][lane]));
+            float x = 0.0f, y = 0.0f;
+            L = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float l = s_l[v][lane], f = l == 0.0f ? 0.0f : fexp2(s_m[v][lane] - M);
+                L += l * f;
+                x = __builtin_fmaf(l == 0.0f ? 0.0f : s_o[v][2 * wave][lane], f, x);
+                y = __builtin_fmaf(l == 0.0f ? 0.0f : s_o[v][2 * wave + 1][lane], f, y);
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            OUTT* orow = reinterpret_cast<OUTT*>(a.out) + ((size_t)(pu.row0 + s_idx) * a.n_q_heads + kh * G + c % G) * HD +
+                         (HD == 256 ? 0 : 256 * (w & 1));
+            // run k: dims tile k/2, 4-row pair k%2
+            OUTT* to = orow + 32 * (k >> 1) + 16 * (k & 1) + 8 * (wave >> 1) + 4 * h + 2 * (wave & 1);
+            store_elem(to, srq(x * inv, a.out_q));
+            store_elem(to + 1, srq(y * inv, a.out_q));
+        }
+        __syncthreads();
     }
 }
 

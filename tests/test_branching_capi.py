@@ -84,6 +84,9 @@ def test_a_workspace_holds_every_smaller_call(kvh, hd, window, kv_f32):
     tokens = [1, 5, 33, 63, 64, 65, 1000, 1024, 1025, 10000, 100000]
     got = np.array([[[sa.paged_tree_ws_bytes(t, n, k, c, **kw) for k in keys] for n in seqs] for t in tokens])
     assert all((np.diff(got, axis=i) >= 0).all() for i in range(3))
+    b = np.array([[[sa.beam_select_ws_bytes(g, 4, v, k) for k in (1, 4, 64)] for v in (1, 500, 32000, 65536, 100000, 131071, 131072, 262144)]
+                  for g in (1, 2, 16, 20, 21, 32, 40, 128, 1000)])
+    assert all((np.diff(b, axis=i) >= 0).all() for i in range(3))
     assert all(sa.paged_fork_ws_bytes(a, n) <= sa.paged_fork_ws_bytes(b, n) for a, b in ((1, 2), (31, 33), (1000, 100000)) for n in (1, 9))
 
 
@@ -160,7 +163,7 @@ def test_definitions():
     assert OB.accept([20], [0, 4], np.array([-1, 0, 0, 2]), np.array([1, 5, 6, 7]), np.array([6, 0, 7, 9]), 3) == ([[0, 2, 3]], [3], [9], [19])
     new, length, free, _ = OB.fork([], np.array([[0, 1, -1], [2, 3, 4]]), [20, 33], [0, 0], [5], 1, 16, 6)
     assert new.tolist() == [[0, 1, -1], [0, 4, -1]] and length == [20, 20] and free == [5, 2, 3]
-    s, p, t = OB.select(np.log([[0.5, 0.25, 0.25], [0.125, 0.875, 0.0]]), np.log([[0.5, 0.5]]), 0.0, 4)
+    s, p, t = OB.select(np.array([[-np.log(2), -np.log(4), -np.log(4)], [np.log(0.125), np.log(0.875), -np.inf]]), np.log([[0.5, 0.5]]), 0.0, 4)
     assert np.allclose(np.exp(s), [[0.4375, 0.25, 0.125, 0.125]]) and p.tolist() == [[1, 0, 0, 0]] and t.tolist() == [[1, 0, 1, 2]]
 
 
