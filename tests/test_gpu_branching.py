@@ -256,6 +256,18 @@ def test_fork_without_enough_pages(free):
         check_fork(pools, table, [20, 25, 30], parent, free, 30, 10, 16)
 
 
+def test_fork_of_lists_that_are_none():
+    """A count outside the list is cut to it; entries that name no page give none."""
+    table, keys = np.array([[0, 1, -1], [2, 3, -1]]), [20, 25]
+    for free, count in (([5, 6], -3), ([99, -7, 2 ** 31 - 1] + [-1] * 7, 10 ** 9)):
+        free_t = np.full(10, -1)
+        free_t[:len(free)] = free
+        got = sa.paged_fork(pools_of(Pages(10, 16), 1, 3), dev(table), dev(keys), dev([0, 0, 0]), dev(free_t), dev([count]),
+                            workspace=sa.Workspace())
+        assert got[0][0].tolist() == [0, 1, -1] and 0 <= got[3].item() <= 10
+        assert all(-1 <= p < 10 for p in got[0].flatten().tolist())
+
+
 def test_fork_tables_alone():
     table, keys, free, n_pages = beams(4, 4, [20, 30, 40, 50], [3, 14, 15, 9], 16, 2)
     check_fork([], table, keys, np.arange(16) // 4 * 4 + np.arange(16)[::-1] % 4, free, 1, n_pages, 16)

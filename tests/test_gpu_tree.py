@@ -373,3 +373,49 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         tree(b, d, workspace=small)
     assert tree(b, dict(d, q=d["q"][:0], parents=d["parents"][:0])).shape == (0, 8, 256)
+
+
+@pytest.mark.parametrize("hd,kvh,n_seq", [(256, 2, 200), (512, 1, 400)])
+@pytest.mark.parametrize("new", [3, 24])
+def test_units_of_many_tiles(hd, kvh, n_seq, new):
+    """More blocks than can be cut, each over more tiles than a wave holds pages of (64), with waves that have no token: all
+    sequences read one history through tables of their own."""
+    keys = 5000
+    b = Trees([keys], [new], hd=hd, kvh=kvh, page=16)
+    d = b.dev()
+    q = torch.randn(n_seq * new, 8, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = sa.paged_tree(q, d["k_pages"], d["v_pages"], d["table"].repeat(n_seq, 1), i32([keys] * n_seq), i32(np.arange(n_seq + 1) * new),
+                        d["parents"].repeat(n_seq), b.cfg(scale=0.3), workspace=sa.Workspace(), q_gain=d["gain"]).cpu().numpy()
+    for s in (0, 1, n_seq // 2, n_seq - 1):
+        b.q = q[s * new:(s + 1) * new].cpu().numpy()
+        out, A, S = b.oracle(cos=None, sin=None, scale=0.3)
+        check(got[s * new:(s + 1) * new], out, bound(out, A, S, q16=True, kv32=False, out16=True), f"sequence {s}")
+
+
+@pytest.mark.parametrize("hd", [256, 512])
+def test_one_long_history_among_many_sequences(hd):
+    """More sequences than a chunk of the list, one of them worth cutting."""
+    new = [5] + [1, 2] * 150
+    keys = [1900] + [20, 9] * 150
+    keys[290] = 1700
+    run(Trees(keys, new, hd=hd, kvh=1), dts=(torch.float16,))
+
+
+@pytest.mark.parametrize("hd,kvh", [(256, 2), (512, 1)])
+@pytest.mark.parametrize("window", [0, 40, 5])
+@pytest.mark.parametrize("kv", [np.float16, np.float32])
+def test_appended_rows_behind_a_window(hd, kvh, window, kv):
+    """Rows stored by the call itself, histories of every alignment, pages in front of the window not there."""
+    new, hist = [12, 1, 40, 7, 0], [100, 63, 17, 300, 0]
+    keys = [a + h for a, h in zip(new, hist)]
+    b = Trees(keys, new, hd=hd, kvh=kvh, kv=kv, window=window, written=False, seed=window)
+    if window:
+        for s, h in enumerate(hist):
+            b.table[s, :max(0, h + 1 - window) // b.page] = -1
+    d = b.dev()
+    got = tree(b, d, append=True).cpu().numpy()
+    b.k_pages, b.v_pages = d["k_pages"].cpu().numpy(), d["v_pages"].cpu().numpy()
+    out, A, S = b.oracle()
+    kv32 = kv is np.float32
+    check(got, out, bound(out, A, S, q16=True, kv32=kv32, out16=True, k16=kv32))
