@@ -100,12 +100,12 @@ def paged_tree(q, k_pages, v_pages, page_table, key_len, cu_q, parents, cfg: Att
     """Attention of packed drafted trees, a tree per sequence, over the cache.
 
     A token attends its sequence's keys in front of the tree, its ancestors and itself, within cfg's window
-    of its position. q f32 [T][nH][hd] raw; normalised and rotated, it enters the products at f32 accuracy (f16 pairs) at
-    head_dim 256 and rounded to f16 at 512. With k_new / v_new ([T][kvH][hd],
-    f32 or f16) the tokens' rows are prepared as ``kv_write`` prepares them, each at its position, and stored
-    by the same call before they are attended; without, the cache holds them. A tree has at most 1024 tokens: rows
-    behind are rows of nobody. Returns out [T][nH][hd] (f16 by default). f32 caches are converted to f16 in the
-    workspace (values beyond 65504 become infinite). `workspace`: the caller's scratch (paged_tree_ws_bytes)."""
+    of its position. q f32 [T][nH][hd] raw; normalised and rotated, it enters the products at f32 accuracy (f16
+    pairs) at head_dim 256 and rounded to f16 at 512. With k_new / v_new ([T][kvH][hd], f32 or f16) the tokens' rows
+    are prepared as ``kv_write`` prepares them, each at its position, and stored by the same call before they are
+    attended; without, the cache holds them. A tree has at most 1024 tokens: rows behind are rows of nobody. Returns
+    out [T][nH][hd] (f16 by default). f32 caches are converted to f16 in the workspace (values beyond 65504 become
+    infinite). `workspace`: the caller's scratch (paged_tree_ws_bytes)."""
     dev, qp, qg = _q(q, cfg, q_gain)
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
     n = q.shape[0]
@@ -210,11 +210,12 @@ def paged_fork(pools, page_table, key_len, parent, free_pages, n_free, *, worksp
                n_pages: int | None = None, page_size: int | None = None, max_key_len: int | None = None):
     """The tables, lengths and free list of sequences that follow their parents (beams after a step's selection).
 
-    New row j continues row parent[j] (int32 [n_new], of any shape) of page_table [n_seq][cols], which lists every sequence that has pages of the pools
-    (one that does not branch is its own parent; a parent outside [0, n_seq) makes an idle row). Full pages are shared;
-    each page that a row will write to, for `room` more keys, becomes its own: the first heir keeps the parent's, the
-    others get pages off the end of free_pages (int32 [n_pages], n_free int32 [1] of them in use), and the filled rows of a
-    partly filled one are copied in every pool. Pages that no new row holds are added to the list first, in order.
+    New row j continues row parent[j] (int32, n_new of them in any shape) of page_table [n_seq][cols], which lists every
+    sequence that has pages of the pools (one that does not branch is its own parent; a parent outside [0, n_seq) makes
+    an idle row). Full pages are shared; each page that a row will write to, for `room` more keys, becomes its own: the
+    first heir keeps the parent's, the others get pages off the end of free_pages (int32 [n_pages], its first n_free
+    (int32 [1]) are free), and the filled rows of a partly filled one are copied in every pool. Pages that no new row
+    holds are added to the list first, in order.
     Returns (table [n_new][cols], key_len [n_new], free_pages, n_free), all new tensors, or the four given as `out` (none of
     them an input: alternate two sets in a captured loop). Too few free pages leave -1 in the last columns that need one;
     n_new * (2 + room // page_size) always suffice. n_pages and page_size are needed where there are no pools.
@@ -257,8 +258,8 @@ def beam_select(logits, scores, *, workspace: DecodeWorkspace, cap: float = 0.0,
                 out=None):
     """The n_out best continuations of each group of beams (default: as many as beams).
 
-    logits f32 or f16 [n_groups * width][V] (rows may lie further apart than V); scores f32 [n_groups][width]: the beams' sums of
-    log probabilities. A candidate scores its beam's plus log softmax(cap * tanh(logits / cap)) (cap 0: of the logits). done
+    logits f32 or f16 [n_groups * width][V], 16-byte aligned (rows may lie further apart than V); scores f32
+    [n_groups][width]: the beams' sums of log probabilities. A candidate scores its beam's plus log softmax(cap * tanh(logits / cap)) (cap 0: of the logits). done
     (bool [n_groups][width]): a finished beam has one candidate, token `pad` at its own score. Logits of -inf or NaN are
     no tokens. Returns (score f32, parent int32, token int32), each [n_groups][n_out], best first, equal scores by beam, then
     token; parent is the row of logits, which ``paged_fork`` takes as it is. Places that no candidate of a score above -inf
