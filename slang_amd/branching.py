@@ -259,11 +259,12 @@ def beam_select(logits, scores, *, workspace: DecodeWorkspace, cap: float = 0.0,
     """The n_out best continuations of each group of beams (default: as many as beams).
 
     logits f32 or f16 [n_groups * width][V], 16-byte aligned (rows may lie further apart than V); scores f32
-    [n_groups][width]: the beams' sums of log probabilities. A candidate scores its beam's plus log softmax(cap * tanh(logits / cap)) (cap 0: of the logits). done
-    (bool [n_groups][width]): a finished beam has one candidate, token `pad` at its own score. Logits of -inf or NaN are
-    no tokens. Returns (score f32, parent int32, token int32), each [n_groups][n_out], best first, equal scores by beam, then
-    token; parent is the row of logits, which ``paged_fork`` takes as it is. Places that no candidate of a score above -inf
-    fills hold -inf, -1, -1. `out`: the three, made by an earlier call. `workspace`: the caller's scratch (beam_select_ws_bytes)."""
+    [n_groups][width]: the beams' sums of log probabilities. A candidate scores its beam's plus log softmax(cap *
+    tanh(logits / cap)) (cap 0: of the logits). done (bool [n_groups][width]): a finished beam has one candidate, token
+    `pad` at its own score. Logits of -inf or NaN are no tokens. Returns (score f32, parent int32, token int32), each
+    [n_groups][n_out], best first, equal scores by beam, then token; parent is the row of logits, which ``paged_fork``
+    takes as it is. Places that no candidate of a score above -inf fills hold -inf, -1, -1. `out`: the three, made by an
+    earlier call. `workspace`: the caller's scratch (beam_select_ws_bytes)."""
     if scores.dim() != 2:
         raise ValueError(f"scores must be [n_groups][width], got {tuple(scores.shape)}")
     dev, (groups, width) = _gpu("logits", logits), scores.shape
