@@ -371,7 +371,9 @@ int g4a_paged_fork(const g4a_pool* pools, int n_pools, const g4a_paged* pg, int 
  *   done        uint8 [n_groups][width] or NULL: a beam that is done has one candidate, token pad at its own score.
  *   out_score   f32, out_parent (the row of logits that the beam continues) and out_token int32 [n_groups][n_out]. A
  *               candidate of score -inf or NaN is none: places without one hold -inf, -1, -1.
- * Scores are formed in 64 bits from a row's sum in 32, and rounded once. Within a beam larger logits come first.
+ * Scores are formed in 64 bits from a row's sum in 32, and rounded once; cap may be any finite number. What a score is
+ * off by, beside that rounding: 2^-18, with a cap up to 64 also 2^-20 of the cap, above 64 2^-19 of the row's largest |x'|.
+ * Within a beam larger logits come first.
  *   ws          at least g4a_beam_select_ws_bytes() bytes, 256-byte aligned, uninitialised.
  * width and n_out are at most G4A_BEAMS_MAX.
  */

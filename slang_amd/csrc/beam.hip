@@ -40,15 +40,48 @@ __device__ __forceinline__ float of_ascending(uint32_t u) {
 }
 __device__ __forceinline__ u64 key_of(float x, int token) { return (u64)ascending(x) << 32 | (uint32_t)~token; }
 
-// x' log2e / unit of a logit: unit is log2e with a cap, cap tanh(x / cap) as cap - 2 cap / (1 + 2^(2 log2e x / cap)), and 1
-// without, so that the difference of two, which is exact where it matters, is rounded last. up2 = 2 log2e / cap
-template <bool CAP>
-__device__ __forceinline__ float capped(float x, float cap2, float up2) {
-    return CAP ? __builtin_fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + fexp2(x * up2)), cap2) : x;
+// A logit x counts as x' = cap tanh(x / cap), or as it is without a cap. What the kernels hold is x' times log2e / unit:
+//   kNoCap    unit log2e: the difference of two logits, which is exact where it matters, is rounded last.
+//   kCap      unit 1: cap - 2 cap / (1 + 2^(2 log2e x / cap)), off by 2.5 2^-23 of the cap, whatever x is. Its reciprocal cap is
+//             kept finite for caps near the smallest numbers, where 0 times infinity would be no number.
+//   kWideCap  unit log2e, for caps above kCapTo: tanh by its series, x + x u^2 (-1/3 + 2/15 u^2 - 17/315 u^4 + 62/2835 u^6), where
+//             |u| = |x / cap| < 0.3 (the next term is below 2^-24), else 1 - 2 / (1 + 2^(2 log2e u)): off by 4.5 2^-23 of x'.
+//             A logit takes twelve instructions more than with kCap: 128 rows of 262144 in f32 54.5 us a call for 46.8.
+enum { kNoCap, kCap, kWideCap };
+constexpr float kCapTo = 64.0f;
+struct Cap {
+    float cap, up;  // kCap: cap log2e, 2 log2e / cap; kWideCap: cap, 1 / cap
+};
+template <int CAP>
+__device__ __forceinline__ Cap cap_of(float cap) {
+    return CAP == kCap ? Cap{cap * kLog2e, fminf(2.0f * kLog2e / cap, 3.40282347e38f)} : Cap{cap, 1.0f / cap};
 }
-// ... in 64 bits, where beams are compared (not by tanh(), whose 64 bits take a microsecond)
-__device__ __forceinline__ double capped64(float x, float cap) {
-    return cap == 0.0f ? (double)x : (double)cap - 2.0 * (double)cap / (1.0 + exp(2.0 * (double)x / (double)cap));
+template <int CAP>
+__device__ __forceinline__ float capped(float x, const Cap& c) {
+    if (CAP == kCap) return __builtin_fmaf(-2.0f * c.cap, __builtin_amdgcn_rcpf(1.0f + fexp2(x * c.up)), c.cap);
+    if (CAP == kWideCap) {
+        const float u = x * c.up, u2 = u * u;
+        const float far = c.cap * __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + fexp2(u * (2.0f * kLog2e))), 1.0f);
+        float p = __builtin_fmaf(u2, 62.0f / 2835.0f, -17.0f / 315.0f);
+        p = __builtin_fmaf(u2, p, 2.0f / 15.0f);
+        p = __builtin_fmaf(u2, p, -1.0f / 3.0f);
+        return fabsf(u) < 0.3f ? __builtin_fmaf(x, u2 * p, x) : far;
+    }
+    return x;
+}
+// 2^ of the difference of two
+template <int CAP>
+__device__ __forceinline__ float weight(float d) { return fexp2(CAP == kCap ? d : d * kLog2e); }
+// x' in 64 bits, where beams are compared (not by tanh(), whose 64 bits take a microsecond): off by 2^-51 of the cap; for
+// caps above kCapTo by the series below |u| = 0.05, whose next term is below 2^-50
+template <int CAP>
+__device__ __forceinline__ double capped64(float x_, float cap_) {
+    const double x = x_, cap = cap_;
+    if (CAP == kNoCap) return x;
+    const double u = x / cap, u2 = u * u;
+    if (CAP == kWideCap && fabs(u) < 0.05)
+        return x + x * (u2 * (-1.0 / 3.0 + u2 * (2.0 / 15.0 + u2 * (-17.0 / 315.0 + u2 * (62.0 / 2835.0)))));
+    return cap - 2.0 * cap / (1.0 + exp(2.0 * u));
 }
 
 __device__ __forceinline__ u64 wave_max64(u64 k) {
@@ -99,14 +132,13 @@ __device__ __forceinline__ int wave_rank(u64* list, int total, int want, int lan
 }
 
 // What a part's sum, relative to its own maximum, counts relative to M
-template <bool CAP>
-__device__ __forceinline__ float part_weight(float2 v, float M, float Mc, float cap2, float up2) {
-    const float d = capped<CAP>(v.x, cap2, up2) - Mc;
-    return v.x == M ? v.y : v.x > kNegInf ? v.y * fexp2(CAP ? d : d * kLog2e) : 0.0f;
+template <int CAP>
+__device__ __forceinline__ float part_weight(float2 v, float M, const Cap& c) {
+    return v.x == M ? v.y : v.x > kNegInf ? v.y * weight<CAP>(capped<CAP>(v.x, c) - capped<CAP>(M, c)) : 0.0f;
 }
 
 // Rows may begin anywhere: a part begins at a multiple of VEC elements of the tensor, at or in front of the row's first.
-template <typename T, int E, bool CAP>
+template <typename T, int E, int CAP>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
     constexpr int VEC = 16 / sizeof(T);
     typedef T vec_t __attribute__((ext_vector_type(VEC)));
@@ -135,7 +167,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
             }
         }
     };
-    const float cap2 = a.cap * kLog2e, up2 = CAP ? 2.0f * kLog2e / a.cap : 0.0f;
+    const Cap cap = cap_of<CAP>(a.cap);
     float m = kNegInf, s = 0.0f;
     float least = -3.40282347e38f;  // what a logit has to reach to be a candidate: nothing below can be among the largest
     int count = 0, sorted = 0;      // candidates in the list; of them in order and above all that came before them
@@ -156,16 +188,16 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
         }
         const float mx = wave_max(mine);
         if (mx > m) {
-            const float d = capped<CAP>(m, cap2, up2) - capped<CAP>(mx, cap2, up2);
-            s = m == kNegInf ? 0.0f : s * fexp2(CAP ? d : d * kLog2e);
+            const float d = capped<CAP>(m, cap) - capped<CAP>(mx, cap);
+            s = m == kNegInf ? 0.0f : s * weight<CAP>(d);
             m = mx;
         }
-        const float mc = capped<CAP>(m, cap2, up2);
+        const float mc = capped<CAP>(m, cap);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float d = capped<CAP>(x[i], cap2, up2) - mc;
-            sum += fexp2(CAP ? d : d * kLog2e);
+            const float d = capped<CAP>(x[i], cap) - mc;
+            sum += weight<CAP>(d);
         }
         // with -inf, which a cap would make finite, or NaN, which are no tokens, or +inf, which is all there is: with care
         if (__ballot(!(sum < __builtin_huge_valf()) || (CAP && low == kNegInf))) {
@@ -173,8 +205,8 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 x[i] = fmaxf(x[i], kNegInf);
-                const float d = capped<CAP>(x[i], cap2, up2) - mc;
-                sum += x[i] == kNegInf ? 0.0f : x[i] == m ? 1.0f : fexp2(CAP ? d : d * kLog2e);
+                const float d = capped<CAP>(x[i], cap) - mc;
+                sum += x[i] == kNegInf ? 0.0f : x[i] == m ? 1.0f : weight<CAP>(d);
             }
         }
         s += sum;
@@ -229,6 +261,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamArgs a) {
 // candidate's place among the group's is its own place in its beam and, of each other beam, the number of candidates in
 // front of it, found by halving.
 constexpr int kGroupWaves = 16;
+template <int CAP>
 __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a) {
     __shared__ u64 s_list[kGroupWaves][kList];
     __shared__ union {
@@ -240,6 +273,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a
     __shared__ double s_score[kBeams];
     __shared__ double s_log[kBeams], s_most[kBeams];  // of a row: log of the sum of exp(x' - the largest x'), and that x'
     const int g = blockIdx.x, tid = threadIdx.x, threads = blockDim.x, W = a.width, K = a.n_out;
+    const Cap cap = cap_of<CAP>(a.cap);
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid < W) {
         s_n[tid] = 0;
@@ -257,15 +291,13 @@ __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a
             top = max(top, (uint32_t)(keys[(size_t)i * K] >> 32));
         }
         m = wave_max(m);
-        const bool cap = a.cap != 0.0f;
-        const float cap2 = a.cap * kLog2e, up2 = 2.0f * kLog2e / a.cap, mc = cap ? capped<true>(m, cap2, up2) : m;
         const uint32_t bound = max(wave_bound(top, K), 1u);  // (0 is no key)
         double s = 0.0;
         int total = 0;
         for (int i0 = 0; i0 < a.parts; i0 += 64) {  // wave-uniform
             const int i = i0 + lane;
             const float2 v = i < a.parts ? sums[i] : make_float2(kNegInf, 0.0f);
-            s += (double)(cap ? part_weight<true>(v, m, mc, cap2, up2) : part_weight<false>(v, m, mc, cap2, up2));
+            s += (double)part_weight<CAP>(v, m, cap);
             bool more = i < a.parts;
             for (int k = 0; k < K; ++k) {
                 const u64 key = more ? keys[(size_t)i * K + k] : 0;
@@ -303,7 +335,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a
     __syncthreads();
     for (int i = tid; i < W * K; i += threads) {
         const u64 key = s_cand[i].key;
-        const double c = capped64(of_ascending((uint32_t)(key >> 32)), a.cap);
+        const double c = capped64<CAP>(of_ascending((uint32_t)(key >> 32)), a.cap);
         s_token[i] = key ? ~(int)(uint32_t)key : -1;
         s_cand[i].score = c;
         if (i % K == 0) s_most[i / K] = c;
@@ -364,13 +396,19 @@ __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a
     }
 }
 
-typedef void (*beam_part_fn)(BeamArgs);
-template <typename T>
-static beam_part_fn pick_each(int each, bool cap) {
-    if (each == 32) return cap ? beam_part_kernel<T, 32, true> : beam_part_kernel<T, 32, false>;
-    return cap ? beam_part_kernel<T, 8, true> : beam_part_kernel<T, 8, false>;
+typedef void (*beam_fn)(BeamArgs);
+template <typename T, int CAP>
+static beam_fn pick_each(int each) { return each == 32 ? beam_part_kernel<T, 32, CAP> : beam_part_kernel<T, 8, CAP>; }
+template <int CAP>
+static beam_fn pick_part(bool f16, int each) { return f16 ? pick_each<half_t, CAP>(each) : pick_each<float, CAP>(each); }
+struct BeamFns {
+    beam_fn part, group;
+};
+static BeamFns pick_beam(bool f16, int each, float cap) {
+    if (cap == 0.0f) return {pick_part<kNoCap>(f16, each), beam_group_kernel<kNoCap>};
+    if (cap > kCapTo) return {pick_part<kWideCap>(f16, each), beam_group_kernel<kWideCap>};
+    return {pick_part<kCap>(f16, each), beam_group_kernel<kCap>};
 }
-static beam_part_fn pick_part(bool f16, int each, bool cap) { return f16 ? pick_each<half_t>(each, cap) : pick_each<float>(each, cap); }
 
 // Few logits: 512 a wave, one step, so that many waves share them. Many, or rows so long that their parts would be many to
 // join: steps of 2048, as many as leave the card kPartWaves waves. A call in a graph with steps of 512 and of 2048: 4 rows
@@ -448,8 +486,9 @@ extern "C" int g4a_beam_select(int n_groups, int width, int vocab, int logits_f1
                      p.parts, p.steps, pad, cap};
     const hipStream_t stream = (hipStream_t)stream_;
     const dim3 grid((unsigned)((p.parts + 3) / 4), (unsigned)(n_groups * width));
-    hipLaunchKernelGGL(pick_part(logits_f16 != 0, p.each, cap > 0.0f), grid, dim3(256), 0, stream, a);
-    hipLaunchKernelGGL(beam_group_kernel, dim3((unsigned)n_groups), dim3(64 * std::min(width, kGroupWaves)), 0, stream, a);
+    const BeamFns fn = pick_beam(logits_f16 != 0, p.each, cap);
+    hipLaunchKernelGGL(fn.part, grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(fn.group, dim3((unsigned)n_groups), dim3(64 * std::min(width, kGroupWaves)), 0, stream, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? G4A_OK : hip_error(e, "beam select launch");
 }
