@@ -422,12 +422,13 @@ static BeamFns pick_beam(bool f16, int each, float cap) {
 }
 
 // Few logits: 512 a wave, one step, so that many waves share them. Many, or rows so long that their parts would be many to
-// join: steps of 2048, as many as leave the card kPartWaves waves. A call in a graph with steps of 512 and of 2048: 4 rows
-// of 32000 10.6 and 14.3 us, of 100000 12.8 and 14.6, of 131072 12.9 and 12.3, of 262144 16.5 and 13.3; 128 rows of 50000
-// 17.5 and 18.6, of 65536 19.5 and 18.3, of 262144 48.0 and 36.9.
+// join: steps of 2048, as many (to the nearest) as leave the card kPartWaves waves. A call in a graph with steps of 512 and of
+// 2048: 4 rows of 32000 9.3 and 10.6 us, of 65536 9.9 and 10.2, of 100000 11.6 and 10.5, of 262144 14.7 and 11.4; 128 rows of
+// 32000 in f16 with a cap 19.2 and 25.1, of 50000 22.1 and 21.5, of 65536 23.9 and 21.8, of 262144 56.5 and 40.3; 1024 rows of
+// 8192 20.1 and 20.4.
 // A wave pays for its first step's bound and order, so longer walks are cheaper, and fewer waves hide less: the kernel takes
-// 35.4 us for 128 rows of 262144 in f32 with a cap with 2 steps of 2048 (3.8 TB/s), 35.5 with 1, 37.6 with 4, 36.5 and 37.5
-// with 4 and 8 of 1024, 43 where the next step's loads were waited for; 30.7 without a cap. What bounds it: a logit with
+// 33.6 us for 128 rows of 262144 in f32 with a cap with 2 steps of 2048 (4.0 TB/s), 33.8 with 1 (whose parts take the join a
+// microsecond more), 34.5 with 4; 29.4 without a cap. What bounds it: a logit with
 // a cap takes two exponentials, a reciprocal and six more instructions, about 72 cycles a wave of 64, 15 us of the card's
 // VALU beside the 26 us that the bytes take, and a wave's first step's ballots and LDS trips.
 constexpr int kPartWaves = 8192;
@@ -438,7 +439,7 @@ struct BeamPlan {
 static BeamPlan beam_plan(int n_groups, int width, int vocab, int n_out) {
     BeamPlan p;
     const int64_t rows = (int64_t)n_groups * width, span = vocab;
-    p.each = vocab >= 1 << 17 || rows * vocab >= (int64_t)64 * 16 * kPartWaves ? 32 : 8;
+    p.each = vocab > 1 << 16 || rows * vocab >= (int64_t)64 * 16 * kPartWaves ? 32 : 8;
     const int64_t step = (int64_t)64 * 32 * kPartWaves;
     p.steps = p.each == 8 ? 1 : (int)std::min<int64_t>(std::max<int64_t>((rows * vocab + step / 2) / step, 1), 64);
     const int64_t part = (int64_t)64 * p.each * p.steps;
