@@ -365,17 +365,17 @@ int g4a_paged_fork(const g4a_pool* pools, int n_pools, const g4a_paged* pg, int 
 /*
  * Beam search's selection. Beam w of group g has the logits x of row g * width + w and the score s; token t makes the
  * candidate of score s + x'[t] - log sum exp x', x' = cap * tanh(x / cap) (cap 0: x' = x). Of a group's width * vocab
- * candidates the n_out of highest score, best first, equal ones by beam and then by token.
+ * candidates the n_out of highest score, best first. A beam's own candidates are in the order of their logits, equal logits by
+ * token: a cap moves none of them, also where it rounds two to one score. Equal scores of two beams are by beam.
  *   logits      f32, or f16 with logits_f16, rows row_stride elements apart, 16-byte aligned. A token whose logit is -inf
  *               or NaN is none: no weight, no candidate. +inf (without a cap) shares the weight with the row's other +inf.
  *   done        uint8 [n_groups][width] or NULL: a beam that is done has one candidate, token pad at its own score.
  *   out_score   f32, out_parent (the row of logits that the beam continues) and out_token int32 [n_groups][n_out]. A
  *               candidate of score -inf or NaN is none: places without one hold -inf, -1, -1.
- * Scores are formed in 64 bits from a row's sum in 32, and rounded once; cap may be any finite number. What a score is
+ * Scores are formed in 64 bits from a row's sum in 32, and rounded once; cap: 0 to below 3e38. What a score is
  * off by, beside that rounding: 2^-18, with a cap up to 64 also 2^-20 of the cap, above 64 2^-19 of the row's largest |x'|.
- * Within a beam larger logits come first.
  *   ws          at least g4a_beam_select_ws_bytes() bytes, 256-byte aligned, uninitialised.
- * width and n_out are at most G4A_BEAMS_MAX.
+ * width and n_out are at most G4A_BEAMS_MAX, n_groups * width at most 65535, vocab at most 2^30.
  */
 #define G4A_BEAMS_MAX 64
 size_t g4a_beam_select_ws_bytes(int n_groups, int width, int vocab, int n_out);

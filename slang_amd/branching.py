@@ -262,9 +262,10 @@ def beam_select(logits, scores, *, workspace: DecodeWorkspace, cap: float = 0.0,
     [n_groups][width]: the beams' sums of log probabilities. A candidate scores its beam's plus log softmax(cap *
     tanh(logits / cap)) (cap 0: of the logits). done (bool [n_groups][width]): a finished beam has one candidate, token
     `pad` at its own score. Logits of -inf or NaN are no tokens. Returns (score f32, parent int32, token int32), each
-    [n_groups][n_out], best first, equal scores by beam, then token; parent is the row of logits, which ``paged_fork``
-    takes as it is. Places that no candidate of a score above -inf fills hold -inf, -1, -1. `out`: the three, made by an
-    earlier call. `workspace`: the caller's scratch (beam_select_ws_bytes)."""
+    [n_groups][n_out], best first: a beam's candidates in the order of their logits (a cap moves none of them), equal
+    logits by token, equal scores of two beams by beam; parent is the row of logits, which ``paged_fork`` takes as it
+    is. Places that no candidate of a score above -inf fills hold -inf, -1, -1. At most 64 beams, 64 places, 65535 rows of
+    logits. `out`: the three, made by an earlier call. `workspace`: the caller's scratch (beam_select_ws_bytes)."""
     if scores.dim() != 2:
         raise ValueError(f"scores must be [n_groups][width], got {tuple(scores.shape)}")
     dev, (groups, width) = _gpu("logits", logits), scores.shape
