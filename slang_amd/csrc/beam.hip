@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a
         if (total <= kList) {
             total = wave_rank(s_list[wave], total, K, lane);
             if (lane < K) s_cand[w * K + lane].key = lane < total ? s_list[wave][lane] : 0;
-        } else {  // many are equal: one after the other
+        } else {  // many are equal, or fewer parts than n_out, where no bound is found, have more than the list holds: one after the other
             u64 last = ~0ull;
             for (int k = 0; k < K; ++k) {
                 u64 best = 0;
