@@ -296,13 +296,14 @@ int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, con
  * and, of the tree, itself and the ancestors whose depth is less than W below its own, all on pages that are there.
  * (A V row that is not finite reaches other tokens of the tree as in g4a_paged_prefill. Masked K rows may hold anything.)
  *   parents     int32 [n_tokens], device, indices within the tree.
- *   q, out      as g4a_paged_prefill, but that at head_dim 256 the prepared q enters the products as f16 pairs (f32
- *               accuracy); at 512 it is rounded to f16 (G4A_Q_HILO refused).
+ *   q, out      as g4a_paged_prefill, but that the prepared q always enters the products as f16 pairs (f32 accuracy;
+ *               G4A_Q_HILO refused).
  *   k_new/v_new [n_tokens][n_kv_heads][head_dim], f32, or f16 with G4A_IN_F16, or both NULL (the cache holds the rows):
  *               prepared as g4a_kv_write prepares rows at the tokens' positions, to the bit, and stored at rows
  *               start + i before they are attended (k_in_q, v_in_q, k_gain as there).
  *   ws          at least g4a_paged_tree_ws_bytes() bytes, 256-byte aligned, uninitialised; concurrent calls need
- *               distinct ones. f32 caches are converted to f16 in it, as in g4a_paged_prefill.
+ *               distinct ones. f32 caches are converted in it, K to f16 pairs, as g4a_paged_decode reads it, and V to f16
+ *               (beyond 65504 a V becomes infinite, a K NaN).
  */
 #define G4A_TREE_MAX 1024
 size_t g4a_paged_tree_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens);

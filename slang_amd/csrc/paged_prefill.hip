@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256) void paged_prep_kernel(PagedPrefillArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void paged_kv16_kernel(PagedKv16Args a) { kv16_rows(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z); }
+__global__ __launch_bounds__(256) void paged_kv16_kernel(PagedKv16Args a) { kv16_rows<false>(a, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z); }
 
 // Merge of the pieces of a split query block, as prefill_merge_kernel: with each piece holding
 // o_p = O_p / l_p, out = sum_p o_p l_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), M = max_p m_p. One workgroup
@@ -415,7 +415,7 @@ typedef void (*paged_prefill_fn)(PagedPrefillArgs);
 
 template <int G>
 static paged_prefill_fn pick_out(int HD, bool out32) {
-    if (HD == 256) return out32 ? paged_prefill_kernel_256<G, float> : paged_prefill_kernel_256<G, half_t>;
+    if (HD == 256) return out32 ? paged_kernel_w256<G, float> : paged_kernel_w256<G, half_t>;
     return out32 ? paged_prefill_kernel_512<G, float> : paged_prefill_kernel_512<G, half_t>;
 }
 static paged_prefill_fn pick_paged(int HD, int G, bool out32) {  // G: 1, 2, 4 or 8 (check_cfg)
@@ -552,6 +552,7 @@ extern "C" int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_
         k.vc = (const float*)pg->v_pages;
         k.ko = (half_t*)(w + p.k16);
         k.vo = (half_t*)(w + p.v16);
+        k.klo = nullptr;
         k.tab = (int32_t*)(w + p.tab16);
         k.n_tokens = n_tokens;
         k.row = (int)cfg->n_kv_heads * HD;

@@ -3,12 +3,14 @@
 // A tree's n tokens are its sequence's last rows, token i at row start + i, start = key_len - n. parents[i] < i names
 // the token that i continues, anything else makes it a root, whose parent is the history's last key. So token i stands at
 // position start + depth(i) and attends the history's keys t with start + depth(i) - t < W, and itself and its ancestors j
-// with depth(i) - depth(j) < W. Everything else is paged_prefill.hip's: the same 128 columns x key tiles unit
-// (paged_tiles.hpp), q and P as f16 operands, sums in f32, K/V rows through the page table.
+// with depth(i) - depth(j) < W. Everything else is paged_prefill.hip's: the same unit of columns x key tiles
+// (paged_tiles.hpp), P and V as f16 operands, sums in f32, K/V rows through the page table. Scores are plain decoding's, so that
+// drafts are checked as it would choose: q is a pair of f16 operands, and so is K of f32 caches (their two products of a
+// remainder, not the one of both).
 //
 // Few tokens over a long history: the rows of K and V are read once for all of a tree's tokens, so the call is bound by
 // them, and the history is what gets cut over the card. Three launches: rows (RoPE by depth, the k/v rows into their
-// pages, q in f16, the tokens' bits, and in the first workgroup the work list), units, and the merge of their partials.
+// pages, q in two f16 operands, the tokens' bits, and in the first workgroup the work list), units, and the merge of their partials.
 #include <algorithm>
 
 #include "paged_tiles.hpp"
@@ -18,6 +20,7 @@ namespace g4a {
 constexpr int kTreeSlots = 768;   // pieces with partials in a call
 constexpr int kTreePieces = 256;  // pieces a query block is cut into
 constexpr int kPlanThreads = 256;
+constexpr int tree_columns(int HD) { return HD == 256 ? 128 : 64; }  // of a unit: tokens times heads of a kv head
 
 struct TreeRowArgs : PagedTreeArgs {
     const void* k_new;
@@ -37,7 +40,8 @@ __device__ __forceinline__ SeqRows tree_rows(const PageTab& t, const int32_t* cu
 }
 
 // ---------------------------------------------------------------- the work list
-// Cost of a piece beside its tiles, of its partial and of the merge, in key tiles (1.9 us at hd 256, 2.4 at 512).
+// Cost of a piece beside its tiles, of its partial and of the merge, in key tiles (about 2 us). (At hd 512 prices of 4 to 9 a piece
+// and 1 to 2.5 a partial are within 1 % of each other over eight batches.)
 struct TreeCost {
     float unit, part, merge;
 };
@@ -226,10 +230,10 @@ __device__ __forceinline__ int walk_up(const int32_t* par, int i, int* lds, int 
     }
 }
 
-// Workgroup 0: the work list. Then a wave per token and four heads: q to f16 as paged_prep_kernel makes it, at the token's
-// depth, and once a token its depth and bits. Then, with new rows, a workgroup per token and kv head: paged_write's row at
-// its own place, rotated by its depth, in the cache and in an f32 cache's f16 copy. Then the copy's other rows, which need
-// none of that: one launch where rows, copy, q and list took three (3 trees of 253, 123 and 60 after 500 to 5000 keys 74 -> 64 us a call).
+// Workgroup 0: the work list. Then a wave per token and four heads: q as paged_prep_kernel makes it, at the token's
+// depth, in f16 and what that leaves, and once a token its depth and bits. Then, with new rows, a workgroup per token and kv head: paged_write's row at
+// its own place, rotated by its depth, in the cache and in an f32 cache's f16 copies. Then the copies' other rows, which need
+// none of that: one launch where rows, copy, q and list took three (3 trees of 253, 123 and 60 after 500 to 5000 keys 10 us a call less).
 template <int HD, typename IT, typename CT>
 __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
     __shared__ int s_par[4][kTreeMax];
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
             if (h0 + i < a.n_q_heads) {
                 const size_t at = ((size_t)tok * a.n_q_heads + h0 + i) * HD + E * lane;
                 *reinterpret_cast<hvec_t*>(a.q16 + at) = hv;
-                if constexpr (HD == 256) *reinterpret_cast<hvec_t*>(a.q16_lo + at) = lo;
+                *reinterpret_cast<hvec_t*>(a.q16_lo + at) = lo;
             }
         }
         return;
@@ -315,7 +319,7 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
         if constexpr (sizeof(CT) == 4) {
             blk -= row_blocks;  // < conv_x * n_seq * conv_z by the grid
             const int x = blk % a.conv_x, bz = blk / a.conv_x;
-            kv16_rows(a.conv, x, bz / a.conv_z, bz % a.conv_z, a.conv_z);
+            kv16_rows<true>(a.conv, x, bz / a.conv_z, bz % a.conv_z, a.conv_z);
         }
         return;
     }
@@ -357,6 +361,8 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
         const size_t copy = paged_row(a.rows, b * a.t.cols + (at >> a.rows.shift), at, a.n_kv_heads * HD) + (size_t)kh * HD;
         a.conv.ko[copy + t] = (half_t)k0;
         a.conv.ko[copy + t + HALF] = (half_t)k1;
+        a.conv.klo[copy + t] = rest16(k0);
+        a.conv.klo[copy + t + HALF] = rest16(k1);
         a.conv.vo[copy + t] = (half_t)v0;
         a.conv.vo[copy + t + HALF] = (half_t)v1;
     }
@@ -364,21 +370,21 @@ __global__ __launch_bounds__(256) void tree_rows_kernel(TreeRowArgs a) {
 
 // ---------------------------------------------------------------- merge
 // out = sum_p o_p l_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), M = max_p m_p, of a block's pieces (o_p = O_p / l_p). A
-// workgroup's item is a wave block of 32 columns x 256 dims of an entry of the merge list, and of its 16 runs of 8 values
+// workgroup's item is a wave's block of 32 columns x 256 dims of an entry of the merge list, and of its 16 runs of 8 values
 // x 64 lanes one, so that many workgroups share the bytes (four runs an item: 8 trees of 16 after 2000 keys 29 -> 35 us a
 // call, 64 after 3000 111 -> 116). Its four waves take every fourth piece, each relative to its own largest m so far, and
 // join through LDS: one trip to memory for up to 16 pieces.
 constexpr int kMergeGrid = 2048;
 template <typename OUTT, int HD>
 __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
-    constexpr int NCOL = 128, NV = NCOL * HD, BLK = NV * 3;  // values and bytes of a piece's block
-    constexpr int NW = 4 * (HD / 256);                       // wave blocks
+    constexpr int NCOL = tree_columns(HD), NV = NCOL * HD, BLK = NV * 3;  // values and bytes of a piece's block
+    constexpr int NW = 4;                                                 // waves' blocks
     __shared__ float s_o[4][8][64], s_l[4][64], s_m[4][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
     const int merges = a.counts[1], G = a.n_q_heads / a.n_kv_heads, BQ = NCOL / G;
     for (int item = blockIdx.x; item < merges * NW * 16; item += gridDim.x) {
         const PagedUnit pu = a.merges[item / (NW * 16)];
-        const int w = item / 16 % NW, k = item % 16, qb = pu.qb, kh = pu.kh, n_pieces = pu.n_pieces, w32 = HD == 256 ? w : w >> 1;
+        const int w = item / 16 % NW, k = item % 16, qb = pu.qb, kh = pu.kh, n_pieces = pu.n_pieces, w32 = HD == 256 ? w : w & 1;
         if (qb * BQ + 32 * w32 / G >= pu.S) continue;  // no token in these 32 columns
         const int c = 32 * w32 + (lane & 31), s_idx = qb * BQ + c / G;
         const bool ok = s_idx < pu.S;
@@ -438,7 +444,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
             }
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             OUTT* orow = reinterpret_cast<OUTT*>(a.out) + ((size_t)(pu.row0 + s_idx) * a.n_q_heads + kh * G + c % G) * HD +
-                         (HD == 256 ? 0 : 256 * (w & 1));
+                         (HD == 256 ? 0 : 256 * (w >> 1));
             // run k: dims tile k/2, 4-row pair k%2
             OUTT* to = orow + 32 * (k >> 1) + 16 * (k & 1) + 8 * (wave >> 1) + 4 * h + 2 * (wave & 1);
             store_elem(to, srq(x * inv, a.out_q));
@@ -452,17 +458,21 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PagedTreeArgs a) {
 typedef void (*tree_fn)(PagedTreeArgs);
 typedef void (*tree_rows_fn)(TreeRowArgs);
 
-template <int G>
-static tree_fn pick_out(int HD, bool out32) {
-    if (HD == 256) return out32 ? paged_prefill_kernel_256<G, float, PagedTreeArgs> : paged_prefill_kernel_256<G, half_t, PagedTreeArgs>;
-    return out32 ? paged_prefill_kernel_512<G, float, PagedTreeArgs> : paged_prefill_kernel_512<G, half_t, PagedTreeArgs>;
+template <int G, int HD, bool K32>
+static tree_fn pick_out(bool out32) {
+    return out32 ? paged_kernel_w256<G, float, PagedTreeArgs, HD, K32> : paged_kernel_w256<G, half_t, PagedTreeArgs, HD, K32>;
 }
-static tree_fn pick_units(int HD, int G, bool out32) {  // G: 1, 2, 4 or 8 (check_cfg)
+template <int G>
+static tree_fn pick_form(int HD, bool kv32, bool out32) {
+    if (HD == 256) return kv32 ? pick_out<G, 256, true>(out32) : pick_out<G, 256, false>(out32);
+    return kv32 ? pick_out<G, 512, true>(out32) : pick_out<G, 512, false>(out32);
+}
+static tree_fn pick_units(int HD, int G, bool kv32, bool out32) {  // G: 1, 2, 4 or 8 (check_cfg)
     switch (G) {
-        case 1: return pick_out<1>(HD, out32);
-        case 2: return pick_out<2>(HD, out32);
-        case 4: return pick_out<4>(HD, out32);
-        default: return pick_out<8>(HD, out32);
+        case 1: return pick_form<1>(HD, kv32, out32);
+        case 2: return pick_form<2>(HD, kv32, out32);
+        case 4: return pick_form<4>(HD, kv32, out32);
+        default: return pick_form<8>(HD, kv32, out32);
     }
 }
 static tree_fn pick_merge(int HD, bool out32) {
@@ -475,16 +485,17 @@ static tree_rows_fn pick_rows(bool in16, bool c32) {
     return c32 ? tree_rows_kernel<HD, float, float> : tree_rows_kernel<HD, float, half_t>;
 }
 
-// What the host can bound, and the workspace [counts][units][merges][depth][bits][q16][its remainders][partials][(m, l)][K16][V16][table16].
+// What the host can bound, and the workspace [counts][units][merges][depth][bits][q16][its remainders][partials][(m, l)][K16][its
+// remainders][V16][table16].
 // Every part grows with n_tokens, n_seq and max_key_len, so that one reserved for the largest call holds all.
 struct TreePlan {
     int bq, kt, max_units, max_slots, words, cols16;
-    size_t units, merges, depth, bits, q16, q16_lo, part_o, part_ml, k16, v16, tab16, total;
+    size_t units, merges, depth, bits, q16, q16_lo, part_o, part_ml, k16, k16_lo, v16, tab16, total;
 };
 static bool tree_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, TreePlan& p) {
     const int HD = (int)cfg->head_dim, G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
     const int64_t kvh = cfg->n_kv_heads;
-    p.bq = 128 / G;
+    p.bq = tree_columns(HD) / G;
     p.kt = HD == 256 ? 64 : 32;
     p.words = tree_words(n_tokens);
     const int64_t blocks = std::min<int64_t>(n_tokens, (int64_t)n_tokens / p.bq + pg->n_seq);
@@ -506,10 +517,10 @@ static bool tree_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, Tre
     p.depth = part((size_t)n_tokens * sizeof(int32_t));
     p.bits = part((size_t)n_tokens * p.words * sizeof(unsigned long long));
     p.q16 = part((size_t)n_tokens * cfg->n_q_heads * HD * sizeof(half_t));
-    p.q16_lo = HD == 256 ? part((size_t)n_tokens * cfg->n_q_heads * HD * sizeof(half_t)) : p.q16;
-    p.part_o = part((size_t)slots * 128 * HD * 3);
-    p.part_ml = part((size_t)slots * 128 * sizeof(float2));
-    p.k16 = p.v16 = p.tab16 = at;
+    p.q16_lo = part((size_t)n_tokens * cfg->n_q_heads * HD * sizeof(half_t));
+    p.part_o = part((size_t)slots * tree_columns(HD) * HD * 3);
+    p.part_ml = part((size_t)slots * tree_columns(HD) * sizeof(float2));
+    p.k16 = p.k16_lo = p.v16 = p.tab16 = at;
     p.cols16 = 0;
     int64_t pages16 = 0;
     if (cfg->flags & G4A_KV_F32) {
@@ -517,6 +528,7 @@ static bool tree_plan(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, Tre
         pages16 = (int64_t)pg->n_seq * p.cols16;
         const size_t pool = (size_t)pages16 * pg->page_size * kvh * HD * sizeof(half_t);
         p.k16 = part(pool);
+        p.k16_lo = part(pool);
         p.v16 = part(pool);
         p.tab16 = part((size_t)pages16 * sizeof(int32_t));
     }
@@ -559,7 +571,7 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
         return G4A_EINVAL;
     }
     if (cfg->flags & G4A_Q_HILO) {
-        set_error("g4a_paged_tree takes q as its head_dim allows (G4A_Q_HILO not supported)");
+        set_error("g4a_paged_tree holds q at f32 accuracy by itself (G4A_Q_HILO not supported)");
         return G4A_EUNSUPPORTED;
     }
     const int HD = (int)cfg->head_dim, G = (int)(cfg->n_q_heads / cfg->n_kv_heads);
@@ -602,6 +614,7 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
     a.bits = (unsigned long long*)(w + p.bits);
     a.depth = (int32_t*)(w + p.depth);
     a.q16_lo = (half_t*)(w + p.q16_lo);
+    a.kc_lo = nullptr;
     a.words = p.words;
     a.k_new = k_new;
     a.v_new = v_new;
@@ -624,6 +637,7 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
         k.vc = (const float*)pg->v_pages;
         k.ko = (half_t*)(w + p.k16);
         k.vo = (half_t*)(w + p.v16);
+        k.klo = (half_t*)(w + p.k16_lo);
         k.tab = (int32_t*)(w + p.tab16);
         k.n_tokens = n_tokens;
         k.row = a.n_kv_heads * HD;
@@ -635,6 +649,7 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
         blocks += (int64_t)a.conv_x * pg->n_seq * a.conv_z;
         // the units read the f16 copy by its own table
         a.kc = w + p.k16;
+        a.kc_lo = w + p.k16_lo;
         a.vc = w + p.v16;
         a.t.table = (const int32_t*)(w + p.tab16);
         a.t.cols = a.t.stride = p.cols16;
@@ -648,10 +663,10 @@ extern "C" int g4a_paged_tree(const g4a_cfg* cfg, const g4a_paged* pg, int n_tok
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged tree preparation launch");
     const bool out32 = (cfg->flags & G4A_OUT_F32) != 0;
     const PagedTreeArgs& t = a;
-    hipLaunchKernelGGL(pick_units(HD, G, out32), dim3((unsigned)p.max_units), dim3(256), 0, stream, t);
+    hipLaunchKernelGGL(pick_units(HD, G, kv32, out32), dim3((unsigned)p.max_units), dim3(256), 0, stream, t);
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged tree launch");
     // a block of the merge list has two slots at least
-    const int items = p.max_slots / 2 * 4 * (HD / 256) * 16;
+    const int items = p.max_slots / 2 * 4 * 16;
     hipLaunchKernelGGL(pick_merge(HD, out32), dim3((unsigned)std::max(std::min(items, kMergeGrid), 1)), dim3(256), 0, stream, t);
     if ((e = hipGetLastError()) != hipSuccess) return hip_error(e, "paged tree merge launch");
     return G4A_OK;
