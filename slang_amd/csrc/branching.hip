@@ -316,10 +316,11 @@ __device__ __forceinline__ void fork_pages(const ForkArgs& a, const ForkMarks& m
     if (tid == 0) a.n_free_out[0] = left;
 }
 
-// All of it by one workgroup, the marks in LDS, where pages and table entries are few. A call without copies, against the
-// three launches: 4 rows of 11 columns 5.6 and 9.2 us, 128 of 67 12.3 and 23.0, 256 of 67 18.5 and 28.5, 1024 of 23
-// 30.6 and 31.5, 512 of 66 (67584 entries) 29.8 and 32.3.
-constexpr int kForkPages = 12288, kForkEntries = 1 << 16, kForkRows = 1024;
+// All of it by one workgroup, the marks in LDS, which holds those of 12288 pages, where table entries are few. A call without
+// copies in a graph, against the three launches: 4 rows of 11 columns 5.5 and 8.7 us (with 12288 pages 7.2 and 9.9), 128 of
+// 67 12.4 and 13.5, 256 of 67 (34304 entries) 19.0 and 18.3, 512 of 66 26.3 and 23.3, 1024 of 66 45.9 and 24.7, 64 of 1000 26.7 and
+// 20.6. (Beyond, the free list is one workgroup's still: 500000 pages, most of them free, take 89 us.)
+constexpr int kForkPages = 12288, kForkEntries = 1 << 15, kForkRows = 1024;
 __global__ __launch_bounds__(kForkThreads) void fork_small_kernel(ForkArgs a) {
     __shared__ int32_t s_owner[kForkPages];
     __shared__ uint32_t s_bits[3][kForkPages / 32];
