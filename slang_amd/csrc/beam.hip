@@ -326,7 +326,8 @@ __global__ __launch_bounds__(64 * kGroupWaves) void beam_group_kernel(BeamArgs a
         if (total <= kList) {
             total = wave_rank(s_list[wave], total, K, lane);
             if (lane < K) s_cand[w * K + lane].key = lane < total ? s_list[wave][lane] : 0;
-        } else {  // many are equal, or fewer parts than n_out, where no bound is found, have more than the list holds: one after the other
+        } else {  // many are equal, or fewer parts than n_out, where no bound is found, have more than the list holds: one after the
+                  // other (4 rows of 32000 in 63 parts: n_out 16 11.2 us a call, 64 112)
             u64 last = ~0ull;
             for (int k = 0; k < K; ++k) {
                 u64 best = 0;

