@@ -163,11 +163,11 @@ __device__ __forceinline__ float4v read_f4(const float* __restrict p) { return *
 //     columns a workgroup, key tiles of 32, as large as those of 64 at hd 256). A wave with all 512 dims of its columns, as in the
 //     prompts' kernel, has no registers for q's second operand (q 128 and O 256 of 512). Against that kernel with q in f16: 8 trees
 //     of 16 after 2000 keys 36 us a call for 41, 3 of 60 to 253 55 for 57; where history streams, twice the columns a K/V
-//     byte tell: 16 of 5 to 40 after up to 16384 97 for 83.
+//     byte tell: 16 of 5 to 40 after up to 16384 92 for 83.
 //   * K32, over f32 caches: K's remainder in f16 is a second tile, multiplied by q's high operand behind the first. Both have
 //     one place in LDS, which is filled again as soon as its products are done: high, low, P.V, each tile is on its way for two
 //     of a round's three phases, and the waits are counted so that the next one's fetch goes on. Half as many bytes again as
-//     with K in f16 alone: 16 trees after up to 8192 keys at hd 512 164 us a call for 129 (179 with each low tile fetched
+//     with K in f16 alone: 16 trees after up to 8192 keys at hd 512 158 us a call for 129 (15 more with each low tile fetched
 //     and waited for in its own round), 32 after up to 2000 at hd 256 51 for 45.
 template <int G, typename OUTT, typename ARGS = PagedPrefillArgs, int HD = 256, bool K32 = false>
 __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {

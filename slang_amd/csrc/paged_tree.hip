@@ -139,7 +139,7 @@ __device__ void plan_trees(const TreeRowArgs& a) {
         st = __builtin_amdgcn_readlane(my, pick);
         __syncthreads();
     }
-    const Over over_st(st), over_kvh(a.n_kv_heads);
+    const Over over_st(st);
     int at[3] = {0, 0, 0};  // units, slots, merges of the chunks before
     for (int c = 0; c < chunks; ++c) {
         if (chunks > 1) load_chunk(c);
@@ -169,9 +169,14 @@ __device__ void plan_trees(const TreeRowArgs& a) {
             }
             const int pieces = max(over_st.up(s_nt[lo]), 1);
             const Over over_pieces(pieces);
-            const int k = u - s_at[0][lo], block = over_pieces(k), p = k - block * pieces;
-            const int qb = over_kvh(block), kh = block - qb * a.n_kv_heads;
             const int start = s_start[lo], S = s_S[lo], b = c * kPlanThreads + lo;
+            // The blocks that read the same keys (stream kh * pieces + p) come every eighth, which is the same XCD: its L2
+            // then reads them once (hd 512: 16 trees after up to 16384 keys 97 -> 92.5 us a call). Eight streams at a time, the last
+            // ones as many as there are.
+            const int k = u - s_at[0][lo], nb = (S + a.bq - 1) >> log_bq, streams = pieces * a.n_kv_heads;
+            const int group = Over(8 * nb)(k), in = k - group * 8 * nb, wide = min(8, streams - 8 * group);
+            const int qb = Over(wide)(in), stream = 8 * group + in - qb * wide;
+            const int kh = over_pieces(stream), p = stream - kh * pieces;
             const int nt = tree_tiles(start, S, qb, a.bq, a.kt, a.window);
             // (pieces of ceil(nt / pieces) tiles or one less, so that no product passes 32 bits)
             const int each = over_pieces(nt), more = nt - each * pieces, t0 = p * each + min(p, more);
