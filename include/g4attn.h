@@ -303,7 +303,7 @@ int g4a_paged_prefill(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens, con
  *               start + i before they are attended (k_in_q, v_in_q, k_gain as there).
  *   ws          at least g4a_paged_tree_ws_bytes() bytes, 256-byte aligned, uninitialised; concurrent calls need
  *               distinct ones. f32 caches are converted in it, K to f16 pairs, as g4a_paged_decode reads it, and V to f16
- *               (beyond 65504 a V becomes infinite, a K NaN).
+ *               (values beyond 65504 make what attends them infinite or NaN).
  */
 #define G4A_TREE_MAX 1024
 size_t g4a_paged_tree_ws_bytes(const g4a_cfg* cfg, const g4a_paged* pg, int n_tokens);

@@ -104,8 +104,8 @@ def paged_tree(q, k_pages, v_pages, page_table, key_len, cu_q, parents, cfg: Att
     pairs), as in ``paged_decode``, and so does K of f32 caches. With k_new / v_new ([T][kvH][hd], f32 or f16) the tokens' rows
     are prepared as ``kv_write`` prepares them, each at its position, and stored by the same call before they are
     attended; without, the cache holds them. A tree has at most 1024 tokens: rows behind are rows of nobody. Returns
-    out [T][nH][hd] (f16 by default). f32 caches are converted in the workspace, K to pairs of f16 and V to f16 (a V
-    beyond 65504 becomes infinite, a K NaN). `workspace`: the caller's scratch (paged_tree_ws_bytes)."""
+    out [T][nH][hd] (f16 by default). f32 caches are converted in the workspace, K to pairs of f16 and V to f16 (values
+    beyond 65504 make what attends them infinite or NaN). `workspace`: the caller's scratch (paged_tree_ws_bytes)."""
     dev, qp, qg = _q(q, cfg, q_gain)
     pg, rc, rs = _cache(dev, k_pages, v_pages, page_table, key_len, cfg, max_key_len, rope_cos, rope_sin)
     n = q.shape[0]

@@ -167,8 +167,10 @@ __device__ __forceinline__ float4v read_f4(const float* __restrict p) { return *
 //   * K32, over f32 caches: K's remainder in f16 is a second tile, multiplied by q's high operand behind the first. Both have
 //     one place in LDS, which is filled again as soon as its products are done: high, low, P.V, each tile is on its way for two
 //     of a round's three phases, and the waits are counted so that the next one's fetch goes on. Half as many bytes again as
-//     with K in f16 alone: 16 trees after up to 8192 keys at hd 512 158 us a call for 129 (15 more with each low tile fetched
-//     and waited for in its own round), 32 after up to 2000 at hd 256 51 for 45.
+//     with K in f16 alone: 16 trees after up to 8192 keys at hd 512 160 us a call for 129 (15 more with each low tile fetched
+//     and waited for in its own round), 32 after up to 2000 at hd 256 52 for 45. P keeps its remainder too, on the V operands that
+//     are there: outputs are 2.9e-4 off, 3.1 to 3.2e-4 without it, of which 2.1e-4 each are V's and the output's rounding to
+//     f16 (1 to 5 % of a call; a V beyond f16 makes its outputs NaN where a weight leaves no remainder).
 template <int G, typename OUTT, typename ARGS = PagedPrefillArgs, int HD = 256, bool K32 = false>
 __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
     constexpr bool TREE = std::is_same<ARGS, PagedTreeArgs>::value;
@@ -488,7 +490,7 @@ __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
         }
         started = true;
         const float msub = m_use == kNegInf ? 0.0f : m_use;
-        half8 pb[2 * NS];
+        half8 pb[2 * NS], pl[K32 ? 2 * NS : 1];
         float ps = 0.0f;
         const rsrc_t rv = tile_rows(a.vc, t + 1, entry), rk = tile_rows(a.kc, t + 2, entry1);
         {
@@ -509,8 +511,9 @@ __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
                     const half_t p = (half_t)ev[s & 1][e];
                     pb[(NS * s + e) >> 3][(NS * s + e) & 7] = p;
                     // (a tree's sum is of the weights as they enter the product: the leading ones' roundings cancel, f16 caches 2.9 ->
-                    // 2.6e-4 off, f32 ones 3.4 -> 3.1e-4, in the same time)
-                    ps += TREE ? (float)p : ev[s & 1][e];
+                    // 2.6e-4 off in the same time)
+                    ps += TREE && !K32 ? (float)p : ev[s & 1][e];
+                    if constexpr (K32) pl[(NS * s + e) >> 3][(NS * s + e) & 7] = (half_t)(ev[s & 1][e] - (float)p);
                 }
             };
             read_k(tile_k(t + 1), 0, kr[0]);
@@ -540,7 +543,10 @@ __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
         l_run += ps;
         // (here, not where they are used behind the masks' branches: the compiler would sink them there)
 #pragma unroll
-        for (int u = 0; u < 2 * NS; ++u) asm volatile("" : "+v"(pb[u]));
+        for (int u = 0; u < 2 * NS; ++u) {
+            asm volatile("" : "+v"(pb[u]));
+            if constexpr (K32) asm volatile("" : "+v"(pl[u]));
+        }
         asm volatile("" : "+v"(l_run));
         if constexpr (K32) {
             meet_but_last();  // K(t + 1)'s low tile is in LDS, V(t + 1) on its way; its high tile fully consumed
@@ -574,6 +580,8 @@ __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
             for (int i = 0; i < kPvAhead; ++i) read_v(i);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
+                // (the remainders' products one behind, so that no two in turn have the same sum)
+                if (K32 && i > 0) mfma32_acc(oacc[(i - 1) & 7], av[(i - 1) % (kPvAhead + 1)], pl[(i - 1) >> 3]);
                 if (i + kPvAhead < N) read_v(i + kPvAhead);
                 mfma32_acc(oacc[i & 7], av[i % (kPvAhead + 1)], pb[i >> 3]);
                 constexpr int I0 = 4 * NS;
@@ -582,6 +590,7 @@ __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
                 if (K32 && i < 8) dma(rkl, tile_k_lo(), i, k_off(i));
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (K32) mfma32_acc(oacc[(N - 1) & 7], av[(N - 1) % (kPvAhead + 1)], pl[(N - 1) >> 3]);
             asm volatile("" : "+v"(mnext));
         }
         if constexpr (LATE) {

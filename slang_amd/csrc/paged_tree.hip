@@ -5,8 +5,8 @@
 // position start + depth(i) and attends the history's keys t with start + depth(i) - t < W, and itself and its ancestors j
 // with depth(i) - depth(j) < W. Everything else is paged_prefill.hip's: the same unit of columns x key tiles
 // (paged_tiles.hpp), P and V as f16 operands, sums in f32, K/V rows through the page table. Scores are plain decoding's, so that
-// drafts are checked as it would choose: q is a pair of f16 operands, and so is K of f32 caches (their two products of a
-// remainder, not the one of both).
+// drafts are checked as it would choose: q is a pair of f16 operands, and so are K and P over f32 caches (products of one
+// remainder, not of two).
 //
 // Few tokens over a long history: the rows of K and V are read once for all of a tree's tokens, so the call is bound by
 // them, and the history is what gets cut over the card. Three launches: rows (RoPE by depth, the k/v rows into their

@@ -71,7 +71,7 @@ def test_a_token_alone_is_a_decode_step(hd, kvh, kv):
 @pytest.mark.parametrize("hd", [256, 512])
 @pytest.mark.parametrize("junk", [1e6, np.inf, np.nan])
 def test_keys_beyond_f16_in_an_f32_cache(hd, junk):
-    """One that is attended shows as NaN, one that is masked reaches nobody; a V beyond f16 is infinite."""
+    """One that is attended shows as NaN, one that is masked reaches nobody; a V beyond f16 shows in all that attend it."""
     b = Trees([60], [20], hd=hd, kvh=1, kv=np.float32, seed=5)
     out, A, S = b.oracle()
     victim = 7
@@ -84,4 +84,16 @@ def test_keys_beyond_f16_in_an_f32_cache(hd, junk):
     assert np.isnan(got[hit]).all()
     v = b.v_pages.copy()
     v[b.table[0, 0], 3] = 1e6
-    assert np.isinf(tree(b, b.dev(v_pages=torch.from_numpy(v).cuda())).cpu().numpy()).all()
+    assert not np.isfinite(tree(b, b.dev(v_pages=torch.from_numpy(v).cuda())).cpu().numpy()).any()
+
+
+@pytest.mark.parametrize("hd,kvh", [(256, 2), (512, 1)])
+def test_weights_over_f32_caches_keep_their_bits(hd, kvh):
+    """With V that f16 holds, an f32 output over an f32 cache has no rounding to f16 left: pairs' remainders (2^-22 of q, K and P,
+    their products), f32 arithmetic on scores (2^-19), partials of 24 bits (2^-16). Four times below a half step of f16."""
+    b = Trees([300, 70, 1500, 33], [20, 70, 9, 1], hd=hd, kvh=kvh, kv=np.float32, seed=4)
+    b.v_pages = b.v_pages.astype(np.float16).astype(np.float32)
+    out, A, S = b.oracle()
+    got = tree(b, b.dev(), out_dtype=torch.float32).cpu().numpy()
+    d = (2.0 ** -21 + 2.0 ** -20 + 2.0 ** -19) * S + 2.0 ** -20
+    check(got, out, (np.expm1(2 * d) + 2.0 ** -16 + 2.0 ** -20) * A + 2.0 ** -24 * np.abs(out) + 2.0 ** -24)
