@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void paged_kernel_w256(ARGS a) {
     // n32 of a row from logical chunk n32 ^ (row % 32)) into the LDS stage that tile t0 + 1 takes over
     // later, then reads them back in that layout; rows past the block's last token read as zeros.
     // (A tree's second operand, what f16 leaves of q, goes straight into registers, and the first too where that stage is not
-    // free or rows are longer. Outputs are 2.1 to 2.9e-4 off 64 bits instead of 4.2 to 5.2e-4 with q in f16, where an f16 output
+    // free or rows are longer. Outputs are 2.1 to 2.6e-4 off 64 bits instead of 4.2 to 5.2e-4 with q in f16, where an f16 output
     // alone is 2.1e-4; 16 long histories take 71 us for 65.7, one short one 10.2 for 8.4.)
     half8 qf[16], ql[TREE ? 16 : 1];
     int entry1, gone0, gone1 = 0;  // tile t + 1's page, the 16-row groups of tiles t and t + 1 without one
