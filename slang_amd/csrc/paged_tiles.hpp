@@ -166,9 +166,9 @@ __device__ __forceinline__ float4v read_f4(const float* __restrict p) { return *
 //     byte tell: 16 of 5 to 40 after up to 16384 92 for 83.
 //   * K32, over f32 caches: K's remainder in f16 is a second tile, multiplied by q's high operand behind the first. Both have
 //     one place in LDS, which is filled again as soon as its products are done: high, low, P.V, each tile is on its way for two
-//     of a round's three phases, and the waits are counted so that the next one's fetch goes on. Half as many bytes again as
+//     of a tile's three phases, and the waits are counted so that the next one's fetch goes on. Half as many bytes again as
 //     with K in f16 alone: 16 trees after up to 8192 keys at hd 512 160 us a call for 129 (15 more with each low tile fetched
-//     and waited for in its own round), 32 after up to 2000 at hd 256 52 for 45. P keeps its remainder too, on the V operands that
+//     and waited for within its own tile), 32 after up to 2000 at hd 256 52 for 45. P keeps its remainder too, on the V operands that
 //     are there: outputs are 2.9e-4 off, 3.1 to 3.2e-4 without it, of which 2.1e-4 each are V's and the output's rounding to
 //     f16 (1 to 5 % of a call; a V beyond f16 makes its outputs NaN where a weight leaves no remainder).
 template <int G, typename OUTT, typename ARGS = PagedPrefillArgs, int HD = 256, bool K32 = false>
